@@ -173,7 +173,7 @@ def _plain_quantize(x, pow2):
     most = v.abs().amax(dim=2).clamp(min=LEAST)
     if pow2:
         mantissa, exponent = torch.frexp(most / E4M3_MAX)
-        scale = torch.ldexp(torch.ones_like(most), exponent - (mantissa == 0.5).int())
+        scale = ((exponent - (mantissa == 0.5).int() + 127) << 23).view(torch.float32)
         q = v / scale.unsqueeze(2)
     else:
         scale = most / E4M3_MAX
@@ -290,7 +290,8 @@ def work(case):
 
 def _e4m3_64(v):
     """Each 64-bit value's nearest e4m3 value, ties to the even significand; |v| <= 448."""
-    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3.0)
+    exponent = torch.frexp(v.abs().clamp(min=2.0 ** -6)).exponent.long()       # v < 2 ** exponent
+    step = ((exponent - 4 + 1023) << 52).view(torch.float64)
     return torch.round(v / step) * step
 
 
@@ -299,10 +300,9 @@ def _quantize64(x, pow2):
     for part in x.double().split(128, dim=1):
         most = part.abs().max(dim=1, keepdim=True).values.clamp(min=LEAST)
         if pow2:
-            e = torch.floor(torch.log2(most / E4M3_MAX)) - 1.0     # then up to the first power that holds it
-            for _ in range(3):
-                e = torch.where(torch.exp2(e) * E4M3_MAX < most, e + 1.0, e)
-            scale = torch.exp2(e)
+            scale = torch.full_like(most, 2.0 ** -126)
+            for _ in range(256):
+                scale = torch.where(scale * E4M3_MAX < most, scale * 2.0, scale)
             values.append(_e4m3_64(part / scale))
         else:
             scale = most / E4M3_MAX
