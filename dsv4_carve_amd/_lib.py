@@ -36,6 +36,14 @@ EXPORTS = (
     "exl3_moe_prefill_scratch_bytes",
     "exl3_moe_prefill",
     "exl3_moe_prefill_routed",
+    "exl3_fp8_quantize",
+    "exl3_fp8_gemm",
+    "exl3_fp8_linear_scratch_bytes",
+    "exl3_fp8_linear",
+    "exl3_fp8_moe_max_rows",
+    "exl3_fp8_moe_scratch_bytes",
+    "exl3_fp8_moe",
+    "exl3_moe_route",
 )
 
 _lock = threading.Lock()
@@ -82,6 +90,15 @@ _SIGS = {
                                  _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                  _P, _I, _P, _I, _P, _L,
                                  _P, _I, _I, _I, _F, _P, _L, _P], _I),
+    "exl3_fp8_quantize": ([_P, _I, _L, _L, _I, _P, _P, _P], _I),
+    "exl3_fp8_gemm": ([_P, _P, _L, _L, _P, _P, _L, _P, _I, _P], _I),
+    "exl3_fp8_linear_scratch_bytes": ([_L, _L, _L], _L),
+    "exl3_fp8_linear": ([_P, _I, _L, _L, _P, _P, _L, _P, _I, _P, _L, _P], _I),
+    "exl3_fp8_moe_max_rows": ([], _I),
+    "exl3_fp8_moe_scratch_bytes": ([_L, _L, _L], _L),
+    "exl3_fp8_moe": ([_P, _I, _P, _I, _L, _L, _L, _L, _L, _P, _P, _P, _P,
+                      _P, _I, _P, _I, _P, _L, _F, _P, _L, _P], _I),
+    "exl3_moe_route": ([_P, _I, _L, _L, _L, _I, _P, _I, _F, _P, _I, _P, _P], _I),
 }
 
 

@@ -1,0 +1,181 @@
+// C-ABI entry points of the block-scaled 8-bit path and the expert router
+// (declared in include/exl3_amd.h).
+#include <cmath>
+
+#include "exl3_fp8_moe.hpp"
+#include "exl3_topk.hpp"
+
+using namespace exl3;
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static int check_blocks(int64_t m, int64_t k, int64_t n) {
+    if (m < 1 || n < 1 || k < 16 || k % 16) return fail("m and n must be positive and k a positive multiple of 16");
+    if (k > (1 << 24) || n > (1 << 24)) return fail("k and n must be at most 2^24");
+    if (m > (int64_t)65535 * 16) return fail("m must be at most 1048560");
+    return 0;
+}
+
+template <int K>
+static int launch_quantize(const void* x, int64_t rows, int k, int groups, bool pow2, uint8_t* q, float* scale,
+                           hipStream_t s) {
+    const bool chunks = k % 16 == 0 && aligned16(x) && aligned16(q);
+    const int64_t blocks = chunks ? (rows * groups * 8 + 255) / 256 : (rows * groups + 3) / 4;
+    if (blocks > 0x7fffffffLL) return fail("too many values");
+    const dim3 grid((unsigned)blocks), block(256);
+    if (chunks) {
+        if (pow2) hipLaunchKernelGGL((fp8_quantize_kernel<K, true>), grid, block, 0, s, x, rows, k, groups, q, scale);
+        else hipLaunchKernelGGL((fp8_quantize_kernel<K, false>), grid, block, 0, s, x, rows, k, groups, q, scale);
+    } else {
+        if (pow2) hipLaunchKernelGGL((fp8_quantize_any_kernel<K, true>), grid, block, 0, s, x, rows, k, groups, q, scale);
+        else hipLaunchKernelGGL((fp8_quantize_any_kernel<K, false>), grid, block, 0, s, x, rows, k, groups, q, scale);
+    }
+    return check_launch();
+}
+
+static int quantize(const void* x, int x_kind, int64_t rows, int64_t k, bool pow2, uint8_t* q, float* scale,
+                    hipStream_t s) {
+    const int groups = (int)((k + FP8_BLOCK - 1) / FP8_BLOCK);
+    if (x_kind == OUT_F16) return launch_quantize<OUT_F16>(x, rows, (int)k, groups, pow2, q, scale, s);
+    if (x_kind == OUT_BF16) return launch_quantize<OUT_BF16>(x, rows, (int)k, groups, pow2, q, scale, s);
+    return launch_quantize<OUT_F32>(x, rows, (int)k, groups, pow2, q, scale, s);
+}
+
+static int gemm(const uint8_t* a, const float* a_scale, int64_t m, int64_t k, const uint8_t* w, const float* w_scale,
+                int64_t n, void* c, int c_kind, hipStream_t s) {
+    hipLaunchKernelGGL((fp8_gemm_rows_kernel<1, 16>), dim3((unsigned)((n + 15) / 16), (unsigned)((m + 15) / 16)),
+                       dim3(1024), 0, s, a, a_scale, m, (int)k, w, w_scale, (int)n, c, c_kind);
+    return check_launch();
+}
+
+static int64_t linear_scratch_bytes(int64_t m, int64_t k) {
+    return align_up(m * k, 256) + m * ((k + FP8_BLOCK - 1) / FP8_BLOCK) * 4;
+}
+
+extern "C" {
+
+int exl3_fp8_quantize(const void* x, int x_kind, int64_t rows, int64_t k, int pow2, uint8_t* q, float* scale,
+                      void* stream) {
+    clear_error();
+    if (!x || !q || !scale) return fail("null pointer");
+    if (x_kind < OUT_F16 || x_kind > OUT_F32) return fail("x_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
+    if (rows < 1 || k < 1) return fail("rows and k must be positive");
+    if (k > (1 << 24)) return fail("k must be at most 2^24");
+    if (rows > (int64_t)1 << 36) return fail("too many values");
+    return quantize(x, x_kind, rows, k, pow2 != 0, q, scale, reinterpret_cast<hipStream_t>(stream));
+}
+
+int exl3_fp8_gemm(const uint8_t* a, const float* a_scale, int64_t m, int64_t k, const uint8_t* w, const float* w_scale,
+                  int64_t n, void* c, int c_kind, void* stream) {
+    clear_error();
+    if (!a || !a_scale || !w || !w_scale || !c) return fail("null pointer");
+    if (c_kind < OUT_F16 || c_kind > OUT_F32) return fail("c_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
+    if (check_blocks(m, k, n)) return -1;
+    if (!aligned16(a) || !aligned16(w) || !aligned16(c)) return fail("a, w and c must be 16-byte aligned");
+    return gemm(a, a_scale, m, k, w, w_scale, n, c, c_kind, reinterpret_cast<hipStream_t>(stream));
+}
+
+int64_t exl3_fp8_linear_scratch_bytes(int64_t m, int64_t k, int64_t n) {
+    clear_error();
+    if (check_blocks(m, k, n)) return -1;
+    return linear_scratch_bytes(m, k);
+}
+
+int exl3_fp8_linear(const void* x, int x_kind, int64_t m, int64_t k, const uint8_t* w, const float* w_scale, int64_t n,
+                    void* c, int c_kind, void* scratch, int64_t scratch_bytes, void* stream) {
+    clear_error();
+    if (!x || !w || !w_scale || !c || !scratch) return fail("null pointer");
+    if (x_kind < OUT_F16 || x_kind > OUT_F32) return fail("x_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
+    if (c_kind < OUT_F16 || c_kind > OUT_F32) return fail("c_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
+    if (check_blocks(m, k, n)) return -1;
+    if (!aligned16(w) || !aligned16(c) || !aligned16(scratch)) return fail("w, c and scratch must be 16-byte aligned");
+    if (scratch_bytes < linear_scratch_bytes(m, k)) return fail("scratch too small");
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    uint8_t* q = static_cast<uint8_t*>(scratch);
+    float* scale = reinterpret_cast<float*>(q + align_up(m * k, 256));
+    const int rc = quantize(x, x_kind, m, k, false, q, scale, s);
+    return rc ? rc : gemm(q, scale, m, k, w, w_scale, n, c, c_kind, s);
+}
+
+int exl3_fp8_moe_max_rows(void) { return FP8_MOE_MAX_ROWS; }
+
+int64_t exl3_fp8_moe_scratch_bytes(int64_t rows, int64_t topk, int64_t intermediate) {
+    clear_error();
+    if (rows < 1 || rows > FP8_MOE_MAX_ROWS) return fail("row count out of range (1 <= rows <= exl3_fp8_moe_max_rows())");
+    if (topk < 1 || topk > FP8_MOE_MAX_TOPK) return fail("topk must be in 1..16");
+    if (intermediate < 128 || intermediate % 128) return fail("intermediate must be a positive multiple of 128");
+    return rows * topk * intermediate * 2;
+}
+
+int exl3_fp8_moe(const void* x, int x_kind, void* out, int out_kind, int64_t rows, int64_t hidden, int64_t intermediate,
+                 int64_t n_experts, int64_t topk, const uint8_t* w13, const float* w13_scale, const uint8_t* w2,
+                 const float* w2_scale, const void* topk_ids, int ids_kind, const void* topk_weights, int weights_kind,
+                 const int64_t* expert_map, int64_t n_global, float swiglu_limit, void* scratch, int64_t scratch_bytes,
+                 void* stream) {
+    clear_error();
+    if (!x || !out || !w13 || !w13_scale || !w2 || !w2_scale || !topk_ids || !topk_weights || !scratch)
+        return fail("null pointer");
+    if (x_kind != OUT_F16 && x_kind != OUT_BF16) return fail("x_kind must be 0 (fp16) or 1 (bf16)");
+    if (out_kind < OUT_F16 || out_kind > OUT_F32) return fail("out_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
+    const int64_t need = exl3_fp8_moe_scratch_bytes(rows, topk, intermediate);
+    if (need < 0) return -1;
+    if (hidden < 128 || hidden % 128) return fail("hidden must be a positive multiple of 128");
+    if (hidden > (1 << 20) || intermediate > (1 << 20)) return fail("hidden and intermediate must be at most 2^20");
+    if (n_experts < 1 || n_experts > (1 << 16)) return fail("n_experts must be in 1..65536");
+    if (!(swiglu_limit > 0.f)) return fail("swiglu_limit must be positive (infinity for none)");
+    if (scratch_bytes < need) return fail("scratch too small");
+    if (!aligned16(x) || !aligned16(out) || !aligned16(w13) || !aligned16(w2) || !aligned16(scratch))
+        return fail("x, out, w13, w2 and scratch must be 16-byte aligned");
+    Fp8MoeArgs A{x, w13, w13_scale, w2, w2_scale, static_cast<uint16_t*>(scratch), out, Route{}, out_kind, (int)rows,
+                 (int)hidden, (int)intermediate, (int)n_experts, (int)topk, swiglu_limit};
+    if (make_route(topk_ids, ids_kind, topk_weights, weights_kind, expert_map, n_global, A.rt)) return -1;
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const dim3 g1((unsigned)(intermediate / 16), (unsigned)(rows * topk)), g2((unsigned)(hidden / 16));
+    const auto launch = [&](auto gu, auto dn) {
+        hipLaunchKernelGGL(gu, g1, dim3(FP8_GU_WAVES * 64), 0, s, A);
+        const int rc = check_launch();
+        if (rc) return rc;
+        hipLaunchKernelGGL(dn, g2, dim3(FP8_DOWN_WAVES * 64), 0, s, A);
+        return check_launch();
+    };
+    if (x_kind == OUT_BF16) {
+        if (rows <= 16) return launch(fp8_moe_gate_up_kernel<true, 1>, fp8_moe_down_kernel<true, 1>);
+        if (rows <= 32) return launch(fp8_moe_gate_up_kernel<true, 2>, fp8_moe_down_kernel<true, 2>);
+        return launch(fp8_moe_gate_up_kernel<true, 4>, fp8_moe_down_kernel<true, 4>);
+    }
+    if (rows <= 16) return launch(fp8_moe_gate_up_kernel<false, 1>, fp8_moe_down_kernel<false, 1>);
+    if (rows <= 32) return launch(fp8_moe_gate_up_kernel<false, 2>, fp8_moe_down_kernel<false, 2>);
+    return launch(fp8_moe_gate_up_kernel<false, 4>, fp8_moe_down_kernel<false, 4>);
+}
+
+int exl3_moe_route(const void* logits, int logits_kind, int64_t rows, int64_t n_experts, int64_t topk, int scoring,
+                   const float* bias, int renormalize, float scale, void* ids, int ids_kind, float* weights,
+                   void* stream) {
+    clear_error();
+    if (!logits || !ids || !weights) return fail("null pointer");
+    if (logits_kind < OUT_F16 || logits_kind > OUT_F32) return fail("logits_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
+    if (ids_kind != IDS_I32 && ids_kind != IDS_I64) return fail("ids_kind must be 0 (int32) or 1 (int64)");
+    if (scoring < SCORE_SOFTMAX || scoring > SCORE_SQRTSOFTPLUS)
+        return fail("scoring must be 0 (softmax), 1 (sigmoid) or 2 (sqrtsoftplus)");
+    if (rows < 1 || n_experts < 1 || n_experts > ROUTE_MAX_EXPERTS)
+        return fail("rows must be positive and n_experts in 1..2048");
+    if (topk < 1 || topk > ROUTE_MAX_TOPK || topk > n_experts) return fail("topk must be in 1..min(64, n_experts)");
+    if (!std::isfinite(scale)) return fail("scale must be finite");
+    if (rows > 4 * 0x7fffffffLL) return fail("too many rows");
+    const int64_t blocks = (rows + 3) / 4;
+    const RouteArgs A{logits, bias, ids, weights, rows, logits_kind, (int)n_experts, (int)topk, scoring,
+                      ids_kind == IDS_I64, renormalize != 0, scale};
+    const int per_lane = (int)(n_experts + 63) / 64;
+    const auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), A);
+        return check_launch();
+    };
+    if (per_lane <= 1) return launch(moe_route_kernel<1>);
+    if (per_lane <= 2) return launch(moe_route_kernel<2>);
+    if (per_lane <= 4) return launch(moe_route_kernel<4>);
+    if (per_lane <= 8) return launch(moe_route_kernel<8>);
+    if (per_lane <= 16) return launch(moe_route_kernel<16>);
+    return launch(moe_route_kernel<32>);
+}
+
+}  // extern "C"

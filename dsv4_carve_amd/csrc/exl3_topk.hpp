@@ -1,0 +1,201 @@
+// Top-k of a router's logits, with the weights of the chosen experts.
+//
+//   score s(l): softmax over the row, 1 / (1 + e^-l), or sqrt(log(1 + e^l))
+//   order:      by l, or by s(l) + bias where a selection bias is given; ties to
+//               the lowest index; a logit (or a biased score) of -inf or NaN is
+//               never chosen
+//   weight:     s of the chosen (without the bias), over their sum if asked for,
+//               times a constant
+//
+// A wave has a row, lane i the experts i, i + 64, ...  The k largest are found one
+// by one: each lane's best, a maximum over the wave, the lowest index that has it.
+//
+// Order by biased scores is the order of the exact scores even where fp32 cannot
+// tell two apart: the k + 1 largest are found in fp32 first, and if two
+// neighbours among them are nearer than fp32's error the row is done again in 64
+// bits (about one row in a hundred of normal logits).  Weights are computed in 64
+// bits: one exponential a lane, and far logits keep their ratios.
+#pragma once
+
+#include "exl3_decode.hpp"
+#include "exl3_capi_util.hpp"
+
+namespace exl3 {
+
+enum Scoring : int { SCORE_SOFTMAX = 0, SCORE_SIGMOID = 1, SCORE_SQRTSOFTPLUS = 2 };
+
+constexpr int ROUTE_MAX_TOPK = 64;
+constexpr int ROUTE_MAX_EXPERTS = 2048;
+
+template <typename T>
+__device__ __forceinline__ T wave_max(T v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const T o = __shfl_xor(v, d);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = min(v, __shfl_xor(v, d));
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ T neg_inf() { return (T)-__builtin_inff(); }
+
+// softplus is max(l, 0) + log(1 + e^-|l|), which neither overflows nor loses small l.
+template <typename T>
+__device__ __forceinline__ T score_of(int scoring, T l, T most, T total) {
+    if (scoring == SCORE_SOFTMAX) return exp(l - most) / total;
+    if (scoring == SCORE_SIGMOID) return (T)1 / ((T)1 + exp(-l));
+    return sqrt((l > 0 ? l : (T)0) + log1p(exp(l > 0 ? -l : l)));
+}
+
+// The `count` largest of the wave's keys in order: lane j keeps the j-th one's index
+// (-1: none left) and key.  Keys are NaN-free; -inf is never chosen.
+template <typename T, int N>
+__device__ __forceinline__ void select_top(T (&key)[N], int count, int lane, int& chosen, T& chosen_key) {
+    chosen = -1;
+    chosen_key = neg_inf<T>();
+    for (int j = 0; j < count; ++j) {
+        T best = key[0];
+        int at = 0;
+#pragma unroll
+        for (int i = 1; i < N; ++i)
+            if (key[i] > best) {
+                best = key[i];
+                at = i;
+            }
+        const T top = wave_max(best);
+        if (!(top > neg_inf<T>())) break;
+        const int idx = wave_min(best == top ? at * 64 + lane : 0x7fffffff);
+        if (lane == j) {
+            chosen = idx;
+            chosen_key = top;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (idx == i * 64 + lane) key[i] = neg_inf<T>();
+    }
+}
+
+struct RouteArgs {
+    const void* logits;         // [rows][E], OutKind
+    const float* bias;          // [E] or null
+    void* ids;                  // [rows][topk], int32 or int64
+    float* weights;             // [rows][topk]
+    int64_t rows;
+    int kind, E, topk, scoring, ids64, renormalize;
+    float scale;
+};
+
+template <int N>
+__global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs A) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= A.rows) return;
+    const int E = A.E;
+    float l[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int e = i * 64 + lane;
+        float v = neg_inf<float>();
+        if (e < E) {
+            const int64_t at = row * E + e;
+            v = A.kind == OUT_F32    ? static_cast<const float*>(A.logits)[at]
+                : A.kind == OUT_BF16 ? bf16_to_f32(static_cast<const uint16_t*>(A.logits)[at])
+                                     : f16_bits_to_f32(static_cast<const uint16_t*>(A.logits)[at]);
+        }
+        l[i] = v == v ? v : neg_inf<float>();
+    }
+    // the softmax's maximum and sum, where something needs them
+    float most = 0.f, total = 1.f;
+    const bool over_row = A.scoring == SCORE_SOFTMAX && (A.bias || !A.renormalize);
+    if (over_row) {
+        most = l[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) most = fmaxf(most, l[i]);
+        most = wave_max(most);
+        total = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) total += l[i] > neg_inf<float>() ? expf(l[i] - most) : 0.f;
+        total = wave_sum(total);
+    }
+    int chosen;
+    if (!A.bias) {
+        float key[N], unused;
+#pragma unroll
+        for (int i = 0; i < N; ++i) key[i] = l[i];
+        select_top<float, N>(key, A.topk, lane, chosen, unused);
+    } else {
+        float key[N], got;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = i * 64 + lane;
+            const float v = l[i] > neg_inf<float>() ? score_of<float>(A.scoring, l[i], most, total) + A.bias[e]
+                                                    : neg_inf<float>();
+            key[i] = v == v ? v : neg_inf<float>();
+        }
+        const int more = min(A.topk + 1, 64);
+        select_top<float, N>(key, more, lane, chosen, got);
+        const float below = __shfl_down(got, 1);
+        // fp32's scores are within 4e-6 of the exact ones (relative above one)
+        const bool near = lane + 1 < more && chosen >= 0 && !(got - below > 0x1p-17f * fmaxf(1.f, fabsf(got)));
+        if (__any(near) || more == A.topk) {
+            double dmost = most, dtotal = 1.0, dkey[N], unused;
+            if (A.scoring == SCORE_SOFTMAX) {
+                dtotal = 0.0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) dtotal += l[i] > neg_inf<float>() ? exp((double)l[i] - dmost) : 0.0;
+                dtotal = wave_sum(dtotal);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int e = i * 64 + lane;
+                const double v = l[i] > neg_inf<float>()
+                                     ? score_of<double>(A.scoring, (double)l[i], dmost, dtotal) + (double)A.bias[e]
+                                     : neg_inf<double>();
+                dkey[i] = v == v ? v : neg_inf<double>();
+            }
+            select_top<double, N>(dkey, A.topk, lane, chosen, unused);
+        }
+        if (lane >= A.topk) chosen = -1;
+    }
+    // the chosen logits, one a lane
+    float mine = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float v = __shfl(l[i], chosen & 63);
+        if ((chosen >> 6) == i) mine = v;
+    }
+    double s = 0.0;
+    if (A.scoring == SCORE_SOFTMAX) {
+        // over their own sum only ratios count: from the largest chosen logit they cannot all underflow
+        const float top = over_row && !A.renormalize ? most : wave_max(chosen >= 0 ? mine : neg_inf<float>());
+        if (chosen >= 0) s = exp((double)mine - (double)top) / (A.renormalize ? 1.0 : (double)total);
+    } else if (chosen >= 0) {
+        s = score_of<double>(A.scoring, (double)mine, 0.0, 1.0);
+    }
+    if (A.renormalize) {
+        const double sum = wave_sum(s);
+        s = sum != 0.0 ? s / sum : 0.0;
+    }
+    if (lane < A.topk) {
+        const int64_t at = row * A.topk + lane;
+        if (A.ids64) static_cast<int64_t*>(A.ids)[at] = chosen;
+        else static_cast<int32_t*>(A.ids)[at] = chosen;
+        A.weights[at] = (float)(s * (double)A.scale);
+    }
+}
+
+}  // namespace exl3

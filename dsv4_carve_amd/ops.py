@@ -13,6 +13,10 @@ Reference call surfaces mirrored here:
   * ``exl3_gemv``        -- vllm_exl3_c, recipe-lna/lna2/bindings.cpp:135-148
   * ``lna2_moe_decode`` and its helpers -- vllm_exl3_c,
     recipe-lna/lna2/lna_moe_ticket.cu:481-581, bindings.cpp:212-219
+
+Beside them, for the layers a checkpoint keeps in block-scaled 8-bit floats
+(``fp8_quantize``, ``fp8_gemm``, ``fp8_linear``, ``fp8_moe``) and for the router
+in front of either expert layer (``moe_route``).
 """
 
 from __future__ import annotations
@@ -749,3 +753,234 @@ def moe_prefill(x: torch.Tensor, out: torch.Tensor, tables, expert_ids: torch.Te
     torch.ops.exl3_amd.moe_prefill(x, out, *tabs, expert_ids, routing_weights, expert_map, expert_bits, b, mask,
                                    int(codebook), float(swiglu_limit), int(hidden), int(intermediate), scratch)
     return out
+
+
+# ------------------------------------------------------------------ block-scaled 8-bit floats
+
+FP8_BLOCK = 128
+E4M3 = torch.float8_e4m3fn
+
+_LIB.define("fp8_quantize(Tensor x, bool pow2, Tensor(a!) q, Tensor(b!) scale) -> ()")
+_LIB.define("fp8_gemm(Tensor a, Tensor a_scale, Tensor w, Tensor w_scale, Tensor(a!) c) -> ()")
+_LIB.define("fp8_linear(Tensor x, Tensor w, Tensor w_scale, Tensor(a!) c, Tensor(b!) scratch) -> ()")
+_LIB.define("fp8_moe(Tensor x, Tensor(a!) out, Tensor w13, Tensor w13_scale, Tensor w2, Tensor w2_scale, "
+            "Tensor expert_ids, Tensor routing_weights, Tensor? expert_map, float swiglu_limit, "
+            "Tensor(b!) scratch) -> ()")
+_LIB.define("moe_route(Tensor logits, int scoring, Tensor? bias, bool renormalize, float scale, Tensor(a!) ids, "
+            "Tensor(b!) weights) -> ()")
+
+
+def _on(device: torch.device):
+    """The guard a launch on `device` needs: HIP launches go to the current device."""
+    return torch.cuda.device(device)
+
+
+def _fp8_quantize_impl(x, pow2, q, scale):
+    k = x.shape[-1]
+    with _on(x.device):
+        _lib.check(_lib.load().exl3_fp8_quantize(_ptr(x), OUT_KIND[x.dtype], x.numel() // k, k, int(pow2), _ptr(q),
+                                                 _ptr(scale), _stream(x.device)))
+
+
+def _fp8_gemm_impl(a, a_scale, w, w_scale, c):
+    with _on(a.device):
+        _lib.check(_lib.load().exl3_fp8_gemm(_ptr(a), _ptr(a_scale), a.shape[0], a.shape[1], _ptr(w), _ptr(w_scale),
+                                             w.shape[0], _ptr(c), OUT_KIND[c.dtype], _stream(a.device)))
+
+
+def _fp8_linear_impl(x, w, w_scale, c, scratch):
+    with _on(x.device):
+        _lib.check(_lib.load().exl3_fp8_linear(_ptr(x), OUT_KIND[x.dtype], x.shape[0], x.shape[1], _ptr(w),
+                                               _ptr(w_scale), w.shape[0], _ptr(c), OUT_KIND[c.dtype], _ptr(scratch),
+                                               scratch.numel(), _stream(x.device)))
+
+
+def _fp8_moe_impl(x, out, w13, w13_scale, w2, w2_scale, ids, weights, emap, limit, scratch):
+    with _on(x.device):
+        _lib.check(_lib.load().exl3_fp8_moe(
+            _ptr(x), X_KIND[x.dtype], _ptr(out), OUT_KIND[out.dtype], x.shape[0], x.shape[1], w2.shape[2], w2.shape[0],
+            ids.shape[1], _ptr(w13), _ptr(w13_scale), _ptr(w2), _ptr(w2_scale), *_route_args(ids, weights, emap),
+            float(limit), _ptr(scratch), scratch.numel(), _stream(x.device)))
+
+
+def _moe_route_impl(logits, scoring, bias, renormalize, scale, ids, weights):
+    with _on(logits.device):
+        _lib.check(_lib.load().exl3_moe_route(
+            _ptr(logits), OUT_KIND[logits.dtype], logits.shape[0], logits.shape[1], ids.shape[1], int(scoring),
+            _ptr(bias), int(renormalize), float(scale), _ptr(ids), IDS_KIND[ids.dtype], _ptr(weights),
+            _stream(logits.device)))
+
+
+_LIB.impl("fp8_quantize", _fp8_quantize_impl, "CUDA")
+_LIB.impl("fp8_gemm", _fp8_gemm_impl, "CUDA")
+_LIB.impl("fp8_linear", _fp8_linear_impl, "CUDA")
+_LIB.impl("fp8_moe", _fp8_moe_impl, "CUDA")
+_LIB.impl("moe_route", _moe_route_impl, "CUDA")
+
+
+def _blocks(n: int) -> int:
+    return -(-n // FP8_BLOCK)
+
+
+def _check_fp8_matrix(w: torch.Tensor, w_scale: torch.Tensor, device: torch.device, what: str = "w") -> None:
+    """w e4m3 [..., n, k] with an fp32 scale for each 128x128 block."""
+    _check(w.dtype == E4M3 and w.is_contiguous() and w.device == device,
+           f"{what} must be contiguous float8_e4m3fn on the input device")
+    _check(w_scale.dtype == torch.float32 and w_scale.is_contiguous() and w_scale.device == device and
+           tuple(w_scale.shape) == (*w.shape[:-2], _blocks(w.shape[-2]), _blocks(w.shape[-1])),
+           f"{what}_scale must be contiguous fp32 on the input device, one value for each 128x128 block of {what}")
+
+
+def fp8_quantize(x: torch.Tensor, *, pow2: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """x [..., k] (fp16, bf16 or fp32, contiguous) as (q float8_e4m3fn [..., k], scale fp32 [..., ceil(k/128)]).
+
+    Each group of 128 values of a row has one scale: a / 448 with a the largest
+    magnitude (at least 448 * 2**-126), q = 448 x / a rounded to the nearest
+    e4m3 value, ties to even; with `pow2` the smallest power of two that is not
+    below a / 448, q = x / scale.  A NaN stays a NaN and does not count for a; an
+    infinity makes its group's scale infinite, its finite values 0 and itself NaN."""
+    _check(x.dim() >= 1 and x.dtype in OUT_KIND and x.is_contiguous(), "x must be contiguous fp16, bf16 or fp32 [..., k]")
+    k = x.shape[-1]
+    _check(1 <= k <= 1 << 24, "k must be in 1..2**24")
+    q = torch.empty(x.shape, dtype=E4M3, device=x.device)
+    scale = torch.empty((*x.shape[:-1], _blocks(k)), dtype=torch.float32, device=x.device)
+    if x.numel():
+        torch.ops.exl3_amd.fp8_quantize(x, bool(pow2), q, scale)
+    return q, scale
+
+
+def _check_fp8_k(k: int) -> None:
+    _check(16 <= k <= 1 << 24 and k % 16 == 0, "in features must be a multiple of 16 in 16..2**24")
+
+
+def fp8_gemm_into(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                  c: torch.Tensor) -> torch.Tensor:
+    """c [m, n] (fp16, bf16 or fp32) = (a with its scales) @ (w with its scales)^T, fp32 accumulation.
+
+    a, a_scale: quantized rows [m, k] as fp8_quantize gives them; w float8_e4m3fn
+    [n, k] with w_scale fp32 [ceil(n/128), ceil(k/128)]; k a multiple of 16.
+    Rows quantized once serve every matrix that reads them."""
+    _check(a.dim() == 2 and a.dtype == E4M3 and a.is_contiguous(), "a must be contiguous float8_e4m3fn [m, k]")
+    m, k = a.shape
+    _check_fp8_k(k)
+    _check(a_scale.dtype == torch.float32 and a_scale.is_contiguous() and a_scale.device == a.device and
+           tuple(a_scale.shape) == (m, _blocks(k)), "a_scale must be contiguous fp32 [m, ceil(k/128)] on a's device")
+    _check(w.dim() == 2 and w.shape[1] == k, "w must be [n, k] with a's feature dimension")
+    _check_fp8_matrix(w, w_scale, a.device)
+    _check(c.dtype in OUT_KIND and c.is_contiguous() and c.device == a.device and tuple(c.shape) == (m, w.shape[0]),
+           "c must be contiguous fp16, bf16 or fp32 [m, n] on a's device")
+    if c.numel():
+        torch.ops.exl3_amd.fp8_gemm(a, a_scale, w, w_scale, c)
+    return c
+
+
+def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+             out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """fp8_gemm_into a new tensor."""
+    _check(a.dim() == 2 and w.dim() == 2, "a must be [m, k] and w [n, k]")
+    c = torch.empty((a.shape[0], w.shape[0]), dtype=out_dtype, device=a.device)
+    return fp8_gemm_into(a, a_scale, w, w_scale, c)
+
+
+@functools.lru_cache(maxsize=4096)
+def _fp8_linear_scratch_bytes(m: int, k: int, n: int) -> int:
+    return int(_lib.check(_lib.load().exl3_fp8_linear_scratch_bytes(m, k, n)))
+
+
+def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+               out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """y [..., n] = x [..., k] through a block-scaled matrix: fp8_gemm(*fp8_quantize(x), w, w_scale), x fp16, bf16
+    or fp32; y in x's dtype unless given.  Its scratch is the call's own (stream-ordered, capturable)."""
+    _check(x.dim() >= 1 and x.dtype in OUT_KIND and x.is_contiguous(), "x must be contiguous fp16, bf16 or fp32 [..., k]")
+    k = x.shape[-1]
+    _check_fp8_k(k)
+    _check(w.dim() == 2 and w.shape[1] == k, "w must be [n, k] with x's feature dimension")
+    _check_fp8_matrix(w, w_scale, x.device)
+    dtype = out_dtype or x.dtype
+    _check(dtype in OUT_KIND, "out_dtype must be fp16, bf16 or fp32")
+    n = w.shape[0]
+    y = torch.empty((*x.shape[:-1], n), dtype=dtype, device=x.device)
+    if y.numel():
+        m = x.numel() // k
+        scratch = torch.empty(_fp8_linear_scratch_bytes(m, k, n), dtype=torch.uint8, device=x.device)
+        torch.ops.exl3_amd.fp8_linear(x.view(m, k), w, w_scale, y.view(m, n), scratch)
+    return y
+
+
+FP8_MOE_MAX_ROWS = 64
+FP8_MOE_MAX_TOPK = 16
+
+
+def fp8_moe(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor,
+            expert_ids: torch.Tensor, routing_weights: torch.Tensor, *, swiglu_limit: float | None = None,
+            expert_map: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """A routed-expert layer of block-scaled matrices for 1..FP8_MOE_MAX_ROWS rows: out [m, hidden] in x's dtype,
+    or the fp16, bf16 or fp32 tensor given.
+
+    x fp16 or bf16 [m, hidden]; w13 float8_e4m3fn [E, 2 * inter, hidden] (gate rows,
+    then up rows), w2 [E, hidden, inter], each with an fp32 scale for each 128x128
+    block; hidden and inter multiples of 128.  expert_ids, routing_weights and
+    expert_map as moe_decode takes them (moe_route makes the first two); an id that
+    no expert here has (-1 among them) contributes nothing.  With `swiglu_limit` L
+    the gate is capped at L and the up projection to [-L, L].  The activation
+    between the two products is rounded to x's dtype, sums are fp32."""
+    _check(x.is_cuda and x.dtype in X_KIND, "input must be HIP fp16 or bf16")
+    _check(x.dim() == 2 and x.is_contiguous(), "input must be contiguous [m, hidden]")
+    m, hidden = x.shape
+    _check(m <= FP8_MOE_MAX_ROWS, f"at most {FP8_MOE_MAX_ROWS} rows")
+    _check(w13.dim() == 3 and w2.dim() == 3 and w13.shape[0] == w2.shape[0] and w13.shape[2] == hidden and
+           w2.shape[1] == hidden and w13.shape[1] == 2 * w2.shape[2],
+           "w13 must be [E, 2 * inter, hidden] and w2 [E, hidden, inter]")
+    inter = w2.shape[2]
+    _check(hidden > 0 and inter > 0 and hidden % FP8_BLOCK == 0 and inter % FP8_BLOCK == 0,
+           "hidden and inter must be multiples of 128")
+    _check_fp8_matrix(w13, w13_scale, x.device, "w13")
+    _check_fp8_matrix(w2, w2_scale, x.device, "w2")
+    _check_route(expert_ids, routing_weights, m, x.device, expert_map, "m")
+    topk = expert_ids.shape[1]
+    _check(1 <= topk <= FP8_MOE_MAX_TOPK, f"topk must be in 1..{FP8_MOE_MAX_TOPK}")
+    _check(swiglu_limit is None or swiglu_limit > 0.0, "swiglu_limit must be positive")
+    if out is None:
+        out = torch.empty_like(x)
+    _check(out.device == x.device and out.shape == x.shape and out.is_contiguous() and out.dtype in OUT_KIND,
+           "output must be contiguous fp16, bf16 or fp32 [m, hidden] on the input device")
+    if m:
+        scratch = torch.empty(m * topk * inter * 2, dtype=torch.uint8, device=x.device)
+        torch.ops.exl3_amd.fp8_moe(x, out, w13, w13_scale, w2, w2_scale, expert_ids, routing_weights, expert_map,
+                                   float("inf") if swiglu_limit is None else float(swiglu_limit), scratch)
+    return out
+
+# ------------------------------------------------------------------ expert routing
+
+SCORING = {"softmax": 0, "sigmoid": 1, "sqrtsoftplus": 2}
+ROUTE_MAX_EXPERTS = 2048
+ROUTE_MAX_TOPK = 64
+
+
+def moe_route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", bias: torch.Tensor | None = None,
+              renormalize: bool = True, scale: float = 1.0,
+              ids_dtype: torch.dtype = torch.int32) -> tuple[torch.Tensor, torch.Tensor]:
+    """The expert_ids [m, topk] and routing_weights fp32 [m, topk] of router logits [m, E] (fp16, bf16 or fp32).
+
+    Experts are taken by logit, or by score + `bias` (fp32 [E]) where one is
+    given, largest first, ties to the lowest index; scores are the row's softmax,
+    the logits' sigmoid or sqrt(softplus).  Weights are the scores (without the
+    bias), divided by their sum with `renormalize`, times `scale`.  A logit (or
+    biased score) of -inf or NaN is never chosen: a slot that is left over has id
+    -1, which the expert layers skip, and weight 0."""
+    _check(logits.dim() == 2 and logits.dtype in OUT_KIND and logits.is_contiguous(),
+           "logits must be contiguous fp16, bf16 or fp32 [m, experts]")
+    m, n_experts = logits.shape
+    _check(1 <= n_experts <= ROUTE_MAX_EXPERTS, f"the number of experts must be in 1..{ROUTE_MAX_EXPERTS}")
+    _check(1 <= topk <= min(ROUTE_MAX_TOPK, n_experts), f"topk must be in 1..min({ROUTE_MAX_TOPK}, experts)")
+    _check(scoring in SCORING, f"scoring must be one of {', '.join(SCORING)}")
+    _check(ids_dtype in IDS_KIND, "ids_dtype must be int32 or int64")
+    _check(float("-inf") < scale < float("inf"), "scale must be finite")
+    if bias is not None:
+        _check(bias.dtype == torch.float32 and bias.is_contiguous() and bias.device == logits.device and
+               tuple(bias.shape) == (n_experts,), "bias must be contiguous fp32 [experts] on the logits' device")
+    ids = torch.empty((m, topk), dtype=ids_dtype, device=logits.device)
+    weights = torch.empty((m, topk), dtype=torch.float32, device=logits.device)
+    if m:
+        torch.ops.exl3_amd.moe_route(logits, SCORING[scoring], bias, bool(renormalize), float(scale), ids, weights)
+    return ids, weights

@@ -283,6 +283,82 @@ int exl3_moe_prefill_routed(const void* x, int x_kind, void* out, int out_kind, 
                             float swiglu_limit, void* scratch, int64_t scratch_bytes, void* stream);
 
 /*
+ * Block-scaled 8-bit floats: matrices that a checkpoint keeps as e4m3 with one
+ * fp32 scale for each 128x128 block, beside the trellis-packed ones.  No
+ * counterpart in the reference, whose plugin leaves such layers to the engine.
+ * Layouts (row-major, contiguous; 16-byte aligned where bytes are read or
+ * written in chunks):
+ *   matrix  w e4m3 [n][k], w_scale fp32 [ceil(n/128)][ceil(k/128)]
+ *   rows    q e4m3 [m][k], scale fp32 [m][ceil(k/128)]
+ *
+ * exl3_fp8_quantize: each group of 128 values of a row (the last may be
+ * shorter) under one scale.  a = max(max|x|, 448 * 2^-126), NaN left out;
+ * scale = a / 448, q = e4m3(448 x / a), ties to even; with pow2 the scale is
+ * the smallest power of two >= a / 448 and q = e4m3(x / scale).  A NaN stays
+ * one; under an infinity the scale is infinite, finite values become 0 and
+ * infinities NaN.  x_kind 0 = fp16, 1 = bf16, 2 = fp32; any rows >= 1,
+ * 1 <= k <= 2^24.
+ */
+int exl3_fp8_quantize(const void* x, int x_kind, int64_t rows, int64_t k, int pow2, uint8_t* q, float* scale,
+                      void* stream);
+
+/*
+ * c[i][j] = sum_b a_scale[i][b] * w_scale[j / 128][b] * sum_{t in block b} a[i][t] * w[j][t],
+ * fp32 accumulation, one rounding to c_kind.  a: quantized rows [m][k]; w: [n][k].
+ * k a multiple of 16 up to 2^24, any n up to 2^24, any m up to 1048560.
+ * a, w and c 16-byte aligned.  Needs no scratch.
+ */
+int exl3_fp8_gemm(const uint8_t* a, const float* a_scale, int64_t m, int64_t k, const uint8_t* w,
+                  const float* w_scale, int64_t n, void* c, int c_kind, void* stream);
+
+/*
+ * exl3_fp8_gemm on exl3_fp8_quantize(x) (scales a / 448).  scratch: >=
+ * exl3_fp8_linear_scratch_bytes(m, k, n) bytes, 16-byte aligned, no zeroing
+ * needed; one call at a time per scratch buffer.
+ */
+int64_t exl3_fp8_linear_scratch_bytes(int64_t m, int64_t k, int64_t n);
+int exl3_fp8_linear(const void* x, int x_kind, int64_t m, int64_t k, const uint8_t* w, const float* w_scale,
+                    int64_t n, void* c, int c_kind, void* scratch, int64_t scratch_bytes, void* stream);
+
+/*
+ * A routed-expert layer of block-scaled matrices for a few rows, two launches:
+ *   [g; u] = W13[e] x[r];  act = silu(min(g, L)) * clamp(u, -L, L);
+ *   out[r] = sum_j topk_weights[r][j] * W2[e] act,  e = topk_ids[r][j]
+ * x, and act between the launches, are 16-bit (x_kind 0 = fp16, 1 = bf16);
+ * sums are fp32.  w13 [E][2*I][H] (gate rows first) with w13_scale
+ * [E][2*I/128][H/128], w2 [E][H][I] with w2_scale [E][H/128][I/128]; H and I
+ * multiples of 128.  1 <= rows <= exl3_fp8_moe_max_rows() = 64, topk <= 16.
+ * swiglu_limit > 0, +infinity for none.  topk_ids, topk_weights, expert_map and
+ * the slots that contribute nothing as in exl3_moe_decode_routed; a row without
+ * a valid slot is 0; an id that a row names twice counts with the sum of its
+ * weights.  scratch: >= exl3_fp8_moe_scratch_bytes(rows, topk, intermediate)
+ * bytes, 16-byte aligned, no zeroing needed; one call at a time per buffer.
+ */
+int exl3_fp8_moe_max_rows(void);
+int64_t exl3_fp8_moe_scratch_bytes(int64_t rows, int64_t topk, int64_t intermediate);
+int exl3_fp8_moe(const void* x, int x_kind, void* out, int out_kind, int64_t rows, int64_t hidden,
+                 int64_t intermediate, int64_t n_experts, int64_t topk, const uint8_t* w13, const float* w13_scale,
+                 const uint8_t* w2, const float* w2_scale, const void* topk_ids, int ids_kind,
+                 const void* topk_weights, int weights_kind, const int64_t* expert_map, int64_t n_global,
+                 float swiglu_limit, void* scratch, int64_t scratch_bytes, void* stream);
+
+/*
+ * Top-k of a router's logits [rows][n_experts], the ids and weights that the
+ * routed-expert entry points read.  scoring s: 0 = softmax over the row,
+ * 1 = sigmoid, 2 = sqrt(softplus).  Order: by logit, or by s + bias where bias
+ * (fp32 [n_experts]) is given, as 64-bit arithmetic orders them; ties go to the
+ * lowest index.  A logit or a biased score of -inf or NaN is never chosen; a
+ * slot that nothing is left for gets id -1 and weight 0.  weights: s of the
+ * chosen (without the bias), over their sum with renormalize (0 where the sum
+ * is 0), times scale.  logits_kind 0 = fp16, 1 = bf16, 2 = fp32; ids_kind
+ * 0 = int32, 1 = int64; n_experts <= 2048, topk <= min(64, n_experts).  The
+ * reference takes both from its engine (recipe-lna/vllm_exl3_exl3.py.lna:2294-2307).
+ */
+int exl3_moe_route(const void* logits, int logits_kind, int64_t rows, int64_t n_experts, int64_t topk, int scoring,
+                   const float* bias, int renormalize, float scale, void* ids, int ids_kind, float* weights,
+                   void* stream);
+
+/*
  * Launch geometry for diagnostics (replaces lna2_moe_info,
  * recipe-lna/lna2/lna_moe_ticket.cu:494-505): writes up to n values
  * {cus, waves_per_launch, threads_per_wave, max_rows, max_pairs, step_k, cols,
