@@ -46,7 +46,7 @@ UNITS += [("exl3_moe_inst.hip", [f"-DEXL3_MOE_MASK=0x{m:03X}u", f"-DEXL3_MOE_CB=
 UNITS += [("exl3_prefill_capi.hip", [], "exl3_prefill_capi.o")]
 UNITS += [("exl3_prefill_inst.hip", [f"-DEXL3_BITS={b}"], f"exl3_pf_b{b}.o") for b in range(1, 9)]
 UNITS += [("exl3_prefill_inst.hip", ["-DEXL3_BITS=3", "-DEXL3_BITS2=2"], "exl3_pf_b32.o")]
-UNITS += [("exl3_fp8_capi.hip", [], "exl3_fp8_capi.o")]
+UNITS += [("exl3_fp8_gemm_capi.hip", [], "exl3_fp8_gemm_capi.o"), ("exl3_fp8_moe_capi.hip", [], "exl3_fp8_moe_capi.o")]
 
 
 def _stale(src: str, out: str) -> bool:

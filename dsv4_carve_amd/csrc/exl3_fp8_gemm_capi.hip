@@ -1,0 +1,194 @@
+// C-ABI entry points of the block-scaled 8-bit quantization and products
+// (declared in include/exl3_amd.h).
+#include <atomic>
+
+#include "exl3_fp8.hpp"
+
+using namespace exl3;
+
+static int check_blocks(int64_t m, int64_t k, int64_t n) {
+    if (m < 1 || n < 1 || k < 16 || k % 16) return fail("m and n must be positive and k a positive multiple of 16");
+    if (k > (1 << 24) || n > (1 << 24)) return fail("k and n must be at most 2^24");
+    if (m > (int64_t)65535 * 16) return fail("m must be at most 1048560");
+    return 0;
+}
+
+template <int K>
+static int launch_quantize(const void* x, int64_t rows, int k, int groups, bool pow2, uint8_t* q, float* scale,
+                           hipStream_t s) {
+    const bool chunks = k % 16 == 0 && aligned16(x) && aligned16(q);
+    const int64_t blocks = chunks ? (rows * groups * 8 + 255) / 256 : (rows * groups + 3) / 4;
+    if (blocks > 0x7fffffffLL) return fail("too many values");
+    const dim3 grid((unsigned)blocks), block(256);
+    if (chunks) {
+        if (pow2) hipLaunchKernelGGL((fp8_quantize_kernel<K, true>), grid, block, 0, s, x, rows, k, groups, q, scale);
+        else hipLaunchKernelGGL((fp8_quantize_kernel<K, false>), grid, block, 0, s, x, rows, k, groups, q, scale);
+    } else {
+        if (pow2) hipLaunchKernelGGL((fp8_quantize_any_kernel<K, true>), grid, block, 0, s, x, rows, k, groups, q, scale);
+        else hipLaunchKernelGGL((fp8_quantize_any_kernel<K, false>), grid, block, 0, s, x, rows, k, groups, q, scale);
+    }
+    return check_launch();
+}
+
+static int quantize(const void* x, int x_kind, int64_t rows, int64_t k, bool pow2, uint8_t* q, float* scale,
+                    hipStream_t s) {
+    const int groups = (int)((k + FP8_BLOCK - 1) / FP8_BLOCK);
+    if (x_kind == OUT_F16) return launch_quantize<OUT_F16>(x, rows, (int)k, groups, pow2, q, scale, s);
+    if (x_kind == OUT_BF16) return launch_quantize<OUT_BF16>(x, rows, (int)k, groups, pow2, q, scale, s);
+    return launch_quantize<OUT_F32>(x, rows, (int)k, groups, pow2, q, scale, s);
+}
+
+// ---------------------------------------------------------------- choice of a tile
+
+struct GemmArgs {
+    const uint8_t* a;
+    const float* a_scale;
+    int64_t m;
+    int k;
+    const uint8_t* w;
+    const float* w_scale;
+    int n;
+    void* c;
+    int c_kind;
+    hipStream_t s;
+};
+
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool WIDE>
+static int launch_tile(const GemmArgs& A) {
+    typedef Fp8Tile<BM, BN, WM, WN, KG, STAGES, WIDE> T;
+    const auto kernel = fp8_gemm_tile_kernel<BM, BN, WM, WN, KG, STAGES, WIDE>;
+    static std::atomic<uint64_t> ready{0};           // devices that know of the LDS size
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= MAX_DEVICES) return fail("no HIP device");
+    if (!(ready.load() >> dev & 1)) {
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                T::LDS) != hipSuccess)
+            return fail("the device does not give the kernel its LDS");
+        ready.fetch_or(1ull << dev);
+    }
+    const int64_t tm = (A.m + BM - 1) / BM, tn = (A.n + BN - 1) / BN;
+    if (tm * tn > 0x7fffffffLL) return fail("too many tiles");
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(T::THREADS), T::LDS, A.s, A.a, A.a_scale, (int)A.m, A.k,
+                       A.w, A.w_scale, A.n, A.c, A.c_kind, (int)tm, (int)tn);
+    return check_launch();
+}
+
+// A tile's share of the time: us for one block of k of a round of workgroups, with
+// one workgroup a CU and with as many as a CU's LDS holds.
+struct TileCost {
+    int bm, bn, resident;
+    float one, full;
+    int (*launch)(const GemmArgs&);
+};
+
+// Measured on 4096-wide k (us, this table's tile / the next one's): 16 rows x 4096
+// 5.0 / 6.5, x 12288 13.1 / 10.4; 32 x 4096 5.9 / 7.3, x 12288 14.7 / 11.8; 128 x
+// 4096 8.3 / 10.1, 256 x 4096 18.2 / 10.8; 512 x 4096 22.0 (64x64) / 15.5 / 24.5,
+// 512 x 12288 42.5 / 34.8; 1024 x 4096 28.8 / 27.3 / 52.7, 4096 x 4096 110 / 74 / 64.
+static const TileCost NARROW[] = {
+    {16, 32, 1, 0.12f, 0.12f, launch_tile<16, 32, 1, 1, 8, 2, false>},
+    {16, 64, 1, 0.20f, 0.20f, launch_tile<16, 64, 1, 2, 4, 3, false>},
+    {32, 32, 1, 0.13f, 0.13f, launch_tile<32, 32, 1, 1, 8, 2, false>},
+    {32, 64, 1, 0.19f, 0.19f, launch_tile<32, 64, 1, 2, 4, 2, false>},
+    {64, 64, 2, 0.21f, 0.42f, launch_tile<64, 64, 2, 2, 2, 2, false>},
+    {64, 128, 1, 0.37f, 0.37f, launch_tile<64, 128, 2, 2, 2, 3, false>},
+    {128, 128, 2, 0.64f, 1.05f, launch_tile<128, 128, 2, 2, 1, 2, false>},
+    {256, 256, 1, 1.90f, 1.90f, launch_tile<256, 256, 2, 4, 1, 2, false>},
+};
+// The 16-bit instruction: 32 x 4096 7.0 / 9.8; 128 x 4096 10.4 / 14.9, 256 x 4096
+// 20.1 / 15.4; 512 x 4096 28.7 / 23.7 / 40.0, 4096 x 4096 213 / 170 / 128.
+static const TileCost WIDE[] = {
+    {32, 32, 1, 0.16f, 0.16f, launch_tile<32, 32, 1, 1, 8, 2, true>},
+    {32, 64, 1, 0.24f, 0.24f, launch_tile<32, 64, 1, 2, 4, 2, true>},
+    {64, 64, 2, 0.36f, 0.80f, launch_tile<64, 64, 2, 2, 2, 2, true>},
+    {64, 128, 1, 0.63f, 0.63f, launch_tile<64, 128, 2, 2, 2, 2, true>},
+    {128, 128, 2, 1.13f, 1.95f, launch_tile<128, 128, 2, 2, 1, 2, true>},
+};
+
+// Rounds of workgroups, each with about 1 us that the blocks do not account for.
+static const TileCost& choose_tile(int64_t m, int64_t k, int64_t n, bool wide) {
+    const TileCost* table = wide ? WIDE : NARROW;
+    const int count = wide ? (int)(sizeof(WIDE) / sizeof(WIDE[0])) : (int)(sizeof(NARROW) / sizeof(NARROW[0]));
+    const int64_t cus = device_cus();
+    const double blocks = (double)((k + FP8_BLOCK - 1) / FP8_BLOCK);
+    const TileCost* best = table;
+    double least = 0;
+    for (const TileCost* t = table; t != table + count; ++t) {
+        const int64_t tiles = ((m + t->bm - 1) / t->bm) * ((n + t->bn - 1) / t->bn);
+        const bool one = tiles <= cus;
+        const int64_t wave = one ? cus : cus * t->resident, rounds = (tiles + wave - 1) / wave;
+        const double us = (double)rounds * (1.0 + blocks * (one ? t->one : t->full));
+        if (t == table || us < least) {
+            least = us;
+            best = t;
+        }
+    }
+    return *best;
+}
+
+// fp32 results come from the 16-bit instruction: the 8-bit one's error, 1e-5 of the
+// result and up to 4e-4 with outlying channels, is next to a 16-bit result's
+// rounding (2e-4 fp16, 2e-3 bf16) and to the operands' own (3e-2), and far above
+// fp32's.  Few fp32 rows have a kernel without LDS tiles (us, against the
+// smallest tile: 1 row x 4096 x 4096 4.9 / 6.1, 16 rows 7.0 / 6.2), and so has a k
+// whose rows are too long for a tile's 32-bit offsets.
+static int gemm(const GemmArgs& A) {
+    const bool wide = A.c_kind == OUT_F32;
+    if ((wide && A.m <= 8) || A.k > FP8_TILE_MAX_K) {
+        hipLaunchKernelGGL((fp8_gemm_rows_kernel<1, 8>), dim3((unsigned)((A.n + 15) / 16), (unsigned)((A.m + 15) / 16)),
+                           dim3(512), 0, A.s, A.a, A.a_scale, A.m, A.k, A.w, A.w_scale, A.n, A.c, A.c_kind);
+        return check_launch();
+    }
+    return choose_tile(A.m, A.k, A.n, wide).launch(A);
+}
+
+static int64_t linear_scratch_bytes(int64_t m, int64_t k) {
+    return align_up(m * k, 256) + m * ((k + FP8_BLOCK - 1) / FP8_BLOCK) * 4;
+}
+
+extern "C" {
+
+int exl3_fp8_quantize(const void* x, int x_kind, int64_t rows, int64_t k, int pow2, uint8_t* q, float* scale,
+                      void* stream) {
+    clear_error();
+    if (!x || !q || !scale) return fail("null pointer");
+    if (x_kind < OUT_F16 || x_kind > OUT_F32) return fail("x_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
+    if (rows < 1 || k < 1) return fail("rows and k must be positive");
+    if (k > (1 << 24)) return fail("k must be at most 2^24");
+    if (rows > (int64_t)1 << 36) return fail("too many values");
+    return quantize(x, x_kind, rows, k, pow2 != 0, q, scale, reinterpret_cast<hipStream_t>(stream));
+}
+
+int exl3_fp8_gemm(const uint8_t* a, const float* a_scale, int64_t m, int64_t k, const uint8_t* w, const float* w_scale,
+                  int64_t n, void* c, int c_kind, void* stream) {
+    clear_error();
+    if (!a || !a_scale || !w || !w_scale || !c) return fail("null pointer");
+    if (c_kind < OUT_F16 || c_kind > OUT_F32) return fail("c_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
+    if (check_blocks(m, k, n)) return -1;
+    if (!aligned16(a) || !aligned16(w) || !aligned16(c)) return fail("a, w and c must be 16-byte aligned");
+    return gemm(GemmArgs{a, a_scale, m, (int)k, w, w_scale, (int)n, c, c_kind, reinterpret_cast<hipStream_t>(stream)});
+}
+
+int64_t exl3_fp8_linear_scratch_bytes(int64_t m, int64_t k, int64_t n) {
+    clear_error();
+    if (check_blocks(m, k, n)) return -1;
+    return linear_scratch_bytes(m, k);
+}
+
+int exl3_fp8_linear(const void* x, int x_kind, int64_t m, int64_t k, const uint8_t* w, const float* w_scale, int64_t n,
+                    void* c, int c_kind, void* scratch, int64_t scratch_bytes, void* stream) {
+    clear_error();
+    if (!x || !w || !w_scale || !c || !scratch) return fail("null pointer");
+    if (x_kind < OUT_F16 || x_kind > OUT_F32) return fail("x_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
+    if (c_kind < OUT_F16 || c_kind > OUT_F32) return fail("c_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
+    if (check_blocks(m, k, n)) return -1;
+    if (!aligned16(w) || !aligned16(c) || !aligned16(scratch)) return fail("w, c and scratch must be 16-byte aligned");
+    if (scratch_bytes < linear_scratch_bytes(m, k)) return fail("scratch too small");
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    uint8_t* q = static_cast<uint8_t*>(scratch);
+    float* scale = reinterpret_cast<float*>(q + align_up(m * k, 256));
+    const int rc = quantize(x, x_kind, m, k, false, q, scale, s);
+    return rc ? rc : gemm(GemmArgs{q, scale, m, (int)k, w, w_scale, (int)n, c, c_kind, s});
+}
+
+}  // extern "C"

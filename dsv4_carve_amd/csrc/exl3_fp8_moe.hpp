@@ -235,7 +235,8 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] += part[s][4 * t + i][lane];
         const int row = 16 * t + r;
-        if (row < A.rows) store_out4(A.out, A.out_kind, row, hidden, n0 + 4 * g, v, true);
+        if (row < A.rows)
+            with_kind(A.out_kind, [&](auto kind) { store_out4<kind()>(A.out, row, hidden, n0 + 4 * g, v, true); });
     }
     static_assert(THREADS == FP8_MOE_MAX_SLOTS, "a thread for each slot");
 }

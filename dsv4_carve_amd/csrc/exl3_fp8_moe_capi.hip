@@ -1,4 +1,4 @@
-// C-ABI entry points of the block-scaled 8-bit path and the expert router
+// C-ABI entry points of the block-scaled expert layer and the expert router
 // (declared in include/exl3_amd.h).
 #include <cmath>
 
@@ -7,95 +7,7 @@
 
 using namespace exl3;
 
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-static int check_blocks(int64_t m, int64_t k, int64_t n) {
-    if (m < 1 || n < 1 || k < 16 || k % 16) return fail("m and n must be positive and k a positive multiple of 16");
-    if (k > (1 << 24) || n > (1 << 24)) return fail("k and n must be at most 2^24");
-    if (m > (int64_t)65535 * 16) return fail("m must be at most 1048560");
-    return 0;
-}
-
-template <int K>
-static int launch_quantize(const void* x, int64_t rows, int k, int groups, bool pow2, uint8_t* q, float* scale,
-                           hipStream_t s) {
-    const bool chunks = k % 16 == 0 && aligned16(x) && aligned16(q);
-    const int64_t blocks = chunks ? (rows * groups * 8 + 255) / 256 : (rows * groups + 3) / 4;
-    if (blocks > 0x7fffffffLL) return fail("too many values");
-    const dim3 grid((unsigned)blocks), block(256);
-    if (chunks) {
-        if (pow2) hipLaunchKernelGGL((fp8_quantize_kernel<K, true>), grid, block, 0, s, x, rows, k, groups, q, scale);
-        else hipLaunchKernelGGL((fp8_quantize_kernel<K, false>), grid, block, 0, s, x, rows, k, groups, q, scale);
-    } else {
-        if (pow2) hipLaunchKernelGGL((fp8_quantize_any_kernel<K, true>), grid, block, 0, s, x, rows, k, groups, q, scale);
-        else hipLaunchKernelGGL((fp8_quantize_any_kernel<K, false>), grid, block, 0, s, x, rows, k, groups, q, scale);
-    }
-    return check_launch();
-}
-
-static int quantize(const void* x, int x_kind, int64_t rows, int64_t k, bool pow2, uint8_t* q, float* scale,
-                    hipStream_t s) {
-    const int groups = (int)((k + FP8_BLOCK - 1) / FP8_BLOCK);
-    if (x_kind == OUT_F16) return launch_quantize<OUT_F16>(x, rows, (int)k, groups, pow2, q, scale, s);
-    if (x_kind == OUT_BF16) return launch_quantize<OUT_BF16>(x, rows, (int)k, groups, pow2, q, scale, s);
-    return launch_quantize<OUT_F32>(x, rows, (int)k, groups, pow2, q, scale, s);
-}
-
-static int gemm(const uint8_t* a, const float* a_scale, int64_t m, int64_t k, const uint8_t* w, const float* w_scale,
-                int64_t n, void* c, int c_kind, hipStream_t s) {
-    hipLaunchKernelGGL((fp8_gemm_rows_kernel<1, 16>), dim3((unsigned)((n + 15) / 16), (unsigned)((m + 15) / 16)),
-                       dim3(1024), 0, s, a, a_scale, m, (int)k, w, w_scale, (int)n, c, c_kind);
-    return check_launch();
-}
-
-static int64_t linear_scratch_bytes(int64_t m, int64_t k) {
-    return align_up(m * k, 256) + m * ((k + FP8_BLOCK - 1) / FP8_BLOCK) * 4;
-}
-
 extern "C" {
-
-int exl3_fp8_quantize(const void* x, int x_kind, int64_t rows, int64_t k, int pow2, uint8_t* q, float* scale,
-                      void* stream) {
-    clear_error();
-    if (!x || !q || !scale) return fail("null pointer");
-    if (x_kind < OUT_F16 || x_kind > OUT_F32) return fail("x_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
-    if (rows < 1 || k < 1) return fail("rows and k must be positive");
-    if (k > (1 << 24)) return fail("k must be at most 2^24");
-    if (rows > (int64_t)1 << 36) return fail("too many values");
-    return quantize(x, x_kind, rows, k, pow2 != 0, q, scale, reinterpret_cast<hipStream_t>(stream));
-}
-
-int exl3_fp8_gemm(const uint8_t* a, const float* a_scale, int64_t m, int64_t k, const uint8_t* w, const float* w_scale,
-                  int64_t n, void* c, int c_kind, void* stream) {
-    clear_error();
-    if (!a || !a_scale || !w || !w_scale || !c) return fail("null pointer");
-    if (c_kind < OUT_F16 || c_kind > OUT_F32) return fail("c_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
-    if (check_blocks(m, k, n)) return -1;
-    if (!aligned16(a) || !aligned16(w) || !aligned16(c)) return fail("a, w and c must be 16-byte aligned");
-    return gemm(a, a_scale, m, k, w, w_scale, n, c, c_kind, reinterpret_cast<hipStream_t>(stream));
-}
-
-int64_t exl3_fp8_linear_scratch_bytes(int64_t m, int64_t k, int64_t n) {
-    clear_error();
-    if (check_blocks(m, k, n)) return -1;
-    return linear_scratch_bytes(m, k);
-}
-
-int exl3_fp8_linear(const void* x, int x_kind, int64_t m, int64_t k, const uint8_t* w, const float* w_scale, int64_t n,
-                    void* c, int c_kind, void* scratch, int64_t scratch_bytes, void* stream) {
-    clear_error();
-    if (!x || !w || !w_scale || !c || !scratch) return fail("null pointer");
-    if (x_kind < OUT_F16 || x_kind > OUT_F32) return fail("x_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
-    if (c_kind < OUT_F16 || c_kind > OUT_F32) return fail("c_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
-    if (check_blocks(m, k, n)) return -1;
-    if (!aligned16(w) || !aligned16(c) || !aligned16(scratch)) return fail("w, c and scratch must be 16-byte aligned");
-    if (scratch_bytes < linear_scratch_bytes(m, k)) return fail("scratch too small");
-    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    uint8_t* q = static_cast<uint8_t*>(scratch);
-    float* scale = reinterpret_cast<float*>(q + align_up(m * k, 256));
-    const int rc = quantize(x, x_kind, m, k, false, q, scale, s);
-    return rc ? rc : gemm(q, scale, m, k, w, w_scale, n, c, c_kind, s);
-}
 
 int exl3_fp8_moe_max_rows(void) { return FP8_MOE_MAX_ROWS; }
 

@@ -72,13 +72,13 @@ def cut(a, w):
 
 
 def gemm(a, a_scale, w, w_scale, dtype):
-    """(result, how far an fp32-accumulated product rounded once to `dtype` may be from it).  A 16-bit result of many
-    rows may come from the 8-bit matrix instruction."""
+    """(result, how far an fp32-accumulated product rounded once to `dtype` may be from it).  A 16-bit result may come
+    from the 8-bit matrix instruction."""
     x, m = rows(a, a_scale), weight(w, w_scale)
     ref = x @ m.t()
     tol = (x.abs() @ m.abs().t()) * steps(a.shape[1]) * U + ref.abs() * half_step(dtype) + 2.0 ** -24 * (
         dtype is torch.float16)
-    return ref, tol + cut(x, m) if dtype is not torch.float32 and a.shape[0] > 32 else tol
+    return ref, tol + cut(x, m) if dtype is not torch.float32 else tol
 
 
 def moe(x, w13, s13, w2, s2, ids, wts, limit, emap, dtype):
