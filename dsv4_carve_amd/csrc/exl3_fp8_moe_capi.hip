@@ -42,22 +42,26 @@ int exl3_fp8_moe(const void* x, int x_kind, void* out, int out_kind, int64_t row
                  (int)hidden, (int)intermediate, (int)n_experts, (int)topk, swiglu_limit};
     if (make_route(topk_ids, ids_kind, topk_weights, weights_kind, expert_map, n_global, A.rt)) return -1;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const dim3 g1((unsigned)(intermediate / 16), (unsigned)(rows * topk)), g2((unsigned)(hidden / 16));
+    // fewer experts than slots: a workgroup row for each expert
+    const int slots = (int)(rows * topk), by_expert = n_experts < slots;
+    const dim3 g1((unsigned)(intermediate / 16), (unsigned)(by_expert ? n_experts : slots)), g2((unsigned)(hidden / 16));
+    // an expert has slots / n_experts rows on average: more than 16 are taken in passes where that is rare
+    const bool few = rows <= 16 || slots <= 4 * n_experts;
     const auto launch = [&](auto gu, auto dn) {
-        hipLaunchKernelGGL(gu, g1, dim3(FP8_GU_WAVES * 64), 0, s, A);
+        hipLaunchKernelGGL(gu, g1, dim3(FP8_GU_WAVES * 64), 0, s, A, by_expert);
         const int rc = check_launch();
         if (rc) return rc;
         hipLaunchKernelGGL(dn, g2, dim3(FP8_DOWN_WAVES * 64), 0, s, A);
         return check_launch();
     };
-    if (x_kind == OUT_BF16) {
-        if (rows <= 16) return launch(fp8_moe_gate_up_kernel<true, 1>, fp8_moe_down_kernel<true, 1>);
-        if (rows <= 32) return launch(fp8_moe_gate_up_kernel<true, 2>, fp8_moe_down_kernel<true, 2>);
-        return launch(fp8_moe_gate_up_kernel<true, 4>, fp8_moe_down_kernel<true, 4>);
-    }
-    if (rows <= 16) return launch(fp8_moe_gate_up_kernel<false, 1>, fp8_moe_down_kernel<false, 1>);
-    if (rows <= 32) return launch(fp8_moe_gate_up_kernel<false, 2>, fp8_moe_down_kernel<false, 2>);
-    return launch(fp8_moe_gate_up_kernel<false, 4>, fp8_moe_down_kernel<false, 4>);
+    const auto pick = [&](auto bf16) {
+        constexpr bool B = decltype(bf16)::value;
+        if (rows <= 16) return launch(fp8_moe_gate_up_kernel<B, 1>, fp8_moe_down_kernel<B, 1>);
+        if (rows <= 32)
+            return launch(few ? fp8_moe_gate_up_kernel<B, 1> : fp8_moe_gate_up_kernel<B, 2>, fp8_moe_down_kernel<B, 2>);
+        return launch(few ? fp8_moe_gate_up_kernel<B, 1> : fp8_moe_gate_up_kernel<B, 4>, fp8_moe_down_kernel<B, 4>);
+    };
+    return x_kind == OUT_BF16 ? pick(std::true_type{}) : pick(std::false_type{});
 }
 
 int exl3_moe_route(const void* logits, int logits_kind, int64_t rows, int64_t n_experts, int64_t topk, int scoring,
