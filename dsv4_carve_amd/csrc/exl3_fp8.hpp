@@ -347,6 +347,99 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_gemm_rows_kernel(const uint8_t
     }
 }
 
+// A few rows (16 at most) of kind K, quantized on the way: the workgroup
+// quantizes them whole into LDS, as fp8_quantize does, while its first weights are
+// on their way, and has 16 outputs of them.  LDS holds a row's blocks (zeros past
+// k) and 64 bytes more, so that four rows' chunks lie in different banks, then the
+// scales.
+constexpr int FP8_LINEAR_WAVES = 8;
+constexpr int FP8_LINEAR_DEEP = 4;                // blocks of a wave on their way
+
+__host__ __device__ inline int fp8_linear_rows_lds(int m, int k) {
+    const int blocks = (k + FP8_BLOCK - 1) / FP8_BLOCK, rows = m * (blocks * FP8_BLOCK + 64 + blocks * 4);
+    const int sums = FP8_LINEAR_WAVES * 64 * 16;
+    return rows > sums ? rows : sums;
+}
+
+template <int K>
+__global__ __launch_bounds__(FP8_LINEAR_WAVES * 64) void fp8_linear_rows_kernel(const void* __restrict__ x, int m, int k,
+                                                                                const uint8_t* __restrict__ w,
+                                                                                const float* __restrict__ w_scale,
+                                                                                int n, void* __restrict__ c, int c_kind) {
+    typedef Half16<true> H;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16, blocks = (k + FP8_BLOCK - 1) / FP8_BLOCK, stride = blocks * FP8_BLOCK + 64;
+    const uint8_t* wr = w + (int64_t)min(n0 + r, n - 1) * k;
+    const float* ws = w_scale + (int64_t)(n0 / FP8_BLOCK) * blocks;
+    float* const scales = reinterpret_cast<float*>(lds + m * stride);        // [m][blocks]
+    int8x32_t wq[FP8_LINEAR_DEEP];
+    float sw[FP8_LINEAR_DEEP];
+#pragma unroll
+    for (int d = 0; d < FP8_LINEAR_DEEP; ++d) {
+        const int kb = wave + d * FP8_LINEAR_WAVES;
+        if (kb < blocks) {
+            wq[d] = load_block(wr, kb, g, k);
+            sw[d] = ws[kb];
+        }
+    }
+    for (int at = tid; at < m * blocks * 8; at += FP8_LINEAR_WAVES * 64) {    // eight lanes a group: whole groups take part
+        const int row = at / (blocks * 8), ch = at - row * (blocks * 8);
+        float v[16] = {};
+        float most = 0.f;
+        if (ch * 16 < k) {
+            load16<K>(static_cast<const char*>(x) + ((int64_t)row * k + ch * 16) * (K == OUT_F32 ? 4 : 2), v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(v[i]));
+        }
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+        const QuantGroup q(most, false);
+        if ((ch & 7) == 0) scales[row * blocks + (ch >> 3)] = q.scale;
+        u32x4_t out;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            out[i] = ch * 16 < k ? pack_e4m3(q(v[4 * i]), q(v[4 * i + 1]), q(v[4 * i + 2]), q(v[4 * i + 3])) : 0u;
+        *reinterpret_cast<u32x4_t*>(lds + row * stride + ch * 16) = out;
+    }
+    __syncthreads();
+    float acc[4] = {};
+    const char* ar = lds + min(r, m - 1) * stride;
+    const float* as = scales + min(r, m - 1) * blocks;
+    for (int base = wave; base < blocks; base += FP8_LINEAR_DEEP * FP8_LINEAR_WAVES) {
+#pragma unroll
+        for (int d = 0; d < FP8_LINEAR_DEEP; ++d) {
+            const int kb = base + d * FP8_LINEAR_WAVES, ahead = kb + FP8_LINEAR_DEEP * FP8_LINEAR_WAVES;
+            if (kb >= blocks) break;
+            const char* p = ar + kb * FP8_BLOCK + g * 16;
+            const BlockW<H> a(join(*reinterpret_cast<const i32x4_t*>(p), *reinterpret_cast<const i32x4_t*>(p + 64)));
+            const float4_t pr = block_product<H>(BlockW<H>(wq[d]), a);
+            const float s = sw[d] * as[kb];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = fmaf(pr[i], s, acc[i]);
+            if (ahead < blocks) {
+                wq[d] = load_block(wr, ahead, g, k);
+                sw[d] = ws[ahead];
+            }
+        }
+    }
+    __syncthreads();                     // the rows are read: their place takes the waves' sums
+    float4_t* const part = reinterpret_cast<float4_t*>(lds);
+    part[wave * 64 + lane] = float4_t{acc[0], acc[1], acc[2], acc[3]};
+    __syncthreads();
+    if (wave) return;
+    float v[4] = {};
+#pragma unroll
+    for (int s = 0; s < FP8_LINEAR_WAVES; ++s) {
+        const float4_t p = part[s * 64 + lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += p[i];
+    }
+    const int nn = n0 + 4 * g;
+    if (r < m && nn < n) with_kind(c_kind, [&](auto kind) { store_out4<kind()>(c, r, n, nn, v, n % 4 == 0); });
+}
+
 // ---------------------------------------------------------------- product, many rows
 
 // An 8-bit instruction for a block, or four 16-bit ones on widened values.

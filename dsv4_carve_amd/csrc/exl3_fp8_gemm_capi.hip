@@ -142,8 +142,18 @@ static int gemm(const GemmArgs& A) {
     return choose_tile(A.m, A.k, A.n, wide).launch(A);
 }
 
-static int64_t linear_scratch_bytes(int64_t m, int64_t k) {
-    return align_up(m * k, 256) + m * ((k + FP8_BLOCK - 1) / FP8_BLOCK) * 4;
+// Whether a linear's rows are quantized by the workgroups that multiply them.
+// Every one of them does all the rows, so it pays while that is little for a CU
+// (us in a captured step, one launch / two: 4096 x 4096 1 row 5.5 / 7.4, 8 rows
+// 8.1 / 7.9; 4096 x 12288 1 row 11.5 / 13.9, 4 rows 14.1 / 14.1; 1536 x 4096 16
+// rows 5.4 / 6.4), and it saves the caller a launch and the scratch.
+static bool linear_in_one(int64_t m, int64_t k, int64_t n) {
+    const int64_t rounds = (n + 16 * device_cus() - 1) / (16 * device_cus());
+    return m <= 16 && m * k * rounds <= 32768 && fp8_linear_rows_lds((int)m, (int)k) <= 64 * 1024;
+}
+
+static int64_t linear_scratch_bytes(int64_t m, int64_t k, int64_t n) {
+    return linear_in_one(m, k, n) ? 0 : align_up(m * k, 256) + m * ((k + FP8_BLOCK - 1) / FP8_BLOCK) * 4;
 }
 
 extern "C" {
@@ -172,19 +182,29 @@ int exl3_fp8_gemm(const uint8_t* a, const float* a_scale, int64_t m, int64_t k, 
 int64_t exl3_fp8_linear_scratch_bytes(int64_t m, int64_t k, int64_t n) {
     clear_error();
     if (check_blocks(m, k, n)) return -1;
-    return linear_scratch_bytes(m, k);
+    return linear_scratch_bytes(m, k, n);
 }
 
 int exl3_fp8_linear(const void* x, int x_kind, int64_t m, int64_t k, const uint8_t* w, const float* w_scale, int64_t n,
                     void* c, int c_kind, void* scratch, int64_t scratch_bytes, void* stream) {
     clear_error();
-    if (!x || !w || !w_scale || !c || !scratch) return fail("null pointer");
+    if (!x || !w || !w_scale || !c) return fail("null pointer");
     if (x_kind < OUT_F16 || x_kind > OUT_F32) return fail("x_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
     if (c_kind < OUT_F16 || c_kind > OUT_F32) return fail("c_kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
     if (check_blocks(m, k, n)) return -1;
-    if (!aligned16(w) || !aligned16(c) || !aligned16(scratch)) return fail("w, c and scratch must be 16-byte aligned");
-    if (scratch_bytes < linear_scratch_bytes(m, k)) return fail("scratch too small");
+    if (!aligned16(x) || !aligned16(w) || !aligned16(c)) return fail("x, w and c must be 16-byte aligned");
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    if (linear_in_one(m, k, n)) {
+        const auto kernel = x_kind == OUT_F16    ? fp8_linear_rows_kernel<OUT_F16>
+                            : x_kind == OUT_BF16 ? fp8_linear_rows_kernel<OUT_BF16>
+                                                 : fp8_linear_rows_kernel<OUT_F32>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((n + 15) / 16)), dim3(FP8_LINEAR_WAVES * 64),
+                           fp8_linear_rows_lds((int)m, (int)k), s, x, (int)m, (int)k, w, w_scale, (int)n, c, c_kind);
+        return check_launch();
+    }
+    if (!scratch) return fail("null pointer");
+    if (!aligned16(scratch)) return fail("scratch must be 16-byte aligned");
+    if (scratch_bytes < linear_scratch_bytes(m, k, n)) return fail("scratch too small");
     uint8_t* q = static_cast<uint8_t*>(scratch);
     float* scale = reinterpret_cast<float*>(q + align_up(m * k, 256));
     const int rc = quantize(x, x_kind, m, k, false, q, scale, s);

@@ -17,8 +17,7 @@
 // bits: one exponential a lane, and far logits keep their ratios.
 #pragma once
 
-#include "exl3_decode.hpp"
-#include "exl3_capi_util.hpp"
+#include "exl3_fp8.hpp"
 
 namespace exl3 {
 
@@ -27,31 +26,60 @@ enum Scoring : int { SCORE_SOFTMAX = 0, SCORE_SIGMOID = 1, SCORE_SQRTSOFTPLUS = 
 constexpr int ROUTE_MAX_TOPK = 64;
 constexpr int ROUTE_MAX_EXPERTS = 2048;
 
-template <typename T>
-__device__ __forceinline__ T wave_max(T v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        const T o = __shfl_xor(v, d);
-        v = o > v ? o : v;
+// v of the lane that a DPP pattern names, `none` where it names no lane.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T lane_of(T v, T none) {
+    if constexpr (sizeof(T) == 8) {
+        const u32x2_t a = __builtin_bit_cast(u32x2_t, v), b = __builtin_bit_cast(u32x2_t, none);
+        return __builtin_bit_cast(T, u32x2_t{(uint32_t)__builtin_amdgcn_update_dpp((int)b[0], (int)a[0], CTRL, ROWS, 0xf, false),
+                                             (uint32_t)__builtin_amdgcn_update_dpp((int)b[1], (int)a[1], CTRL, ROWS, 0xf, false)});
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
+                                                                 CTRL, ROWS, 0xf, false));
     }
-    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ T read_lane(T v, int lane) {
+    if constexpr (sizeof(T) == 8) {
+        const u32x2_t a = __builtin_bit_cast(u32x2_t, v);
+        return __builtin_bit_cast(T, u32x2_t{(uint32_t)__builtin_amdgcn_readlane((int)a[0], lane),
+                                             (uint32_t)__builtin_amdgcn_readlane((int)a[1], lane)});
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    }
+}
+
+// op over the wave's lanes (each lane's value once), as a wave-uniform value: a
+// scan of each row of 16 lanes, then of the rows; lane 63 has it all.
+template <typename T, typename Op>
+__device__ __forceinline__ T wave_all(T v, T none, Op op) {
+    v = op(v, lane_of<0x111, 0xf>(v, none));        // row_shr:1, 2, 4, 8
+    v = op(v, lane_of<0x112, 0xf>(v, none));
+    v = op(v, lane_of<0x114, 0xf>(v, none));
+    v = op(v, lane_of<0x118, 0xf>(v, none));
+    v = op(v, lane_of<0x142, 0xa>(v, none));        // row_bcast:15, 31
+    v = op(v, lane_of<0x143, 0xc>(v, none));
+    return read_lane(v, 63);
 }
 
 template <typename T>
 __device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
-}
-
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = min(v, __shfl_xor(v, d));
-    return v;
+    return wave_all(v, (T)0, [](T a, T b) { return a + b; });
 }
 
 template <typename T>
 __device__ __forceinline__ T neg_inf() { return (T)-__builtin_inff(); }
+
+// NaN-free values only.
+template <typename T>
+__device__ __forceinline__ T wave_max(T v) {
+    return wave_all(v, neg_inf<T>(), [](T a, T b) { return a > b ? a : b; });
+}
+
+__device__ __forceinline__ int wave_min(int v) {
+    return wave_all(v, 0x7fffffff, [](int a, int b) { return min(a, b); });
+}
 
 // softplus is max(l, 0) + log(1 + e^-|l|), which neither overflows nor loses small l.
 template <typename T>
@@ -78,7 +106,10 @@ __device__ __forceinline__ void select_top(T (&key)[N], int count, int lane, int
             }
         const T top = wave_max(best);
         if (!(top > neg_inf<T>())) break;
-        const int idx = wave_min(best == top ? at * 64 + lane : 0x7fffffff);
+        const uint64_t have = __ballot(best == top);
+        const int owner = __builtin_ctzll(have);
+        const int idx = have & (have - 1) ? wave_min(best == top ? at * 64 + lane : 0x7fffffff)
+                                          : __builtin_amdgcn_readlane(at, owner) * 64 + owner;
         if (lane == j) {
             chosen = idx;
             chosen_key = top;

@@ -762,7 +762,7 @@ E4M3 = torch.float8_e4m3fn
 
 _LIB.define("fp8_quantize(Tensor x, bool pow2, Tensor(a!) q, Tensor(b!) scale) -> ()")
 _LIB.define("fp8_gemm(Tensor a, Tensor a_scale, Tensor w, Tensor w_scale, Tensor(a!) c) -> ()")
-_LIB.define("fp8_linear(Tensor x, Tensor w, Tensor w_scale, Tensor(a!) c, Tensor(b!) scratch) -> ()")
+_LIB.define("fp8_linear(Tensor x, Tensor w, Tensor w_scale, Tensor(a!) c, Tensor(b!)? scratch) -> ()")
 _LIB.define("fp8_moe(Tensor x, Tensor(a!) out, Tensor w13, Tensor w13_scale, Tensor w2, Tensor w2_scale, "
             "Tensor expert_ids, Tensor routing_weights, Tensor? expert_map, float swiglu_limit, "
             "Tensor(b!) scratch) -> ()")
@@ -770,45 +770,47 @@ _LIB.define("moe_route(Tensor logits, int scoring, Tensor? bias, bool renormaliz
             "Tensor(b!) weights) -> ()")
 
 
-def _on(device: torch.device):
-    """The guard a launch on `device` needs: HIP launches go to the current device."""
-    return torch.cuda.device(device)
+def _launch(device: torch.device, entry: str, *args) -> None:
+    """A library call on `device`'s current stream.  HIP launches go to the current device: another one is made
+    current for the call."""
+    index = device.index
+    fn = getattr(_lib.load(), entry)
+    if index == torch.cuda.current_device():
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def _fp8_quantize_impl(x, pow2, q, scale):
     k = x.shape[-1]
-    with _on(x.device):
-        _lib.check(_lib.load().exl3_fp8_quantize(_ptr(x), OUT_KIND[x.dtype], x.numel() // k, k, int(pow2), _ptr(q),
-                                                 _ptr(scale), _stream(x.device)))
+    _launch(x.device, "exl3_fp8_quantize", x.data_ptr(), OUT_KIND[x.dtype], x.numel() // k, k, int(pow2), q.data_ptr(),
+            scale.data_ptr())
 
 
 def _fp8_gemm_impl(a, a_scale, w, w_scale, c):
-    with _on(a.device):
-        _lib.check(_lib.load().exl3_fp8_gemm(_ptr(a), _ptr(a_scale), a.shape[0], a.shape[1], _ptr(w), _ptr(w_scale),
-                                             w.shape[0], _ptr(c), OUT_KIND[c.dtype], _stream(a.device)))
+    m, k = a.shape
+    _launch(a.device, "exl3_fp8_gemm", a.data_ptr(), a_scale.data_ptr(), m, k, w.data_ptr(), w_scale.data_ptr(),
+            w.shape[0], c.data_ptr(), OUT_KIND[c.dtype])
 
 
 def _fp8_linear_impl(x, w, w_scale, c, scratch):
-    with _on(x.device):
-        _lib.check(_lib.load().exl3_fp8_linear(_ptr(x), OUT_KIND[x.dtype], x.shape[0], x.shape[1], _ptr(w),
-                                               _ptr(w_scale), w.shape[0], _ptr(c), OUT_KIND[c.dtype], _ptr(scratch),
-                                               scratch.numel(), _stream(x.device)))
+    n, k = w.shape
+    _launch(x.device, "exl3_fp8_linear", x.data_ptr(), OUT_KIND[x.dtype], x.numel() // k, k, w.data_ptr(),
+            w_scale.data_ptr(), n, c.data_ptr(), OUT_KIND[c.dtype], _ptr(scratch),
+            0 if scratch is None else scratch.numel())
 
 
 def _fp8_moe_impl(x, out, w13, w13_scale, w2, w2_scale, ids, weights, emap, limit, scratch):
-    with _on(x.device):
-        _lib.check(_lib.load().exl3_fp8_moe(
-            _ptr(x), X_KIND[x.dtype], _ptr(out), OUT_KIND[out.dtype], x.shape[0], x.shape[1], w2.shape[2], w2.shape[0],
-            ids.shape[1], _ptr(w13), _ptr(w13_scale), _ptr(w2), _ptr(w2_scale), *_route_args(ids, weights, emap),
-            float(limit), _ptr(scratch), scratch.numel(), _stream(x.device)))
+    _launch(x.device, "exl3_fp8_moe", x.data_ptr(), X_KIND[x.dtype], out.data_ptr(), OUT_KIND[out.dtype], x.shape[0],
+            x.shape[1], w2.shape[2], w2.shape[0], ids.shape[1], w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(),
+            w2_scale.data_ptr(), *_route_args(ids, weights, emap), float(limit), scratch.data_ptr(), scratch.numel())
 
 
 def _moe_route_impl(logits, scoring, bias, renormalize, scale, ids, weights):
-    with _on(logits.device):
-        _lib.check(_lib.load().exl3_moe_route(
-            _ptr(logits), OUT_KIND[logits.dtype], logits.shape[0], logits.shape[1], ids.shape[1], int(scoring),
-            _ptr(bias), int(renormalize), float(scale), _ptr(ids), IDS_KIND[ids.dtype], _ptr(weights),
-            _stream(logits.device)))
+    _launch(logits.device, "exl3_moe_route", logits.data_ptr(), OUT_KIND[logits.dtype], logits.shape[0],
+            logits.shape[1], ids.shape[1], int(scoring), _ptr(bias), int(renormalize), float(scale), ids.data_ptr(),
+            IDS_KIND[ids.dtype], weights.data_ptr())
 
 
 _LIB.impl("fp8_quantize", _fp8_quantize_impl, "CUDA")
@@ -886,14 +888,15 @@ def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: t
 
 
 @functools.lru_cache(maxsize=4096)
-def _fp8_linear_scratch_bytes(m: int, k: int, n: int) -> int:
+def _fp8_linear_scratch_bytes(device_index: int, m: int, k: int, n: int) -> int:
     return int(_lib.check(_lib.load().exl3_fp8_linear_scratch_bytes(m, k, n)))
 
 
 def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """y [..., n] = x [..., k] through a block-scaled matrix: fp8_gemm(*fp8_quantize(x), w, w_scale), x fp16, bf16
-    or fp32; y in x's dtype unless given.  Its scratch is the call's own (stream-ordered, capturable)."""
+    or fp32; y in x's dtype unless given.  A few rows take one launch.  Its scratch is the call's own
+    (stream-ordered, capturable)."""
     _check(x.dim() >= 1 and x.dtype in OUT_KIND and x.is_contiguous(), "x must be contiguous fp16, bf16 or fp32 [..., k]")
     k = x.shape[-1]
     _check_fp8_k(k)
@@ -904,9 +907,9 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
     n = w.shape[0]
     y = torch.empty((*x.shape[:-1], n), dtype=dtype, device=x.device)
     if y.numel():
-        m = x.numel() // k
-        scratch = torch.empty(_fp8_linear_scratch_bytes(m, k, n), dtype=torch.uint8, device=x.device)
-        torch.ops.exl3_amd.fp8_linear(x.view(m, k), w, w_scale, y.view(m, n), scratch)
+        nbytes = _fp8_linear_scratch_bytes(x.device.index, x.numel() // k, k, n) if x.is_cuda else 0
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        torch.ops.exl3_amd.fp8_linear(x, w, w_scale, y, scratch)
     return y
 
 

@@ -100,10 +100,13 @@ def test_gemm_argument_errors_without_device(change, msg):
 
 def test_linear_scratch_is_checked():
     L = _lib.load()
-    need = L.exl3_fp8_linear_scratch_bytes(5, 400, 64)
-    assert need >= 5 * 400 + 5 * 4 * 4
-    refused(L.exl3_fp8_linear(P, 1, 5, 400, P, P, 64, P, 1, P, need - 1, None), "scratch too small")
-    refused(L.exl3_fp8_linear(P, 1, 5, 400, P, P, 64, P, 1, P + 4, need, None), "aligned")
+    need = L.exl3_fp8_linear_scratch_bytes(50, 400, 64)
+    assert need >= 50 * 400 + 50 * 4 * 4
+    refused(L.exl3_fp8_linear(P, 1, 50, 400, P, P, 64, P, 1, P, need - 1, None), "scratch too small")
+    refused(L.exl3_fp8_linear(P, 1, 50, 400, P, P, 64, P, 1, P + 4, need, None), "aligned")
+    refused(L.exl3_fp8_linear(P, 1, 50, 400, P, P, 64, P, 1, None, need, None), "null")
+    refused(L.exl3_fp8_linear(P + 2, 1, 5, 400, P, P, 64, P, 1, P, need, None), "aligned")
+    assert L.exl3_fp8_linear_scratch_bytes(1, 4096, 4096) == 0
     refused(L.exl3_fp8_linear_scratch_bytes(5, 40, 64), "multiple of 16")
 
 
