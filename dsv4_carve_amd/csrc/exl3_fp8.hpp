@@ -103,8 +103,7 @@ struct BlockX {
 };
 
 template <typename H, typename X>
-__device__ __forceinline__ float4_t block_product(const BlockW<H>& w, const X& x) {
-    float4_t p = {0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ float4_t block_product(const BlockW<H>& w, const X& x, float4_t p = {0.f, 0.f, 0.f, 0.f}) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) p = H::mfma(w.v[i], x.v[i], p);
     return p;

@@ -4,13 +4,15 @@
 //             g = W13[e][:I] x[row], u = W13[e][I:] x[row]
 //   down      out[row] = sum_e wt(row, e) * (W2[e] act[s])
 //
-// Activations stay 16-bit and the e4m3 weights are widened to their type
-// (exactly) before the 16x16x32 matrix instruction: at a few rows the layer reads
-// weights, and rounding activations to 8 bits would cost accuracy for nothing.
-// Sums are fp32: a block of 128 is four instructions into a cleared
-// accumulator, scaled into the running sum by one multiply-add a value.  The
-// activation is rounded to 16 bits between the launches, the only rounding
-// besides the output's.
+// Activations are not quantized: at a few rows the layer reads weights, and
+// rounding activations to 8 bits would cost accuracy for nothing.  The e4m3
+// weights are widened (exactly) to the type of x for the first product, and to
+// bf16 for the second, whose activation is the sum of two bf16 values (its
+// rounding and the rounding of what that leaves, 2^-17 of it, and no overflow):
+// one instruction more a block, which the weights' traffic hides, and the
+// output's rounding is the only one that counts.  Sums are fp32: a block of 128
+// is four 16x16x32 instructions (eight) into a cleared accumulator, scaled into
+// the running sum by one multiply-add a value.
 //
 // Routing is read in each workgroup, lane r of a wave holding row r (64 rows at
 // most).  A row that names an expert more than once counts as its first slot,
@@ -36,7 +38,7 @@ struct Fp8MoeArgs {
     const float* s13;           // [E][2 I / 128][hidden / 128]
     const uint8_t* w2;          // [E][hidden][I]
     const float* s2;            // [E][hidden / 128][I / 128]
-    uint16_t* act;              // [rows * topk][I], 16-bit
+    uint16_t* act;              // [rows * topk][I / 16][2][16]: 16 activations as bf16, then what that leaves of them
     void* out;                  // [rows][hidden]
     Route rt;
     int out_kind, rows, hidden, inter, E, topk;
@@ -50,14 +52,16 @@ constexpr int FP8_GU_WAVES = 4;
 // first slot does the work, or with by_expert an expert; the others' workgroups
 // end at once, and there are fewer of those with fewer experts than slots.  The
 // expert's rows are the columns of the matrix instruction, 16 MT at a time: with
-// few rows an expert, the columns left over cost neither traffic nor time.  Four
-// waves a workgroup, each with two blocks of both matrices on their way: 5.6 TB/s
-// of weights (the layer above, 303 us), 4.2 with eight waves of twice the
-// registers a workgroup.
+// few rows an expert, the columns left over cost neither traffic nor time.  MT 0
+// is for rows that are few an expert, 4 at a time: their inputs come as down's do,
+// one load for four rows.  Four waves a workgroup, each with two blocks of both
+// matrices on their way.
 template <bool BF16, int MT>
 __global__ __launch_bounds__(FP8_GU_WAVES * 64) void fp8_moe_gate_up_kernel(const Fp8MoeArgs A, int by_expert) {
     typedef Half16<BF16> H;
-    __shared__ float part[FP8_GU_WAVES][2 * MT * 4][64];
+    constexpr int TILES = MT ? MT : 1, COLS = MT ? 16 * MT : 4;
+    __shared__ float part[FP8_GU_WAVES][2 * TILES * 4][64];
+    __shared__ i32x4_t columns[MT ? 1 : FP8_GU_WAVES][64];      // a wave's inputs of one block, 256 bytes a row
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, g = lane >> 4;
     const int S = A.rows * A.topk;
@@ -99,21 +103,26 @@ __global__ __launch_bounds__(FP8_GU_WAVES * 64) void fp8_moe_gate_up_kernel(cons
     const int place = __popcll(mask & ((1ull << lane) - 1));
     const int col_slot = __builtin_amdgcn_ds_permute((mine >= 0 ? place : cnt + lane - place) * 4, mine);
 
-    for (int c0 = 0; c0 < cnt; c0 += 16 * MT) {
-        const uint16_t* xr[MT];
+    for (int c0 = 0; c0 < cnt; c0 += COLS) {
+        // a column past the last row has that row's inputs, and is not stored
+        const auto input_row = [&](int col) {
+            return static_cast<const uint16_t*>(A.x) + (int64_t)(__shfl(col_slot, min(col, cnt - 1)) / A.topk) * hidden;
+        };
+        const uint16_t* xr[TILES];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const int col = c0 + 16 * t + r, cs = __shfl(col_slot, col & 63);
-            xr[t] = col < cnt ? static_cast<const uint16_t*>(A.x) + (int64_t)(cs / A.topk) * hidden : nullptr;
-        }
-        float ag[MT][4] = {}, au[MT][4] = {};
+        for (int t = 0; t < TILES; ++t) xr[t] = MT ? input_row(c0 + 16 * t + r) : input_row(c0 + g) + 8 * r;
+        float ag[TILES][4] = {}, au[TILES][4] = {};
         const auto compute = [&](const Unit& u, int kb) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
+            for (int t = 0; t < TILES; ++t) {
                 if (t > 0 && c0 + 16 * t >= cnt) break;
                 BlockX<H> bx;
-                if (xr[t]) bx.load(xr[t] + kb * FP8_BLOCK, g);
-                else bx.clear();
+                if constexpr (MT) {
+                    bx.load(xr[t] + kb * FP8_BLOCK, g);
+                } else {
+                    columns[wave][lane] = *reinterpret_cast<const i32x4_t*>(xr[t] + kb * FP8_BLOCK);
+                    bx.load(reinterpret_cast<const uint16_t*>(columns[wave] + 16 * min(r, 3)), g);
+                }
                 const float4_t pg = block_product<H>(BlockW<H>(u.g), bx), pu = block_product<H>(BlockW<H>(u.u), bx);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -124,21 +133,21 @@ __global__ __launch_bounds__(FP8_GU_WAVES * 64) void fp8_moe_gate_up_kernel(cons
         };
         if (c0 && wave < kb_n) fetch(u0, wave);
         for (int kb = wave; kb < kb_n; kb += 2 * FP8_GU_WAVES) {
-            if (kb + FP8_GU_WAVES < kb_n) fetch(u1, kb + FP8_GU_WAVES);
+            fetch(u1, min(kb + FP8_GU_WAVES, kb_n - 1));
             compute(u0, kb);
-            if (kb + 2 * FP8_GU_WAVES < kb_n) fetch(u0, kb + 2 * FP8_GU_WAVES);
+            fetch(u0, min(kb + 2 * FP8_GU_WAVES, kb_n - 1));
             if (kb + FP8_GU_WAVES < kb_n) compute(u1, kb + FP8_GU_WAVES);
         }
         if (c0) __syncthreads();
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < TILES; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 part[wave][8 * t + i][lane] = ag[t][i];
                 part[wave][8 * t + 4 + i][lane] = au[t][i];
             }
         __syncthreads();
-        for (int t = wave; t < MT; t += FP8_GU_WAVES) {
+        for (int t = wave; t < TILES; t += FP8_GU_WAVES) {
             float gs[4] = {}, us[4] = {};
 #pragma unroll
             for (int s = 0; s < FP8_GU_WAVES; ++s)
@@ -148,17 +157,21 @@ __global__ __launch_bounds__(FP8_GU_WAVES * 64) void fp8_moe_gate_up_kernel(cons
                     us[i] += part[s][8 * t + 4 + i][lane];
                 }
             const int col = c0 + 16 * t + r, cs = __shfl(col_slot, col & 63);
-            if (col >= cnt) continue;
-            uint16_t h[4];
+            if (col >= cnt || (!MT && r >= COLS)) continue;
+            float act[4], rest[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 // comparisons, not fminf: a NaN stays one
                 const float gv = gs[i] > A.limit ? A.limit : gs[i];
                 const float uv = us[i] > A.limit ? A.limit : us[i] < -A.limit ? -A.limit : us[i];
-                h[i] = H::bits(gv / (1.0f + expf(-gv)) * uv);
+                act[i] = gv / (1.0f + expf(-gv)) * uv;
+                const float top = (float)(__bf16)act[i];
+                rest[i] = fabsf(top) < __builtin_inff() ? act[i] - top : 0.f;
             }
-            *reinterpret_cast<u32x2_t*>(A.act + (int64_t)cs * I + n0 + 4 * g) =
-                u32x2_t{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
+            uint16_t* p = A.act + 2 * ((int64_t)cs * I + n0) + 4 * g;
+            *reinterpret_cast<u32x2_t*>(p) = u32x2_t{pack_bf16(act[0], act[1]), pack_bf16(act[2], act[3])};
+            *reinterpret_cast<u32x2_t*>(p + 16) =
+                u32x2_t{pack_bf16(rest[0], rest[1]), pack_bf16(rest[2], rest[3])};
         }
     }
 }
@@ -169,58 +182,66 @@ constexpr int FP8_DOWN_WAVES = 16;
 // experts, in the order of their first slots; a column of the matrix
 // instruction is a row of the batch, and a row's routing weight joins the block's
 // scale, so that the sum over experts needs no second pass and no atomics.  A
-// wave takes every 16th block of (expert, k), the next one's bytes on their way
-// while it computes; of its row groups of 16 only those that name the expert are
-// read and multiplied.  5.1 TB/s of weights with 16 rows (101 of 256 experts of
-// 4096 x 2048, 165 us); three or four blocks ahead, or the inputs ahead too,
-// change nothing.
-template <bool BF16, int MT>
+// wave takes every 16th (8th) block of an expert and 16 rows that some of name it,
+// the next ones' bytes on their way while it computes.
+template <int MT>
 __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const Fp8MoeArgs A) {
-    typedef Half16<BF16> H;
-    static_assert(FP8_DOWN_WAVES * 64 == FP8_MOE_MAX_SLOTS, "a thread for each slot");
+    typedef Half16<true> H;
+    constexpr int WAVES = FP8_DOWN_WAVES;
+    static_assert(WAVES * 64 == FP8_MOE_MAX_SLOTS, "a thread for each slot");
+    constexpr int COLS = 4;        // rows whose inputs two loads bring
     struct Entry {
         int slot;
         float weight;
     };
     struct Expert {
         uint64_t rows;             // bit r: row r names it
-        int id, first;             // its first entry
+        int id;
+    };
+    struct Group {                 // an expert and up to COLS of 16 rows that name it
+        int id;
+        uint16_t rows;             // which of the 16
+        uint16_t first;            // the first one's entry, below 1024, and the 16 rows' number in the two bits above
     };
     __shared__ __attribute__((aligned(16))) int ids[FP8_MOE_MAX_SLOTS];      // local expert of a slot, or -1
     __shared__ float wts[FP8_MOE_MAX_SLOTS];
     __shared__ Expert experts[FP8_MOE_MAX_SLOTS];                            // the active ones
     __shared__ Entry entries[FP8_MOE_MAX_SLOTS];                             // their rows, in order
+    __shared__ Group groups[FP8_MOE_MAX_SLOTS];
     __shared__ uint16_t place[FP8_MOE_MAX_SLOTS];                            // of a first slot's expert among them
-    __shared__ int wave_n[FP8_DOWN_WAVES];
-    __shared__ float part[FP8_DOWN_WAVES][MT * 4][64];
+    __shared__ uint16_t first_of[FP8_MOE_MAX_SLOTS];                         // an expert's first entry
+    __shared__ int wave_n[2][WAVES];
+    __shared__ __attribute__((aligned(16))) float part[WAVES][MT * 4][64];
+    __shared__ i32x4_t columns[WAVES][COLS * 32];       // a wave's inputs of one block, 512 bytes a row
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = lane & 15, g = lane >> 4;
-    const int S = A.rows * A.topk, row = tid / A.topk;
+    const int S = A.rows * A.topk;
+    const uint64_t below = (1ull << lane) - 1;
+    const int row = tid / A.topk;
     const int e = tid < S ? A.rt.local(tid, A.E) : -1;
     ids[tid] = e;
     if (e >= 0) wts[tid] = A.rt.weight(tid);
     __syncthreads();
     // the first slot of this one's expert, and whether it is its row's first of it
     int first = tid;
-    bool row_first = false;
+    bool row_first = e >= 0;
     if (wave * 64 < S) {
         for (int s = (min(S, wave * 64 + 64) - 1) & ~3; s >= 0; s -= 4) {
             const i32x4_t v = *reinterpret_cast<const i32x4_t*>(&ids[s]);
 #pragma unroll
             for (int i = 3; i >= 0; --i) first = v[i] == e && s + i < first ? s + i : first;
         }
-        row_first = e >= 0;
         for (int s = row * A.topk; s < tid; ++s) row_first = row_first && ids[s] != e;
     }
     const bool owner = e >= 0 && first == tid;
-    const uint64_t below = (1ull << lane) - 1, own = __ballot(owner);
-    if (lane == 0) wave_n[wave] = __popcll(own);
+    const uint64_t own = __ballot(owner);
+    if (lane == 0) wave_n[0][wave] = __popcll(own);
     __syncthreads();
     int before = 0, active = 0;
 #pragma unroll
-    for (int i = 0; i < FP8_DOWN_WAVES; ++i) {
-        before += i < wave ? wave_n[i] : 0;
-        active += wave_n[i];
+    for (int i = 0; i < WAVES; ++i) {
+        before += i < wave ? wave_n[0][i] : 0;
+        active += wave_n[0][i];
     }
     if (owner) {
         const int at = before + __popcll(own & below);
@@ -231,88 +252,137 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
     __syncthreads();
     if (row_first) atomicOr(reinterpret_cast<unsigned long long*>(&experts[place[first]].rows), 1ull << row);
     __syncthreads();
-    // entries of the experts before each: a scan over the waves' experts
-    const int mine = tid < active ? __popcll(experts[tid].rows) : 0;
+    // entries and row groups of the experts before each: a scan over the waves' experts, groups from bit 16 up
+    const uint64_t named = tid < active ? experts[tid].rows : 0;
+    int mine = __popcll(named);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) mine += (__popc((named >> (16 * t)) & 0xffff) + COLS - 1) / COLS << 16;
     int sum = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const int o = __shfl_up(sum, d);
         sum += lane >= d ? o : 0;
     }
-    if (lane == 63) wave_n[wave] = sum;
+    if (lane == 63) wave_n[1][wave] = sum;
     __syncthreads();
+    int total = 0;
 #pragma unroll
-    for (int i = 0; i < FP8_DOWN_WAVES; ++i) sum += i < wave ? wave_n[i] : 0;
-    if (tid < active) experts[tid].first = sum - mine;
+    for (int i = 0; i < WAVES; ++i) {
+        sum += i < wave ? wave_n[1][i] : 0;
+        total += wave_n[1][i];
+    }
+    if (tid < active) {
+        int at = (sum - mine) >> 16, entry = (sum - mine) & 0xffff;
+        first_of[tid] = (uint16_t)entry;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            for (uint32_t left = (named >> (16 * t)) & 0xffff; left;) {
+                uint32_t rest = left;
+                for (int i = 0; i < COLS; ++i) rest &= rest - 1;
+                groups[at++] = Group{experts[tid].id, (uint16_t)(left ^ rest), (uint16_t)(entry | t << 10)};
+                entry += __popc(left ^ rest);
+                left = rest;
+            }
+        }
+    }
     __syncthreads();
     if (row_first) {
         float w = 0.f;
         for (int s = tid; s < (row + 1) * A.topk; ++s) w += ids[s] == e ? wts[s] : 0.f;
-        const Expert& x = experts[place[first]];
-        entries[x.first + __popcll(x.rows & ((1ull << row) - 1))] = Entry{tid, w};
+        const int j = place[first];
+        entries[first_of[j] + __popcll(experts[j].rows & ((1ull << row) - 1))] = Entry{tid, w};
     }
     __syncthreads();
 
-    const int n0 = blockIdx.x * 16, I = A.inter, hidden = A.hidden, kb_n = I / FP8_BLOCK, units = active * kb_n;
-    // a row group's inputs, and this lane's routing weight
-    const auto inputs = [&](BlockX<H>& x, float& wt, uint64_t rows, int first, int kb, int t) {
-        const int at = 16 * t + r;
-        x.clear();
-        wt = 0.f;
-        if ((rows >> at) & 1) {
-            const Entry n = entries[first + __popcll(rows & ((1ull << at) - 1))];
-            wt = n.weight;
-            x.load(A.act + (int64_t)n.slot * I + kb * FP8_BLOCK, g);
-        }
-    };
-    struct Unit {
+    const int n0 = blockIdx.x * 16, I = A.inter, hidden = A.hidden, kb_n = I / FP8_BLOCK;
+    const int units = (total >> 16) * kb_n;
+    // Block kb of group j's expert, and the inputs of the group's rows there: the vector memory path takes 16 lanes
+    // that read neighbouring bytes together and lanes of different rows one by one, so the inputs (512 bytes a row,
+    // two rows a load) come in their own order and take the matrix unit's by way of LDS.  Straight to the lanes that
+    // multiply them they are eight loads of four useful lanes each, and bound the kernel (231 us where it is 165).
+    struct Weights {
         int8x32_t w;
-        uint64_t rows;
         float sc;
-        int first, kb;
     };
-    const auto fetch = [&](Unit& u, int at) {
-        const int j = at / kb_n;
-        u.kb = at - j * kb_n;
-        const Expert x = experts[j];
-        u.rows = x.rows;
-        u.first = x.first;
-        u.w = load_whole_block(A.w2 + ((int64_t)x.id * hidden + n0 + r) * I + u.kb * FP8_BLOCK, g);
-        u.sc = A.s2[((int64_t)x.id * hidden + n0) / FP8_BLOCK * kb_n + u.kb];
+    struct Inputs {
+        i32x4_t v[COLS / 2];
+        float wt;
+        uint32_t rows;
+        int t;
+    };
+    const auto fetch_w = [&](Weights& u, int at) {
+        const int j = at / kb_n, kb = at - j * kb_n, id = __builtin_amdgcn_readfirstlane(groups[j].id);
+        u.w = load_whole_block(A.w2 + ((int64_t)id * hidden + n0 + r) * I + kb * FP8_BLOCK, g);
+        u.sc = A.s2[((int64_t)id * hidden + n0) / FP8_BLOCK * kb_n + kb];
+    };
+    const auto fetch_x = [&](Inputs& u, int at) {
+        const int j = at / kb_n, kb = at - j * kb_n;
+        const int first = __builtin_amdgcn_readfirstlane(groups[j].first), entry = first & 0x3ff;
+        u.rows = __builtin_amdgcn_readfirstlane(groups[j].rows);
+        u.t = MT == 1 ? 0 : first >> 10;
+        const int last = (int)__popc(u.rows) - 1;
+        u.wt = entries[entry + min((int)__popc(u.rows & ((1u << r) - 1)), last)].weight;
+#pragma unroll
+        for (int i = 0; i < COLS / 2; ++i) {
+            const int slot = entries[entry + min(2 * i + (lane >> 5), last)].slot;
+            u.v[i] = reinterpret_cast<const i32x4_t*>(A.act + 2 * ((int64_t)slot * I + kb * FP8_BLOCK))[lane & 31];
+        }
     };
     float acc[MT][4] = {};
-    const auto compute = [&](const Unit& u) {
+    const auto compute = [&](const Weights& u, const Inputs& x) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            if (MT > 1 && !((u.rows >> (16 * t)) & 0xffff)) continue;
-            BlockX<H> x;
-            float wt;
-            inputs(x, wt, u.rows, u.first, u.kb, t);
-            const float4_t p = block_product<H>(BlockW<H>(u.w), x);
-            const bool has = (u.rows >> (16 * t + r)) & 1;      // 0 times a weight that is NaN is not 0
-            wt *= u.sc;
+        for (int i = 0; i < COLS / 2; ++i) columns[wave][64 * i + lane] = x.v[i];
+        const bool has = (x.rows >> r) & 1;           // the other columns are no row's: any inputs do
+        const i32x4_t* col = columns[wave] + (has ? __popc(x.rows & ((1u << r) - 1)) : 0) * 32 + 4 * g;
+        BlockX<H> in[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][i] = has ? fmaf(p[i], wt, acc[t][i]) : acc[t][i];
-        }
+        for (int i = 0; i < 2; ++i)                   // chunks g and g + 4 of 16: two of 8 values, two of what they leave
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                in[0].v[2 * i + h] = __builtin_bit_cast(H::vec8, col[16 * i + h]);
+                in[1].v[2 * i + h] = __builtin_bit_cast(H::vec8, col[16 * i + 2 + h]);
+            }
+        const BlockW<H> w(u.w);
+        const float4_t p = block_product<H>(w, in[0], block_product<H>(w, in[1]));
+        const float s = x.wt * u.sc;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            if (t == x.t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[t][i] = has ? fmaf(p[i], s, acc[t][i]) : acc[t][i];
     };
-    Unit u0, u1;
-    int at = __builtin_amdgcn_readfirstlane(wave);
-    if (at < units) fetch(u0, at);
-    for (; at < units; at += 2 * FP8_DOWN_WAVES) {
-        if (at + FP8_DOWN_WAVES < units) fetch(u1, at + FP8_DOWN_WAVES);
-        compute(u0);
-        if (at + 2 * FP8_DOWN_WAVES < units) fetch(u0, at + 2 * FP8_DOWN_WAVES);
-        if (at + FP8_DOWN_WAVES < units) compute(u1);
+    // Loads are waited for in their order, so a unit's inputs are asked for one unit ahead and before the weights of
+    // two units ahead: those are still on their way while the unit is computed.  For the same reason no load is in a
+    // branch (a wait behind one counts the loads of the shorter side): a group of fewer rows reads its last one's
+    // inputs again, and past the end the last unit is.
+    constexpr int AHEAD = 2, RING = AHEAD + 1, TURN = 2 * RING;
+    Weights uw[RING];
+    Inputs ux[2];
+    const int me = __builtin_amdgcn_readfirstlane(wave);
+    if (me < units) {
+        fetch_x(ux[0], me);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) fetch_w(uw[i], min(me + i * WAVES, units - 1));
+    }
+    for (int base = me; base < units; base += TURN * WAVES) {
+#pragma unroll
+        for (int i = 0; i < TURN; ++i) {
+            const int at = base + i * WAVES;
+            if (at >= units) break;
+            fetch_x(ux[(i + 1) % 2], min(at + WAVES, units - 1));
+            fetch_w(uw[(i + AHEAD) % RING], min(at + AHEAD * WAVES, units - 1));
+            compute(uw[i % RING], ux[i % 2]);
+        }
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) part[wave][4 * t + i][lane] = acc[t][i];
     __syncthreads();
-    for (int t = wave; t < MT; t += FP8_DOWN_WAVES) {
+    for (int t = wave; t < MT; t += WAVES) {
         float v[4] = {};
 #pragma unroll
-        for (int s = 0; s < FP8_DOWN_WAVES; ++s)
+        for (int s = 0; s < WAVES; ++s)
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] += part[s][4 * t + i][lane];
         const int orow = 16 * t + r;

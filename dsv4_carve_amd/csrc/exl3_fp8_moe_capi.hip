@@ -16,7 +16,7 @@ int64_t exl3_fp8_moe_scratch_bytes(int64_t rows, int64_t topk, int64_t intermedi
     if (rows < 1 || rows > FP8_MOE_MAX_ROWS) return fail("row count out of range (1 <= rows <= exl3_fp8_moe_max_rows())");
     if (topk < 1 || topk > FP8_MOE_MAX_TOPK) return fail("topk must be in 1..16");
     if (intermediate < 128 || intermediate % 128) return fail("intermediate must be a positive multiple of 128");
-    return rows * topk * intermediate * 2;
+    return rows * topk * intermediate * 4;
 }
 
 int exl3_fp8_moe(const void* x, int x_kind, void* out, int out_kind, int64_t rows, int64_t hidden, int64_t intermediate,
@@ -45,8 +45,9 @@ int exl3_fp8_moe(const void* x, int x_kind, void* out, int out_kind, int64_t row
     // fewer experts than slots: a workgroup row for each expert
     const int slots = (int)(rows * topk), by_expert = n_experts < slots;
     const dim3 g1((unsigned)(intermediate / 16), (unsigned)(by_expert ? n_experts : slots)), g2((unsigned)(hidden / 16));
-    // an expert has slots / n_experts rows on average: more than 16 are taken in passes where that is rare
-    const bool few = rows <= 16 || slots <= 4 * n_experts;
+    // An expert has slots / n_experts rows on average: with three at most, more than four are rare, and the expert's
+    // weights are read again for them (us, 41 rows x 8 on half of 256 experts: 306, with 64 columns 327).
+    const bool few = slots <= 3 * n_experts;
     const auto launch = [&](auto gu, auto dn) {
         hipLaunchKernelGGL(gu, g1, dim3(FP8_GU_WAVES * 64), 0, s, A, by_expert);
         const int rc = check_launch();
@@ -56,10 +57,11 @@ int exl3_fp8_moe(const void* x, int x_kind, void* out, int out_kind, int64_t row
     };
     const auto pick = [&](auto bf16) {
         constexpr bool B = decltype(bf16)::value;
-        if (rows <= 16) return launch(fp8_moe_gate_up_kernel<B, 1>, fp8_moe_down_kernel<B, 1>);
+        if (rows <= 16)
+            return launch(few ? fp8_moe_gate_up_kernel<B, 0> : fp8_moe_gate_up_kernel<B, 1>, fp8_moe_down_kernel<1>);
         if (rows <= 32)
-            return launch(few ? fp8_moe_gate_up_kernel<B, 1> : fp8_moe_gate_up_kernel<B, 2>, fp8_moe_down_kernel<B, 2>);
-        return launch(few ? fp8_moe_gate_up_kernel<B, 1> : fp8_moe_gate_up_kernel<B, 4>, fp8_moe_down_kernel<B, 4>);
+            return launch(few ? fp8_moe_gate_up_kernel<B, 0> : fp8_moe_gate_up_kernel<B, 2>, fp8_moe_down_kernel<2>);
+        return launch(few ? fp8_moe_gate_up_kernel<B, 0> : fp8_moe_gate_up_kernel<B, 4>, fp8_moe_down_kernel<4>);
     };
     return x_kind == OUT_BF16 ? pick(std::true_type{}) : pick(std::false_type{});
 }

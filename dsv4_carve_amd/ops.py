@@ -928,8 +928,8 @@ def fp8_moe(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: tor
     block; hidden and inter multiples of 128.  expert_ids, routing_weights and
     expert_map as moe_decode takes them (moe_route makes the first two); an id that
     no expert here has (-1 among them) contributes nothing.  With `swiglu_limit` L
-    the gate is capped at L and the up projection to [-L, L].  The activation
-    between the two products is rounded to x's dtype, sums are fp32."""
+    the gate is capped at L and the up projection to [-L, L].  Sums are fp32, and
+    the activation between the two products keeps 16 bits and fp32's range."""
     _check(x.is_cuda and x.dtype in X_KIND, "input must be HIP fp16 or bf16")
     _check(x.dim() == 2 and x.is_contiguous(), "input must be contiguous [m, hidden]")
     m, hidden = x.shape
@@ -951,7 +951,7 @@ def fp8_moe(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: tor
     _check(out.device == x.device and out.shape == x.shape and out.is_contiguous() and out.dtype in OUT_KIND,
            "output must be contiguous fp16, bf16 or fp32 [m, hidden] on the input device")
     if m:
-        scratch = torch.empty(m * topk * inter * 2, dtype=torch.uint8, device=x.device)
+        scratch = torch.empty(m * topk * inter * 4, dtype=torch.uint8, device=x.device)
         torch.ops.exl3_amd.fp8_moe(x, out, w13, w13_scale, w2, w2_scale, expert_ids, routing_weights, expert_map,
                                    float("inf") if swiglu_limit is None else float(swiglu_limit), scratch)
     return out

@@ -118,7 +118,7 @@ MOE = {"x": P, "x_kind": 1, "out_kind": 1, "rows": 2, "hidden": 256, "inter": 12
     ({"x": None}, "null"), ({"x_kind": 2}, "x_kind"), ({"out_kind": 3}, "out_kind"), ({"rows": 0}, "row count"),
     ({"rows": 65}, "row count"), ({"topk": 0}, "topk"), ({"topk": 17}, "topk"), ({"inter": 64}, "intermediate"),
     ({"hidden": 192}, "hidden"), ({"hidden": 1 << 21}, "2^20"), ({"E": 0}, "n_experts"), ({"limit": 0.0}, "swiglu_limit"),
-    ({"limit": float("nan")}, "swiglu_limit"), ({"bytes": 1023}, "scratch too small"), ({"scratch": P + 8}, "aligned"),
+    ({"limit": float("nan")}, "swiglu_limit"), ({"bytes": 2047}, "scratch too small"), ({"scratch": P + 8}, "aligned"),
     ({"x": P + 2}, "aligned"), ({"ids_kind": 2}, "int32 or int64"), ({"w_kind": 3}, "routing weights"),
     ({"emap": P, "n_global": 0}, "expert map")])
 def test_moe_argument_errors_without_device(change, msg):
@@ -131,7 +131,7 @@ def test_moe_argument_errors_without_device(change, msg):
 def test_moe_limits_agree():
     L = _lib.load()
     assert L.exl3_fp8_moe_max_rows() == ops.FP8_MOE_MAX_ROWS
-    assert L.exl3_fp8_moe_scratch_bytes(64, ops.FP8_MOE_MAX_TOPK, 128) == 64 * 16 * 128 * 2
+    assert L.exl3_fp8_moe_scratch_bytes(64, ops.FP8_MOE_MAX_TOPK, 128) == 64 * 16 * 128 * 4
 
 
 @pytest.mark.parametrize("change,msg", [({"logits": None}, "null"), ({"kind": 3}, "logits_kind"), ({"ids": 2}, "ids_kind"),

@@ -291,12 +291,12 @@ def routed(gen, rows, experts, topk, dtype=torch.int32):
 
 def check_moe(x, mats, ids, wts, limit=None, emap=None, out=None):
     y = ops.fp8_moe(x, *mats, ids, wts, swiglu_limit=limit, expert_map=emap, out=out)
-    ref, tol, low = R.moe(x, *mats, ids.cpu(), wts.cpu(), limit, None if emap is None else emap.cpu(), y.dtype)
+    ref, tol = R.moe(x, *mats, ids.cpu(), wts.cpu(), limit, None if emap is None else emap.cpu(), y.dtype)
     within(y, ref, tol, "moe")
-    # rounding errors are independent: in the 2-norm the activation's and the output's add up to two half steps at most
-    # (a subnormal fp16 value's half step is 2^-25 whatever its size)
+    # in the 2-norm: the output's half step (2^-25 where fp16 is subnormal) and little else
+    low = ref.numel() ** 0.5 * 2.0 ** -25 if y.dtype is torch.float16 else 0.0
     norm = torch.linalg.norm
-    assert norm(y.double() - ref) <= norm(ref) * (R.half_step(x.dtype) + R.half_step(y.dtype) + 1e-6) + norm(low)
+    assert norm(y.double() - ref) <= norm(ref) * (R.half_step(y.dtype) + 2.0 ** -16) + low
     return y
 
 
@@ -374,7 +374,7 @@ def test_moe_full_size_layer(dev):
     ids[0, 0] = 255
     y = ops.fp8_moe(x, w13.view(R.E4M3), s13, w2.view(R.E4M3), s2, ids, wts, swiglu_limit=10.0)
     pick = [0, 9, 15]
-    ref, tol, _ = R.moe(x[pick], w13.view(R.E4M3), s13, w2.view(R.E4M3), s2, ids[pick].cpu(), wts[pick].cpu(), 10.0, None,
+    ref, tol = R.moe(x[pick], w13.view(R.E4M3), s13, w2.view(R.E4M3), s2, ids[pick].cpu(), wts[pick].cpu(), 10.0, None,
                      y.dtype)
     within(y[pick], ref, tol, "full size")
 
@@ -402,7 +402,7 @@ def test_together_captured_and_on_another_stream(dev, rows):
         logits = ops.fp8_gemm(q, s, *gate, out_dtype=torch.float32)
         ref_ids, ref_w = R.route(logits, 3, "sigmoid", None, True, 1.0)
         assert torch.equal(ids.long(), ref_ids)
-        within(y, *R.moe(h, *mats, ref_ids.cpu(), ref_w.cpu(), 4.0, None, y.dtype)[:2], "block")
+        within(y, *R.moe(h, *mats, ref_ids.cpu(), ref_w.cpu(), 4.0, None, y.dtype), "block")
     static = xs[0].clone()
     graphs = []
     for _ in range(2):                                     # two graphs over the same inputs, replayed in turn
