@@ -9,6 +9,8 @@
 //
 // A wave has a row, lane i the experts i, i + 64, ...  The k largest are found one
 // by one: each lane's best, a maximum over the wave, the lowest index that has it.
+// Instructions bound it (8000 rows of 256 experts read 8 MB): keys are integers
+// that order as their numbers do, a step of a maximum one DPP instruction.
 //
 // Order by biased scores is the order of the exact scores even where fp32 cannot
 // tell two apart: the k + 1 largest are found in fp32 first, and if two
@@ -71,14 +73,9 @@ __device__ __forceinline__ T wave_sum(T v) {
 template <typename T>
 __device__ __forceinline__ T neg_inf() { return (T)-__builtin_inff(); }
 
-// NaN-free values only.
-template <typename T>
-__device__ __forceinline__ T wave_max(T v) {
-    return wave_all(v, neg_inf<T>(), [](T a, T b) { return a > b ? a : b; });
-}
-
-__device__ __forceinline__ int wave_min(int v) {
-    return wave_all(v, 0x7fffffff, [](int a, int b) { return min(a, b); });
+template <typename K>
+__device__ __forceinline__ K wave_max(K v, K none) {
+    return wave_all(v, none, [](K a, K b) { return a > b ? a : b; });
 }
 
 // softplus is max(l, 0) + log(1 + e^-|l|), which neither overflows nor loses small l.
@@ -89,34 +86,66 @@ __device__ __forceinline__ T score_of(int scoring, T l, T most, T total) {
     return sqrt((l > 0 ? l : (T)0) + log1p(exp(l > 0 ? -l : l)));
 }
 
+// A key that orders as its number does, so that maxima are one integer
+// instruction; -inf (and a NaN) is NO_KEY, which is never chosen, and 0 has one key.
+template <typename T>
+struct KeyOf;
+template <>
+struct KeyOf<float> {
+    typedef int type;
+    static constexpr int NO_KEY = INT32_MIN;
+    static __device__ __forceinline__ int of(float v) {
+        const int b = __float_as_int(v + 0.f);
+        return v > -__builtin_inff() ? b ^ (b >> 31 & 0x7fffffff) : NO_KEY;
+    }
+};
+template <>
+struct KeyOf<double> {
+    typedef long type;
+    static constexpr long NO_KEY = INT64_MIN;
+    static __device__ __forceinline__ long of(double v) {
+        const long b = __builtin_bit_cast(long, v + 0.0);
+        return v > -(double)__builtin_inff() ? b ^ (b >> 63 & 0x7fffffffffffffffl) : NO_KEY;
+    }
+};
+
 // The `count` largest of the wave's keys in order: lane j keeps the j-th one's index
-// (-1: none left) and key.  Keys are NaN-free; -inf is never chosen.
-template <typename T, int N>
-__device__ __forceinline__ void select_top(T (&key)[N], int count, int lane, int& chosen, T& chosen_key) {
+// (-1: none left), key and logit.
+template <typename K, int N>
+__device__ __forceinline__ void select_top(K (&key)[N], const float (&l)[N], K none, int count, int& chosen, K& chosen_key,
+                                           float& logit) {
+    const int lane = threadIdx.x & 63;
     chosen = -1;
-    chosen_key = neg_inf<T>();
+    chosen_key = none;
+    logit = 0.f;
     for (int j = 0; j < count; ++j) {
-        T best = key[0];
+        K best = key[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) best = key[i] > best ? key[i] : best;
+        const K top = wave_max(best, none);
+        if (top == none) break;
+        // the lowest index that has it: the first register, then the first lane
+        uint64_t have = 0;
         int at = 0;
 #pragma unroll
-        for (int i = 1; i < N; ++i)
-            if (key[i] > best) {
-                best = key[i];
-                at = i;
-            }
-        const T top = wave_max(best);
-        if (!(top > neg_inf<T>())) break;
-        const uint64_t have = __ballot(best == top);
-        const int owner = __builtin_ctzll(have);
-        const int idx = have & (have - 1) ? wave_min(best == top ? at * 64 + lane : 0x7fffffff)
-                                          : __builtin_amdgcn_readlane(at, owner) * 64 + owner;
-        if (lane == j) {
-            chosen = idx;
-            chosen_key = top;
+        for (int i = N - 1; i >= 0; --i) {
+            const uint64_t h = __ballot(key[i] == top);
+            at = h ? i : at;
+            have = h ? h : have;
         }
+        const int owner = __builtin_ctzll(have);
+        float value = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (idx == i * 64 + lane) key[i] = neg_inf<T>();
+            if (at == i) {
+                value = read_lane(l[i], owner);
+                key[i] = lane == owner ? none : key[i];
+            }
+        if (lane == j) {
+            chosen = at * 64 + owner;
+            chosen_key = top;
+            logit = value;
+        }
     }
 }
 
@@ -155,35 +184,37 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs A) {
     if (over_row) {
         most = l[0];
 #pragma unroll
-        for (int i = 1; i < N; ++i) most = fmaxf(most, l[i]);
-        most = wave_max(most);
+        for (int i = 1; i < N; ++i) most = l[i] > most ? l[i] : most;
+        most = wave_max(most, neg_inf<float>());
         total = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) total += l[i] > neg_inf<float>() ? expf(l[i] - most) : 0.f;
         total = wave_sum(total);
     }
     int chosen;
+    float mine;                     // the chosen logit, one a lane
+    typedef KeyOf<float> Key;
+    int key[N], got;
     if (!A.bias) {
-        float key[N], unused;
 #pragma unroll
-        for (int i = 0; i < N; ++i) key[i] = l[i];
-        select_top<float, N>(key, A.topk, lane, chosen, unused);
+        for (int i = 0; i < N; ++i) key[i] = Key::of(l[i]);
+        select_top<int, N>(key, l, Key::NO_KEY, A.topk, chosen, got, mine);
     } else {
-        float key[N], got;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = i * 64 + lane;
-            const float v = l[i] > neg_inf<float>() ? score_of<float>(A.scoring, l[i], most, total) + A.bias[e]
-                                                    : neg_inf<float>();
-            key[i] = v == v ? v : neg_inf<float>();
-        }
+        for (int i = 0; i < N; ++i)
+            key[i] = l[i] > neg_inf<float>()
+                         ? Key::of(score_of<float>(A.scoring, l[i], most, total) + A.bias[i * 64 + lane])
+                         : Key::NO_KEY;
         const int more = min(A.topk + 1, 64);
-        select_top<float, N>(key, more, lane, chosen, got);
-        const float below = __shfl_down(got, 1);
-        // fp32's scores are within 4e-6 of the exact ones (relative above one)
-        const bool near = lane + 1 < more && chosen >= 0 && !(got - below > 0x1p-17f * fmaxf(1.f, fabsf(got)));
+        select_top<int, N>(key, l, Key::NO_KEY, more, chosen, got, mine);
+        // fp32's scores are within 4e-6 of the exact ones (relative above one); a key turned back is its score
+        const float here = __int_as_float(got ^ (got >> 31 & 0x7fffffff)), below = __shfl_down(here, 1);
+        const bool last = __shfl_down(chosen, 1) < 0;
+        const bool near = lane + 1 < more && chosen >= 0 && !last && !(here - below > 0x1p-17f * fmaxf(1.f, fabsf(here)));
         if (__any(near) || more == A.topk) {
-            double dmost = most, dtotal = 1.0, dkey[N], unused;
+            typedef KeyOf<double> Key64;
+            double dmost = most, dtotal = 1.0;
+            long dkey[N], unused;
             if (A.scoring == SCORE_SOFTMAX) {
                 dtotal = 0.0;
 #pragma unroll
@@ -191,28 +222,19 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs A) {
                 dtotal = wave_sum(dtotal);
             }
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int e = i * 64 + lane;
-                const double v = l[i] > neg_inf<float>()
-                                     ? score_of<double>(A.scoring, (double)l[i], dmost, dtotal) + (double)A.bias[e]
-                                     : neg_inf<double>();
-                dkey[i] = v == v ? v : neg_inf<double>();
-            }
-            select_top<double, N>(dkey, A.topk, lane, chosen, unused);
+            for (int i = 0; i < N; ++i)
+                dkey[i] = l[i] > neg_inf<float>()
+                              ? Key64::of(score_of<double>(A.scoring, (double)l[i], dmost, dtotal) +
+                                          (double)A.bias[i * 64 + lane])
+                              : Key64::NO_KEY;
+            select_top<long, N>(dkey, l, Key64::NO_KEY, A.topk, chosen, unused, mine);
         }
         if (lane >= A.topk) chosen = -1;
-    }
-    // the chosen logits, one a lane
-    float mine = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float v = __shfl(l[i], chosen & 63);
-        if ((chosen >> 6) == i) mine = v;
     }
     double s = 0.0;
     if (A.scoring == SCORE_SOFTMAX) {
         // over their own sum only ratios count: from the largest chosen logit they cannot all underflow
-        const float top = over_row && !A.renormalize ? most : wave_max(chosen >= 0 ? mine : neg_inf<float>());
+        const float top = over_row && !A.renormalize ? most : wave_max(chosen >= 0 ? mine : neg_inf<float>(), neg_inf<float>());
         if (chosen >= 0) s = exp((double)mine - (double)top) / (A.renormalize ? 1.0 : (double)total);
     } else if (chosen >= 0) {
         s = score_of<double>(A.scoring, (double)mine, 0.0, 1.0);

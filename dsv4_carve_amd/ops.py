@@ -844,8 +844,8 @@ def fp8_quantize(x: torch.Tensor, *, pow2: bool = False) -> tuple[torch.Tensor, 
     _check(x.dim() >= 1 and x.dtype in OUT_KIND and x.is_contiguous(), "x must be contiguous fp16, bf16 or fp32 [..., k]")
     k = x.shape[-1]
     _check(1 <= k <= 1 << 24, "k must be in 1..2**24")
-    q = torch.empty(x.shape, dtype=E4M3, device=x.device)
-    scale = torch.empty((*x.shape[:-1], _blocks(k)), dtype=torch.float32, device=x.device)
+    q = torch.empty_like(x, dtype=E4M3)
+    scale = x.new_empty((*x.shape[:-1], _blocks(k)), dtype=torch.float32)
     if x.numel():
         torch.ops.exl3_amd.fp8_quantize(x, bool(pow2), q, scale)
     return q, scale
@@ -883,7 +883,7 @@ def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: t
              out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """fp8_gemm_into a new tensor."""
     _check(a.dim() == 2 and w.dim() == 2, "a must be [m, k] and w [n, k]")
-    c = torch.empty((a.shape[0], w.shape[0]), dtype=out_dtype, device=a.device)
+    c = a.new_empty((a.shape[0], w.shape[0]), dtype=out_dtype)
     return fp8_gemm_into(a, a_scale, w, w_scale, c)
 
 
@@ -905,10 +905,10 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
     dtype = out_dtype or x.dtype
     _check(dtype in OUT_KIND, "out_dtype must be fp16, bf16 or fp32")
     n = w.shape[0]
-    y = torch.empty((*x.shape[:-1], n), dtype=dtype, device=x.device)
+    y = x.new_empty((*x.shape[:-1], n), dtype=dtype)
     if y.numel():
         nbytes = _fp8_linear_scratch_bytes(x.device.index, x.numel() // k, k, n) if x.is_cuda else 0
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        scratch = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         torch.ops.exl3_amd.fp8_linear(x, w, w_scale, y, scratch)
     return y
 
@@ -951,7 +951,7 @@ def fp8_moe(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: tor
     _check(out.device == x.device and out.shape == x.shape and out.is_contiguous() and out.dtype in OUT_KIND,
            "output must be contiguous fp16, bf16 or fp32 [m, hidden] on the input device")
     if m:
-        scratch = torch.empty(m * topk * inter * 4, dtype=torch.uint8, device=x.device)
+        scratch = x.new_empty(m * topk * inter * 4, dtype=torch.uint8)
         torch.ops.exl3_amd.fp8_moe(x, out, w13, w13_scale, w2, w2_scale, expert_ids, routing_weights, expert_map,
                                    float("inf") if swiglu_limit is None else float(swiglu_limit), scratch)
     return out
@@ -985,8 +985,8 @@ def moe_route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", bias
     if bias is not None:
         _check(bias.dtype == torch.float32 and bias.is_contiguous() and bias.device == logits.device and
                tuple(bias.shape) == (n_experts,), "bias must be contiguous fp32 [experts] on the logits' device")
-    ids = torch.empty((m, topk), dtype=ids_dtype, device=logits.device)
-    weights = torch.empty((m, topk), dtype=torch.float32, device=logits.device)
+    ids = logits.new_empty((m, topk), dtype=ids_dtype)
+    weights = logits.new_empty((m, topk), dtype=torch.float32)
     if m:
         torch.ops.exl3_amd.moe_route(logits, SCORING[scoring], bias, bool(renormalize), float(scale), ids, weights)
     return ids, weights
