@@ -190,10 +190,18 @@ __device__ __forceinline__ void load16(const void* p, float (&v)[16]) {
 template <int K, bool POW2>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const void* __restrict__ x, int64_t rows, int k, int groups,
                                                            uint8_t* __restrict__ q, float* __restrict__ scale) {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const uint32_t chunks = (uint32_t)groups * 8;
-    const int64_t row = t / chunks;
-    const int c = (int)(t - row * chunks);
+    int64_t row;
+    int c;
+    if (gridDim.x < 1u << 24) {         // a division in 32 bits is a quarter of one in 64
+        const uint32_t t = blockIdx.x * 256 + threadIdx.x;
+        row = t / chunks;
+        c = (int)(t - (uint32_t)row * chunks);
+    } else {
+        const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        row = t / chunks;
+        c = (int)(t - row * chunks);
+    }
     const bool in = row < rows && c * 16 < k;
     float v[16];
     float most = 0.f;
@@ -509,6 +517,14 @@ __device__ __forceinline__ void wait_loads() {
     __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
 }
 
+// A workgroup barrier that waits for no load (__syncthreads would, for those of the steps ahead); the compiler moves no
+// memory access over it.
+__device__ __forceinline__ void bare_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool WIDE>
 __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu(2))) void fp8_gemm_tile_kernel(const uint8_t* __restrict__ a,
                                                                         const float* __restrict__ a_scale, int m, int k,
@@ -615,7 +631,7 @@ __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu
     for (int step = 0; step < steps; ++step) {
         // this step has come, and every wave is done with the buffer of the one before
         wait_loads<(STAGES - 2) * (T::NA + T::NW)>();
-        __builtin_amdgcn_s_barrier();
+        bare_barrier();
         // (no branch below these: the compiler would move the sums' updates behind it, and hold every product until there)
         if (step % T::GROUP == 0) fetch_scales(sv, step + T::GROUP);
         if (step % T::GROUP == T::GROUP / 2) put_scales(sv, step + T::GROUP / 2);

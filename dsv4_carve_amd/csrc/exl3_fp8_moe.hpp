@@ -120,7 +120,9 @@ __global__ __launch_bounds__(FP8_GU_WAVES * 64) void fp8_moe_gate_up_kernel(cons
                 if constexpr (MT) {
                     bx.load(xr[t] + kb * FP8_BLOCK, g);
                 } else {
+                    __builtin_amdgcn_wave_barrier();
                     columns[wave][lane] = *reinterpret_cast<const i32x4_t*>(xr[t] + kb * FP8_BLOCK);
+                    __builtin_amdgcn_wave_barrier();
                     bx.load(reinterpret_cast<const uint16_t*>(columns[wave] + 16 * min(r, 3)), g);
                 }
                 const float4_t pg = block_product<H>(BlockW<H>(u.g), bx), pu = block_product<H>(BlockW<H>(u.u), bx);
@@ -330,8 +332,10 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
     };
     float acc[MT][4] = {};
     const auto compute = [&](const Weights& u, const Inputs& x) {
+        __builtin_amdgcn_wave_barrier();              // the wave's own place: its LDS operations are in order
 #pragma unroll
         for (int i = 0; i < COLS / 2; ++i) columns[wave][64 * i + lane] = x.v[i];
+        __builtin_amdgcn_wave_barrier();
         const bool has = (x.rows >> r) & 1;           // the other columns are no row's: any inputs do
         const i32x4_t* col = columns[wave] + (has ? __popc(x.rows & ((1u << r) - 1)) : 0) * 32 + 4 * g;
         BlockX<H> in[2];

@@ -824,6 +824,11 @@ def _blocks(n: int) -> int:
     return -(-n // FP8_BLOCK)
 
 
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """x, or a copy of it where it begins off the 16-byte borders that the kernels read by (a slice of a flat tensor)."""
+    return x.clone() if x.data_ptr() & 15 else x
+
+
 def _check_fp8_matrix(w: torch.Tensor, w_scale: torch.Tensor, device: torch.device, what: str = "w") -> None:
     """w e4m3 [..., n, k] with an fp32 scale for each 128x128 block."""
     _check(w.dtype == E4M3 and w.is_contiguous() and w.device == device,
@@ -909,7 +914,7 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
     if y.numel():
         nbytes = _fp8_linear_scratch_bytes(x.device.index, x.numel() // k, k, n) if x.is_cuda else 0
         scratch = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        torch.ops.exl3_amd.fp8_linear(x, w, w_scale, y, scratch)
+        torch.ops.exl3_amd.fp8_linear(_aligned(x), w, w_scale, y, scratch)
     return y
 
 
@@ -952,7 +957,7 @@ def fp8_moe(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: tor
            "output must be contiguous fp16, bf16 or fp32 [m, hidden] on the input device")
     if m:
         scratch = x.new_empty(m * topk * inter * 4, dtype=torch.uint8)
-        torch.ops.exl3_amd.fp8_moe(x, out, w13, w13_scale, w2, w2_scale, expert_ids, routing_weights, expert_map,
+        torch.ops.exl3_amd.fp8_moe(_aligned(x), out, w13, w13_scale, w2, w2_scale, expert_ids, routing_weights, expert_map,
                                    float("inf") if swiglu_limit is None else float(swiglu_limit), scratch)
     return out
 

@@ -137,6 +137,17 @@ def test_gemm_row_counts(dev, m):
     within(ops.fp8_gemm(a, sa, w, sw, out_dtype=torch.float32), *R.gemm(a, sa, w, sw, torch.float32), str(m))
 
 
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n", [(5, 4084), (16, 4090), (15, 12200), (33, 4084), (50, 4090), (120, 4084), (250, 4090),
+                                 (500, 4084), (500, 4090), (1000, 4090), (2000, 8180), (4000, 4090)])
+def test_gemm_tile_shapes(dev, m, n, out):
+    """Rows and columns that every tile shape is chosen for, ragged in both, and a last block of 16."""
+    gen = gen_of(dev, m + n)
+    a, sa = rows_of(gen, m, 272)
+    w, sw = R.matrix(gen, n, 272)
+    within(ops.fp8_gemm(a, sa, w, sw, out_dtype=out), *R.gemm(a, sa, w, sw, out), f"{m}x{n}")
+
+
 @pytest.mark.parametrize("m,k,n", [(3, 400, 40), (40, 400, 200), (300, 400, 330), (600, 1040, 600)])
 def test_gemm_writes_its_rows_only_and_keeps_nan_in_them(dev, m, k, n):
     """Rows around c stay; a NaN in one row of a, or of w, reaches that row, or column, only; bytes past k are not used."""
@@ -336,6 +347,34 @@ def test_moe_skipped_repeated_and_mapped_ids(dev):
     none = torch.full((20, 4), -1, dtype=torch.int32, device=dev)
     assert (ops.fp8_moe(x, *mats, none, wts) == 0).all()
     assert ops.fp8_moe(x[:0], *mats, none[:0], wts[:0]).shape == (0, 256)
+
+
+@pytest.mark.parametrize("rows,experts,topk", [(16, 64, 4), (31, 64, 3), (64, 64, 3), (64, 9, 2)])
+def test_moe_crowded_expert(dev, rows, experts, topk):
+    """One expert that every row names, more rows than are taken at once, among experts of few rows."""
+    gen = gen_of(dev, rows)
+    mats = layer(gen, experts, 256, 128, size=1.0)
+    x = normal(gen, rows, 256, spread=False)
+    ids, wts = routed(gen, rows, experts, topk)
+    ids[:, 0] = 5
+    ids[:5, 1] = 7
+    check_moe(x, mats, ids, wts, 8.0)
+
+
+def test_unaligned_inputs_and_own_output(dev):
+    """x two bytes off a 16-byte border; the layer's output over its input."""
+    gen = gen_of(dev, 21)
+    w, sw = R.matrix(gen, 64, 256)
+    mats = layer(gen, 4, 256, 128, size=1.0)
+    for rows in (2, 20):
+        flat = normal(gen, 1 + rows * 256, spread=False)
+        x = flat[1:].view(rows, 256)
+        assert torch.equal(ops.fp8_linear(x, w, sw), ops.fp8_linear(x.clone(), w, sw))
+        ids, wts = routed(gen, rows, 4, 2)
+        want = ops.fp8_moe(x.clone(), *mats, ids, wts)
+        assert torch.equal(ops.fp8_moe(x, *mats, ids, wts), want)
+        y = x.clone()
+        assert ops.fp8_moe(y, *mats, ids, wts, out=y) is y and torch.equal(y, want)
 
 
 def test_moe_rows_are_apart(dev):
