@@ -207,10 +207,18 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs A) {
                          : Key::NO_KEY;
         const int more = min(A.topk + 1, 64);
         select_top<int, N>(key, l, Key::NO_KEY, more, chosen, got, mine);
-        // fp32's scores are within 4e-6 of the exact ones (relative above one); a key turned back is its score
+        // fp32's keys are within 4e-6 of the exact ones, relative to what they are made of where that is above one: the
+        // key itself, or a score that a bias takes back, of any expert (sqrt(log(1 + e^l)) < 1.4 sqrt(l) from l = 1 on).
+        // A key turned back is its number.
+        float size = 1.f;
+        if (A.scoring == SCORE_SQRTSOFTPLUS) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) size = fmaxf(size, l[i]);
+            size = sqrtf(wave_max(size, 1.f));
+        }
         const float here = __int_as_float(got ^ (got >> 31 & 0x7fffffff)), below = __shfl_down(here, 1);
         const bool last = __shfl_down(chosen, 1) < 0;
-        const bool near = lane + 1 < more && chosen >= 0 && !last && !(here - below > 0x1p-17f * fmaxf(1.f, fabsf(here)));
+        const bool near = lane + 1 < more && chosen >= 0 && !last && !(here - below > 0x1p-17f * fmaxf(size, fabsf(here)));
         if (__any(near) || more == A.topk) {
             typedef KeyOf<double> Key64;
             double dmost = most, dtotal = 1.0;

@@ -262,6 +262,20 @@ def test_route_ties_and_near_ties(dev, scoring):
     check_route(far, 8, scoring, torch.randn(256, generator=gen, device=dev) * 1e-7)
 
 
+def test_route_scores_that_a_bias_takes_back(dev):
+    """A key's error is that of its score, which may be far above the key."""
+    gen = gen_of(dev, 11)
+    logits = torch.randn((500, 6), generator=gen, device=dev)
+    logits[:, ::2] = 1e6 + torch.randint(-32, 32, (500, 3), generator=gen, device=dev) * 0.0625
+    score = torch.sqrt(logits.double().clamp(min=0) + torch.log1p(torch.exp(-logits.double().abs())))
+    for shift in (0.0, 0.5):
+        for row in range(0, 500, 10):
+            bias = (shift - score[row]).float()             # this row's keys lie within fp32's error of each other
+            check_route(logits[row:row + 10].contiguous(), 2, "sqrtsoftplus", bias)
+            check_route(logits[row:row + 10].contiguous(), 6, "sqrtsoftplus", bias + torch.randint(
+                -8, 8, (6,), generator=gen, device=dev) * 2.0 ** -16)
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid", "sqrtsoftplus"])
 @pytest.mark.parametrize("biased", [False, True])
 def test_route_masked_and_extreme_logits(dev, scoring, biased):
