@@ -33,9 +33,9 @@ typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int FP8_BLOCK = 128;
+constexpr float FP8_MAX = 448.0f;
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-constexpr float FP8_MAX = 448.0f;
 
 __device__ __forceinline__ int8x32_t join(i32x4_t lo, i32x4_t hi) {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -56,7 +56,6 @@ struct Half16 {
         const f16x2_t p3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
         return vec8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
     }
-    static __device__ __forceinline__ uint16_t bits(float f) { return f32_to_f16_bits(f); }
 };
 
 template <>
@@ -72,7 +71,6 @@ struct Half16<true> {
         const bf16x2_t p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
         return vec8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
     }
-    static __device__ __forceinline__ uint16_t bits(float f) { return f32_to_bf16_rne(f); }
 };
 
 // A lane's 32 weights of one block (two 16-byte loads, as in exl3_fp8.hpp) and the inputs at the same k.
@@ -95,10 +93,6 @@ struct BlockX {
         v[1] = lo[1];
         v[2] = hi[0];
         v[3] = hi[1];
-    }
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = typename H::vec8{};
     }
 };
 
@@ -186,7 +180,8 @@ __device__ __forceinline__ void load16(const void* p, float (&v)[16]) {
 }
 
 // Rows of a multiple of 16 values, 16-byte aligned: a lane has 16 neighbouring
-// values, eight lanes a group.
+// values, eight lanes a group.  Memory bounds it: 8000 x 4096 fp16 15.9 us, 6.2 TB/s
+// read and written; 13 rows are a launch's 2.9 us.
 template <int K, bool POW2>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const void* __restrict__ x, int64_t rows, int k, int groups,
                                                            uint8_t* __restrict__ q, float* __restrict__ scale) {
@@ -222,7 +217,8 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const void* __restric
     *reinterpret_cast<u32x4_t*>(q + at) = out;
 }
 
-// Any row length and alignment: a wave for each group, two values a lane.
+// Any row length and alignment: a wave for each group, two values a lane, whose
+// loads of two or four bytes bound it.
 template <int K, bool POW2>
 __global__ __launch_bounds__(256) void fp8_quantize_any_kernel(const void* __restrict__ x, int64_t rows, int k,
                                                                int groups, uint8_t* __restrict__ q,
@@ -301,6 +297,8 @@ __device__ __forceinline__ int8x32_t load_block(const uint8_t* row, int kb, int 
 // A workgroup has 16 outputs of 16 MT rows; its waves take every WAVES-th block
 // of k, with both operands straight from memory to registers and through the
 // 16-bit instruction, and their sums are joined in LDS in the order of the waves.
+// Latency bounds it: 2 rows x 1536 x 4096 3.9 us, 1 row x 4096 x 4096 4.9 us (3.4
+// TB/s of weights).
 template <int MT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void fp8_gemm_rows_kernel(const uint8_t* __restrict__ a,
                                                                    const float* __restrict__ a_scale, int64_t m, int k,
@@ -358,7 +356,8 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_gemm_rows_kernel(const uint8_t
 // quantizes them whole into LDS, as fp8_quantize does, while its first weights are
 // on their way, and has 16 outputs of them.  LDS holds a row's blocks (zeros past
 // k) and 64 bytes more, so that four rows' chunks lie in different banks, then the
-// scales.
+// scales.  1 row x 4096 x 4096 5.5 to 6.3 us (2.7 to 3.1 TB/s of weights): the first
+// loads' latency and the row's way through LDS.
 constexpr int FP8_LINEAR_WAVES = 8;
 constexpr int FP8_LINEAR_DEEP = 4;                // blocks of a wave on their way
 

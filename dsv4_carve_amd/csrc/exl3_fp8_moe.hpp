@@ -9,7 +9,7 @@
 // weights are widened (exactly) to the type of x for the first product, and to
 // bf16 for the second, whose activation is the sum of two bf16 values (its
 // rounding and the rounding of what that leaves, 2^-17 of it, and no overflow):
-// one instruction more a block, which the weights' traffic hides, and the
+// four instructions more a block, which the weights' traffic hides, and the
 // output's rounding is the only one that counts.  Sums are fp32: a block of 128
 // is four 16x16x32 instructions (eight) into a cleared accumulator, scaled into
 // the running sum by one multiply-add a value.
@@ -55,7 +55,8 @@ constexpr int FP8_GU_WAVES = 4;
 // few rows an expert, the columns left over cost neither traffic nor time.  MT 0
 // is for rows that are few an expert, 4 at a time: their inputs come as down's do,
 // one load for four rows.  Four waves a workgroup, each with two blocks of both
-// matrices on their way.
+// matrices on their way.  Memory bounds it: 5.4 to 5.7 TB/s of weights with 16 rows
+// (101 of 256 experts of 4096 x 2048, 299 to 314 us).
 template <bool BF16, int MT>
 __global__ __launch_bounds__(FP8_GU_WAVES * 64) void fp8_moe_gate_up_kernel(const Fp8MoeArgs A, int by_expert) {
     typedef Half16<BF16> H;
