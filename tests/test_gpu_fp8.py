@@ -195,6 +195,25 @@ def test_gemm_past_32_bit_offsets(dev, m, k, n):
     within(c[-40:, last], *R.gemm(a[-40:], sa[-40:], w[last], sw[-1:], torch.bfloat16), "corner")
 
 
+@pytest.mark.parametrize("out", [torch.float16, torch.float32])
+def test_gemm_longest_rows(dev, out):
+    """Rows too long for a tile's 32-bit offsets; no value is negative, so that the sum's size is its own."""
+    gen = gen_of(dev, 8)
+    m, k, n = 17, (1 << 22) + 16, 20
+    a, w = (torch.randint(0, 0x40, shape, generator=gen, device=dev, dtype=torch.uint8).view(R.E4M3)
+            for shape in ((m, k), (n, k)))
+    sa = torch.rand((m, -(-k // 128)), generator=gen, device=dev)
+    sw = torch.rand((1, -(-k // 128)), generator=gen, device=dev) * 2.0 ** -10
+    c = ops.fp8_gemm(a, sa, w, sw, out_dtype=out)
+    ref = torch.zeros((m, n), dtype=torch.float64, device=dev)
+    for at in range(0, k, 1 << 20):
+        part = slice(at, min(at + (1 << 20), k))
+        b = slice(at // 128, -(-part.stop // 128))
+        ref += R.rows(a[:, part], sa[:, b]) @ R.weight(w[:, part], sw[:, b]).t()
+    # an eighth of the blocks is a wave's sum, and eight of them are joined
+    within(c, ref, ref * (R.steps(k // 8) * R.U + R.half_step(out)), "longest")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 13, 16, 17, 40, 300])
 @pytest.mark.parametrize("k,n", [(1536, 384), (272, 70)])
@@ -361,6 +380,18 @@ def test_moe_skipped_repeated_and_mapped_ids(dev):
     none = torch.full((20, 4), -1, dtype=torch.int32, device=dev)
     assert (ops.fp8_moe(x, *mats, none, wts) == 0).all()
     assert ops.fp8_moe(x[:0], *mats, none[:0], wts[:0]).shape == (0, 256)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_moe_small_and_large_inputs(dev, dtype):
+    """Inputs in fp16's subnormal range, and activations past fp16's largest value."""
+    gen = gen_of(dev, 17)
+    mats = layer(gen, 8, 256, 256, size=1.0)
+    x = normal(gen, 6, 256, dtype=torch.float32, spread=False)
+    ids, wts = routed(gen, 6, 8, 2)
+    out = torch.empty((6, 256), dtype=torch.float32, device=dev)
+    check_moe((x * 2.0 ** -19).to(dtype), mats, ids, wts, out=out)
+    check_moe((x * 64).to(dtype), (mats[0], mats[1] * 64, mats[2], mats[3]), ids, wts, out=out)
 
 
 @pytest.mark.parametrize("rows,experts,topk", [(16, 64, 4), (31, 64, 3), (64, 64, 3), (64, 9, 2)])
