@@ -37,6 +37,18 @@ constexpr float FP8_MAX = 448.0f;
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// A wave-uniform lane's value of 4 or 8 bytes.
+template <typename T>
+__device__ __forceinline__ T read_lane(T v, int lane) {
+    if constexpr (sizeof(T) == 8) {
+        const u32x2_t a = __builtin_bit_cast(u32x2_t, v);
+        return __builtin_bit_cast(T, u32x2_t{(uint32_t)__builtin_amdgcn_readlane((int)a[0], lane),
+                                             (uint32_t)__builtin_amdgcn_readlane((int)a[1], lane)});
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    }
+}
+
 __device__ __forceinline__ int8x32_t join(i32x4_t lo, i32x4_t hi) {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }

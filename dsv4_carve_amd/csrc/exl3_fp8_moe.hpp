@@ -187,13 +187,17 @@ constexpr int FP8_DOWN_WAVES = 16;
 // scale, so that the sum over experts needs no second pass and no atomics.  A
 // wave takes every 16th block of an expert and up to four rows that name it, the
 // next ones' bytes on their way while it computes.  5.7 TB/s of weights with 16
-// rows (101 of 256 experts of 4096 x 2048, 149 us).
+// rows (101 of 256 experts of 4096 x 2048, 149 us).  MT 0 is for a single row, whose
+// experts one wave tells apart: one barrier before the first load, not eight (a
+// layer of one row 46.1 to 47.7 us a call, 48.5 to 50.7 with MT 1).
 template <int MT>
 __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const Fp8MoeArgs A) {
     typedef Half16<true> H;
     constexpr int WAVES = FP8_DOWN_WAVES;
     static_assert(WAVES * 64 == FP8_MOE_MAX_SLOTS, "a thread for each slot");
-    constexpr int COLS = 4;        // rows whose inputs two loads bring
+    constexpr bool ONE = MT == 0;
+    constexpr int TILES = ONE ? 1 : MT;
+    constexpr int COLS = ONE ? 1 : 4, LOADS = (COLS + 1) / 2;      // rows of a group, and the loads that bring their inputs
     struct Entry {
         uint16_t slot, row;
         float weight;
@@ -214,98 +218,124 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
     __shared__ uint16_t place[FP8_MOE_MAX_SLOTS];                            // of a first slot's expert among them
     __shared__ uint16_t first_of[FP8_MOE_MAX_SLOTS];                         // an expert's first entry
     __shared__ int wave_n[2][WAVES];
-    __shared__ __attribute__((aligned(16))) float part[WAVES][MT * 4][64];
-    __shared__ i32x4_t columns[WAVES][COLS * 32];       // a wave's inputs of one block, 512 bytes a row
+    __shared__ __attribute__((aligned(16))) float part[WAVES][TILES * 4][64];
+    __shared__ i32x4_t columns[WAVES][LOADS * 64];       // a wave's inputs of one block, 512 bytes a row
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = lane & 15, g = lane >> 4;
     const int S = A.rows * A.topk;
     const uint64_t below = (1ull << lane) - 1;
     const int row = tid / A.topk;
     const int e = tid < S ? A.rt.local(tid, A.E) : -1;
-    ids[tid] = e;
-    if (e >= 0) wts[tid] = A.rt.weight(tid);
-    __syncthreads();
-    // the first slot of this one's expert, and whether it is its row's first of it
-    int first = tid;
-    bool row_first = e >= 0;
-    if (wave * 64 < S) {
-        for (int s = (min(S, wave * 64 + 64) - 1) & ~3; s >= 0; s -= 4) {
-            const i32x4_t v = *reinterpret_cast<const i32x4_t*>(&ids[s]);
+    int total;                     // entries, groups from bit 16 up
+    if constexpr (ONE) {
+        // an expert's first slot is an entry and a group, with the weights of all its slots
+        if (wave == 0) {
+            const float w = e >= 0 ? A.rt.weight(tid) : 0.f;
+            float sum = 0.f;
+            bool is_first = e >= 0;
 #pragma unroll
-            for (int i = 3; i >= 0; --i) first = v[i] == e && s + i < first ? s + i : first;
-        }
-        for (int s = row * A.topk; s < tid; ++s) row_first = row_first && ids[s] != e;
-    }
-    const bool owner = e >= 0 && first == tid;
-    const uint64_t own = __ballot(owner);
-    if (lane == 0) wave_n[0][wave] = __popcll(own);
-    __syncthreads();
-    int before = 0, active = 0;
-#pragma unroll
-    for (int i = 0; i < WAVES; ++i) {
-        before += i < wave ? wave_n[0][i] : 0;
-        active += wave_n[0][i];
-    }
-    if (owner) {
-        const int at = before + __popcll(own & below);
-        place[tid] = (uint16_t)at;
-        experts[at].id = e;
-        experts[at].rows = 0;
-    }
-    __syncthreads();
-    if (row_first) atomicOr(reinterpret_cast<unsigned long long*>(&experts[place[first]].rows), 1ull << row);
-    __syncthreads();
-    // An expert's rows in order, cut into groups: a group's rows are columns of the matrix instruction by their number
-    // mod 16.
-    const auto split = [](uint64_t rows, auto&& group) {
-        int first = 0, count = 0;
-        for (uint32_t used = 0; rows; rows &= rows - 1) {
-            const uint32_t column = 1u << (__builtin_ctzll(rows) & 15);
-            if (count == COLS || (used & column)) {
-                group(first, count);
-                first += count;
-                count = 0;
-                used = 0;
+            for (int s = 0; s < FP8_MOE_MAX_TOPK; ++s) {
+                const bool same = read_lane(e, s) == e;
+                sum += same ? read_lane(w, s) : 0.f;
+                is_first = is_first && !(same && s < lane);
             }
-            used |= column;
-            ++count;
+            const uint64_t active = __ballot(is_first);
+            const int at = __popcll(active & below);
+            if (is_first) {
+                groups[at] = Group{e, (uint16_t)at, 1};
+                entries[at] = Entry{(uint16_t)tid, 0, sum};
+            }
+            if (lane == 0) wave_n[1][0] = __popcll(active);
         }
-        if (count) group(first, count);
-    };
-    // entries and groups of the experts before each: a scan over the waves' experts, groups from bit 16 up
-    const uint64_t named = tid < active ? experts[tid].rows : 0;
-    int mine = __popcll(named);
-    split(named, [&](int, int) { mine += 1 << 16; });
-    int sum = mine;
+        __syncthreads();
+        total = wave_n[1][0] << 16;
+    } else {
+        ids[tid] = e;
+        if (e >= 0) wts[tid] = A.rt.weight(tid);
+        __syncthreads();
+        // the first slot of this one's expert, and whether it is its row's first of it
+        int first = tid;
+        bool row_first = e >= 0;
+        if (wave * 64 < S) {
+            for (int s = (min(S, wave * 64 + 64) - 1) & ~3; s >= 0; s -= 4) {
+                const i32x4_t v = *reinterpret_cast<const i32x4_t*>(&ids[s]);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(sum, d);
-        sum += lane >= d ? o : 0;
-    }
-    if (lane == 63) wave_n[1][wave] = sum;
-    __syncthreads();
-    int total = 0;
+                for (int i = 3; i >= 0; --i) first = v[i] == e && s + i < first ? s + i : first;
+            }
+            for (int s = row * A.topk; s < tid; ++s) row_first = row_first && ids[s] != e;
+        }
+        const bool owner = e >= 0 && first == tid;
+        const uint64_t own = __ballot(owner);
+        if (lane == 0) wave_n[0][wave] = __popcll(own);
+        __syncthreads();
+        int before = 0, active = 0;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) {
-        sum += i < wave ? wave_n[1][i] : 0;
-        total += wave_n[1][i];
+        for (int i = 0; i < WAVES; ++i) {
+            before += i < wave ? wave_n[0][i] : 0;
+            active += wave_n[0][i];
+        }
+        if (owner) {
+            const int at = before + __popcll(own & below);
+            place[tid] = (uint16_t)at;
+            experts[at].id = e;
+            experts[at].rows = 0;
+        }
+        __syncthreads();
+        if (row_first) atomicOr(reinterpret_cast<unsigned long long*>(&experts[place[first]].rows), 1ull << row);
+        __syncthreads();
+        // An expert's rows in order, cut into groups: a group's rows are columns of the matrix instruction by their number
+        // mod 16.
+        const auto split = [](uint64_t rows, auto&& group) {
+            int first = 0, count = 0;
+            for (uint32_t used = 0; rows; rows &= rows - 1) {
+                const uint32_t column = 1u << (__builtin_ctzll(rows) & 15);
+                if (count == COLS || (used & column)) {
+                    group(first, count);
+                    first += count;
+                    count = 0;
+                    used = 0;
+                }
+                used |= column;
+                ++count;
+            }
+            if (count) group(first, count);
+        };
+        // entries and groups of the experts before each: a scan over the waves' experts, groups from bit 16 up
+        const uint64_t named = tid < active ? experts[tid].rows : 0;
+        int mine = __popcll(named);
+        split(named, [&](int, int) { mine += 1 << 16; });
+        int sum = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(sum, d);
+            sum += lane >= d ? o : 0;
+        }
+        if (lane == 63) wave_n[1][wave] = sum;
+        __syncthreads();
+        total = 0;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            sum += i < wave ? wave_n[1][i] : 0;
+            total += wave_n[1][i];
+        }
+        if (tid < active) {
+            int at = (sum - mine) >> 16;
+            const int entry = (sum - mine) & 0xffff;
+            first_of[tid] = (uint16_t)entry;
+            split(named, [&](int first, int count) {
+                groups[at++] = Group{experts[tid].id, (uint16_t)(entry + first), (uint16_t)count};
+            });
+        }
+        __syncthreads();
+        if (row_first) {
+            float w = 0.f;
+            for (int s = tid; s < (row + 1) * A.topk; ++s) w += ids[s] == e ? wts[s] : 0.f;
+            const int j = place[first];
+            entries[first_of[j] + __popcll(experts[j].rows & ((1ull << row) - 1))] = Entry{(uint16_t)tid, (uint16_t)row, w};
+        }
+        __syncthreads();
+
     }
-    if (tid < active) {
-        int at = (sum - mine) >> 16;
-        const int entry = (sum - mine) & 0xffff;
-        first_of[tid] = (uint16_t)entry;
-        split(named, [&](int first, int count) {
-            groups[at++] = Group{experts[tid].id, (uint16_t)(entry + first), (uint16_t)count};
-        });
-    }
-    __syncthreads();
-    if (row_first) {
-        float w = 0.f;
-        for (int s = tid; s < (row + 1) * A.topk; ++s) w += ids[s] == e ? wts[s] : 0.f;
-        const int j = place[first];
-        entries[first_of[j] + __popcll(experts[j].rows & ((1ull << row) - 1))] = Entry{(uint16_t)tid, (uint16_t)row, w};
-    }
-    __syncthreads();
 
     const int n0 = blockIdx.x * 16, I = A.inter, hidden = A.hidden, kb_n = I / FP8_BLOCK;
     const int units = (total >> 16) * kb_n;
@@ -318,7 +348,7 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
         float sc;
     };
     struct Inputs {
-        i32x4_t v[COLS / 2];
+        i32x4_t v[LOADS];
         float wt;
         int col, t;                // this lane's row's: which of the group's (-1: none), which 16 of the batch
     };
@@ -344,16 +374,16 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
             }
         }
 #pragma unroll
-        for (int i = 0; i < COLS / 2; ++i) {
+        for (int i = 0; i < LOADS; ++i) {
             const int slot = entries[first + min(2 * i + (lane >> 5), last)].slot;
             u.v[i] = reinterpret_cast<const i32x4_t*>(A.act + 2 * ((int64_t)slot * I + kb * FP8_BLOCK))[lane & 31];
         }
     };
-    float acc[MT][4] = {};
+    float acc[TILES][4] = {};
     const auto compute = [&](const Weights& u, const Inputs& x) {
         __builtin_amdgcn_wave_barrier();              // the wave's own place: its LDS operations are in order
 #pragma unroll
-        for (int i = 0; i < COLS / 2; ++i) columns[wave][64 * i + lane] = x.v[i];
+        for (int i = 0; i < LOADS; ++i) columns[wave][64 * i + lane] = x.v[i];
         __builtin_amdgcn_wave_barrier();
         const bool has = x.col >= 0;                  // the other columns are no row's: any inputs do
         const i32x4_t* col = columns[wave] + (has ? x.col : 0) * 32 + 4 * g;
@@ -369,8 +399,8 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
         const float4_t p = block_product<H>(w, in[0], block_product<H>(w, in[1]));
         const float s = x.wt * u.sc;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const bool here = has && (MT == 1 || x.t == t);
+        for (int t = 0; t < TILES; ++t) {
+            const bool here = has && (TILES == 1 || x.t == t);
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[t][i] = here ? fmaf(p[i], s, acc[t][i]) : acc[t][i];
         }
@@ -399,11 +429,11 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
         }
     }
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) part[wave][4 * t + i][lane] = acc[t][i];
     __syncthreads();
-    for (int t = wave; t < MT; t += WAVES) {
+    for (int t = wave; t < TILES; t += WAVES) {
         float v[4] = {};
 #pragma unroll
         for (int s = 0; s < WAVES; ++s)

@@ -57,6 +57,7 @@ int exl3_fp8_moe(const void* x, int x_kind, void* out, int out_kind, int64_t row
     };
     const auto pick = [&](auto bf16) {
         constexpr bool B = decltype(bf16)::value;
+        if (rows == 1) return launch(few ? fp8_moe_gate_up_kernel<B, 0> : fp8_moe_gate_up_kernel<B, 1>, fp8_moe_down_kernel<0>);
         if (rows <= 16)
             return launch(few ? fp8_moe_gate_up_kernel<B, 0> : fp8_moe_gate_up_kernel<B, 1>, fp8_moe_down_kernel<1>);
         if (rows <= 32)

@@ -43,17 +43,6 @@ __device__ __forceinline__ T lane_of(T v, T none) {
     }
 }
 
-template <typename T>
-__device__ __forceinline__ T read_lane(T v, int lane) {
-    if constexpr (sizeof(T) == 8) {
-        const u32x2_t a = __builtin_bit_cast(u32x2_t, v);
-        return __builtin_bit_cast(T, u32x2_t{(uint32_t)__builtin_amdgcn_readlane((int)a[0], lane),
-                                             (uint32_t)__builtin_amdgcn_readlane((int)a[1], lane)});
-    } else {
-        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
-    }
-}
-
 // op over the wave's lanes (each lane's value once), as a wave-uniform value: a
 // scan of each row of 16 lanes, then of the rows; lane 63 has it all.
 template <typename T, typename Op>

@@ -382,6 +382,19 @@ def test_moe_skipped_repeated_and_mapped_ids(dev):
     assert ops.fp8_moe(x[:0], *mats, none[:0], wts[:0]).shape == (0, 256)
 
 
+@pytest.mark.parametrize("ids", [[3, 3, 0, -1, 7, 3], [-1, -1, 5], [9, 5000, -7], [2], list(range(16))])
+@pytest.mark.parametrize("mapped", [False, True])
+def test_moe_one_row(dev, ids, mapped):
+    """A single token: an expert named twice, none at all, ids out of range, every slot that there may be."""
+    gen = gen_of(dev, 18)
+    mats = layer(gen, 8, 256, 384, size=1.0)
+    emap = torch.tensor([4, -1, 0, 7, 7, 2], device=dev) if mapped else None
+    wts = torch.rand((1, len(ids)), generator=gen, device=dev)
+    y = check_moe(normal(gen, 1, 256, spread=False), mats, torch.tensor([ids], device=dev, dtype=torch.int32), wts, emap=emap)
+    if ids[0] == 9:
+        assert (y == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_moe_small_and_large_inputs(dev, dtype):
     """Inputs in fp16's subnormal range, and activations past fp16's largest value."""
