@@ -14,11 +14,11 @@
 // the instruction's row operand: a lane's four results are then four
 // neighbouring outputs of one row of a, under one scale.
 //
-// Two instructions do it.  The 8-bit one (16x16x128, a block in one) cuts each
-// product to a multiple of 2^-13 of the largest power of two among its group of
-// eight before it adds them: 1e-5 of the result in the 2-norm on normal values,
-// 1e-4 to 4e-4 where some channels are twenty times the others.  The 16-bit one
-// (16x16x32, four a block, on values widened exactly) is at 3e-8 and half as fast.
+// The instruction is the 16-bit one (16x16x32, four a block) on values widened
+// exactly, so that sums are fp32's.  The 8-bit one (16x16x128, a block in one) is
+// twice as fast and is not used: it cuts each product to a multiple of 2^-13 of
+// the largest power of two among its group of eight before it adds them, which a
+// result that cancels feels far more than its own rounding.
 #pragma once
 
 #include "exl3_decode.hpp"
@@ -460,59 +460,46 @@ __global__ __launch_bounds__(FP8_LINEAR_WAVES * 64) void fp8_linear_rows_kernel(
 
 // ---------------------------------------------------------------- product, many rows
 
-// An 8-bit instruction for a block, or four 16-bit ones on widened values.
-template <bool WIDE>
-struct Frag;
-
-template <>
-struct Frag<false> {
-    int8x32_t v;
-    __device__ __forceinline__ void set(const i32x4_t& lo, const i32x4_t& hi) { v = join(lo, hi); }
-    static __device__ __forceinline__ float4_t product(const Frag& w, const Frag& a) {
-        const float4_t zero = {0.f, 0.f, 0.f, 0.f};
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, a.v, zero, 0, 0, 0, 0, 0, 0);
-    }
-};
-
-template <>
-struct Frag<true> {
-    BlockX<Half16<true>> v;
+// A lane's 32 values of a block, as they come from LDS, and the product of two of them.
+struct Frag {
+    typedef Half16<true> H;
+    H::vec8 v[4];
     __device__ __forceinline__ void set(const i32x4_t& lo, const i32x4_t& hi) {
-        const BlockW<Half16<true>> b(join(lo, hi));
+        const BlockW<H> b(join(lo, hi));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v.v[i] = b.v[i];
+        for (int i = 0; i < 4; ++i) v[i] = b.v[i];
     }
     static __device__ __forceinline__ float4_t product(const Frag& w, const Frag& a) {
         float4_t p = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p = Half16<true>::mfma(w.v.v[i], a.v.v[i], p);
+        for (int i = 0; i < 4; ++i) p = H::mfma(w.v[i], a.v[i], p);
         return p;
     }
 };
 
 // Tiles of BM rows of a and BN rows of w; WM x WN waves share one, KG such sets
 // take alternate blocks of k (their sums are joined in LDS at the end).  A step
-// is KG blocks, which go from memory straight to LDS, STAGES - 1 steps ahead.  A
-// row of a block is eight 16-byte chunks there, chunk c of row r at place
-// c ^ (r & 7), so that eight rows' chunks of one k lie in different banks.
-template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool WIDE>
+// is KG blocks, which go from memory straight to LDS, one step ahead.  A row of a
+// block is eight 16-byte chunks there, chunk c of row r at place c ^ (r & 7), so
+// that eight rows' chunks of one k lie in different banks.
+template <int BM, int BN, int WM, int WN, int KG>
 struct Fp8Tile {
     static constexpr int SET = WM * WN * 64;              // threads of one set
     static constexpr int THREADS = SET * KG;
     static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
     static constexpr int NA = BM * 8 / SET, NW = BN * 8 / SET;      // chunks a thread moves in a step
     static constexpr int BUF = (BM + BN) * FP8_BLOCK;     // bytes of a block
-    static constexpr int NB = (BN + 127) / 128;           // scale blocks of w beside each other
     static constexpr int GROUP = KG < 4 ? 8 : 4;          // steps whose scales are staged together
-    static constexpr int SCALES = KG * GROUP * (BM + NB); // values of a group
+    static constexpr int SCALES = KG * GROUP * (BM + 1);  // values of a group
     static constexpr int NS = (SCALES + THREADS - 1) / THREADS;
-    static constexpr int LDS = STAGES * KG * BUF + 2 * SCALES * 4;
+    static constexpr int LDS = 2 * KG * BUF + 2 * SCALES * 4;
     static_assert(BM * 8 % SET == 0 && BN * 8 % SET == 0 && SET % 64 == 0, "whole chunks, in rows of eight");
+    static_assert(128 % BN == 0, "one block of w's scales");
     static_assert(KG == 1 || BM * BN * 4 * (KG - 1) <= LDS, "the sums are joined in the buffers");
     static_assert(LDS <= 160 * 1024, "LDS of a CU");
 };
 
-constexpr int FP8_TILE_MAX_K = 1 << 22;        // 256 rows of k bytes, and a few blocks more, stay below 2^31
+constexpr int FP8_TILE_MAX_K = 1 << 22;        // 128 rows of k bytes, and a few blocks more, stay below 2^31
 
 // 16 bytes a lane from base + at + step to dst + 16 * lane, zeros where at is OUTSIDE: the buffer has 2^31 bytes, and
 // an offset past its end reads as zero.
@@ -521,29 +508,24 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t base, char* d
     __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (__attribute__((address_space(3))) void*)dst, 16, (int)at, step, 0, 0);
 }
 
-// Until at most N of this wave's loads are on their way, and none of its LDS operations.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-    static_assert(N >= 0 && N < 64, "");
-    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
-}
+// Until none of this wave's loads and LDS operations is on its way.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(7 << 4); }
 
-// A workgroup barrier that waits for no load (__syncthreads would, for those of the steps ahead); the compiler moves no
-// memory access over it.
+// A workgroup barrier without a wait of its own; the compiler moves no memory access over it.
 __device__ __forceinline__ void bare_barrier() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
 
-template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool WIDE>
+template <int BM, int BN, int WM, int WN, int KG>
 __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu(2))) void fp8_gemm_tile_kernel(const uint8_t* __restrict__ a,
                                                                         const float* __restrict__ a_scale, int m, int k,
                                                                         const uint8_t* __restrict__ w,
                                                                         const float* __restrict__ w_scale, int n,
                                                                         void* __restrict__ c, int c_kind, int tiles_m,
                                                                         int tiles_n) {
-    typedef Fp8Tile<BM, BN, WM, WN, KG, STAGES, WIDE> T;
+    typedef Fp8Tile<BM, BN, WM, WN, KG> T;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int set = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid / T::SET), st = tid - set * T::SET;
@@ -590,15 +572,15 @@ __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu
             for (int i = 0; i < T::NW; ++i) load_to_lds(tw, dst + (BM + i * ROWS) * FP8_BLOCK, in ? ow[i] : OUTSIDE, at);
         }
     };
-    // scales of a group of steps as [block][BM rows of a, NB blocks of w]; a block past the end has any
-    float* const scales = reinterpret_cast<float*>(lds + STAGES * KG * T::BUF);
+    // scales of a group of steps as [block][BM rows of a, w's block]; a block past the end has any
+    float* const scales = reinterpret_cast<float*>(lds + 2 * KG * T::BUF);
     const auto fetch_scales = [&](float (&v)[T::NS], int first) {
 #pragma unroll
         for (int i = 0; i < T::NS; ++i) {
             const int at = tid + i * T::THREADS, row = at / (KG * T::GROUP), b = at - row * (KG * T::GROUP);
             const int kb = min(first * KG + b, blocks - 1);
             const float* p = row < BM ? a_scale + (int64_t)min(m0 + row, m - 1) * blocks
-                                      : w_scale + (int64_t)min(n0 / FP8_BLOCK + row - BM, (n - 1) / FP8_BLOCK) * blocks;
+                                      : w_scale + (int64_t)(n0 / FP8_BLOCK) * blocks;
             v[i] = p[kb];
         }
     };
@@ -607,7 +589,7 @@ __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
         for (int i = 0; i < T::NS; ++i) {
             const int at = tid + i * T::THREADS, row = at / (KG * T::GROUP), b = at - row * (KG * T::GROUP);
-            if (at < T::SCALES) p[b * (BM + T::NB) + row] = v[i];
+            if (at < T::SCALES) p[b * (BM + 1) + row] = v[i];
         }
     };
 
@@ -624,45 +606,43 @@ __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu
     float acc[T::MT][T::NT][4] = {};
     float sv[T::NS];
     fetch_scales(sv, 0);
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) fetch(s, s);
+    fetch(0, 0);
     put_scales(sv, 0);
     // Row groups i = 0 .. LAST of a step, each NT products; a product is read (into its sum) one row group after it
     // began.  A step's last row group is computed after the next step's barrier, while that step's first operands are
     // on their way from LDS.
     constexpr int LAST = T::MT - 1;
-    Frag<WIDE> fa = {}, fw[T::NT] = {};
+    Frag fa = {}, fw[T::NT] = {};
     float4_t p[T::NT] = {};
     float s = 0.f, sw = 0.f, sc = 0.f;      // scales: of fa's rows, of w's block, of the products in p
     const auto sum_up = [&](int i, int j) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) acc[i][j][q] = fmaf(p[j][q], sc, acc[i][j][q]);
     };
-    int stage = 0;
     for (int step = 0; step < steps; ++step) {
         // this step has come, and every wave is done with the buffer of the one before
-        wait_loads<(STAGES - 2) * (T::NA + T::NW)>();
+        wait_loads();
         bare_barrier();
         // (no branch below these: the compiler would move the sums' updates behind it, and hold every product until there)
         if (step % T::GROUP == 0) fetch_scales(sv, step + T::GROUP);
         if (step % T::GROUP == T::GROUP / 2) put_scales(sv, step + T::GROUP / 2);
-        fetch(step + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-        const char* base = lds + (stage * KG + set) * T::BUF;
-        const float* sp = scales + (step / T::GROUP & 1) * T::SCALES + (step % T::GROUP * KG + set) * (BM + T::NB);
-        const auto read = [&](Frag<WIDE>& f, const int (&at)[2], int i) {
+        fetch(step + 1, (step + 1) & 1);
+        const char* base = lds + ((step & 1) * KG + set) * T::BUF;
+        const float* sp = scales + (step / T::GROUP & 1) * T::SCALES + (step % T::GROUP * KG + set) * (BM + 1);
+        const auto read = [&](Frag& f, const int (&at)[2], int i) {
             f.set(*reinterpret_cast<const i32x4_t*>(base + at[0] + i * 16 * FP8_BLOCK),
                   *reinterpret_cast<const i32x4_t*>(base + at[1] + i * 16 * FP8_BLOCK));
         };
-        Frag<WIDE> next;
+        Frag next;
         read(next, aa, 0);
-        const float sw_next = sp[BM + wn * (BN / WN) / FP8_BLOCK];
+        const float sw_next = sp[BM];
         sp += wm * (BM / WM) + r;
         float s_next = sp[0];
 #pragma unroll
         for (int j = 0; j < T::NT; ++j) {
             if (LAST > 0) sum_up(LAST - 1, j);
             else sum_up(0, j);
-            p[j] = Frag<WIDE>::product(fw[j], fa);
+            p[j] = Frag::product(fw[j], fa);
             read(fw[j], aw, j);
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -677,24 +657,23 @@ __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
             for (int j = 0; j < T::NT; ++j) {
                 sum_up(i ? i - 1 : LAST, j);
-                p[j] = Frag<WIDE>::product(fw[j], fa);
+                p[j] = Frag::product(fw[j], fa);
                 __builtin_amdgcn_sched_barrier(0);
             }
             sc = s * sw;
             fa = next;
             s = s_next;
         }
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
 #pragma unroll
     for (int j = 0; j < T::NT; ++j) {
         sum_up(LAST > 0 ? LAST - 1 : 0, j);
-        p[j] = Frag<WIDE>::product(fw[j], fa);
+        p[j] = Frag::product(fw[j], fa);
     }
     sc = s * sw;
 #pragma unroll
     for (int j = 0; j < T::NT; ++j) sum_up(LAST, j);
-    wait_loads<0>();                // the zeros of the steps past the end, before the buffers are used again or given back
+    wait_loads();                   // the zeros of the steps past the end, before the buffers are used again or given back
     __syncthreads();
     if constexpr (KG > 1) {
         float4_t* sums = reinterpret_cast<float4_t*>(lds);

@@ -53,10 +53,10 @@ struct GemmArgs {
     hipStream_t s;
 };
 
-template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool WIDE>
+template <int BM, int BN, int WM, int WN, int KG>
 static int launch_tile(const GemmArgs& A) {
-    typedef Fp8Tile<BM, BN, WM, WN, KG, STAGES, WIDE> T;
-    const auto kernel = fp8_gemm_tile_kernel<BM, BN, WM, WN, KG, STAGES, WIDE>;
+    typedef Fp8Tile<BM, BN, WM, WN, KG> T;
+    const auto kernel = fp8_gemm_tile_kernel<BM, BN, WM, WN, KG>;
     static std::atomic<uint64_t> ready{0};           // devices that know of the LDS size
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= MAX_DEVICES) return fail("no HIP device");
@@ -81,65 +81,47 @@ struct TileCost {
     int (*launch)(const GemmArgs&);
 };
 
-// Measured on 4096-wide k (us, this table's tile / the next one's): 16 rows x 4096
-// 5.0 / 6.5, x 12288 13.1 / 10.4; 32 x 4096 5.9 / 7.3, x 12288 14.7 / 11.8; 128 x
-// 4096 8.3 / 10.1, 256 x 4096 18.2 / 10.8; 512 x 4096 22.0 (64x64) / 15.5 / 24.5,
-// 512 x 12288 42.5 / 34.8; 1024 x 4096 28.8 / 27.3 / 52.7, 4096 x 4096 110 / 74 / 64.
-static const TileCost NARROW[] = {
-    {16, 32, 1, 0.12f, 0.12f, launch_tile<16, 32, 1, 1, 8, 2, false>},
-    {16, 64, 1, 0.20f, 0.20f, launch_tile<16, 64, 1, 2, 4, 3, false>},
-    {32, 32, 1, 0.13f, 0.13f, launch_tile<32, 32, 1, 1, 8, 2, false>},
-    {32, 64, 1, 0.19f, 0.19f, launch_tile<32, 64, 1, 2, 4, 2, false>},
-    {64, 64, 2, 0.21f, 0.42f, launch_tile<64, 64, 2, 2, 2, 2, false>},
-    {64, 128, 1, 0.37f, 0.37f, launch_tile<64, 128, 2, 2, 2, 3, false>},
-    {128, 128, 2, 0.64f, 1.05f, launch_tile<128, 128, 2, 2, 1, 2, false>},
-    {256, 256, 1, 1.90f, 1.90f, launch_tile<256, 256, 2, 4, 1, 2, false>},
-};
-// The 16-bit instruction: 32 x 4096 7.0 / 9.8; 128 x 4096 10.4 / 14.9, 256 x 4096
-// 20.1 / 15.4; 512 x 4096 28.7 / 23.7 / 40.0, 4096 x 4096 213 / 170 / 128.
-static const TileCost WIDE[] = {
-    {32, 32, 1, 0.16f, 0.16f, launch_tile<32, 32, 1, 1, 8, 2, true>},
-    {32, 64, 1, 0.24f, 0.24f, launch_tile<32, 64, 1, 2, 4, 2, true>},
-    {64, 64, 2, 0.36f, 0.80f, launch_tile<64, 64, 2, 2, 2, 2, true>},
-    {64, 128, 1, 0.63f, 0.63f, launch_tile<64, 128, 2, 2, 2, 2, true>},
-    {128, 128, 2, 1.13f, 1.95f, launch_tile<128, 128, 2, 2, 1, 2, true>},
+// Measured on 4096-wide k (us, this table's tile / the next one's): 32 rows x 4096
+// 7.0 / 9.8; 128 x 4096 10.4 / 14.9, 256 x 4096 20.1 / 15.4; 512 x 4096 28.7 (64x64)
+// / 23.7 / 40.0, 4096 x 4096 213 / 170 / 128.
+static const TileCost TILES[] = {
+    {32, 32, 1, 0.16f, 0.16f, launch_tile<32, 32, 1, 1, 8>},
+    {32, 64, 1, 0.24f, 0.24f, launch_tile<32, 64, 1, 2, 4>},
+    {64, 64, 2, 0.36f, 0.80f, launch_tile<64, 64, 2, 2, 2>},
+    {64, 128, 1, 0.63f, 0.63f, launch_tile<64, 128, 2, 2, 2>},
+    {128, 128, 2, 1.13f, 1.95f, launch_tile<128, 128, 2, 2, 1>},
 };
 
 // Rounds of workgroups, each with about 1 us that the blocks do not account for.
-static const TileCost& choose_tile(int64_t m, int64_t k, int64_t n, bool wide) {
-    const TileCost* table = wide ? WIDE : NARROW;
-    const int count = wide ? (int)(sizeof(WIDE) / sizeof(WIDE[0])) : (int)(sizeof(NARROW) / sizeof(NARROW[0]));
+static const TileCost& choose_tile(int64_t m, int64_t k, int64_t n) {
     const int64_t cus = device_cus();
     const double blocks = (double)((k + FP8_BLOCK - 1) / FP8_BLOCK);
-    const TileCost* best = table;
+    const TileCost* best = TILES;
     double least = 0;
-    for (const TileCost* t = table; t != table + count; ++t) {
-        const int64_t tiles = ((m + t->bm - 1) / t->bm) * ((n + t->bn - 1) / t->bn);
+    for (const TileCost& t : TILES) {
+        const int64_t tiles = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
         const bool one = tiles <= cus;
-        const int64_t wave = one ? cus : cus * t->resident, rounds = (tiles + wave - 1) / wave;
-        const double us = (double)rounds * (1.0 + blocks * (one ? t->one : t->full));
-        if (t == table || us < least) {
+        const int64_t wave = one ? cus : cus * t.resident, rounds = (tiles + wave - 1) / wave;
+        const double us = (double)rounds * (1.0 + blocks * (one ? t.one : t.full));
+        if (&t == TILES || us < least) {
             least = us;
-            best = t;
+            best = &t;
         }
     }
     return *best;
 }
 
-// fp32 results come from the 16-bit instruction: the 8-bit one's error, 1e-5 of the
-// result and up to 4e-4 with outlying channels, is next to a 16-bit result's
-// rounding (2e-4 fp16, 2e-3 bf16) and to the operands' own (3e-2), and far above
-// fp32's.  Few fp32 rows have a kernel without LDS tiles (us, against the
+// The kernel goes by the sizes, not by the result's type: a 16-bit result is the
+// fp32 one rounded.  Few rows have a kernel without LDS tiles (us, against the
 // smallest tile: 1 row x 4096 x 4096 4.9 / 6.1, 16 rows 7.0 / 6.2), and so has a k
 // whose rows are too long for a tile's 32-bit offsets.
 static int gemm(const GemmArgs& A) {
-    const bool wide = A.c_kind == OUT_F32;
-    if ((wide && A.m <= 8) || A.k > FP8_TILE_MAX_K) {
+    if (A.m <= 8 || A.k > FP8_TILE_MAX_K) {
         hipLaunchKernelGGL((fp8_gemm_rows_kernel<1, 8>), dim3((unsigned)((A.n + 15) / 16), (unsigned)((A.m + 15) / 16)),
                            dim3(512), 0, A.s, A.a, A.a_scale, A.m, A.k, A.w, A.w_scale, A.n, A.c, A.c_kind);
         return check_launch();
     }
-    return choose_tile(A.m, A.k, A.n, wide).launch(A);
+    return choose_tile(A.m, A.k, A.n).launch(A);
 }
 
 // Whether a linear's rows are quantized by the workgroups that multiply them.

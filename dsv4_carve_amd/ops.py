@@ -866,10 +866,8 @@ def fp8_gemm_into(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_sca
 
     a, a_scale: quantized rows [m, k] as fp8_quantize gives them; w float8_e4m3fn
     [n, k] with w_scale fp32 [ceil(n/128), ceil(k/128)]; k a multiple of 16.
-    Rows quantized once serve every matrix that reads them.  A 16-bit c comes from
-    the 8-bit matrix instruction, which drops what is below 2**-13 of the largest
-    of eight neighbouring products (1e-5 of the result on normal values, 4e-4 with
-    channels twenty times the others); an fp32 c is exact to fp32."""
+    Rows quantized once serve every matrix that reads them.  A 16-bit c is the fp32
+    one rounded."""
     _check(a.dim() == 2 and a.dtype == E4M3 and a.is_contiguous(), "a must be contiguous float8_e4m3fn [m, k]")
     m, k = a.shape
     _check_fp8_k(k)

@@ -304,10 +304,7 @@ int exl3_fp8_quantize(const void* x, int x_kind, int64_t rows, int64_t k, int po
 
 /*
  * c[i][j] = sum_b a_scale[i][b] * w_scale[j / 128][b] * sum_{t in block b} a[i][t] * w[j][t],
- * fp32 accumulation, one rounding to c_kind.  A block's inner product for a
- * 16-bit c comes from the 8-bit matrix instruction, which cuts each product to a
- * multiple of 2^-13 of the largest power of two among its eight neighbours (1e-5
- * of the result on normal values); for an fp32 c it is exact to fp32.
+ * fp32 accumulation, one rounding to c_kind.
  * a: quantized rows [m][k]; w: [n][k].
  * k a multiple of 16 up to 2^24, any n up to 2^24, any m up to 1048560.
  * a, w and c 16-byte aligned.  Needs no scratch.
@@ -317,7 +314,7 @@ int exl3_fp8_gemm(const uint8_t* a, const float* a_scale, int64_t m, int64_t k, 
 
 /*
  * exl3_fp8_gemm on exl3_fp8_quantize(x) (scales a / 448), for a few rows in one
- * launch (products then exact to fp32 for every c_kind).  x 16-byte aligned.
+ * launch.  x 16-byte aligned.
  * scratch: >= exl3_fp8_linear_scratch_bytes(m, k, n) bytes, 16-byte aligned, no
  * zeroing needed (where the size is 0 it may be null); one call at a time per
  * scratch buffer.

@@ -166,6 +166,44 @@ def test_gemm_writes_its_rows_only_and_keeps_nan_in_them(dev, m, k, n):
     assert torch.equal(torch.isnan(c), bad) and torch.equal(c[~bad], plain[~bad])
 
 
+@pytest.mark.parametrize("m,k,n", [(5, 4368, 330), (20, 9552, 500), (50, 9552, 4084), (60, 4784, 5002), (120, 9232, 4084),
+                                   (250, 4368, 4090), (120, 4784, 8000), (500, 4368, 4084), (1000, 2320, 4090),
+                                   (4000, 2320, 4090)])
+def test_gemm_long_rows_of_every_tile(dev, m, k, n):
+    """More than two groups of staged scales for every tile shape, their number no multiple of a group, a ragged last
+    block, scales far apart: the fp32 result against the reference, a 16-bit one against its rounding."""
+    gen = gen_of(dev, m + k)
+    a, sa = rows_of(gen, m, k)
+    w, sw = R.matrix(gen, n, k)
+    sw = sw * torch.exp2(torch.randint(-6, 7, sw.shape, generator=gen, device=dev).float())
+    c = ops.fp8_gemm(a, sa, w, sw, out_dtype=torch.float32)
+    ref, tol = R.gemm(a, sa, w, sw, torch.float32)
+    within(c, ref, tol, f"{m}x{k}x{n}")
+    # Partial sums of terms of either sign are no larger than the whole in the mean, and their roundings (one step at
+    # most each) no more alike than the terms: the 2-norm grows with the root of their number.
+    assert torch.linalg.norm(c.double() - ref) <= torch.linalg.norm(ref) * R.steps(k) ** 0.5 * R.U
+    for dtype in (torch.float16, torch.bfloat16):
+        s = 2.0 ** -8 if dtype is torch.float16 else 1.0          # into fp16's range
+        assert torch.equal(ops.fp8_gemm(a, sa * s, w, sw, out_dtype=dtype), (c * s).to(dtype))
+
+
+@pytest.mark.parametrize("m", [1, 3, 8, 9, 16, 40, 77, 300])
+@pytest.mark.parametrize("wide", [1.0, 20.0])
+def test_16_bit_results_are_the_fp32_sum_rounded_once(dev, m, wide):
+    """Whatever the row count, with and without channels that stand out."""
+    gen = gen_of(dev, m)
+    x = torch.randn((m, 1024), generator=gen, device=dev)
+    x[:, torch.rand(1024, generator=gen, device=dev) < 0.005] *= wide
+    x = x.to(torch.bfloat16)
+    w, sw = R.matrix(gen, 512, 1024)
+    sw = sw * 2.0 ** -8
+    a, sa = ops.fp8_quantize(x)
+    for dtype in (torch.float16, torch.bfloat16):
+        assert torch.equal(ops.fp8_gemm(a, sa, w, sw, out_dtype=dtype),
+                           ops.fp8_gemm(a, sa, w, sw, out_dtype=torch.float32).to(dtype))
+        assert torch.equal(ops.fp8_linear(x, w, sw, out_dtype=dtype), ops.fp8_linear(x, w, sw, out_dtype=torch.float32).to(dtype))
+
+
 def test_gemm_is_repeatable(dev):
     gen = gen_of(dev, 9)
     for m in (1, 20, 100, 700):
