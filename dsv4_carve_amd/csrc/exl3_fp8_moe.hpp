@@ -7,12 +7,10 @@
 // Activations are not quantized: at a few rows the layer reads weights, and
 // rounding activations to 8 bits would cost accuracy for nothing.  The e4m3
 // weights are widened (exactly) to the type of x for the first product, and to
-// bf16 for the second, whose activation is the sum of two bf16 values (its
-// rounding and the rounding of what that leaves, 2^-17 of it, and no overflow):
-// four instructions more a block, which the weights' traffic hides, and the
-// output's rounding is the only one that counts.  Sums are fp32: a block of 128
-// is four 16x16x32 instructions (eight) into a cleared accumulator, scaled into
-// the running sum by one multiply-add a value.
+// bf16 for the second, whose activation is fp32: 24 bits, the sum of three bf16
+// values, each its highest 8 bits left (exact, and no overflow).  Sums are fp32: a
+// block of 128 is four 16x16x32 instructions (twelve) into a cleared accumulator,
+// scaled into the running sum by one multiply-add a value.
 //
 // Routing is read in each workgroup, lane r of a wave holding row r (64 rows at
 // most).  A row that names an expert more than once counts as its first slot,
@@ -38,7 +36,7 @@ struct Fp8MoeArgs {
     const float* s13;           // [E][2 I / 128][hidden / 128]
     const uint8_t* w2;          // [E][hidden][I]
     const float* s2;            // [E][hidden / 128][I / 128]
-    uint16_t* act;              // [rows * topk][I / 16][2][16]: 16 activations as bf16, then what that leaves of them
+    float* act;                 // [rows * topk][I]
     void* out;                  // [rows][hidden]
     Route rt;
     int out_kind, rows, hidden, inter, E, topk;
@@ -161,25 +159,36 @@ __global__ __launch_bounds__(FP8_GU_WAVES * 64) void fp8_moe_gate_up_kernel(cons
                 }
             const int col = c0 + 16 * t + r, cs = __shfl(col_slot, col & 63);
             if (col >= cnt || (!MT && r >= COLS)) continue;
-            float act[4], rest[4];
+            float4_t act;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 // comparisons, not fminf: a NaN stays one
                 const float gv = gs[i] > A.limit ? A.limit : gs[i];
                 const float uv = us[i] > A.limit ? A.limit : us[i] < -A.limit ? -A.limit : us[i];
                 act[i] = gv / (1.0f + expf(-gv)) * uv;
-                const float top = (float)(__bf16)act[i];
-                rest[i] = fabsf(top) < __builtin_inff() ? act[i] - top : 0.f;
             }
-            uint16_t* p = A.act + 2 * ((int64_t)cs * I + n0) + 4 * g;
-            *reinterpret_cast<u32x2_t*>(p) = u32x2_t{pack_bf16(act[0], act[1]), pack_bf16(act[2], act[3])};
-            *reinterpret_cast<u32x2_t*>(p + 16) =
-                u32x2_t{pack_bf16(rest[0], rest[1]), pack_bf16(rest[2], rest[3])};
+            *reinterpret_cast<float4_t*>(A.act + (int64_t)cs * I + n0 + 4 * g) = act;
         }
     }
 }
 
 constexpr int FP8_DOWN_WAVES = 16;
+
+// Four fp32 values as three planes of bf16: their upper halves, those of what that leaves, and the 8 bits left then.
+__device__ __forceinline__ void split_bf16(const float4_t& v, u32x2_t (&plane)[3]) {
+    float4_t rest = v;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u[i] = __float_as_uint(rest[i]);
+            const float top = __uint_as_float(u[i] & 0xffff0000u);
+            rest[i] = p == 0 && fabsf(top) == __builtin_inff() ? 0.f : rest[i] - top;      // an infinity leaves nothing
+        }
+        plane[p] = u32x2_t{__builtin_amdgcn_perm(u[1], u[0], 0x07060302), __builtin_amdgcn_perm(u[3], u[2], 0x07060302)};
+    }
+}
 
 // down: a workgroup has 16 outputs of every row and goes through all active
 // experts, in the order of their first slots; a column of the matrix
@@ -219,7 +228,9 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
     __shared__ uint16_t first_of[FP8_MOE_MAX_SLOTS];                         // an expert's first entry
     __shared__ int wave_n[2][WAVES];
     __shared__ __attribute__((aligned(16))) float part[WAVES][TILES * 4][64];
-    __shared__ i32x4_t columns[WAVES][LOADS * 64];       // a wave's inputs of one block, 512 bytes a row
+    // a wave's inputs of one block: a row is three planes of 256 bytes, and 16 more, so that rows lie in different banks
+    constexpr int COLUMN = 3 * 256 + 16;
+    __shared__ __attribute__((aligned(16))) char columns[WAVES][2 * LOADS * COLUMN];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = lane & 15, g = lane >> 4;
     const int S = A.rows * A.topk;
@@ -348,7 +359,7 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
         float sc;
     };
     struct Inputs {
-        i32x4_t v[LOADS];
+        float4_t v[LOADS];
         float wt;
         int col, t;                // this lane's row's: which of the group's (-1: none), which 16 of the batch
     };
@@ -376,27 +387,31 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int slot = entries[first + min(2 * i + (lane >> 5), last)].slot;
-            u.v[i] = reinterpret_cast<const i32x4_t*>(A.act + 2 * ((int64_t)slot * I + kb * FP8_BLOCK))[lane & 31];
+            u.v[i] = reinterpret_cast<const float4_t*>(A.act + (int64_t)slot * I + kb * FP8_BLOCK)[lane & 31];
         }
     };
     float acc[TILES][4] = {};
     const auto compute = [&](const Weights& u, const Inputs& x) {
         __builtin_amdgcn_wave_barrier();              // the wave's own place: its LDS operations are in order
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) columns[wave][64 * i + lane] = x.v[i];
+        for (int i = 0; i < LOADS; ++i) {
+            u32x2_t plane[3];
+            split_bf16(x.v[i], plane);
+            char* at = columns[wave] + (2 * i + (lane >> 5)) * COLUMN + (lane & 31) * 8;
+#pragma unroll
+            for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x2_t*>(at + 256 * q) = plane[q];
+        }
         __builtin_amdgcn_wave_barrier();
         const bool has = x.col >= 0;                  // the other columns are no row's: any inputs do
-        const i32x4_t* col = columns[wave] + (has ? x.col : 0) * 32 + 4 * g;
-        BlockX<H> in[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)                   // chunks g and g + 4 of 16: two of 8 values, two of what they leave
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                in[0].v[2 * i + h] = __builtin_bit_cast(H::vec8, col[16 * i + h]);
-                in[1].v[2 * i + h] = __builtin_bit_cast(H::vec8, col[16 * i + 2 + h]);
-            }
+        const char* col = columns[wave] + (has ? x.col : 0) * COLUMN;
         const BlockW<H> w(u.w);
-        const float4_t p = block_product<H>(w, in[0], block_product<H>(w, in[1]));
+        float4_t p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 2; q >= 0; --q) {                // the smallest first
+            BlockX<H> in;
+            in.load(reinterpret_cast<const uint16_t*>(col + 256 * q), g);
+            p = block_product<H>(w, in, p);
+        }
         const float s = x.wt * u.sc;
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {

@@ -38,7 +38,7 @@ int exl3_fp8_moe(const void* x, int x_kind, void* out, int out_kind, int64_t row
     if (scratch_bytes < need) return fail("scratch too small");
     if (!aligned16(x) || !aligned16(out) || !aligned16(w13) || !aligned16(w2) || !aligned16(scratch))
         return fail("x, out, w13, w2 and scratch must be 16-byte aligned");
-    Fp8MoeArgs A{x, w13, w13_scale, w2, w2_scale, static_cast<uint16_t*>(scratch), out, Route{}, out_kind, (int)rows,
+    Fp8MoeArgs A{x, w13, w13_scale, w2, w2_scale, static_cast<float*>(scratch), out, Route{}, out_kind, (int)rows,
                  (int)hidden, (int)intermediate, (int)n_experts, (int)topk, swiglu_limit};
     if (make_route(topk_ids, ids_kind, topk_weights, weights_kind, expert_map, n_global, A.rt)) return -1;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);

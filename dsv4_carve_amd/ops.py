@@ -931,8 +931,8 @@ def fp8_moe(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: tor
     block; hidden and inter multiples of 128.  expert_ids, routing_weights and
     expert_map as moe_decode takes them (moe_route makes the first two); an id that
     no expert here has (-1 among them) contributes nothing.  With `swiglu_limit` L
-    the gate is capped at L and the up projection to [-L, L].  Sums are fp32, and
-    the activation between the two products keeps 16 bits and fp32's range."""
+    the gate is capped at L and the up projection to [-L, L].  Sums and the
+    activation between the two products are fp32."""
     _check(x.is_cuda and x.dtype in X_KIND, "input must be HIP fp16 or bf16")
     _check(x.dim() == 2 and x.is_contiguous(), "input must be contiguous [m, hidden]")
     m, hidden = x.shape

@@ -445,6 +445,36 @@ def test_moe_small_and_large_inputs(dev, dtype):
     check_moe((x * 64).to(dtype), (mats[0], mats[1] * 64, mats[2], mats[3]), ids, wts, out=out)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,experts,topk", [(1, 4, 3), (5, 16, 2), (20, 3, 2), (40, 64, 2), (64, 4, 3)])
+def test_moe_activation_is_fp32(dev, dtype, rows, experts, topk):
+    """One input and one value of each down row other than zero: the output is a sum of the activations themselves."""
+    gen = gen_of(dev, rows)
+    n = 256
+    w13, s13 = R.matrix(gen, experts, 2 * n, n)
+    w13 = (w13.float() / 448).clamp(-1, 1).to(R.E4M3)
+    s13 = s13 * 64
+    w2 = torch.eye(n, device=dev).expand(experts, n, n).contiguous().to(R.E4M3)
+    s2 = torch.ones((experts, 2, 2), device=dev)
+    x = torch.zeros((rows, n), dtype=dtype, device=dev)
+    at = torch.randint(0, n, (rows,), generator=gen, device=dev)
+    x[torch.arange(rows, device=dev), at] = (torch.rand(rows, generator=gen, device=dev) * 4 + 0.5).to(dtype)
+    ids = torch.rand((rows, experts), generator=gen, device=dev).argsort(1)[:, :topk].contiguous()
+    wts = torch.ones((rows, topk), device=dev)
+    out = ops.fp8_moe(x, w13, s13, w2, s2, ids, wts, swiglu_limit=8.0, out=torch.empty((rows, n), device=dev))
+    ref, tol = torch.zeros((rows, n), dtype=torch.float64, device=dev), 0.0
+    full = R.weight(w13, s13)
+    for j in range(topk):
+        h = (full[ids[:, j]] @ x.double().unsqueeze(2)).squeeze(2)
+        g, u = h[:, :n].clamp(max=8.0), h[:, n:].clamp(-8.0, 8.0)
+        act = g * torch.sigmoid(g) * u
+        ref += act
+        # half steps: a rounding each of g (which silu's slope makes 1 + |g| of at most), u, 1 + e^-g, the quotient, the
+        # product, the scaled sum and the joined one, four of the exponential
+        tol = tol + act.abs() * (11 + g.abs()) * 2.0 ** -24
+    within(out, ref, tol + 2.0 ** -126, "act")
+
+
 @pytest.mark.parametrize("rows,experts,topk", [(16, 64, 4), (31, 64, 3), (64, 64, 3), (64, 9, 2)])
 def test_moe_crowded_expert(dev, rows, experts, topk):
     """One expert that every row names, more rows than are taken at once, among experts of few rows."""
