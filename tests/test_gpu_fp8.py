@@ -306,6 +306,18 @@ def test_route(dev, scoring, biased, rows, experts, topk):
         check_route(logits, topk, scoring, bias, renormalize=False, scale=2.5, ids_dtype=torch.int64)
 
 
+@pytest.mark.parametrize("rows,experts,topk", [(40, 64, 8), (40, 300, 8), (200, 2048, 16)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_route_softmax_over_the_row_is_64_bit(dev, rows, experts, topk, biased):
+    gen = gen_of(dev, experts)
+    bias = torch.randn(experts, generator=gen, device=dev) * 0.1 if biased else None
+    logits = torch.randn((rows, experts), generator=gen, device=dev) * 3
+    ids, wts = ops.moe_route(logits, topk, bias=bias, renormalize=False)
+    want_ids, want = R.route(logits, topk, "softmax", bias, False, 1.0)
+    assert torch.equal(ids.long(), want_ids)
+    assert ((wts.double() - want).abs() <= want * 2.0 ** -24 * 1.001 + 2.0 ** -150).all()     # one rounding
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid", "sqrtsoftplus"])
 def test_route_ties_and_near_ties(dev, scoring):
     """Equal logits go by index; scores that fp32 cannot tell apart go by their exact order."""
