@@ -572,7 +572,8 @@ __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu
             for (int i = 0; i < T::NW; ++i) load_to_lds(tw, dst + (BM + i * ROWS) * FP8_BLOCK, in ? ow[i] : OUTSIDE, at);
         }
     };
-    // scales of a group of steps as [block][BM rows of a, w's block]; a block past the end has any
+    // scales of a group of steps as [block][BM rows of a, w's block]; a block past the end has zeros, not a neighbour's
+    // value: that may be infinite
     float* const scales = reinterpret_cast<float*>(lds + 2 * KG * T::BUF);
     const auto fetch_scales = [&](float (&v)[T::NS], int first) {
 #pragma unroll
@@ -589,7 +590,7 @@ __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
         for (int i = 0; i < T::NS; ++i) {
             const int at = tid + i * T::THREADS, row = at / (KG * T::GROUP), b = at - row * (KG * T::GROUP);
-            if (at < T::SCALES) p[b * (BM + 1) + row] = v[i];
+            if (at < T::SCALES) p[b * (BM + 1) + row] = first * KG + b < blocks ? v[i] : 0.f;
         }
     };
 

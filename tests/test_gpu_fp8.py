@@ -204,6 +204,22 @@ def test_16_bit_results_are_the_fp32_sum_rounded_once(dev, m, wide):
         assert torch.equal(ops.fp8_linear(x, w, sw, out_dtype=dtype), ops.fp8_linear(x, w, sw, out_dtype=torch.float32).to(dtype))
 
 
+@pytest.mark.parametrize("m", [3, 20, 50, 100, 300])
+@pytest.mark.parametrize("out", TYPES)
+def test_gemm_infinite_scales(dev, m, out):
+    """An infinite scale makes its products infinite, none of them a NaN, wherever the blocks of k end."""
+    gen = gen_of(dev, m)
+    for k in (272, 640):
+        a, w = (torch.randint(0x30, 0x40, s, generator=gen, device=dev, dtype=torch.uint8).view(R.E4M3) for s in ((m, k), (200, k)))
+        sa, sw = torch.ones((m, -(-k // 128)), device=dev), torch.ones((2, -(-k // 128)), device=dev)
+        good = ops.fp8_gemm(a, sa, w, sw, out_dtype=out)
+        sa[1, -1], sw[1, -1] = torch.inf, torch.inf
+        c = ops.fp8_gemm(a, sa, w, sw, out_dtype=out)
+        assert (c[1] == torch.inf).all() and (c[:, 128:] == torch.inf).all()
+        keep = [r for r in range(m) if r != 1]
+        assert torch.equal(c[keep, :128], good[keep, :128])
+
+
 def test_gemm_is_repeatable(dev):
     gen = gen_of(dev, 9)
     for m in (1, 20, 100, 700):
