@@ -28,6 +28,9 @@ inline int check_launch() {
     return 0;
 }
 
+// HIP takes fewer than 2^32 threads along a grid's dimension: workgroups of 256 and fewer.
+constexpr int64_t MAX_GRID = (1 << 24) - 1;
+
 inline int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 constexpr int MAX_DEVICES = 64;

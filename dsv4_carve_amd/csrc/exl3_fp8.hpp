@@ -198,17 +198,9 @@ template <int K, bool POW2>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const void* __restrict__ x, int64_t rows, int k, int groups,
                                                            uint8_t* __restrict__ q, float* __restrict__ scale) {
     const uint32_t chunks = (uint32_t)groups * 8;
-    int64_t row;
-    int c;
-    if (gridDim.x < 1u << 24) {         // a division in 32 bits is a quarter of one in 64
-        const uint32_t t = blockIdx.x * 256 + threadIdx.x;
-        row = t / chunks;
-        c = (int)(t - (uint32_t)row * chunks);
-    } else {
-        const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-        row = t / chunks;
-        c = (int)(t - row * chunks);
-    }
+    const uint32_t t = blockIdx.x * 256 + threadIdx.x, in_rows = t / chunks;        // fewer than 2^32 threads a launch
+    const int64_t row = in_rows;
+    const int c = (int)(t - in_rows * chunks);
     const bool in = row < rows && c * 16 < k;
     float v[16];
     float most = 0.f;

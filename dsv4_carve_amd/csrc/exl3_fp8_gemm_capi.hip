@@ -13,21 +13,22 @@ static int check_blocks(int64_t m, int64_t k, int64_t n) {
     return 0;
 }
 
+// As many launches as the rows need: one takes MAX_GRID workgroups of 32 groups, or of 4.
 template <int K>
 static int launch_quantize(const void* x, int64_t rows, int k, int groups, bool pow2, uint8_t* q, float* scale,
                            hipStream_t s) {
     const bool chunks = k % 16 == 0 && aligned16(x) && aligned16(q);
-    const int64_t blocks = chunks ? (rows * groups * 8 + 255) / 256 : (rows * groups + 3) / 4;
-    if (blocks > 0x7fffffffLL) return fail("too many values");
-    const dim3 grid((unsigned)blocks), block(256);
-    if (chunks) {
-        if (pow2) hipLaunchKernelGGL((fp8_quantize_kernel<K, true>), grid, block, 0, s, x, rows, k, groups, q, scale);
-        else hipLaunchKernelGGL((fp8_quantize_kernel<K, false>), grid, block, 0, s, x, rows, k, groups, q, scale);
-    } else {
-        if (pow2) hipLaunchKernelGGL((fp8_quantize_any_kernel<K, true>), grid, block, 0, s, x, rows, k, groups, q, scale);
-        else hipLaunchKernelGGL((fp8_quantize_any_kernel<K, false>), grid, block, 0, s, x, rows, k, groups, q, scale);
+    const auto kernel = chunks ? (pow2 ? fp8_quantize_kernel<K, true> : fp8_quantize_kernel<K, false>)
+                               : (pow2 ? fp8_quantize_any_kernel<K, true> : fp8_quantize_any_kernel<K, false>);
+    const int64_t per = chunks ? 32 : 4, most = MAX_GRID * per / groups;
+    for (int64_t at = 0; at < rows; at += most) {
+        const int64_t here = rows - at < most ? rows - at : most;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((here * groups + per - 1) / per)), dim3(256), 0, s,
+                           static_cast<const char*>(x) + at * k * (K == OUT_F32 ? 4 : 2), here, k, groups, q + at * k,
+                           scale + at * groups);
+        if (check_launch()) return -1;
     }
-    return check_launch();
+    return 0;
 }
 
 static int quantize(const void* x, int x_kind, int64_t rows, int64_t k, bool pow2, uint8_t* q, float* scale,
@@ -67,7 +68,7 @@ static int launch_tile(const GemmArgs& A) {
         ready.fetch_or(1ull << dev);
     }
     const int64_t tm = (A.m + BM - 1) / BM, tn = (A.n + BN - 1) / BN;
-    if (tm * tn > 0x7fffffffLL) return fail("too many tiles");
+    if (tm * tn * T::THREADS > 0xffffffffLL) return fail("too many tiles");
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(T::THREADS), T::LDS, A.s, A.a, A.a_scale, (int)A.m, A.k,
                        A.w, A.w_scale, A.n, A.c, A.c_kind, (int)tm, (int)tn);
     return check_launch();

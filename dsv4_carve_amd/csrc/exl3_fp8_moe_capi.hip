@@ -80,14 +80,20 @@ int exl3_moe_route(const void* logits, int logits_kind, int64_t rows, int64_t n_
         return fail("rows must be positive and n_experts in 1..2048");
     if (topk < 1 || topk > ROUTE_MAX_TOPK || topk > n_experts) return fail("topk must be in 1..min(64, n_experts)");
     if (!std::isfinite(scale)) return fail("scale must be finite");
-    if (rows > 4 * 0x7fffffffLL) return fail("too many rows");
-    const int64_t blocks = (rows + 3) / 4;
-    const RouteArgs A{logits, bias, ids, weights, rows, logits_kind, (int)n_experts, (int)topk, scoring,
-                      ids_kind == IDS_I64, renormalize != 0, scale};
+    if (rows > (int64_t)1 << 36) return fail("too many rows");
     const int per_lane = (int)(n_experts + 63) / 64;
-    const auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), A);
-        return check_launch();
+    const auto launch = [&](auto kernel) {        // as often as the rows need: a workgroup has four
+        for (int64_t at = 0; at < rows; at += 4 * MAX_GRID) {
+            const int64_t here = rows - at < 4 * MAX_GRID ? rows - at : 4 * MAX_GRID;
+            const RouteArgs A{static_cast<const char*>(logits) + at * n_experts * (logits_kind == OUT_F32 ? 4 : 2), bias,
+                              static_cast<char*>(ids) + at * topk * (ids_kind == IDS_I64 ? 8 : 4), weights + at * topk,
+                              here, logits_kind, (int)n_experts, (int)topk, scoring, ids_kind == IDS_I64,
+                              renormalize != 0, scale};
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((here + 3) / 4)), dim3(256), 0,
+                               reinterpret_cast<hipStream_t>(stream), A);
+            if (check_launch()) return -1;
+        }
+        return 0;
     };
     if (per_lane <= 1) return launch(moe_route_kernel<1>);
     if (per_lane <= 2) return launch(moe_route_kernel<2>);

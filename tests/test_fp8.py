@@ -142,3 +142,7 @@ def test_route_argument_errors_without_device(change, msg):
     a = {"logits": P, "kind": 2, "rows": 3, "E": 8, "topk": 2, "scoring": 0, "scale": 1.0, "ids": 0, **change}
     refused(_lib.load().exl3_moe_route(a["logits"], a["kind"], a["rows"], a["E"], a["topk"], a["scoring"], None, 1,
                                        a["scale"], P, a["ids"], P, None), msg)
+
+
+def test_route_refuses_rows_past_any_memory():
+    refused(_lib.load().exl3_moe_route(P, 1, (1 << 36) + 1, 1, 1, 0, None, 1, 1.0, P, 0, P, None), "too many rows")

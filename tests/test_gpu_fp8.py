@@ -110,6 +110,23 @@ def test_quantize_empty_leading_dims_and_unaligned(dev):
     check_quantized(flat, *ops.fp8_quantize(flat), False)
 
 
+@pytest.mark.parametrize("rows,k", [((1 << 26) + 6, 1), ((1 << 25) + 9, 130), ((1 << 29) + 40, 16)])
+def test_quantize_more_rows_than_a_launch_takes(dev, rows, k):
+    """Rows on either side of a launch's last one, and the last rows, are as in a call of their own."""
+    gen = gen_of(dev, k)
+    x = torch.empty((rows, k), dtype=torch.int16, device=dev)
+    for part in x.split(1 << 24):
+        part.random_(0, 0x7f00, generator=gen)
+    x = x.view(torch.bfloat16)
+    q, s = ops.fp8_quantize(x)
+    a_launch = ((1 << 24) - 1) * (32 if k % 16 == 0 else 4) // s.shape[1]
+    assert rows > a_launch
+    for at in (0, a_launch - 5, a_launch, rows - 37):
+        at = min(at, rows - 37)
+        want_q, want_s = ops.fp8_quantize(x[at:at + 37].clone())
+        assert torch.equal(q[at:at + 37].view(torch.uint8), want_q.view(torch.uint8)) and torch.equal(s[at:at + 37], want_s)
+
+
 # ---------------------------------------------------------------- product
 
 
@@ -359,6 +376,17 @@ def test_route_scores_that_a_bias_takes_back(dev):
             check_route(logits[row:row + 10].contiguous(), 2, "sqrtsoftplus", bias)
             check_route(logits[row:row + 10].contiguous(), 6, "sqrtsoftplus", bias + torch.randint(
                 -8, 8, (6,), generator=gen, device=dev) * 2.0 ** -16)
+
+
+@pytest.mark.parametrize("ids_dtype", [torch.int32, torch.int64])
+def test_route_more_rows_than_a_launch_takes(dev, ids_dtype):
+    rows = (1 << 26) + 5
+    logits = torch.empty((rows, 2), dtype=torch.bfloat16, device=dev).normal_(generator=gen_of(dev, 7))
+    ids, wts = ops.moe_route(logits, 1, scoring="sigmoid", renormalize=False, ids_dtype=ids_dtype)
+    assert torch.equal(ids[:, 0], (logits[:, 1] > logits[:, 0]).to(ids_dtype))
+    for at in (0, 4 * ((1 << 24) - 1) - 9, rows - 20):
+        want = R.route(logits[at:at + 20], 1, "sigmoid", None, False, 1.0)[1]
+        assert ((wts[at:at + 20].double() - want).abs() <= want * 2.0 ** -24 * 1.001).all()
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid", "sqrtsoftplus"])
