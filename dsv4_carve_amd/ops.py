@@ -892,7 +892,9 @@ def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: t
 
 @functools.lru_cache(maxsize=4096)
 def _fp8_linear_scratch_bytes(device_index: int, m: int, k: int, n: int) -> int:
-    return int(_lib.check(_lib.load().exl3_fp8_linear_scratch_bytes(m, k, n)))
+    """What a call on that device needs: the library goes by the current one."""
+    with torch.cuda.device(device_index):
+        return int(_lib.check(_lib.load().exl3_fp8_linear_scratch_bytes(m, k, n)))
 
 
 def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,

@@ -315,9 +315,9 @@ int exl3_fp8_gemm(const uint8_t* a, const float* a_scale, int64_t m, int64_t k, 
 /*
  * exl3_fp8_gemm on exl3_fp8_quantize(x) (scales a / 448), for a few rows in one
  * launch.  x 16-byte aligned.
- * scratch: >= exl3_fp8_linear_scratch_bytes(m, k, n) bytes, 16-byte aligned, no
- * zeroing needed (where the size is 0 it may be null); one call at a time per
- * scratch buffer.
+ * scratch: >= exl3_fp8_linear_scratch_bytes(m, k, n) bytes, asked for with the
+ * call's device current, 16-byte aligned, no zeroing needed (where the size is 0
+ * it may be null); one call at a time per scratch buffer.
  */
 int64_t exl3_fp8_linear_scratch_bytes(int64_t m, int64_t k, int64_t n);
 int exl3_fp8_linear(const void* x, int x_kind, int64_t m, int64_t k, const uint8_t* w, const float* w_scale,

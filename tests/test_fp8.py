@@ -110,6 +110,31 @@ def test_linear_scratch_is_checked():
     refused(L.exl3_fp8_linear_scratch_bytes(5, 40, 64), "multiple of 16")
 
 
+def test_linear_scratch_goes_by_the_calls_device(monkeypatch):
+    """Whether a call needs scratch depends on the number of CUs: that of its own device, whichever is current."""
+    current = [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *_):
+            current.pop()
+
+    class Lib:
+        def exl3_fp8_linear_scratch_bytes(self, m, k, n):
+            return 1000 + current[-1]
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_lib, "load", Lib)
+    ops._fp8_linear_scratch_bytes.cache_clear()
+    assert [ops._fp8_linear_scratch_bytes(i, 2, 256, 64) for i in (1, 0, 1)] == [1001, 1000, 1001]
+    ops._fp8_linear_scratch_bytes.cache_clear()
+
+
 MOE = {"x": P, "x_kind": 1, "out_kind": 1, "rows": 2, "hidden": 256, "inter": 128, "E": 4, "topk": 2, "ids_kind": 0,
        "w_kind": 2, "emap": None, "n_global": 0, "limit": 1.0, "scratch": P, "bytes": 1 << 20}
 
