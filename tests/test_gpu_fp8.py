@@ -300,6 +300,21 @@ def test_linear_is_quantize_then_gemm(dev, dtype, rows, k, n):
     assert torch.equal(ops.fp8_linear(x3, w, sw)[0], ops.fp8_linear(x, w, sw))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,k", [(1, 7168), (2, 7168), (1, 12288), (2, 12288), (1, 4224), (1, 8208)])
+def test_linear_long_rows(dev, dtype, rows, k):
+    """More blocks than a wave has on their way at once."""
+    gen = gen_of(dev, rows + k)
+    x = normal(gen, rows, k, dtype=dtype)
+    w, sw = R.matrix(gen, 84, k)
+    sw = sw * torch.exp2(torch.randint(-3, 4, sw.shape, generator=gen, device=dev).float()) * 2.0 ** -6
+    q, s = ops.fp8_quantize(x)
+    y = ops.fp8_linear(x, w, sw, out_dtype=torch.float32)
+    ref, tol = R.gemm(q, s, w, sw, torch.float32)
+    within(y, ref, tol, f"{rows}x{k}")
+    assert torch.equal(ops.fp8_linear(x, w, sw, out_dtype=torch.bfloat16), y.to(torch.bfloat16))
+
+
 @pytest.mark.parametrize("rows", [1, 4, 12])
 def test_linear_nan_infinity_and_zero_rows(dev, rows):
     gen = gen_of(dev, 6)
