@@ -866,8 +866,9 @@ def fp8_gemm_into(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_sca
 
     a, a_scale: quantized rows [m, k] as fp8_quantize gives them; w float8_e4m3fn
     [n, k] with w_scale fp32 [ceil(n/128), ceil(k/128)]; k a multiple of 16.
-    Rows quantized once serve every matrix that reads them.  A 16-bit c is the fp32
-    one rounded."""
+    At most 1048560 rows; a, w and c begin on 16-byte borders (whole tensors do, a
+    slice may not and is refused then).  Rows quantized once serve every matrix that
+    reads them.  A 16-bit c is the fp32 one rounded."""
     _check(a.dim() == 2 and a.dtype == E4M3 and a.is_contiguous(), "a must be contiguous float8_e4m3fn [m, k]")
     m, k = a.shape
     _check_fp8_k(k)
@@ -900,8 +901,8 @@ def _fp8_linear_scratch_bytes(device_index: int, m: int, k: int, n: int) -> int:
 def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """y [..., n] = x [..., k] through a block-scaled matrix: fp8_gemm(*fp8_quantize(x), w, w_scale), x fp16, bf16
-    or fp32; y in x's dtype unless given.  A few rows take one launch.  Its scratch is the call's own
-    (stream-ordered, capturable)."""
+    or fp32; y in x's dtype unless given.  At most 1048560 rows; w begins on a 16-byte border.  A few rows take one
+    launch.  Its scratch is the call's own (stream-ordered, capturable)."""
     _check(x.dim() >= 1 and x.dtype in OUT_KIND and x.is_contiguous(), "x must be contiguous fp16, bf16 or fp32 [..., k]")
     k = x.shape[-1]
     _check_fp8_k(k)
@@ -934,7 +935,8 @@ def fp8_moe(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: tor
     expert_map as moe_decode takes them (moe_route makes the first two); an id that
     no expert here has (-1 among them) contributes nothing.  With `swiglu_limit` L
     the gate is capped at L and the up projection to [-L, L].  Sums and the
-    activation between the two products are fp32."""
+    activation between the two products are fp32.  w13, w2 and an `out` given begin
+    on 16-byte borders."""
     _check(x.is_cuda and x.dtype in X_KIND, "input must be HIP fp16 or bf16")
     _check(x.dim() == 2 and x.is_contiguous(), "input must be contiguous [m, hidden]")
     m, hidden = x.shape

@@ -306,7 +306,8 @@ int exl3_fp8_quantize(const void* x, int x_kind, int64_t rows, int64_t k, int po
  * c[i][j] = sum_b a_scale[i][b] * w_scale[j / 128][b] * sum_{t in block b} a[i][t] * w[j][t],
  * fp32 accumulation, one rounding to c_kind.
  * a: quantized rows [m][k]; w: [n][k].
- * k a multiple of 16 up to 2^24, any n up to 2^24, any m up to 1048560.
+ * k a multiple of 16 up to 2^24, any n up to 2^24, any m up to 1048560.  The
+ * product of two scales is taken in fp32, and loses bits below its normal range.
  * a, w and c 16-byte aligned.  Needs no scratch.
  */
 int exl3_fp8_gemm(const uint8_t* a, const float* a_scale, int64_t m, int64_t k, const uint8_t* w,

@@ -574,6 +574,25 @@ def test_unaligned_inputs_and_own_output(dev):
         assert ops.fp8_moe(y, *mats, ids, wts, out=y) is y and torch.equal(y, want)
 
 
+def test_unaligned_matrices_and_outputs_are_refused(dev):
+    """What a kernel reads or writes by 16 bytes and is too large to copy for a call."""
+    off = lambda t: torch.cat([t.flatten().view(torch.uint8)[:8], t.flatten().view(torch.uint8)])[8:].view(t.dtype).view(t.shape)  # noqa: E731
+    gen = gen_of(dev, 22)
+    w, sw = R.matrix(gen, 64, 256)
+    a, sa = rows_of(gen, 20, 256)
+    x = normal(gen, 20, 256, spread=False)
+    mats = layer(gen, 4, 256, 128)
+    ids, wts = routed(gen, 20, 4, 2)
+    c = torch.empty((20, 64), dtype=torch.bfloat16, device=dev)
+    for call in (lambda: ops.fp8_gemm(off(a), sa, w, sw), lambda: ops.fp8_gemm(a, sa, off(w), sw),
+                 lambda: ops.fp8_gemm_into(a, sa, w, sw, off(c)), lambda: ops.fp8_linear(x, off(w), sw),
+                 lambda: ops.fp8_moe(x, off(mats[0]), *mats[1:], ids, wts),
+                 lambda: ops.fp8_moe(x, *mats[:2], off(mats[2]), mats[3], ids, wts),
+                 lambda: ops.fp8_moe(x, *mats, ids, wts, out=off(x))):
+        with pytest.raises(RuntimeError, match="16-byte aligned"):
+            call()
+
+
 def test_moe_rows_are_apart(dev):
     """NaN and infinities of a row, or of an expert that only it names, stay in it."""
     gen = gen_of(dev, 12)
