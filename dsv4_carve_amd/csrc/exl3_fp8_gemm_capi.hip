@@ -82,9 +82,10 @@ struct TileCost {
     int (*launch)(const GemmArgs&);
 };
 
-// Measured on 4096-wide k (us, this table's tile / the next one's): 32 rows x 4096
-// 7.0 / 9.8; 128 x 4096 10.4 / 14.9, 256 x 4096 20.1 / 15.4; 512 x 4096 28.7 (64x64)
-// / 23.7 / 40.0, 4096 x 4096 213 / 170 / 128.
+// Measured in captured launches on 4096-wide k (us, this table's shapes in turn): 48
+// rows x 4096 8.6 / 10.8 / 15.6 / 22.6; 128 x 4096 14.7 / 11.5 / 16.2 / 23.0; 256 x
+// 4096 27.8 / 21.0 / 17.2 / 23.5 / 38.7; 512 x 4096 51.4 / 37.8 / 29.8 / 24.2 / 39.2;
+// 4096 x 4096 - / - / 208 / 169 / 120.
 static const TileCost TILES[] = {
     {32, 32, 1, 0.16f, 0.16f, launch_tile<32, 32, 1, 1, 8>},
     {32, 64, 1, 0.24f, 0.24f, launch_tile<32, 64, 1, 2, 4>},
@@ -93,7 +94,12 @@ static const TileCost TILES[] = {
     {128, 128, 2, 1.13f, 1.95f, launch_tile<128, 128, 2, 2, 1>},
 };
 
-// Rounds of workgroups, each with about 1 us that the blocks do not account for.
+// Rounds of workgroups, each with about 1 us that the blocks do not account for; a
+// last round of one workgroup a CU takes what one takes.  Of 135 sizes (k 1536,
+// 4096 and 7168, n 1536, 4096 and 12288, 4 to 4096 rows) the choice is 1% above the
+// fastest kernel in the mean and more than 10% above it in two: 32 rows x 1536 x
+// 1536, 6.0 us where the kernel without tiles takes 4.5, and 4096 rows
+// 7168 -> 1536, 108 where 128x128 takes 98.
 static const TileCost& choose_tile(int64_t m, int64_t k, int64_t n) {
     const int64_t cus = device_cus();
     const double blocks = (double)((k + FP8_BLOCK - 1) / FP8_BLOCK);
@@ -101,9 +107,9 @@ static const TileCost& choose_tile(int64_t m, int64_t k, int64_t n) {
     double least = 0;
     for (const TileCost& t : TILES) {
         const int64_t tiles = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
-        const bool one = tiles <= cus;
-        const int64_t wave = one ? cus : cus * t.resident, rounds = (tiles + wave - 1) / wave;
-        const double us = (double)rounds * (1.0 + blocks * (one ? t.one : t.full));
+        const int64_t rounds = tiles / (cus * t.resident), rest = tiles - rounds * cus * t.resident;
+        const double us = (double)rounds * (1.0 + blocks * t.full) +
+                          (rest ? 1.0 + blocks * (rest <= cus ? t.one : t.full) : 0.0);
         if (&t == TILES || us < least) {
             least = us;
             best = &t;
@@ -113,11 +119,13 @@ static const TileCost& choose_tile(int64_t m, int64_t k, int64_t n) {
 }
 
 // The kernel goes by the sizes, not by the result's type: a 16-bit result is the
-// fp32 one rounded.  Few rows have a kernel without LDS tiles (us, against the
-// smallest tile: 1 row x 4096 x 4096 4.9 / 6.1, 16 rows 7.0 / 6.2), and so has a k
-// whose rows are too long for a tile's 32-bit offsets.
+// fp32 one rounded.  Few rows have a kernel without LDS tiles: 8, and 16 where its
+// workgroups are one round (us, against the best tile: 4096 x 4096 8 rows 6.5 / 7.6,
+// 16 rows 7.5 / 7.7, 1536 x 4096 16 rows 4.4 / 5.9, 7168 x 4096 11.0 / 10.7; 4096 x
+// 12288 8 rows 13.7 / 13.1, 16 rows 16.6 / 13.1), and so has a k whose rows are too
+// long for a tile's 32-bit offsets.
 static int gemm(const GemmArgs& A) {
-    if (A.m <= 8 || A.k > FP8_TILE_MAX_K) {
+    if (A.m <= (A.n <= 16 * (int64_t)device_cus() ? 16 : 8) || A.k > FP8_TILE_MAX_K) {
         hipLaunchKernelGGL((fp8_gemm_rows_kernel<1, 8>), dim3((unsigned)((A.n + 15) / 16), (unsigned)((A.m + 15) / 16)),
                            dim3(512), 0, A.s, A.a, A.a_scale, A.m, A.k, A.w, A.w_scale, A.n, A.c, A.c_kind);
         return check_launch();
@@ -127,9 +135,9 @@ static int gemm(const GemmArgs& A) {
 
 // Whether a linear's rows are quantized by the workgroups that multiply them.
 // Every one of them does all the rows, so it pays while that is little for a CU
-// (us in a captured step, one launch / two: 4096 x 4096 1 row 5.5 / 7.4, 8 rows
-// 8.1 / 7.9; 4096 x 12288 1 row 11.5 / 13.9, 4 rows 14.1 / 14.1; 1536 x 4096 16
-// rows 5.4 / 6.4), and it saves the caller a launch and the scratch.
+// (us in a captured step, one launch / two: 4096 x 4096 1 row 6.3 / 8.0, 8 rows
+// 9.2 / 9.1; 4096 x 12288 1 row 12.0 / 13.7, 4 rows 15.0 / 14.8; 1536 x 4096 16
+// rows 6.2 / 6.8), and it saves the caller a launch and the scratch.
 static bool linear_in_one(int64_t m, int64_t k, int64_t n) {
     const int64_t rounds = (n + 16 * device_cus() - 1) / (16 * device_cus());
     return m <= 16 && m * k * rounds <= 32768 && fp8_linear_rows_lds((int)m, (int)k) <= 64 * 1024;
