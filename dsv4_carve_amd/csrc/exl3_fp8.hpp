@@ -85,10 +85,11 @@ struct Half16<true> {
     }
 };
 
-// A lane's 32 weights of one block (two 16-byte loads, as in exl3_fp8.hpp) and the inputs at the same k.
+// A lane's 32 e4m3 values of one block (two 16-byte loads) and 16-bit inputs at the same k.
 template <typename H>
 struct BlockW {
     typename H::vec8 v[4];
+    BlockW() = default;
     __device__ __forceinline__ explicit BlockW(const int8x32_t& q) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = H::widen((uint32_t)q[2 * i], (uint32_t)q[2 * i + 1]);
@@ -452,23 +453,6 @@ __global__ __launch_bounds__(FP8_LINEAR_WAVES * 64) void fp8_linear_rows_kernel(
 
 // ---------------------------------------------------------------- product, many rows
 
-// A lane's 32 values of a block, as they come from LDS, and the product of two of them.
-struct Frag {
-    typedef Half16<true> H;
-    H::vec8 v[4];
-    __device__ __forceinline__ void set(const i32x4_t& lo, const i32x4_t& hi) {
-        const BlockW<H> b(join(lo, hi));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = b.v[i];
-    }
-    static __device__ __forceinline__ float4_t product(const Frag& w, const Frag& a) {
-        float4_t p = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p = H::mfma(w.v[i], a.v[i], p);
-        return p;
-    }
-};
-
 // Tiles of BM rows of a and BN rows of w; WM x WN waves share one, KG such sets
 // take alternate blocks of k (their sums are joined in LDS at the end).  A step
 // is KG blocks, which go from memory straight to LDS, one step ahead.  A row of a
@@ -605,6 +589,7 @@ __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu
     // began.  A step's last row group is computed after the next step's barrier, while that step's first operands are
     // on their way from LDS.
     constexpr int LAST = T::MT - 1;
+    typedef BlockW<Half16<true>> Frag;
     Frag fa = {}, fw[T::NT] = {};
     float4_t p[T::NT] = {};
     float s = 0.f, sw = 0.f, sc = 0.f;      // scales: of fa's rows, of w's block, of the products in p
@@ -623,8 +608,8 @@ __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu
         const char* base = lds + ((step & 1) * KG + set) * T::BUF;
         const float* sp = scales + (step / T::GROUP & 1) * T::SCALES + (step % T::GROUP * KG + set) * (BM + 1);
         const auto read = [&](Frag& f, const int (&at)[2], int i) {
-            f.set(*reinterpret_cast<const i32x4_t*>(base + at[0] + i * 16 * FP8_BLOCK),
-                  *reinterpret_cast<const i32x4_t*>(base + at[1] + i * 16 * FP8_BLOCK));
+            f = Frag(join(*reinterpret_cast<const i32x4_t*>(base + at[0] + i * 16 * FP8_BLOCK),
+                          *reinterpret_cast<const i32x4_t*>(base + at[1] + i * 16 * FP8_BLOCK)));
         };
         Frag next;
         read(next, aa, 0);
@@ -635,7 +620,7 @@ __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu
         for (int j = 0; j < T::NT; ++j) {
             if (LAST > 0) sum_up(LAST - 1, j);
             else sum_up(0, j);
-            p[j] = Frag::product(fw[j], fa);
+            p[j] = block_product(fw[j], fa);
             read(fw[j], aw, j);
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -650,7 +635,7 @@ __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
             for (int j = 0; j < T::NT; ++j) {
                 sum_up(i ? i - 1 : LAST, j);
-                p[j] = Frag::product(fw[j], fa);
+                p[j] = block_product(fw[j], fa);
                 __builtin_amdgcn_sched_barrier(0);
             }
             sc = s * sw;
@@ -661,7 +646,7 @@ __global__ __launch_bounds__(WM* WN* KG * 64) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
     for (int j = 0; j < T::NT; ++j) {
         sum_up(LAST > 0 ? LAST - 1 : 0, j);
-        p[j] = Frag::product(fw[j], fa);
+        p[j] = block_product(fw[j], fa);
     }
     sc = s * sw;
 #pragma unroll
