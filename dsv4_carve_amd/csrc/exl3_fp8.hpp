@@ -49,6 +49,19 @@ __device__ __forceinline__ T read_lane(T v, int lane) {
     }
 }
 
+// v of the lane that a DPP pattern names, `none` where it names no lane.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T lane_of(T v, T none) {
+    if constexpr (sizeof(T) == 8) {
+        const u32x2_t a = __builtin_bit_cast(u32x2_t, v), b = __builtin_bit_cast(u32x2_t, none);
+        return __builtin_bit_cast(T, u32x2_t{(uint32_t)__builtin_amdgcn_update_dpp((int)b[0], (int)a[0], CTRL, ROWS, 0xf, false),
+                                             (uint32_t)__builtin_amdgcn_update_dpp((int)b[1], (int)a[1], CTRL, ROWS, 0xf, false)});
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
+                                                                 CTRL, ROWS, 0xf, false));
+    }
+}
+
 __device__ __forceinline__ int8x32_t join(i32x4_t lo, i32x4_t hi) {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }

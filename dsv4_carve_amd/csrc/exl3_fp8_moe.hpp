@@ -9,8 +9,9 @@
 // weights are widened (exactly) to the type of x for the first product, and to
 // bf16 for the second, whose activation is fp32: 24 bits, the sum of three bf16
 // values, each its highest 8 bits left (exact, and no overflow).  Sums are fp32: a
-// block of 128 is four 16x16x32 instructions (twelve) into a cleared accumulator,
-// scaled into the running sum by one multiply-add a value.
+// block of 128 is four 16x16x32 instructions into a cleared accumulator, scaled into
+// the running sum by one multiply-add a value; the three parts of an activation are
+// three columns of the instruction, whose results are added before that.
 //
 // Routing is read in each workgroup, lane r of a wave holding row r (64 rows at
 // most).  A row that names an expert more than once counts as its first slot,
@@ -211,26 +212,24 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
         uint16_t slot, row;
         float weight;
     };
-    struct Expert {
-        uint64_t rows;             // bit r: row r names it
-        int id;
-    };
     struct Group {                 // an expert and up to COLS rows that name it, no two of them alike mod 16
         int id;
         uint16_t first, count;     // entries
     };
     __shared__ __attribute__((aligned(16))) int ids[FP8_MOE_MAX_SLOTS];      // local expert of a slot, or -1
     __shared__ float wts[FP8_MOE_MAX_SLOTS];
-    __shared__ Expert experts[FP8_MOE_MAX_SLOTS];                            // the active ones
+    __shared__ int expert_id[FP8_MOE_MAX_SLOTS];                             // the active ones
+    __shared__ uint64_t expert_rows[FP8_MOE_MAX_SLOTS];                      // bit r: row r names it
     __shared__ Entry entries[FP8_MOE_MAX_SLOTS];                             // their rows, in order
     __shared__ Group groups[FP8_MOE_MAX_SLOTS];
     __shared__ uint16_t place[FP8_MOE_MAX_SLOTS];                            // of a first slot's expert among them
     __shared__ uint16_t first_of[FP8_MOE_MAX_SLOTS];                         // an expert's first entry
     __shared__ int wave_n[2][WAVES];
     __shared__ __attribute__((aligned(16))) float part[WAVES][TILES * 4][64];
-    // a wave's inputs of one block: a row is three planes of 256 bytes, and 16 more, so that rows lie in different banks
-    constexpr int COLUMN = 3 * 256 + 16;
-    __shared__ __attribute__((aligned(16))) char columns[WAVES][2 * LOADS * COLUMN];
+    // a wave's inputs of one block: sixteen chunks of 8 values, each of twelve columns, plane 0, 1 and 2 of the group's four
+    // rows in turn, and 16 bytes more, so that chunks lie in different banks
+    constexpr int CHUNK = 13 * 16;
+    __shared__ __attribute__((aligned(16))) char columns[WAVES][16 * CHUNK];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = lane & 15, g = lane >> 4;
     const int S = A.rows * A.topk;
@@ -288,11 +287,11 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
         if (owner) {
             const int at = before + __popcll(own & below);
             place[tid] = (uint16_t)at;
-            experts[at].id = e;
-            experts[at].rows = 0;
+            expert_id[at] = e;
+            expert_rows[at] = 0;
         }
         __syncthreads();
-        if (row_first) atomicOr(reinterpret_cast<unsigned long long*>(&experts[place[first]].rows), 1ull << row);
+        if (row_first) atomicOr(reinterpret_cast<unsigned long long*>(&expert_rows[place[first]]), 1ull << row);
         __syncthreads();
         // An expert's rows in order, cut into groups: a group's rows are columns of the matrix instruction by their number
         // mod 16.
@@ -312,7 +311,7 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
             if (count) group(first, count);
         };
         // entries and groups of the experts before each: a scan over the waves' experts, groups from bit 16 up
-        const uint64_t named = tid < active ? experts[tid].rows : 0;
+        const uint64_t named = tid < active ? expert_rows[tid] : 0;
         int mine = __popcll(named);
         split(named, [&](int, int) { mine += 1 << 16; });
         int sum = mine;
@@ -334,7 +333,7 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
             const int entry = (sum - mine) & 0xffff;
             first_of[tid] = (uint16_t)entry;
             split(named, [&](int first, int count) {
-                groups[at++] = Group{experts[tid].id, (uint16_t)(entry + first), (uint16_t)count};
+                groups[at++] = Group{expert_id[tid], (uint16_t)(entry + first), (uint16_t)count};
             });
         }
         __syncthreads();
@@ -342,7 +341,7 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
             float w = 0.f;
             for (int s = tid; s < (row + 1) * A.topk; ++s) w += ids[s] == e ? wts[s] : 0.f;
             const int j = place[first];
-            entries[first_of[j] + __popcll(experts[j].rows & ((1ull << row) - 1))] = Entry{(uint16_t)tid, (uint16_t)row, w};
+            entries[first_of[j] + __popcll(expert_rows[j] & ((1ull << row) - 1))] = Entry{(uint16_t)tid, (uint16_t)row, w};
         }
         __syncthreads();
 
@@ -362,6 +361,7 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
         float4_t v[LOADS];
         float wt;
         int col, t;                // this lane's row's: which of the group's (-1: none), which 16 of the batch
+        int last;                  // of the group's rows
     };
     const auto fetch_w = [&](Weights& u, int at) {
         const int j = at / kb_n, kb = at - j * kb_n, id = __builtin_amdgcn_readfirstlane(groups[j].id);
@@ -372,6 +372,7 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
         const int j = at / kb_n, kb = at - j * kb_n;
         const int first = __builtin_amdgcn_readfirstlane(groups[j].first);
         const int last = __builtin_amdgcn_readfirstlane(groups[j].count) - 1;
+        u.last = last;
         u.col = -1;
         u.t = 0;
         u.wt = 0.f;
@@ -395,22 +396,27 @@ __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const
         __builtin_amdgcn_wave_barrier();              // the wave's own place: its LDS operations are in order
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
+            if (2 * i > x.last) break;                // its last rows again
             u32x2_t plane[3];
             split_bf16(x.v[i], plane);
-            char* at = columns[wave] + (2 * i + (lane >> 5)) * COLUMN + (lane & 31) * 8;
+            char* at = columns[wave] + ((lane & 31) >> 1) * CHUNK + (2 * i + (lane >> 5)) * 16 + (lane & 1) * 8;
 #pragma unroll
-            for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x2_t*>(at + 256 * q) = plane[q];
+            for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x2_t*>(at + 64 * q) = plane[q];
         }
         __builtin_amdgcn_wave_barrier();
-        const bool has = x.col >= 0;                  // the other columns are no row's: any inputs do
-        const char* col = columns[wave] + (has ? x.col : 0) * COLUMN;
-        const BlockW<H> w(u.w);
-        float4_t p = {0.f, 0.f, 0.f, 0.f};
+        const char* col = columns[wave] + 2 * g * CHUNK + (r < 12 ? r : r - 4) * 16;        // columns from 12 on are no row's
+        BlockX<H> in;
 #pragma unroll
-        for (int q = 2; q >= 0; --q) {                // the smallest first
-            BlockX<H> in;
-            in.load(reinterpret_cast<const uint16_t*>(col + 256 * q), g);
-            p = block_product<H>(w, in, p);
+        for (int i = 0; i < 4; ++i)                   // chunks 2g, 2g + 1, 8 + 2g and 9 + 2g
+            in.v[i] = *reinterpret_cast<const H::vec8*>(col + ((i & 1) + (i >> 1) * 8) * CHUNK);
+        const float4_t p3 = block_product<H>(BlockW<H>(u.w), in);
+        const bool has = x.col >= 0;
+        const int from = ((lane & 48) + (has ? x.col : 0)) * 4;
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                 // the parts of column c are c, c + 4 and c + 8: row_shl:4, 8
+            const float sum = p3[i] + lane_of<0x104, 0xf>(p3[i], 0.f) + lane_of<0x108, 0xf>(p3[i], 0.f);
+            p[i] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(sum)));
         }
         const float s = x.wt * u.sc;
 #pragma unroll

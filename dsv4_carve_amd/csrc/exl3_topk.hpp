@@ -32,19 +32,6 @@ enum Scoring : int { SCORE_SOFTMAX = 0, SCORE_SIGMOID = 1, SCORE_SQRTSOFTPLUS = 
 constexpr int ROUTE_MAX_TOPK = 64;
 constexpr int ROUTE_MAX_EXPERTS = 2048;
 
-// v of the lane that a DPP pattern names, `none` where it names no lane.
-template <int CTRL, int ROWS, typename T>
-__device__ __forceinline__ T lane_of(T v, T none) {
-    if constexpr (sizeof(T) == 8) {
-        const u32x2_t a = __builtin_bit_cast(u32x2_t, v), b = __builtin_bit_cast(u32x2_t, none);
-        return __builtin_bit_cast(T, u32x2_t{(uint32_t)__builtin_amdgcn_update_dpp((int)b[0], (int)a[0], CTRL, ROWS, 0xf, false),
-                                             (uint32_t)__builtin_amdgcn_update_dpp((int)b[1], (int)a[1], CTRL, ROWS, 0xf, false)});
-    } else {
-        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
-                                                                 CTRL, ROWS, 0xf, false));
-    }
-}
-
 // op over the wave's lanes (each lane's value once), as a wave-uniform value: a
 // scan of each row of 16 lanes, then of the rows; lane 63 has it all.
 template <typename T, typename Op>

@@ -546,6 +546,23 @@ def test_moe_activation_is_fp32(dev, dtype, rows, experts, topk):
     within(out, ref, tol + 2.0 ** -126, "act")
 
 
+@pytest.mark.parametrize("rows", [1, 7, 40])
+def test_moe_infinite_activations(dev, rows):
+    """An activation past fp32 is infinite, and so is what positive weights make of it: no NaN, and no other row's."""
+    gen = gen_of(dev, rows)
+    w13 = torch.randint(0x30, 0x40, (3, 512, 128), generator=gen, device=dev, dtype=torch.uint8).view(R.E4M3)
+    w2 = torch.randint(0x30, 0x40, (3, 128, 256), generator=gen, device=dev, dtype=torch.uint8).view(R.E4M3)
+    s13, s2 = torch.ones((3, 4, 1), device=dev), torch.ones((3, 1, 2), device=dev) * 2.0 ** -20
+    x = torch.rand((rows, 128), generator=gen, device=dev).to(torch.bfloat16)
+    ids = torch.arange(rows, device=dev).reshape(-1, 1) % 3
+    want = ops.fp8_moe(x, w13, s13, w2, s2, ids, torch.ones((rows, 1), device=dev))
+    x[rows // 2] = 2.0 ** 80
+    y = ops.fp8_moe(x, w13, s13, w2, s2, ids, torch.ones((rows, 1), device=dev))
+    assert (y[rows // 2] == torch.inf).all() and torch.isfinite(want).all()
+    keep = [r for r in range(rows) if r != rows // 2]
+    assert torch.equal(y[keep], want[keep])
+
+
 @pytest.mark.parametrize("rows,experts,topk", [(16, 64, 4), (31, 64, 3), (64, 64, 3), (64, 9, 2)])
 def test_moe_crowded_expert(dev, rows, experts, topk):
     """One expert that every row names, more rows than are taken at once, among experts of few rows."""
