@@ -11,7 +11,7 @@
 // by one: each lane's best, a maximum over the wave, the lowest index that has it.
 // Instructions bound it (8000 rows of 256 experts read 8 MB): keys are integers
 // that order as their numbers do, a step of a maximum one DPP instruction (8000
-// rows with a bias 14.7 us, 974 instructions a row; 16 rows 4.9 us, a launch and one
+// rows with a bias 14.5 us, 982 instructions a row; 16 rows 4.9 us, a launch and one
 // row's chain).
 //
 // Order by biased scores is the order of the exact scores even where fp32 cannot

@@ -72,8 +72,9 @@ def cut(a, w):
 
 
 def gemm(a, a_scale, w, w_scale, dtype):
-    """(result, how far an fp32-accumulated product rounded once to `dtype` may be from it).  A 16-bit result may come
-    from the 8-bit matrix instruction."""
+    """(result, how far an fp32-accumulated product rounded once to `dtype` may be from it).  For 16 bits the bound has
+    room for the 8-bit matrix instruction, which no kernel uses: tests of a 16-bit result against the rounded fp32 one
+    go without it."""
     x, m = rows(a, a_scale), weight(w, w_scale)
     ref = x @ m.t()
     tol = (x.abs() @ m.abs().t()) * steps(a.shape[1]) * U + ref.abs() * half_step(dtype) + 2.0 ** -24 * (
