@@ -197,9 +197,10 @@ __device__ __forceinline__ void split_bf16(const float4_t& v, u32x2_t (&plane)[3
 // scale, so that the sum over experts needs no second pass and no atomics.  A
 // wave takes every 16th block of an expert and up to four rows that name it, the
 // next ones' bytes on their way while it computes.  5.3 to 5.5 TB/s of weights with
-// 16 rows (101 of 256 experts of 4096 x 2048, 154 to 160 us).  MT 0 is for a single row, whose
-// experts one wave tells apart: one barrier before the first load, not eight (a
-// layer of one row 46.1 to 47.7 us a call, 48.5 to 50.7 with MT 1).
+// 16 rows (101 of 256 experts of 4096 x 2048, 154 to 160 us).  MT 0 is for a
+// single row, whose experts one wave tells apart: one barrier before the first
+// load, not eight (a layer of one row 46.1 to 47.7 us a call, 48.5 to 50.7 with
+// MT 1).
 template <int MT>
 __global__ __launch_bounds__(FP8_DOWN_WAVES * 64) void fp8_moe_down_kernel(const Fp8MoeArgs A) {
     typedef Half16<true> H;

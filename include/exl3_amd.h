@@ -329,8 +329,8 @@ int exl3_fp8_linear(const void* x, int x_kind, int64_t m, int64_t k, const uint8
  *   [g; u] = W13[e] x[r];  act = silu(min(g, L)) * clamp(u, -L, L);
  *   out[r] = sum_j topk_weights[r][j] * W2[e] act,  e = topk_ids[r][j]
  * x is 16-bit (x_kind 0 = fp16, 1 = bf16), act and sums are fp32.  w13
- * [E][2*I][H] (gate rows first) with w13_scale [E][2*I/128][H/128], w2 [E][H][I] with w2_scale [E][H/128][I/128]; H and I
- * multiples of 128.  1 <= rows <= exl3_fp8_moe_max_rows() = 64, topk <= 16.
+ * [E][2*I][H] (gate rows first) with w13_scale [E][2*I/128][H/128], w2
+ * [E][H][I] with w2_scale [E][H/128][I/128]; H and I multiples of 128.  1 <= rows <= exl3_fp8_moe_max_rows() = 64, topk <= 16.
  * swiglu_limit > 0, +infinity for none.  topk_ids, topk_weights, expert_map and
  * the slots that contribute nothing as in exl3_moe_decode_routed; a row without
  * a valid slot is 0; an id that a row names twice counts with the sum of its
