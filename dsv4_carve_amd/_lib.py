@@ -44,6 +44,10 @@ EXPORTS = (
     "exl3_fp8_moe_scratch_bytes",
     "exl3_fp8_moe",
     "exl3_moe_route",
+    "exl3_fp8_norm",
+    "exl3_fp8_cache_append",
+    "exl3_fp8_attention_scratch_bytes",
+    "exl3_fp8_attention",
 )
 
 _lock = threading.Lock()
@@ -99,6 +103,12 @@ _SIGS = {
     "exl3_fp8_moe": ([_P, _I, _P, _I, _L, _L, _L, _L, _L, _P, _P, _P, _P,
                       _P, _I, _P, _I, _P, _L, _F, _P, _L, _P], _I),
     "exl3_moe_route": ([_P, _I, _L, _L, _L, _I, _P, _I, _F, _P, _I, _P, _P], _I),
+    "exl3_fp8_norm": ([_P, _I, _P, _I, _P, _I, _L, _L, _F, _I, _P, _P, _P, _P, _I, _P], _I),
+    "exl3_fp8_cache_append": ([_P, _L, _L, _P, _L, _L, _I, _L, _P, _P, _P, _P, _L, _L, _L, _L, _P, _L, _L, _P, _P, _L,
+                               _P], _I),
+    "exl3_fp8_attention_scratch_bytes": ([_L, _L, _L, _L, _L, _L, _L, _L], _L),
+    "exl3_fp8_attention": ([_P, _I, _L, _L, _L, _L, _P, _P, _P, _P, _L, _L, _L, _L, _P, _L, _L, _P, _P, _L, _F, _L, _P,
+                            _P, _P, _I, _P, _L, _P], _I),
 }
 
 

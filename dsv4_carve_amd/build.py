@@ -47,6 +47,8 @@ UNITS += [("exl3_prefill_capi.hip", [], "exl3_prefill_capi.o")]
 UNITS += [("exl3_prefill_inst.hip", [f"-DEXL3_BITS={b}"], f"exl3_pf_b{b}.o") for b in range(1, 9)]
 UNITS += [("exl3_prefill_inst.hip", ["-DEXL3_BITS=3", "-DEXL3_BITS2=2"], "exl3_pf_b32.o")]
 UNITS += [("exl3_fp8_gemm_capi.hip", [], "exl3_fp8_gemm_capi.o"), ("exl3_fp8_moe_capi.hip", [], "exl3_fp8_moe_capi.o")]
+UNITS += [("exl3_norm_capi.hip", [], "exl3_norm_capi.o"), ("exl3_attn_capi.hip", [], "exl3_attn_capi.o")]
+UNITS += [("exl3_attn_inst.hip", [f"-DEXL3_ATTN_DIM={d}"], f"exl3_attn_d{d}.o") for d in (64, 128, 192, 256)]
 
 
 def _stale(src: str, out: str) -> bool:

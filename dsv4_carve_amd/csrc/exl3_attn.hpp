@@ -1,0 +1,826 @@
+// A paged cache of e4m3 keys and values with one power-of-two scale for each page
+// and head, the write into it, and causal attention over it.
+//
+//   k  [pages][kv][page][dim]   k_scale [pages][kv]
+//   v  [pages][kv][dim][page]   v_scale [pages][kv]      (a value's tokens are neighbours)
+//
+//   s_ij = scale * q_i . k_j for the keys j that query i sees (j <= i, j > i - window)
+//   out_i = sum_j e^(s_ij) v_j / (sum_j e^(s_ij) + e^sink),  lse_i = log of that sum
+//
+// A power of two as the scale keeps a value's bits where the scale of a begun page
+// grows (but for those that fall below e4m3's normal range), and e4m3's relative
+// error does not depend on where in its range a value lies.
+#pragma once
+
+#include "exl3_fp8.hpp"
+#include "exl3_topk.hpp"
+
+namespace exl3 {
+
+struct CacheView {
+    uint8_t* k;
+    float* k_scale;
+    uint8_t* v;
+    float* v_scale;
+    const int* table;            // [seqs][width] pages
+    int64_t table_stride;
+    const int* lengths;          // [seqs], the new tokens counted
+    const int* starts;           // [seqs + 1] first token of each sequence, or null: one token each
+    int seqs, tokens, kv, dim, page_shift, width, pages;
+};
+
+// A sequence's tokens in a call and its length.  What a table, a length or a start
+// names past its range is cut to it: no index leaves a buffer.
+struct Seq {
+    int first, n, len;
+};
+
+__device__ __forceinline__ Seq get_seq(const CacheView& C, int s) {
+    Seq q;
+    if (C.starts) {
+        const int a = C.starts[s], b = C.starts[s + 1];
+        q.first = min(max(a, 0), C.tokens);
+        q.n = max(min(b, C.tokens) - q.first, 0);
+    } else {
+        q.first = s;
+        q.n = 1;
+    }
+    const int64_t room = (int64_t)C.width << C.page_shift;
+    const int len = max(C.lengths[s], 0);
+    q.len = (int64_t)len < room ? len : (int)room;
+    return q;
+}
+
+// A value that all lanes have alike, known as such to the compiler: control flow and
+// addresses that follow from it are scalar.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const u32x2_t a = __builtin_bit_cast(u32x2_t, v);
+    return __builtin_bit_cast(int64_t, u32x2_t{(uint32_t)uniform((int)a[0]), (uint32_t)uniform((int)a[1])});
+}
+
+// Exclusive prefix sum of one value a thread over a workgroup of WAVES waves, and the total.
+template <int WAVES>
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t (&lds)[WAVES], int64_t& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t sum = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t up = __shfl_up(sum, d);
+        if (lane >= d) sum += up;
+    }
+    __syncthreads();
+    if (lane == 63) lds[wave] = sum;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) before += lds[w];
+        total += lds[w];
+    }
+    return before + sum - v;
+}
+
+// The sequence that unit `at` of all sequences' units lies in, by a scan over the
+// sequences; count(s) units each.  Returns the total; found[0] is -1 where `at` is
+// behind it, found[1] the unit within the sequence.
+template <int WAVES, typename Count>
+__device__ __forceinline__ int64_t find_seq(int seqs, int64_t at, int64_t (&lds)[WAVES], int64_t (&found)[2], Count&& count) {
+    int64_t sum = 0;
+    if (threadIdx.x == 0) found[0] = -1;
+    for (int s0 = 0; s0 < seqs; s0 += WAVES * 64) {
+        const int s = s0 + threadIdx.x;
+        const int64_t c = s < seqs ? count(s) : 0;
+        int64_t total;
+        const int64_t before = sum + block_scan<WAVES>(c, lds, total);
+        if (at >= before && at < before + c) {
+            found[0] = s;
+            found[1] = at - before;
+        }
+        sum += total;
+    }
+    __syncthreads();
+    return uniform(sum);
+}
+
+// ---------------------------------------------------------------- the write
+
+constexpr int APPEND_WAVES = 4;
+
+struct AppendArgs {
+    CacheView c;
+    const void* k;
+    const void* v;
+    int64_t k_token, k_head, v_token, v_head;          // strides in values
+};
+
+// The pages that a sequence's new tokens lie in.
+__device__ __forceinline__ int touched_pages(const CacheView& C, const Seq& q) {
+    const int from = max(q.len - q.n, 0);
+    return q.len > from ? ((q.len - 1) >> C.page_shift) - (from >> C.page_shift) + 1 : 0;
+}
+
+// Eight neighbouring values (16-byte aligned) as fp32; an infinity as a NaN.
+template <int K>
+__device__ __forceinline__ void load8_finite(const void* p, int64_t at, float (&v)[8]) {
+    if constexpr (K == OUT_F32) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float4_t f = reinterpret_cast<const float4_t*>(static_cast<const float*>(p) + at)[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * i + j] = f[j];
+        }
+    } else {
+        const u32x4_t u = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[2 * j] = K == OUT_BF16 ? __uint_as_float(u[j] << 16) : f16_bits_to_f32((uint16_t)u[j]);
+            v[2 * j + 1] = K == OUT_BF16 ? __uint_as_float(u[j] & 0xffff0000u) : f16_bits_to_f32((uint16_t)(u[j] >> 16));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = fabsf(v[j]) == __builtin_inff() ? __builtin_nanf("") : v[j];
+}
+
+// Four codes times a power of two, rounded to e4m3 again.
+__device__ __forceinline__ uint32_t rescale4(uint32_t u, float by) {
+    return pack_e4m3(__builtin_amdgcn_cvt_f32_fp8((int)u, 0) * by, __builtin_amdgcn_cvt_f32_fp8((int)u, 1) * by,
+                     __builtin_amdgcn_cvt_f32_fp8((int)u, 2) * by, __builtin_amdgcn_cvt_f32_fp8((int)u, 3) * by);
+}
+
+// A workgroup has one page of one head, of the keys or of the values: the new
+// tokens' largest magnitude, the scale, the old codes where it grew, the new ones.
+// The inputs are read twice (the second time from cache).
+template <int K>
+__global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(AppendArgs A) {
+    __shared__ int64_t lds[APPEND_WAVES];
+    __shared__ int64_t found[2];
+    __shared__ float most_of[APPEND_WAVES];
+    const CacheView& C = A.c;
+    const int tid = threadIdx.x, head = blockIdx.y;
+    const bool values = blockIdx.z;
+    int s = blockIdx.x, nth = 0;
+    if (C.starts) {
+        find_seq<APPEND_WAVES>(C.seqs, blockIdx.x, lds, found, [&](int i) { return (int64_t)touched_pages(C, get_seq(C, i)); });
+        if (found[0] < 0) return;
+        s = uniform((int)found[0]);
+        nth = uniform((int)found[1]);
+    }
+    const Seq q = get_seq(C, s);
+    const int page = 1 << C.page_shift, base = q.len - q.n, from = max(base, 0);
+    if (q.len <= from) return;
+    const int at = (from >> C.page_shift) + nth;                                  // the page's place in the sequence
+    const int id = C.table[s * C.table_stride + at];
+    if ((unsigned)id >= (unsigned)C.pages) return;
+    const int lo = max(from - (at << C.page_shift), 0), hi = min(q.len - (at << C.page_shift), page);
+    const int64_t token = q.first + (at << C.page_shift) - base;                  // the token of the page's place 0
+    const int64_t stride = values ? A.v_token : A.k_token;
+    const int64_t in0 = token * stride + head * (values ? A.v_head : A.k_head);
+    const void* in = values ? A.v : A.k;
+    const int64_t block = (int64_t)id * C.kv + head;
+    uint8_t* code = (values ? C.v : C.k) + (block << C.page_shift) * C.dim;
+    float* scale = (values ? C.v_scale : C.k_scale) + block;
+
+    const int per = C.dim >> 3;                                                   // chunks of eight a token
+    float most = 0.f;
+    float x[8];
+    for (int i = tid; i < (hi - lo) * per; i += APPEND_WAVES * 64) {
+        const int t = i / per;
+        load8_finite<K>(in, in0 + (lo + t) * stride + (i - t * per) * 8, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+    }
+    most = wave_max(most, 0.f);
+    if ((tid & 63) == 0) most_of[tid >> 6] = most;
+    const float before = lo ? *scale : 0.f;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < APPEND_WAVES; ++w) most = fmaxf(most, most_of[w]);
+    const float now = fmaxf(QuantGroup(most, true).scale, before);
+    const float inverse = 1.0f / now, by = before / now;
+    const bool grew = lo && by != 1.0f;
+    if (!values) {
+        if (grew)
+            for (int i = tid; i < lo * C.dim / 16; i += APPEND_WAVES * 64) {
+                u32x4_t u = reinterpret_cast<u32x4_t*>(code)[i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) u[j] = rescale4(u[j], by);
+                reinterpret_cast<u32x4_t*>(code)[i] = u;
+            }
+        for (int i = tid; i < (hi - lo) * per; i += APPEND_WAVES * 64) {
+            const int t = i / per, d = (i - t * per) * 8;
+            load8_finite<K>(in, in0 + (lo + t) * stride + d, x);
+            *reinterpret_cast<u32x2_t*>(code + (lo + t) * C.dim + d) =
+                u32x2_t{pack_e4m3(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse),
+                        pack_e4m3(x[4] * inverse, x[5] * inverse, x[6] * inverse, x[7] * inverse)};
+        }
+    } else {
+        // 16 tokens of one value's channel at once; what is outside [lo, hi) goes back as it was, or rescaled below lo
+        const int first = grew ? 0 : lo >> 4, groups = ((hi + 15) >> 4) - first;
+        for (int i = tid; i < groups * C.dim; i += APPEND_WAVES * 64) {
+            const int b = i / C.dim, d = i - b * C.dim, t0 = (first + b) * 16;
+            u32x4_t* p = reinterpret_cast<u32x4_t*>(code + ((int64_t)d << C.page_shift) + t0);
+            u32x4_t u = {0, 0, 0, 0};
+            if (t0 < lo || t0 + 16 > hi) u = *p;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t moved = grew ? rescale4(u[j], by) : u[j];
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int t = t0 + 4 * j + e;
+                    const float f = t >= lo && t < hi ? load_kind<K>(in, in0 + t * stride + d) : 0.f;
+                    y[e] = (fabsf(f) == __builtin_inff() ? __builtin_nanf("") : f) * inverse;
+                }
+                const uint32_t made = pack_e4m3(y[0], y[1], y[2], y[3]);
+                uint32_t r = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int t = t0 + 4 * j + e;
+                    const uint32_t m = 0xffu << (8 * e);
+                    r |= m & (t < lo ? moved : t < hi ? made : u[j]);
+                }
+                u[j] = r;
+            }
+            *p = u;
+        }
+    }
+    if (tid == 0) *scale = now;
+}
+
+// ---------------------------------------------------------------- attention
+
+constexpr int ATTN_WAVES = 4;
+constexpr int ATTN_KEYS = 64;                 // keys of a block
+constexpr float ATTN_LOW = -3.402823466e+38f; // a row's reference before its first key
+constexpr float ATTN_SLACK = 6.f;             // how far a logit may pass the reference (log2) before sums are rescaled
+constexpr int ATTN_HEADROOM = 8;              // 16-bit weights are below 2^(SLACK + HEADROOM) < 65504
+
+struct AttnArgs {
+    CacheView c;
+    const uint16_t* q;
+    int64_t q_token, q_head;                  // strides in values
+    int heads, group;                         // query heads, and of each cache head
+    float qk_scale;                           // scale * log2(e)
+    int window;                               // 0: none
+    const float* sinks;                       // [heads] or null
+    uint16_t* out;                            // [tokens][heads][dim]
+    float* lse;                               // [tokens][heads] or null
+    float* part;                              // partial results of shared items, or null: a workgroup an item
+    int least;                                // units that a workgroup has at least
+    bool clear;                               // rows that no sequence has are zeroed
+};
+
+// Rows of a tile: ROWS neighbouring (query, head of the group) pairs of one sequence and cache head.
+struct Tile {
+    int r0, rows;                             // rows within the sequence, and how many there are
+    int lo, hi;                               // keys that some row sees
+    int full_lo, full_hi;                     // keys that every row sees
+};
+
+__device__ __forceinline__ Tile get_tile(const AttnArgs& A, const Seq& q, int t, int ROWS) {
+    Tile x;
+    x.r0 = t * ROWS;
+    x.rows = min(ROWS, q.n * A.group - x.r0);
+    const int base = q.len - q.n;
+    const int qa = x.r0 / A.group, qb = (x.r0 + x.rows - 1) / A.group;
+    x.hi = min(max(base + qb + 1, 0), q.len);
+    x.full_hi = max(base + qa + 1, 0);
+    x.lo = x.full_lo = 0;
+    if (A.window) {
+        x.lo = min(max(base + qa + 1 - A.window, 0), x.hi);
+        x.full_lo = max(base + qb + 1 - A.window, 0);
+    }
+    return x;
+}
+
+__device__ __forceinline__ int tiles_of(const AttnArgs& A, const Seq& q, int ROWS) {
+    return (int)(((int64_t)q.n * A.group + ROWS - 1) / ROWS);
+}
+
+// Blocks of keys that a tile goes through, one at least: a row without keys has a result too.
+__device__ __forceinline__ int blocks_of(const Tile& x) {
+    return max((x.hi + ATTN_KEYS - 1) / ATTN_KEYS - x.lo / ATTN_KEYS, 1);
+}
+
+__device__ __forceinline__ int64_t units_of(const AttnArgs& A, const Seq& q, int ROWS) {
+    const int tiles = tiles_of(A, q, ROWS);
+    int64_t n = 0;
+    for (int t = 0; t < tiles; ++t) n += blocks_of(get_tile(A, q, t, ROWS));
+    return n;
+}
+
+__device__ __forceinline__ float xor_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t u) {       // 0x80 in each byte that is an e4m3 NaN
+    return ((u & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+// One wave's rows against blocks of 64 keys.  The products are transposed: keys are
+// the rows of S^T = K Q^T, so that a lane has logits of one row only (row lane % 16 of
+// each 16), and lane group g = lane / 16 has keys 16 g .. 16 g + 15 of the block: key
+// 16 g + 4 t + i is row 4 g + i of the t-th product.  The weights are then, as they
+// are, the column operand of O^T = V^T P^T, for which a lane reads 16 neighbouring
+// tokens of one channel.  A lane's 16 keys are of one page: one pair of scales.
+//
+// Softmax: weights are 2^(s - m) against a reference m that follows the row's largest
+// logit with some slack, and the values' scale joins the weight, as 2^(s - m) * vs *
+// 2^(HEADROOM - c), where c follows the row's largest log2 of weight times scale: so
+// the 16-bit operand neither overflows nor loses a row whose values are small.  Sums
+// are fp32.  A 16-bit weight has 11 bits, three more than a bf16 result; for an fp16
+// result the rest of the weight goes through the product as well (FINE).
+template <int DIM, bool BF16, int RB>
+struct AttnWave {
+    static constexpr bool FINE = !BF16;
+    static constexpr int KC = DIM / 64, DT = DIM / 16;
+    typedef Half16<BF16> H;
+    typedef Half16<false> W;
+
+    float4_t o[DT][RB];
+    float m[RB], top[RB], c[RB], l[RB];
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            m[rb] = top[rb] = ATTN_LOW;
+            c[rb] = l[rb] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d][rb] = float4_t{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+
+    // blocks first, first + step, ... < last of the tile's keys
+    __device__ __forceinline__ void run(const AttnArgs& A, const Seq& q, const Tile& x, int s, int head, int first, int last,
+                                        int step) {
+        const CacheView& C = A.c;
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+        const int base = q.len - q.n;
+        typename H::vec8 qf[RB][KC][2];
+        int see_lo[RB], see_hi[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const int row = 16 * rb + r, at = (x.r0 + row) / A.group, hg = x.r0 + row - at * A.group;
+            const bool in = row < x.rows;
+            const uint16_t* p = A.q + (int64_t)(q.first + at) * A.q_token + (int64_t)(head * A.group + hg) * A.q_head;
+#pragma unroll
+            for (int k = 0; k < KC; ++k)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int d = 64 * k + 16 * g + 8 * u;
+                    qf[rb][k][u] = __builtin_bit_cast(typename H::vec8, u32x4_t{0, 0, 0, 0});
+                    if (in && d < C.dim) qf[rb][k][u] = *reinterpret_cast<const typename H::vec8*>(p + d);
+                }
+            see_hi[rb] = in ? min(base + at + 1, q.len) : 0;
+            see_lo[rb] = in && A.window ? base + at + 1 - A.window : 0;
+        }
+        const int* table = C.table + s * C.table_stride;
+        const int pages = (q.len + (1 << C.page_shift) - 1) >> C.page_shift;
+        const int gk = r >> 2;                                    // the group of the key that this lane reads
+        // No branch here or in the loads: lanes that a branch divides may stay apart in the loop around the products.
+        const auto page_id = [&](int b, int group) {
+            const int i = (b * ATTN_KEYS + 16 * group) >> C.page_shift, id = table[min(i, pages - 1)];
+            return i < pages ? id : -1;
+        };
+        const int mask = (1 << C.page_shift) - 1;
+        u32x4_t kraw[4][KC], vraw[DT];
+        float ks, vs;
+        int idk, idv;                                             // pages of the block whose keys are read next
+        const auto valid = [&](int id) { return (unsigned)id < (unsigned)C.pages; };
+        const auto load_k = [&](int b, int id) {
+            const int64_t block = (int64_t)(valid(id) ? id : 0) * C.kv + head;
+            const uint8_t* p = C.k + ((block << C.page_shift) + ((b * ATTN_KEYS + 16 * gk + (r & 3)) & mask)) * C.dim;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int k = 0; k < KC; ++k) {
+                    const int d = 64 * k + 16 * g;                // behind the row's end: its first values, against zeros
+                    kraw[t][k] = *reinterpret_cast<const u32x4_t*>(p + 4 * t * C.dim + (d < C.dim ? d : 0));
+                }
+        };
+        const auto load_v = [&](int b, int id) {
+            const int64_t block = (int64_t)(valid(id) ? id : 0) * C.kv + head;
+            const uint8_t* p = C.v + ((block * C.dim) << C.page_shift) + ((b * ATTN_KEYS + 16 * g) & mask);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const int channel = 16 * d < C.dim ? 16 * d + r : r;          // behind the last: not stored
+                vraw[d] = *reinterpret_cast<const u32x4_t*>(p + (channel << C.page_shift));
+            }
+        };
+        const auto load_scales = [&](int id) {
+            const int64_t block = (int64_t)(valid(id) ? id : 0) * C.kv + head;
+            ks = C.k_scale[block];
+            vs = C.v_scale[block];
+        };
+        if (first >= last) return;
+        idk = page_id(first, gk);
+        idv = page_id(first, g);
+        load_k(first, idk);
+        load_scales(idv);
+        load_v(first, idv);
+        int id_now = idv;
+        if (first + step < last) {
+            idk = page_id(first + step, gk);
+            idv = page_id(first + step, g);
+        }
+        for (int b = first; b < last; b += step) {
+            const bool more = b + step < last;
+            float4_t p[4][RB];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) p[t][rb] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int k = 0; k < KC; ++k)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const typename H::vec8 key = H::widen(kraw[t][k][2 * u], kraw[t][k][2 * u + 1]);
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) p[t][rb] = H::mfma(key, qf[rb][k][u], p[t][rb]);
+                    }
+            const float kc = ks * A.qk_scale, vscale = vs;
+            const int id_here = id_now;
+            if (more) {
+                load_k(b + step, idk);
+                load_scales(idv);
+                id_now = idv;
+                if (b + 2 * step < last) idk = page_id(b + 2 * step, gk);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[t][rb][i] *= kc;
+            const int key0 = b * ATTN_KEYS + 16 * g;
+            const bool here = valid(id_here);
+            const bool whole = b * ATTN_KEYS >= x.full_lo && (b + 1) * ATTN_KEYS <= x.full_hi &&
+                               __builtin_amdgcn_ballot_w64(here) == ~0ull;
+            if (!whole) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = key0 + 4 * t + i;
+                            if (!(here && key >= see_lo[rb] && key < see_hi[rb])) p[t][rb][i] = -__builtin_inff();
+                        }
+                // Nothing that no row sees may reach a sum: a weight of 0 leaves a NaN one.
+                uint32_t keep[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    keep[j] = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0 + 4 * j + e;
+                        if (here && key >= x.lo && key < x.hi) keep[j] |= 0xffu << (8 * e);
+                    }
+                }
+                uint32_t nan = 0;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        vraw[d][j] &= keep[j];
+                        nan |= nan_bytes(vraw[d][j]);
+                    }
+                // A NaN that only some of the rows see: counted for those in a product of its own, and 0 in the others'.
+                if (__builtin_amdgcn_ballot_w64(nan != 0)) {
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        half8_t sees[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const int key = key0 + 8 * u + j;
+                                sees[u][j] = here && key >= see_lo[rb] && key < see_hi[rb] ? (_Float16)1.f : (_Float16)0.f;
+                            }
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) {
+                            float4_t n = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int u = 0; u < 2; ++u)
+                                n = W::mfma(W::widen((nan_bytes(vraw[d][2 * u]) >> 7) * 0x38u,        // 0x38: one
+                                                     (nan_bytes(vraw[d][2 * u + 1]) >> 7) * 0x38u), sees[u], n);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (n[i] > 0.f) o[d][rb][i] = __builtin_nanf("");
+                        }
+                    }
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) vraw[d][j] &= ~((nan_bytes(vraw[d][j]) >> 7) * 0xffu);
+                }
+            }
+            // log2 of a bound of the values' scale: vscale < 2^ev
+            const float ev = (float)((int)(__float_as_uint(vscale) >> 23 & 0xff) - 126);
+            float most[RB];
+            bool grew = false;
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                most[rb] = p[0][rb][0];
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (t + i) most[rb] = fmaxf(most[rb], p[t][rb][i]);
+                grew |= most[rb] > m[rb] + ATTN_SLACK || most[rb] + ev > top[rb] + ATTN_SLACK;
+            }
+            if (__builtin_amdgcn_ballot_w64(grew)) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    const float m1 = fmaxf(m[rb], xor_max(most[rb])), top1 = fmaxf(top[rb], xor_max(most[rb] + ev));
+                    const float c1 = ceilf(top1 - m1);
+                    const float fl = __builtin_amdgcn_exp2f(m[rb] - m1);
+                    const float fo = __builtin_amdgcn_exp2f(m[rb] - m1 + (c[rb] - c1));
+                    m[rb] = m1;
+                    top[rb] = top1;
+                    c[rb] = c1;
+                    l[rb] *= fl;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[d][rb][i] *= fo;
+                }
+            }
+            half8_t hi[RB][2], lo[RB][2];
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const float f = ldexpf(vscale, ATTN_HEADROOM - (int)c[rb]);
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float e = __builtin_amdgcn_exp2f(p[t][rb][i] - m[rb]);
+                        l[rb] += e;
+                        const float w = e * f;
+                        const _Float16 h = (_Float16)w;
+                        hi[rb][t >> 1][4 * (t & 1) + i] = h;
+                        if constexpr (FINE) lo[rb][t >> 1][4 * (t & 1) + i] = (_Float16)(w - (float)h);
+                    }
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const half8_t v = W::widen(vraw[d][2 * u], vraw[d][2 * u + 1]);
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        o[d][rb] = W::mfma(v, hi[rb][u], o[d][rb]);
+                        if constexpr (FINE) o[d][rb] = W::mfma(v, lo[rb][u], o[d][rb]);
+                    }
+                }
+            if (more) {
+                load_v(b + step, id_now);
+                if (b + 2 * step < last) idv = page_id(b + 2 * step, g);
+            }
+        }
+    }
+};
+
+template <int DIM, int RB>
+struct AttnSize {
+    static constexpr int ROWS = 16 * RB, PITCH = DIM + 4;
+    static constexpr int LDS = ATTN_WAVES * ROWS * (PITCH + 2) * 4;
+    static constexpr int PART = ROWS * (DIM + 2);                 // floats of a partial result: rows of sums, then m and l
+};
+
+// Four outputs of one row.
+template <bool BF16>
+__device__ __forceinline__ void store_row4(uint16_t* p, float4_t v) {
+    const uint32_t a = BF16 ? pack_bf16(v[0], v[1]) : f32_to_f16_bits(v[0]) | (uint32_t)f32_to_f16_bits(v[1]) << 16;
+    const uint32_t b = BF16 ? pack_bf16(v[2], v[3]) : f32_to_f16_bits(v[2]) | (uint32_t)f32_to_f16_bits(v[3]) << 16;
+    *reinterpret_cast<u32x2_t*>(p) = u32x2_t{a, b};
+}
+
+// A row's final factor and the logarithm of its sum, from its reference and sum.
+__device__ __forceinline__ float finish_row(const AttnArgs& A, int head, float m, float l, float& lse) {
+    float f = 1.f;
+    if (A.sinks) {
+        const float s = A.sinks[head] * 1.4426950408889634f, m1 = fmaxf(m, s);
+        f = __builtin_amdgcn_exp2f(m - m1);
+        l = l * f + __builtin_amdgcn_exp2f(s - m1);
+        m = m1;
+    }
+    lse = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    return l == 0.f ? 0.f : f / l;
+}
+
+// Rows of q whose tokens no sequence has: zeros, and -inf for the logarithm.
+__device__ __forceinline__ void clear_rows(const AttnArgs& A) {
+    const CacheView& C = A.c;
+    if (!A.clear || !C.starts) return;
+    const int a = min(max(C.starts[0], 0), C.tokens), b = min(max(C.starts[C.seqs], a), C.tokens);
+    const int rows = C.tokens - (b - a);
+    const int64_t each = (int64_t)A.heads * C.dim / 8;
+    for (int i = blockIdx.x; i < rows; i += gridDim.x) {
+        const int64_t t = i < a ? i : i + (b - a);
+        for (int64_t j = threadIdx.x; j < each; j += blockDim.x)
+            reinterpret_cast<u32x4_t*>(A.out + t * A.heads * C.dim)[j] = u32x4_t{0, 0, 0, 0};
+        if (A.lse)
+            for (int j = threadIdx.x; j < A.heads; j += blockDim.x) A.lse[t * A.heads + j] = -__builtin_inff();
+    }
+}
+
+// Units are (cache head, tile, block of keys), in this order; a workgroup has an
+// equal share of them, next to each other, whatever sequences they are of.  Its four
+// waves go through a tile's blocks in turn and join their sums in LDS.  A tile whose
+// blocks one workgroup has all is finished; of the others each workgroup leaves a
+// partial result: in its first place where the tile began before its share, in its
+// second where it goes on behind it.  Without a place for partial results a workgroup
+// has a tile: blockIdx.x is the tile (the last, longest ones first), blockIdx.y the head.
+template <int DIM, bool BF16, int RB>
+__global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_kernel(AttnArgs A) {
+    typedef AttnSize<DIM, RB> Z;
+    extern __shared__ float lds[];
+    __shared__ int64_t scan[ATTN_WAVES];
+    __shared__ int64_t found[2];
+    const CacheView& C = A.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, g = lane >> 4;
+    int64_t u = 0, u1 = 0, total = 0;
+    int s = 0, t = 0, head = 0, done = 0;                       // done: the tile's blocks before the share
+    Seq q;
+    Tile x;
+    int n = 0;
+    clear_rows(A);
+    if (A.part) {
+        const auto count = [&](int i) { return units_of(A, get_seq(C, i), Z::ROWS); };
+        total = find_seq<ATTN_WAVES>(C.seqs, 0, scan, found, count);
+        const int64_t all = total * C.kv;
+        int64_t share = (all + gridDim.x - 1) / gridDim.x;
+        if (share < A.least) share = A.least;
+        u = share * blockIdx.x;
+        u1 = u + share < all ? u + share : all;
+        if (u >= u1) return;
+        head = (int)(u / total);
+        find_seq<ATTN_WAVES>(C.seqs, u - head * total, scan, found, count);
+        s = uniform((int)found[0]);
+        int64_t left = uniform(found[1]);
+        q = get_seq(C, s);
+        for (;; ++t) {
+            x = get_tile(A, q, t, Z::ROWS);
+            n = blocks_of(x);
+            if (left < n) break;
+            left -= n;
+        }
+        done = (int)left;
+    } else {
+        const int64_t at = (int64_t)gridDim.x - 1 - blockIdx.x;
+        find_seq<ATTN_WAVES>(C.seqs, at, scan, found, [&](int i) { return (int64_t)tiles_of(A, get_seq(C, i), Z::ROWS); });
+        if (found[0] < 0) return;
+        s = uniform((int)found[0]);
+        t = uniform((int)found[1]);
+        head = blockIdx.y;
+        q = get_seq(C, s);
+        x = get_tile(A, q, t, Z::ROWS);
+        n = blocks_of(x);
+        u1 = n;
+    }
+    float* sums = lds;                                          // [wave][row][PITCH]
+    float* ml = lds + ATTN_WAVES * Z::ROWS * Z::PITCH;          // [wave][row][2]
+    for (;;) {
+        const int64_t want = u1 - u;
+        const int here = (int)(n - done < want ? n - done : want);
+        const int b0 = x.lo / ATTN_KEYS + done;
+        AttnWave<DIM, BF16, RB> W;
+        W.clear();
+        W.run(A, q, x, s, head, b0 + wave, min(b0 + here, (x.hi + ATTN_KEYS - 1) / ATTN_KEYS), ATTN_WAVES);
+        __syncthreads();
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const int row = 16 * rb + r;
+            float l = W.l[rb];
+            l += __shfl_xor(l, 16);
+            l += __shfl_xor(l, 32);
+            if (g == 0) {
+                ml[(wave * Z::ROWS + row) * 2] = W.m[rb];
+                ml[(wave * Z::ROWS + row) * 2 + 1] = l;
+            }
+            const int back = (int)W.c[rb] - ATTN_HEADROOM;
+#pragma unroll
+            for (int d = 0; d < DIM / 16; ++d) {
+                float4_t v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = ldexpf(W.o[d][rb][i], back);
+                *reinterpret_cast<float4_t*>(sums + (wave * Z::ROWS + row) * Z::PITCH + 16 * d + 4 * g) = v;
+            }
+        }
+        __syncthreads();
+        const bool final = here == n;
+        float* part = A.part + ((int64_t)blockIdx.x * 2 + (done == 0 ? 1 : 0)) * Z::PART;
+        const int quads = C.dim / 4;
+        for (int i = tid; i < x.rows * quads; i += ATTN_WAVES * 64) {
+            const int row = i / quads, d = (i - row * quads) * 4;
+            float m = ATTN_LOW, l = 0.f;
+#pragma unroll
+            for (int w = 0; w < ATTN_WAVES; ++w) m = fmaxf(m, ml[(w * Z::ROWS + row) * 2]);
+            float4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < ATTN_WAVES; ++w) {
+                const float f = __builtin_amdgcn_exp2f(ml[(w * Z::ROWS + row) * 2] - m);
+                l += f * ml[(w * Z::ROWS + row) * 2 + 1];
+                const float4_t a = *reinterpret_cast<const float4_t*>(sums + (w * Z::ROWS + row) * Z::PITCH + d);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = fmaf(f, a[j], v[j]);
+            }
+            if (final) {
+                const int at = (x.r0 + row) / A.group, h = head * A.group + x.r0 + row - at * A.group;
+                const int64_t o = (int64_t)(q.first + at) * A.heads + h;
+                float lse;
+                const float f = finish_row(A, h, m, l, lse);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] *= f;
+                store_row4<BF16>(A.out + o * C.dim + d, v);
+                if (A.lse && d == 0) A.lse[o] = lse;
+            } else {
+                *reinterpret_cast<float4_t*>(part + row * C.dim + d) = v;
+                if (d == 0) {
+                    part[Z::ROWS * DIM + 2 * row] = m;
+                    part[Z::ROWS * DIM + 2 * row + 1] = l;
+                }
+            }
+        }
+        u += here;
+        if (u >= u1) break;
+        done = 0;
+        if (++t == tiles_of(A, q, Z::ROWS)) {
+            t = 0;
+            do {
+                if (++s == C.seqs) {
+                    s = 0;
+                    ++head;
+                }
+                q = get_seq(C, s);
+            } while (q.n == 0);
+        }
+        x = get_tile(A, q, t, Z::ROWS);
+        n = blocks_of(x);
+    }
+}
+
+// The tiles that a border between two workgroups' shares divides, joined by the
+// workgroup of the first such border; blockIdx.y takes every gridDim.y-th row.
+template <int DIM, bool BF16, int RB>
+__global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_join_kernel(AttnArgs A, int shares) {
+    typedef AttnSize<DIM, RB> Z;
+    __shared__ int64_t scan[ATTN_WAVES];
+    __shared__ int64_t found[2];
+    const CacheView& C = A.c;
+    const auto count = [&](int i) { return units_of(A, get_seq(C, i), Z::ROWS); };
+    const int64_t total = find_seq<ATTN_WAVES>(C.seqs, 0, scan, found, count);
+    const int64_t all = total * C.kv;
+    int64_t share = (all + shares - 1) / shares;
+    if (share < A.least) share = A.least;
+    const int64_t u = share * ((int64_t)blockIdx.x + 1);
+    if (u >= all) return;
+    const int head = (int)(u / total);
+    find_seq<ATTN_WAVES>(C.seqs, u - head * total, scan, found, count);
+    const int s = uniform((int)found[0]);
+    int64_t left = uniform(found[1]);
+    const Seq q = get_seq(C, s);
+    Tile x;
+    int n;
+    for (int t = 0;; ++t) {
+        x = get_tile(A, q, t, Z::ROWS);
+        n = blocks_of(x);
+        if (left < n) break;
+        left -= n;
+    }
+    if (left == 0 || left > share) return;                       // the tile begins here, or a border before this divides it
+    const int last = (int)((u - left + n - 1) / share);          // the workgroup of the tile's last unit
+    const int first = blockIdx.x;
+    const auto place = [&](int w) { return A.part + ((int64_t)w * 2 + (w == first ? 1 : 0)) * Z::PART; };
+    const int quads = C.dim / 4, rows = (x.rows - (int)blockIdx.y + (int)gridDim.y - 1) / (int)gridDim.y;
+    for (int i = threadIdx.x; i < rows * quads; i += ATTN_WAVES * 64) {
+        const int nth = i / quads, d = (i - nth * quads) * 4, row = nth * gridDim.y + blockIdx.y;
+        float m = ATTN_LOW, l = 0.f;
+        for (int w = first; w <= last; ++w) m = fmaxf(m, place(w)[Z::ROWS * DIM + 2 * row]);
+        float4_t v = {0.f, 0.f, 0.f, 0.f};
+        for (int w = first; w <= last; ++w) {
+            const float* p = place(w);
+            const float f = __builtin_amdgcn_exp2f(p[Z::ROWS * DIM + 2 * row] - m);
+            l += f * p[Z::ROWS * DIM + 2 * row + 1];
+            const float4_t a = *reinterpret_cast<const float4_t*>(p + row * C.dim + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = fmaf(f, a[j], v[j]);
+        }
+        const int at = (x.r0 + row) / A.group, h = head * A.group + x.r0 + row - at * A.group;
+        const int64_t o = (int64_t)(q.first + at) * A.heads + h;
+        float lse;
+        const float f = finish_row(A, h, m, l, lse);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] *= f;
+        store_row4<BF16>(A.out + o * C.dim + d, v);
+        if (A.lse && d == 0) A.lse[o] = lse;
+    }
+}
+
+}  // namespace exl3

@@ -1,0 +1,128 @@
+// C-ABI entry points of the 8-bit cache and the attention over it (declared in
+// include/exl3_amd.h).
+#include <algorithm>
+#include <cmath>
+
+#include "exl3_attn_launch.hpp"
+
+using namespace exl3;
+
+static int check_cache(const void* k, const void* k_scale, const void* v, const void* v_scale, int64_t pages, int64_t kv_heads,
+                       int64_t page_size, int64_t dim, const void* table, int64_t width, const void* lengths,
+                       const void* starts, int64_t seqs, int64_t tokens) {
+    if (!k || !k_scale || !v || !v_scale || !table || !lengths) return fail("null pointer");
+    if (pages < 1 || pages > INT32_MAX) return fail("pages must be in 1..2^31-1");
+    if (kv_heads < 1 || kv_heads > 1024) return fail("kv_heads must be in 1..1024");
+    if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+        return fail("page_size must be 16, 32, 64, 128 or 256");
+    if (dim < 16 || dim > 256 || dim % 16) return fail("dim must be a multiple of 16 in 16..256");
+    if (width < 1 || width > INT32_MAX / page_size) return fail("a table's row must have 1..(2^31-1)/page_size pages");
+    if (seqs < 1 || seqs > (1 << 20)) return fail("seqs must be in 1..2^20");
+    if (tokens < 1 || tokens > (1 << 22)) return fail("tokens must be in 1..2^22");
+    if (!starts && tokens != seqs) return fail("without starts there is one token for each sequence");
+    if (!aligned16(k) || !aligned16(v)) return fail("k and v must be 16-byte aligned");
+    return 0;
+}
+
+static int log2_of(int64_t v) { return 63 - __builtin_clzll((unsigned long long)v); }
+
+// Work is shared out where there are fewer than two tiles a CU.
+static AttnPlan plan_attention(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t keys) {
+    const int64_t group = heads / kv_heads, rows = (tokens + seqs - 1) / seqs * group, cus = device_cus();
+    AttnPlan P{};
+    P.rb = rows <= 16 ? 1 : rows <= 32 || dim > 128 ? 2 : 4;
+    const int64_t tiles = tokens * group / (16 * P.rb) + std::min(seqs, tokens), blocks = (keys + ATTN_KEYS - 1) / ATTN_KEYS;
+    P.tiles = (unsigned)tiles;
+    if (tiles * kv_heads < 2 * cus || P.rb == 1) {
+        const int64_t most = cus * (P.rb == 4 ? 1 : 2), units = tiles * kv_heads * std::max<int64_t>(blocks, 1);
+        P.shares = (unsigned)std::max<int64_t>(1, std::min(most, (units + ATTN_WAVES - 1) / ATTN_WAVES));
+        P.join_rows = 4;
+    }
+    return P;
+}
+
+static int64_t part_bytes(const AttnPlan& P, int64_t dim) {
+    const int64_t padded = (dim + 63) / 64 * 64;
+    return (int64_t)P.shares * 2 * 16 * P.rb * (padded + 2) * 4;
+}
+
+static int64_t keys_of(int64_t width, int64_t page_size, int64_t tokens, int64_t window) {
+    return window ? std::min(width * page_size, window + tokens + 2 * ATTN_KEYS) : width * page_size;
+}
+
+extern "C" {
+
+int exl3_fp8_cache_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                          int kind, int64_t tokens, uint8_t* k_cache, float* k_scale, uint8_t* v_cache, float* v_scale,
+                          int64_t pages, int64_t kv_heads, int64_t page_size, int64_t dim, const int32_t* table,
+                          int64_t table_stride, int64_t width, const int32_t* lengths, const int32_t* starts, int64_t seqs,
+                          void* stream) {
+    clear_error();
+    if (!k || !v) return fail("null pointer");
+    if (kind < OUT_F16 || kind > OUT_F32) return fail("kind must be 0 (fp16), 1 (bf16) or 2 (fp32)");
+    if (check_cache(k_cache, k_scale, v_cache, v_scale, pages, kv_heads, page_size, dim, table, width, lengths, starts, seqs,
+                    tokens))
+        return -1;
+    const int64_t each = kind == OUT_F32 ? 4 : 8;
+    if (!aligned16(k) || !aligned16(v) || k_token % each || k_head % each || v_token % each || v_head % each)
+        return fail("rows of k and v must be 16-byte aligned");
+    const AppendArgs A{{k_cache, k_scale, v_cache, v_scale, table, table_stride, lengths, starts, (int)seqs, (int)tokens,
+                        (int)kv_heads, (int)dim, log2_of(page_size), (int)width, (int)pages},
+                       k, v, k_token, k_head, v_token, v_head};
+    // pages that may be touched: each sequence's first and last one, and those that its tokens fill
+    const int64_t bound = starts ? std::min(tokens, tokens / page_size + 2 * seqs) : tokens;
+    const auto kernel = kind == OUT_F16    ? fp8_cache_append_kernel<OUT_F16>
+                        : kind == OUT_BF16 ? fp8_cache_append_kernel<OUT_BF16>
+                                           : fp8_cache_append_kernel<OUT_F32>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)bound, (unsigned)kv_heads, 2), dim3(APPEND_WAVES * 64), 0,
+                       reinterpret_cast<hipStream_t>(stream), A);
+    return check_launch();
+}
+
+int64_t exl3_fp8_attention_scratch_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs,
+                                         int64_t width, int64_t page_size, int64_t window) {
+    clear_error();
+    if (tokens < 1 || tokens > (1 << 22) || seqs < 1 || seqs > (1 << 20) || kv_heads < 1 || heads < kv_heads ||
+        heads % kv_heads || heads > 65536 || dim < 16 || dim > 256 || dim % 16 || page_size < 16 || page_size > 256 ||
+        width < 1 || width > INT32_MAX / page_size || window < 0)
+        return fail("sizes out of range");
+    return part_bytes(plan_attention(tokens, heads, kv_heads, dim, seqs, keys_of(width, page_size, tokens, window)), dim);
+}
+
+int exl3_fp8_attention(const void* q, int kind, int64_t q_token, int64_t q_head, int64_t tokens, int64_t heads,
+                       const uint8_t* k_cache, const float* k_scale, const uint8_t* v_cache, const float* v_scale,
+                       int64_t pages, int64_t kv_heads, int64_t page_size, int64_t dim, const int32_t* table,
+                       int64_t table_stride, int64_t width, const int32_t* lengths, const int32_t* starts, int64_t seqs,
+                       float scale, int64_t window, const float* sinks, void* out, float* lse, int clear, void* scratch,
+                       int64_t scratch_bytes, void* stream) {
+    clear_error();
+    if (!q || !out) return fail("null pointer");
+    if (kind != OUT_F16 && kind != OUT_BF16) return fail("kind must be 0 (fp16) or 1 (bf16)");
+    if (check_cache(k_cache, k_scale, v_cache, v_scale, pages, kv_heads, page_size, dim, table, width, lengths, starts, seqs,
+                    tokens))
+        return -1;
+    if (heads < kv_heads || heads % kv_heads || heads > 65536) return fail("heads must be a multiple of kv_heads up to 65536");
+    if (tokens * heads > INT32_MAX) return fail("too many rows");
+    if (!std::isfinite(scale)) return fail("scale must be finite");
+    if (window < 0 || window > INT32_MAX / 2) return fail("window must be in 0..2^30");
+    if (!aligned16(q) || !aligned16(out) || q_token % 8 || q_head % 8) return fail("rows of q and out must be 16-byte aligned");
+    const AttnPlan P = plan_attention(tokens, heads, kv_heads, dim, seqs, keys_of(width, page_size, tokens, window));
+    const int64_t need = part_bytes(P, dim);
+    if (need && !scratch) return fail("null pointer");
+    if (!aligned16(scratch)) return fail("scratch must be 16-byte aligned");
+    if (scratch_bytes < need) return fail("scratch too small");
+    AttnArgs A{{const_cast<uint8_t*>(k_cache), const_cast<float*>(k_scale), const_cast<uint8_t*>(v_cache),
+                const_cast<float*>(v_scale), table, table_stride, lengths, starts, (int)seqs, (int)tokens, (int)kv_heads,
+                (int)dim, log2_of(page_size), (int)width, (int)pages},
+               static_cast<const uint16_t*>(q), q_token, q_head, (int)heads, (int)(heads / kv_heads),
+               scale * 1.4426950408889634f, (int)window, sinks, static_cast<uint16_t*>(out), lse,
+               P.shares ? static_cast<float*>(scratch) : nullptr, ATTN_WAVES, clear != 0};
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const bool bf16 = kind == OUT_BF16;
+    if (dim <= 64) return launch_attention_64(A, P, bf16, s);
+    if (dim <= 128) return launch_attention_128(A, P, bf16, s);
+    if (dim <= 192) return launch_attention_192(A, P, bf16, s);
+    return launch_attention_256(A, P, bf16, s);
+}
+
+}  // extern "C"

@@ -15,14 +15,18 @@ Reference call surfaces mirrored here:
     recipe-lna/lna2/lna_moe_ticket.cu:481-581, bindings.cpp:212-219
 
 Beside them, for the layers a checkpoint keeps in block-scaled 8-bit floats
-(``fp8_quantize``, ``fp8_gemm``, ``fp8_linear``, ``fp8_moe``) and for the router
-in front of either expert layer (``moe_route``).
+(``fp8_quantize``, ``fp8_gemm``, ``fp8_linear``, ``fp8_moe``), for the router in
+front of either expert layer (``moe_route``), and for what such layers have between
+their products: the norm that makes 8-bit rows (``fp8_norm``), an 8-bit paged cache
+and the attention over it (``fp8_cache_append``, ``fp8_attention``).
 """
 
 from __future__ import annotations
 
 import functools
+import math
 import threading
+from typing import NamedTuple
 
 import torch
 
@@ -997,3 +1001,223 @@ def moe_route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", bias
     if m:
         torch.ops.exl3_amd.moe_route(logits, SCORING[scoring], bias, bool(renormalize), float(scale), ids, weights)
     return ids, weights
+
+
+# ------------------------------------------------------------------ between the 8-bit products
+
+_LIB.define("fp8_norm(Tensor x, Tensor? residual, Tensor weight, float eps, bool pow2, Tensor(a!) q, Tensor(b!) scale, "
+            "Tensor(c!)? total, Tensor(d!)? normed) -> ()")
+_LIB.define("fp8_cache_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) k_scale, Tensor(c!) v_cache, "
+            "Tensor(d!) v_scale, Tensor table, Tensor lengths, Tensor? starts) -> ()")
+_LIB.define("fp8_attention(Tensor q, Tensor k_cache, Tensor k_scale, Tensor v_cache, Tensor v_scale, Tensor table, "
+            "Tensor lengths, Tensor? starts, float scale, int window, Tensor? sinks, Tensor(a!) out, Tensor(b!)? lse, "
+            "bool clear, Tensor(c!)? scratch) -> ()")
+
+
+def _fp8_norm_impl(x, residual, weight, eps, pow2, q, scale, total, normed):
+    k = x.shape[-1]
+    _launch(x.device, "exl3_fp8_norm", x.data_ptr(), OUT_KIND[x.dtype], _ptr(residual),
+            0 if residual is None else OUT_KIND[residual.dtype], weight.data_ptr(), OUT_KIND[weight.dtype], x.numel() // k, k,
+            float(eps), int(pow2), q.data_ptr(), scale.data_ptr(), _ptr(total), _ptr(normed),
+            0 if normed is None else OUT_KIND[normed.dtype])
+
+
+def _cache_args(k_cache, k_scale, v_cache, v_scale, table, lengths, starts):
+    pages, heads, page, dim = k_cache.shape
+    return (k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(), pages, heads, page, dim,
+            table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(), _ptr(starts), table.shape[0])
+
+
+def _fp8_cache_append_impl(k, v, k_cache, k_scale, v_cache, v_scale, table, lengths, starts):
+    _launch(k.device, "exl3_fp8_cache_append", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+            OUT_KIND[k.dtype], k.shape[0], *_cache_args(k_cache, k_scale, v_cache, v_scale, table, lengths, starts))
+
+
+def _fp8_attention_impl(q, k_cache, k_scale, v_cache, v_scale, table, lengths, starts, scale, window, sinks, out, lse, clear,
+                        scratch):
+    _launch(q.device, "exl3_fp8_attention", q.data_ptr(), X_KIND[q.dtype], q.stride(0), q.stride(1), q.shape[0], q.shape[1],
+            *_cache_args(k_cache, k_scale, v_cache, v_scale, table, lengths, starts), float(scale), int(window), _ptr(sinks),
+            out.data_ptr(), _ptr(lse), int(clear), _ptr(scratch), 0 if scratch is None else scratch.numel())
+
+
+_LIB.impl("fp8_norm", _fp8_norm_impl, "CUDA")
+_LIB.impl("fp8_cache_append", _fp8_cache_append_impl, "CUDA")
+_LIB.impl("fp8_attention", _fp8_attention_impl, "CUDA")
+
+
+class Fp8Norm(NamedTuple):
+    """What fp8_norm makes: quantized rows and their scales; the new residual and the rows in 16 or 32 bits, or None."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+    residual: torch.Tensor | None
+    normed: torch.Tensor | None
+
+
+def fp8_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None, eps: float = 1e-6,
+             pow2: bool = False, normed_dtype: torch.dtype | None = None) -> Fp8Norm:
+    """The root-mean-square norm of x [..., k] (+ residual), quantized for fp8_gemm.
+
+    h = x + residual, y = h / sqrt(mean(h**2) + eps) * weight; q float8_e4m3fn
+    [..., k] and scale fp32 [..., ceil(k/128)] are fp8_quantize's formula on y, which
+    is not rounded before.  x, weight [k]: fp16, bf16 or fp32; residual of x's shape,
+    in x's dtype or fp32: the result's `residual` is h in that dtype, a tensor of its
+    own.  With `normed_dtype` (fp16, bf16 or fp32) y comes in it as well, for readers
+    that take 16-bit rows.  A row with a NaN is NaN; a row with an infinity has 0 for
+    its finite values and NaN for the others."""
+    _check(x.dim() >= 1 and x.dtype in OUT_KIND and x.is_contiguous(), "x must be contiguous fp16, bf16 or fp32 [..., k]")
+    k = x.shape[-1]
+    _check(1 <= k <= 1 << 24, "k must be in 1..2**24")
+    _check(weight.dtype in OUT_KIND and weight.is_contiguous() and weight.device == x.device and tuple(weight.shape) == (k,),
+           "weight must be contiguous fp16, bf16 or fp32 [k] on x's device")
+    _check(0.0 <= eps < float("inf"), "eps must be finite and not negative")
+    _check(normed_dtype is None or normed_dtype in OUT_KIND, "normed_dtype must be fp16, bf16 or fp32")
+    total = None
+    if residual is not None:
+        _check(residual.dtype in (x.dtype, torch.float32) and residual.is_contiguous() and residual.device == x.device and
+               residual.shape == x.shape, "residual must be contiguous, of x's shape, device and dtype (or fp32)")
+        total = torch.empty_like(residual)
+    q = torch.empty_like(x, dtype=E4M3)
+    scale = x.new_empty((*x.shape[:-1], _blocks(k)), dtype=torch.float32)
+    normed = None if normed_dtype is None else torch.empty_like(x, dtype=normed_dtype)
+    if x.numel():
+        torch.ops.exl3_amd.fp8_norm(x, residual, weight, float(eps), bool(pow2), q, scale, total, normed)
+    return Fp8Norm(q, scale, total, normed)
+
+
+class Fp8Cache(NamedTuple):
+    """A paged cache of e4m3 keys and values with an fp32 scale for each page and head; a value's tokens are neighbours."""
+
+    k: torch.Tensor            # float8_e4m3fn [pages, kv_heads, page, dim]
+    k_scale: torch.Tensor      # fp32 [pages, kv_heads]
+    v: torch.Tensor            # float8_e4m3fn [pages, kv_heads, dim, page]
+    v_scale: torch.Tensor      # fp32 [pages, kv_heads]
+
+
+FP8_CACHE_PAGES = (16, 32, 64, 128, 256)
+FP8_CACHE_MAX_DIM = 256
+
+
+def fp8_cache(pages: int, kv_heads: int, page: int, dim: int, device: torch.device | str = "cuda") -> Fp8Cache:
+    """An empty cache of `pages` pages of `page` tokens (16, 32, 64, 128 or 256), dim a multiple of 16 up to 256."""
+    _check(page in FP8_CACHE_PAGES, "page must be 16, 32, 64, 128 or 256")
+    _check(dim % 16 == 0 and 16 <= dim <= FP8_CACHE_MAX_DIM, "dim must be a multiple of 16 in 16..256")
+    _check(1 <= pages < 1 << 31 and 1 <= kv_heads <= 1024, "pages must be in 1..2**31-1 and kv_heads in 1..1024")
+    k = torch.zeros((pages, kv_heads, page, dim), dtype=torch.uint8, device=device).view(E4M3)
+    v = torch.zeros((pages, kv_heads, dim, page), dtype=torch.uint8, device=device).view(E4M3)
+    scale = torch.zeros((2, pages, kv_heads), dtype=torch.float32, device=device)
+    return Fp8Cache(k, scale[0], v, scale[1])
+
+
+def _check_cache(cache: Fp8Cache, table, lengths, starts, tokens: int, device: torch.device) -> None:
+    k, k_scale, v, v_scale = cache
+    _check(k.dim() == 4 and k.dtype == E4M3 and k.is_contiguous() and k.device == device,
+           "the cache's k must be contiguous float8_e4m3fn [pages, kv_heads, page, dim] on the input device")
+    pages, heads, page, dim = k.shape
+    _check(page in FP8_CACHE_PAGES, "page must be 16, 32, 64, 128 or 256")
+    _check(dim % 16 == 0 and 16 <= dim <= FP8_CACHE_MAX_DIM, "dim must be a multiple of 16 in 16..256")
+    _check(pages >= 1 and 1 <= heads <= 1024, "the cache must have a page and 1..1024 heads")
+    _check(v.dtype == E4M3 and v.is_contiguous() and v.device == device and tuple(v.shape) == (pages, heads, dim, page),
+           "the cache's v must be contiguous float8_e4m3fn [pages, kv_heads, dim, page] on the input device")
+    for t in (k_scale, v_scale):
+        _check(t.dtype == torch.float32 and t.is_contiguous() and t.device == device and tuple(t.shape) == (pages, heads),
+               "the cache's scales must be contiguous fp32 [pages, kv_heads] on the input device")
+    _check(table.dim() == 2 and table.dtype == torch.int32 and table.device == device and table.stride(1) == 1 and
+           table.shape[1] >= 1, "table must be int32 [seqs, pages] on the input device, rows contiguous")
+    seqs = table.shape[0]
+    _check(lengths.dtype == torch.int32 and lengths.is_contiguous() and lengths.device == device and
+           tuple(lengths.shape) == (seqs,), "lengths must be contiguous int32 [seqs] on the input device")
+    if starts is None:
+        _check(tokens == seqs, "without starts there is one token for each sequence")
+    else:
+        _check(starts.dtype == torch.int32 and starts.is_contiguous() and starts.device == device and
+               tuple(starts.shape) == (seqs + 1,), "starts must be contiguous int32 [seqs + 1] on the input device")
+
+
+def _token_rows(t: torch.Tensor) -> torch.Tensor:
+    """t [tokens, heads, dim], or a copy of it where a row's values are apart or off the 16-byte borders that the kernels read
+    by (a slice of a fused projection is taken as it is)."""
+    each = 16 // t.element_size()
+    if t.stride(2) == 1 and t.stride(0) % each == 0 and t.stride(1) % each == 0 and t.data_ptr() & 15 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def fp8_cache_append(k: torch.Tensor, v: torch.Tensor, cache: Fp8Cache, table: torch.Tensor, lengths: torch.Tensor,
+                     starts: torch.Tensor | None = None) -> Fp8Cache:
+    """Writes new keys and values [tokens, kv_heads, dim] (fp16, bf16 or fp32) into their sequences' pages.
+
+    table int32 [seqs, n]: a sequence's pages, in order; lengths int32 [seqs]: its
+    tokens, the new ones counted, which are its last; starts int32 [seqs + 1]:
+    sequence s has the call's tokens starts[s] .. starts[s + 1] - 1 (None: one token
+    each).  A page's scale is the smallest power of two that is not below its largest
+    magnitude / 448: over the new tokens, and where the page holds tokens of the
+    sequence already, not below the one it has; where it grows, their codes are
+    rounded to it.  A NaN or an infinity is kept as a NaN.  What the tables name out
+    of range is left out: tokens before position 0 or behind the table's room, pages
+    outside the cache.  A page that two sequences of one call write has a mixture of
+    both: sequences share pages that are full.  Returns the cache."""
+    _check(k.dim() == 3 and k.dtype in OUT_KIND, "k must be fp16, bf16 or fp32 [tokens, kv_heads, dim]")
+    _check(v.dtype == k.dtype and v.shape == k.shape and v.device == k.device, "v must be of k's shape, dtype and device")
+    _check_cache(cache, table, lengths, starts, k.shape[0], k.device)
+    _check(k.shape[1] == cache.k.shape[1] and k.shape[2] == cache.k.shape[3], "k must have the cache's heads and dim")
+    if k.shape[0] and table.shape[0]:
+        torch.ops.exl3_amd.fp8_cache_append(_token_rows(k), _token_rows(v), *cache, table, lengths, starts)
+    return cache
+
+
+@functools.lru_cache(maxsize=4096)
+def _fp8_attention_scratch_bytes(device_index: int, *sizes: int) -> int:
+    """What a call on that device needs: the library goes by the current one."""
+    with torch.cuda.device(device_index):
+        return int(_lib.check(_lib.load().exl3_fp8_attention_scratch_bytes(*sizes)))
+
+
+def fp8_attention(q: torch.Tensor, cache: Fp8Cache, table: torch.Tensor, lengths: torch.Tensor,
+                  starts: torch.Tensor | None = None, *, scale: float | None = None, window: int | None = None,
+                  sinks: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                  return_lse: bool = False) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Causal attention of the last tokens of each sequence over an 8-bit cache: out [tokens, heads, dim] in q's dtype.
+
+    q fp16 or bf16 [tokens, heads, dim], heads a multiple of the cache's kv_heads
+    (query head h reads cache head h // (heads // kv_heads)); table, lengths and starts
+    as fp8_cache_append takes them, with which the tokens' own keys are written first.
+    The query at position i sees the keys j <= i, with `window` those j > i - window.
+    scale: of the products, 1 / sqrt(dim) unless given; sinks fp32 [heads]: a logit
+    that joins each row's denominator.  With return_lse also the logarithm of the
+    denominator, fp32 [tokens, heads].  A query that sees no key has 0 (and -inf, or
+    its sink); a key that it does not see has no part in its result, whatever the
+    cache holds there.  Tokens outside every sequence are left as they were in an
+    `out` given, and are 0 otherwise.  Scratch is the call's own (stream-ordered,
+    capturable)."""
+    _check(q.dim() == 3 and q.dtype in X_KIND, "q must be fp16 or bf16 [tokens, heads, dim]")
+    tokens, heads, dim = q.shape
+    _check_cache(cache, table, lengths, starts, tokens, q.device)
+    _, kv_heads, page, cache_dim = cache.k.shape
+    _check(dim == cache_dim and heads >= kv_heads and heads % kv_heads == 0,
+           "q must have the cache's dim, and a multiple of its heads")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    _check(math.isfinite(scale), "scale must be finite")
+    _check(window is None or 1 <= window <= 1 << 30, "window must be in 1..2**30")
+    if sinks is not None:
+        _check(sinks.dtype == torch.float32 and sinks.is_contiguous() and sinks.device == q.device and
+               tuple(sinks.shape) == (heads,), "sinks must be contiguous fp32 [heads] on q's device")
+    clear = out is None
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+    _check(out.dtype == q.dtype and out.device == q.device and out.is_contiguous() and out.shape == q.shape,
+           "out must be contiguous, of q's shape, dtype and device")
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    if tokens and table.shape[0]:
+        scratch = None
+        if q.is_cuda:
+            nbytes = _fp8_attention_scratch_bytes(q.device.index, tokens, heads, kv_heads, dim, table.shape[0], table.shape[1],
+                                                  page, window or 0)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        torch.ops.exl3_amd.fp8_attention(_token_rows(q), *cache, table, lengths, starts, scale, window or 0, sinks, out, lse,
+                                         clear, scratch)
+    elif clear:
+        out.zero_()
+        if lse is not None:
+            lse.fill_(float("-inf"))
+    return (out, lse) if return_lse else out

@@ -362,6 +362,71 @@ int exl3_moe_route(const void* logits, int logits_kind, int64_t rows, int64_t n_
                    void* stream);
 
 /*
+ * The residual's addition and the root-mean-square norm, quantized as the
+ * block-scaled products read it: h = x + residual (or x), y = h / sqrt(mean(h^2)
+ * + eps) * weight, (q, scale) = exl3_fp8_quantize's formula on y, all of it in 64
+ * bits up to each result's rounding.  sum: h in the residual's type (may be the
+ * residual itself).  normed: y as normed_kind, or null.  A row whose sum of squares
+ * is not finite has what 64-bit arithmetic makes of y: NaN (its scales 2^-126), or
+ * 0 beside an infinity.  Kinds 0 = fp16, 1 = bf16, 2 = fp32; the residual is of x's
+ * kind or fp32, or null; any rows >= 1, 1 <= k <= 2^24, 0 <= eps finite.
+ */
+int exl3_fp8_norm(const void* x, int x_kind, const void* residual, int residual_kind, const void* weight,
+                  int weight_kind, int64_t rows, int64_t k, float eps, int pow2, uint8_t* q, float* scale, void* sum,
+                  void* normed, int normed_kind, void* stream);
+
+/*
+ * A paged cache of e4m3 keys and values with an fp32 scale for each page and head:
+ *   k [pages][kv_heads][page_size][dim]   k_scale [pages][kv_heads]
+ *   v [pages][kv_heads][dim][page_size]   v_scale [pages][kv_heads]
+ * k and v 16-byte aligned; page_size 16, 32, 64, 128 or 256, dim a multiple of 16 up
+ * to 256.  A sequence's pages are the first ones of its row of `table` (int32
+ * [seqs][table_stride], width columns); lengths int32 [seqs] count its tokens, those
+ * of the call included.  starts int32 [seqs + 1]: sequence s has the call's tokens
+ * starts[s] .. starts[s + 1] - 1, which are its last ones; null for one token each
+ * (tokens == seqs).  All four are read on the device: a length past the table's row
+ * counts as the row's room, a page outside the cache is left out, and starts are cut
+ * to 0..tokens.
+ *
+ * exl3_fp8_cache_append writes the call's keys and values (strides in values, rows
+ * 16-byte aligned; kind 0 = fp16, 1 = bf16, 2 = fp32).  A page's scale becomes the
+ * smallest power of two s with max|x| <= 448 s over its new tokens (at least 2^-126;
+ * NaN and infinities left out), or stays where the page holds tokens of the sequence
+ * already and has a larger one; where it grows, their codes are rounded to it.  A NaN
+ * or an infinity becomes a NaN.  Tokens before position 0 are left out.  A page that
+ * two sequences of one call write has a mixture of both.
+ */
+int exl3_fp8_cache_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                          int64_t v_head, int kind, int64_t tokens, uint8_t* k_cache, float* k_scale,
+                          uint8_t* v_cache, float* v_scale, int64_t pages, int64_t kv_heads, int64_t page_size,
+                          int64_t dim, const int32_t* table, int64_t table_stride, int64_t width,
+                          const int32_t* lengths, const int32_t* starts, int64_t seqs, void* stream);
+
+/*
+ * Causal attention of the call's tokens over that cache: query head h reads cache
+ * head h / (heads / kv_heads); the query at position i sees keys j <= i, with
+ * window > 0 those with j > i - window.
+ *   out = sum_j e^(scale q.k_j) v_j / (sum_j e^(scale q.k_j) + e^sinks[h])
+ * q (kind 0 = fp16, 1 = bf16; strides in values, rows 16-byte aligned), out [tokens]
+ * [heads][dim] of the same kind, 16-byte aligned; sinks fp32 [heads] or null; lse
+ * fp32 [tokens][heads] or null: the logarithm of the denominator.  A query that sees
+ * nothing has out 0 and lse -inf (its sink, where there is one).  A key that a query
+ * does not see has no part in its result, whatever its bytes.  Tokens outside every
+ * sequence are left as they were; with `clear` they become 0 and -inf.
+ * scratch: >= exl3_fp8_attention_scratch_bytes(...) bytes, asked for with the call's
+ * device current, 16-byte aligned, no zeroing needed (may be null where the size is
+ * 0); one call at a time per buffer.
+ */
+int64_t exl3_fp8_attention_scratch_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs,
+                                         int64_t width, int64_t page_size, int64_t window);
+int exl3_fp8_attention(const void* q, int kind, int64_t q_token, int64_t q_head, int64_t tokens, int64_t heads,
+                       const uint8_t* k_cache, const float* k_scale, const uint8_t* v_cache, const float* v_scale,
+                       int64_t pages, int64_t kv_heads, int64_t page_size, int64_t dim, const int32_t* table,
+                       int64_t table_stride, int64_t width, const int32_t* lengths, const int32_t* starts,
+                       int64_t seqs, float scale, int64_t window, const float* sinks, void* out, float* lse, int clear,
+                       void* scratch, int64_t scratch_bytes, void* stream);
+
+/*
  * Launch geometry for diagnostics (replaces lna2_moe_info,
  * recipe-lna/lna2/lna_moe_ticket.cu:494-505): writes up to n values
  * {cus, waves_per_launch, threads_per_wave, max_rows, max_pairs, step_k, cols,
