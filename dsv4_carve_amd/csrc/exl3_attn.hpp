@@ -262,7 +262,8 @@ struct AttnArgs {
     const uint16_t* q;
     int64_t q_token, q_head;                  // strides in values
     int heads, group;                         // query heads, and of each cache head
-    float qk_scale;                           // scale * log2(e)
+    float qk_scale;                           // |scale| * log2(e)
+    bool negative;                            // scale < 0
     int window;                               // 0: none
     const float* sinks;                       // [heads] or null
     uint16_t* out;                            // [tokens][heads][dim]
@@ -327,12 +328,121 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t u) {       // 0x80 in eac
 // are, the column operand of O^T = V^T P^T, for which a lane reads 16 neighbouring
 // tokens of one channel.  A lane's 16 keys are of one page: one pair of scales.
 //
-// Softmax: weights are 2^(s - m) against a reference m that follows the row's largest
-// logit with some slack, and the values' scale joins the weight, as 2^(s - m) * vs *
-// 2^(HEADROOM - c), where c follows the row's largest log2 of weight times scale: so
-// the 16-bit operand neither overflows nor loses a row whose values are small.  Sums
-// are fp32.  A 16-bit weight has 11 bits, three more than a bf16 result; for an fp16
-// result the rest of the weight goes through the product as well (FINE).
+// Softmax: the 16-bit operand of the second product is w = 2^(s - m + k), with a
+// reference m that follows the row's largest logit with some slack, and k = log2(value
+// scale) + HEADROOM - c, where c follows the row's largest log2 of weight times scale:
+// so it neither overflows nor loses a row whose values are small.  (k is -64 at least:
+// less counts as nothing beside the row's largest.)  The denominator is the sum of w
+// 2^-k.  Sums are fp32.  A 16-bit weight has 11 bits, three more than a bf16 result;
+// for an fp16 result the rest of the weight goes through the product as well (FINE).
+//
+// Memory wants neighbouring lanes on neighbouring bytes, the products lanes of
+// different keys and channels: a wave's loads go by whole rows (16 bytes a lane) and are
+// turned in LDS, in a place of its own, so that no barrier is needed.  Chunks of 16
+// bytes are XORed with their row: neither side meets a bank twice in eight lanes.
+// Loads are of buffers that end with the page: what lies outside is not read and comes
+// back as zeros, so a call's end and a page that is none need no branch.
+template <int DIM>
+struct AttnStage {
+    static constexpr int SUB = DIM % 128 == 0 ? 128 : 64, CS = SUB / 16, SUBS = DIM / SUB, KEYS = 64 / CS;
+    static constexpr int LOADS = DIM / 16;                    // loads of 16 bytes a lane for the keys or values of a block
+    static constexpr int K_BYTES = ATTN_KEYS * DIM, BYTES = 2 * K_BYTES;
+
+    char* lds;                   // keys [64][DIM], values [DIM][64]
+    int k_write, v_write, k_read[2], v_read;
+    uint32_t k_off[SUBS], v_off;
+    int lg;                      // log2 of the neighbouring chunks of a value's row
+
+    __device__ __forceinline__ AttnStage(const CacheView& C, char* lds_) : lds(lds_) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+        const int key = lane / CS, chunk = lane % CS;
+        const int sw = SUB == 128 ? key & 3 : (key >> 1) & 1;
+        k_write = key * DIM + ((chunk ^ sw) << 4);
+        const int sr = SUB == 128 ? (r & 3) | (r >> 2 & 1) << 2 : (r >> 1 & 1) | (r >> 2 & 1) << 1;
+        const int row = (16 * (r >> 2) + (r & 3)) * DIM;
+        k_read[0] = row + ((g ^ sr) << 4);
+        k_read[1] = SUB == 128 ? row + (((4 + g) ^ sr) << 4) : k_read[0] + 64;
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s) {
+            const int c = s * SUB + chunk * 16;
+            k_off[s] = c < C.dim ? key * C.dim + c : OUTSIDE; // behind the row's end: zeros
+        }
+        lg = min(C.page_shift, 6) - 4;
+        const int v_row = lane >> lg, v_chunk = (lane & ((1 << lg) - 1)) << 4;
+        v_off = (v_row << C.page_shift) + v_chunk;            // channels behind the last are outside the page
+        v_write = K_BYTES + v_row * 64 + (v_chunk ^ ((v_row >> 1 & 3) << 4));
+        v_read = K_BYTES + r * 64 + ((g ^ (r >> 1 & 3)) << 4);
+    }
+
+    // Bytes of a page and head from `at` on; none where ids' lane group g names no page, or without `on`.
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t part(const CacheView& C, const uint8_t* p, int head, int ids, int g,
+                                                                  int at, bool on) {
+        const int id = __builtin_amdgcn_readlane(ids, 16 * g);
+        const bool is = on && (unsigned)id < (unsigned)C.pages;
+        const uint32_t bytes = (uint32_t)C.dim << C.page_shift;                   // below 2^16, and 1024 heads of it below 2^32
+        return __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(p) + (uint64_t)(uint32_t)(is ? id : 0) * ((uint32_t)C.kv * bytes) + (head * bytes + at), 0,
+            is ? bytes - at : 0, 0x27000);
+    }
+
+    __device__ __forceinline__ void load_k(const CacheView& C, int head, int b, int ids, bool on, u32x4_t (&z)[LOADS]) const {
+        const int mask = (1 << C.page_shift) - 1;
+        __amdgpu_buffer_rsrc_t p[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) p[g] = part(C, C.k, head, ids, g, ((b * ATTN_KEYS + 16 * g) & mask) * C.dim, on);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int key = j / SUBS * KEYS;
+            z[j] = __builtin_amdgcn_raw_buffer_load_b128(p[key >> 4], k_off[j % SUBS], (key & 15) * C.dim, 0);
+        }
+    }
+
+    __device__ __forceinline__ void load_v(const CacheView& C, int head, int b, int ids, bool on, u32x4_t (&z)[LOADS]) const {
+        const int mask = (1 << C.page_shift) - 1;
+        __amdgpu_buffer_rsrc_t p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int g = (i & ((1 << (2 - lg)) - 1)) << lg;
+            p[i] = part(C, C.v, head, ids, g, (b * ATTN_KEYS + 16 * g) & mask, on);
+        }
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+            z[j] = __builtin_amdgcn_raw_buffer_load_b128(p[j & 3], v_off + (j >> (2 - lg) << (6 - lg + C.page_shift)), 0, 0);
+    }
+
+    // Between what some lanes of the wave write and others read: LDS keeps a wave's order, the compiler has to.
+    static __device__ __forceinline__ void order() { asm volatile("" ::: "memory"); }
+
+    __device__ __forceinline__ void put_k(const u32x4_t (&z)[LOADS]) const {
+        order();
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int key = j / SUBS * KEYS;
+            const int at = key >> 4 & 1 ? k_write ^ (SUB == 128 ? 64 : 32) : k_write;
+            *reinterpret_cast<u32x4_t*>(lds + at + key * DIM + j % SUBS * SUB) = z[j];
+        }
+        order();
+    }
+
+    __device__ __forceinline__ void put_v(const u32x4_t (&z)[LOADS]) const {
+        order();
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int g = (j & ((1 << (2 - lg)) - 1)) << lg, channel = j >> (2 - lg) << (6 - lg);
+            *reinterpret_cast<u32x4_t*>(lds + (v_write ^ (g << 4)) + channel * 64) = z[j];
+        }
+        order();
+    }
+
+    // 16 values of key 16 (lane % 16 / 4) + 4 t + lane % 4, from 64 k + 16 (lane / 16) on
+    __device__ __forceinline__ u32x4_t key(int t, int k) const {
+        return *reinterpret_cast<const u32x4_t*>(lds + k_read[k & 1] + k / 2 * 128 + 4 * t * DIM);
+    }
+
+    // 16 tokens, from 16 (lane / 16) on, of channel 16 d + lane % 16
+    __device__ __forceinline__ u32x4_t& value(int d) const { return *reinterpret_cast<u32x4_t*>(lds + v_read + d * 1024); }
+};
+
 template <int DIM, bool BF16, int RB>
 struct AttnWave {
     static constexpr bool FINE = !BF16;
@@ -353,9 +463,11 @@ struct AttnWave {
         }
     }
 
-    // blocks first, first + step, ... < last of the tile's keys
-    __device__ __forceinline__ void run(const AttnArgs& A, const Seq& q, const Tile& x, int s, int head, int first, int last,
-                                        int step) {
+    // Blocks first, first + step, ... < last of the tile's keys.  No branch divides lanes in here: the compiler may leave
+    // them apart in the loop around the products, and may place copies of other lanes' registers before they are back.
+    __device__ __forceinline__ void run(const AttnArgs& A, const AttnStage<DIM>& S, const Seq& q, const Tile& x, int s, int head,
+                                        int first, int last, int step) {
+        if (first >= last) return;
         const CacheView& C = A.c;
         const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
         const int base = q.len - q.n;
@@ -363,181 +475,138 @@ struct AttnWave {
         int see_lo[RB], see_hi[RB];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            const int row = 16 * rb + r, at = (x.r0 + row) / A.group, hg = x.r0 + row - at * A.group;
+            const int row = 16 * rb + r;
             const bool in = row < x.rows;
+            const int of = x.r0 + (in ? row : 0), at = of / A.group, hg = of - at * A.group;
             const uint16_t* p = A.q + (int64_t)(q.first + at) * A.q_token + (int64_t)(head * A.group + hg) * A.q_head;
 #pragma unroll
             for (int k = 0; k < KC; ++k)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int d = 64 * k + 16 * g + 8 * u;
-                    qf[rb][k][u] = __builtin_bit_cast(typename H::vec8, u32x4_t{0, 0, 0, 0});
-                    if (in && d < C.dim) qf[rb][k][u] = *reinterpret_cast<const typename H::vec8*>(p + d);
+                    const bool is = in && d < C.dim;
+                    const u32x4_t z = *reinterpret_cast<const u32x4_t*>(p + (d < C.dim ? d : 0));
+                    u32x4_t v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = is ? A.negative ? z[i] ^ 0x80008000u : z[i] : 0u;
+                    qf[rb][k][u] = __builtin_bit_cast(typename H::vec8, v);
                 }
             see_hi[rb] = in ? min(base + at + 1, q.len) : 0;
             see_lo[rb] = in && A.window ? base + at + 1 - A.window : 0;
         }
         const int* table = C.table + s * C.table_stride;
         const int pages = (q.len + (1 << C.page_shift) - 1) >> C.page_shift;
-        const int gk = r >> 2;                                    // the group of the key that this lane reads
-        // No branch here or in the loads: lanes that a branch divides may stay apart in the loop around the products.
-        const auto page_id = [&](int b, int group) {
-            const int i = (b * ATTN_KEYS + 16 * group) >> C.page_shift, id = table[min(i, pages - 1)];
+        // The page of lane group g's 16 keys.
+        const auto pages_of = [&](int b) {
+            const int i = (min(b, last - 1) * ATTN_KEYS + 16 * g) >> C.page_shift, id = table[min(i, pages - 1)];
             return i < pages ? id : -1;
         };
-        const int mask = (1 << C.page_shift) - 1;
-        u32x4_t kraw[4][KC], vraw[DT];
-        float ks, vs;
-        int idk, idv;                                             // pages of the block whose keys are read next
         const auto valid = [&](int id) { return (unsigned)id < (unsigned)C.pages; };
-        const auto load_k = [&](int b, int id) {
-            const int64_t block = (int64_t)(valid(id) ? id : 0) * C.kv + head;
-            const uint8_t* p = C.k + ((block << C.page_shift) + ((b * ATTN_KEYS + 16 * gk + (r & 3)) & mask)) * C.dim;
+        const auto scale_of = [&](const float* p, int id) { return p[(int64_t)(valid(id) ? id : 0) * C.kv + head]; };
+        // In a block that not every row sees whole, what no row sees may hold anything: its bytes become zeros (a weight of 0
+        // would leave a NaN one).  A NaN that only some rows see becomes a zero too, and `nans` has it counted later.
+        bool nans = false;
+        const auto hide_values = [&](int b, bool here, bool keep_nans) {
+            const int key0 = b * ATTN_KEYS + 16 * g;
+            uint32_t keep[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int j = 0; j < 4; ++j) {
+                keep[j] = 0;
 #pragma unroll
-                for (int k = 0; k < KC; ++k) {
-                    const int d = 64 * k + 16 * g;                // behind the row's end: its first values, against zeros
-                    kraw[t][k] = *reinterpret_cast<const u32x4_t*>(p + 4 * t * C.dim + (d < C.dim ? d : 0));
+                for (int e = 0; e < 4; ++e) {
+                    const int key = key0 + 4 * j + e;
+                    if (here && key >= x.lo && key < x.hi) keep[j] |= 0xffu << (8 * e);
                 }
-        };
-        const auto load_v = [&](int b, int id) {
-            const int64_t block = (int64_t)(valid(id) ? id : 0) * C.kv + head;
-            const uint8_t* p = C.v + ((block * C.dim) << C.page_shift) + ((b * ATTN_KEYS + 16 * g) & mask);
+            }
+            uint32_t nan = 0;
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const int channel = 16 * d < C.dim ? 16 * d + r : r;          // behind the last: not stored
-                vraw[d] = *reinterpret_cast<const u32x4_t*>(p + (channel << C.page_shift));
+                u32x4_t v = S.value(d);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] &= keep[j];
+                    const uint32_t bad = nan_bytes(v[j]);
+                    nan |= bad;
+                    if (!keep_nans) v[j] &= ~((bad >> 7) * 0xffu);
+                }
+                S.value(d) = v;
             }
+            S.order();
+            nans |= __builtin_amdgcn_ballot_w64(nan != 0) != 0;
         };
-        const auto load_scales = [&](int id) {
-            const int64_t block = (int64_t)(valid(id) ? id : 0) * C.kv + head;
-            ks = C.k_scale[block];
-            vs = C.v_scale[block];
-        };
-        if (first >= last) return;
-        idk = page_id(first, gk);
-        idv = page_id(first, g);
-        load_k(first, idk);
-        load_scales(idv);
-        load_v(first, idv);
-        int id_now = idv;
-        if (first + step < last) {
-            idk = page_id(first + step, gk);
-            idv = page_id(first + step, g);
-        }
+
+        u32x4_t kreg[DT], vreg[DT];
+        int ids = pages_of(first), next = pages_of(first + step);  // asked for two blocks ahead: loads come back in order
+        S.load_k(C, head, first, ids, true, kreg);
+        float ks = scale_of(C.k_scale, ids), vs = scale_of(C.v_scale, ids);
+        S.load_v(C, head, first, ids, true, vreg);
         for (int b = first; b < last; b += step) {
+            const int id_here = ids;
+            float kc = fmaxf(ks * A.qk_scale, 0x1p-126f), vscale = vs;
+            const int after = pages_of(b + 2 * step);
             const bool more = b + step < last;
+            S.put_k(kreg);
+            S.load_k(C, head, b + step, next, more, kreg);
+            ks = scale_of(C.k_scale, next);
+            vs = scale_of(C.v_scale, next);
             float4_t p[4][RB];
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) p[t][rb] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int k = 0; k < KC; ++k)
 #pragma unroll
-                for (int k = 0; k < KC; ++k)
+                for (int t = 0; t < 4; ++t) {
+                    const u32x4_t z = S.key(t, k);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const typename H::vec8 key = H::widen(kraw[t][k][2 * u], kraw[t][k][2 * u + 1]);
+                        const typename H::vec8 key = H::widen(z[2 * u], z[2 * u + 1]);
 #pragma unroll
                         for (int rb = 0; rb < RB; ++rb) p[t][rb] = H::mfma(key, qf[rb][k][u], p[t][rb]);
                     }
-            const float kc = ks * A.qk_scale, vscale = vs;
-            const int id_here = id_now;
-            if (more) {
-                load_k(b + step, idk);
-                load_scales(idv);
-                id_now = idv;
-                if (b + 2 * step < last) idk = page_id(b + 2 * step, gk);
-            }
+                }
+            S.put_v(vreg);
+            S.load_v(C, head, b + step, next, more, vreg);
+            ids = next;
+            next = after;
+            if (b * ATTN_KEYS < x.full_lo || (b + 1) * ATTN_KEYS > x.full_hi ||
+                __builtin_amdgcn_ballot_w64(valid(id_here)) != ~0ull) {
+                const int key0 = b * ATTN_KEYS + 16 * g;
+                const bool here = valid(id_here) && key0 + 15 >= x.lo && key0 < x.hi;
+                kc = here ? kc : 1.f;
+                vscale = here ? vscale : 1.f;
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) p[t][rb][i] *= kc;
-            const int key0 = b * ATTN_KEYS + 16 * g;
-            const bool here = valid(id_here);
-            const bool whole = b * ATTN_KEYS >= x.full_lo && (b + 1) * ATTN_KEYS <= x.full_hi &&
-                               __builtin_amdgcn_ballot_w64(here) == ~0ull;
-            if (!whole) {
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
+                for (int rb = 0; rb < RB; ++rb) {
+                    const int lo = here ? see_lo[rb] - key0 : 16, n = see_hi[rb] - key0;
 #pragma unroll
                     for (int t = 0; t < 4; ++t)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int key = key0 + 4 * t + i;
-                            if (!(here && key >= see_lo[rb] && key < see_hi[rb])) p[t][rb][i] = -__builtin_inff();
+                            const int key = 4 * t + i;
+                            p[t][rb][i] = key >= lo && key < n ? p[t][rb][i] : -__builtin_inff();
                         }
-                // Nothing that no row sees may reach a sum: a weight of 0 leaves a NaN one.
-                uint32_t keep[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    keep[j] = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = key0 + 4 * j + e;
-                        if (here && key >= x.lo && key < x.hi) keep[j] |= 0xffu << (8 * e);
-                    }
                 }
-                uint32_t nan = 0;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        vraw[d][j] &= keep[j];
-                        nan |= nan_bytes(vraw[d][j]);
-                    }
-                // A NaN that only some of the rows see: counted for those in a product of its own, and 0 in the others'.
-                if (__builtin_amdgcn_ballot_w64(nan != 0)) {
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) {
-                        half8_t sees[2];
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const int key = key0 + 8 * u + j;
-                                sees[u][j] = here && key >= see_lo[rb] && key < see_hi[rb] ? (_Float16)1.f : (_Float16)0.f;
-                            }
-#pragma unroll
-                        for (int d = 0; d < DT; ++d) {
-                            float4_t n = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                            for (int u = 0; u < 2; ++u)
-                                n = W::mfma(W::widen((nan_bytes(vraw[d][2 * u]) >> 7) * 0x38u,        // 0x38: one
-                                                     (nan_bytes(vraw[d][2 * u + 1]) >> 7) * 0x38u), sees[u], n);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (n[i] > 0.f) o[d][rb][i] = __builtin_nanf("");
-                        }
-                    }
-#pragma unroll
-                    for (int d = 0; d < DT; ++d)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) vraw[d][j] &= ~((nan_bytes(vraw[d][j]) >> 7) * 0xffu);
-                }
+                hide_values(b, here, false);
             }
-            // log2 of a bound of the values' scale: vscale < 2^ev
-            const float ev = (float)((int)(__float_as_uint(vscale) >> 23 & 0xff) - 126);
-            float most[RB];
+            const float lv = __builtin_amdgcn_logf(vscale);
             bool grew = false;
+            float most[RB];
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-                most[rb] = p[0][rb][0];
+                float a = p[0][rb][0];
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (t + i) most[rb] = fmaxf(most[rb], p[t][rb][i]);
-                grew |= most[rb] > m[rb] + ATTN_SLACK || most[rb] + ev > top[rb] + ATTN_SLACK;
+                        if (t + i) a = fmaxf(a, p[t][rb][i]);
+                most[rb] = a * kc;
+                grew |= most[rb] > m[rb] + ATTN_SLACK || most[rb] + lv > top[rb] + ATTN_SLACK;
             }
             if (__builtin_amdgcn_ballot_w64(grew)) {
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    const float m1 = fmaxf(m[rb], xor_max(most[rb])), top1 = fmaxf(top[rb], xor_max(most[rb] + ev));
+                    const float m1 = fmaxf(m[rb], xor_max(most[rb])), top1 = fmaxf(top[rb], xor_max(most[rb] + lv));
                     const float c1 = ceilf(top1 - m1);
                     const float fl = __builtin_amdgcn_exp2f(m[rb] - m1);
                     const float fo = __builtin_amdgcn_exp2f(m[rb] - m1 + (c[rb] - c1));
@@ -554,33 +623,64 @@ struct AttnWave {
             half8_t hi[RB][2], lo[RB][2];
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-                const float f = ldexpf(vscale, ATTN_HEADROOM - (int)c[rb]);
+                const float k = fmaxf(lv + (ATTN_HEADROOM - c[rb]), -64.f), add = k - m[rb];
+                float sum = 0.f;
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(p[t][rb][i] - m[rb]);
-                        l[rb] += e;
-                        const float w = e * f;
+                        const float w = __builtin_amdgcn_exp2f(fmaf(p[t][rb][i], kc, add));
+                        sum += w;
                         const _Float16 h = (_Float16)w;
                         hi[rb][t >> 1][4 * (t & 1) + i] = h;
                         if constexpr (FINE) lo[rb][t >> 1][4 * (t & 1) + i] = (_Float16)(w - (float)h);
                     }
+                l[rb] = fmaf(sum, __builtin_amdgcn_exp2f(-k), l[rb]);
             }
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+            for (int d = 0; d < DT; ++d) {
+                const u32x4_t z = S.value(d);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const half8_t v = W::widen(vraw[d][2 * u], vraw[d][2 * u + 1]);
+                    const half8_t v = W::widen(z[2 * u], z[2 * u + 1]);
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb) {
                         o[d][rb] = W::mfma(v, hi[rb][u], o[d][rb]);
                         if constexpr (FINE) o[d][rb] = W::mfma(v, lo[rb][u], o[d][rb]);
                     }
                 }
-            if (more) {
-                load_v(b + step, id_now);
-                if (b + 2 * step < last) idv = page_id(b + 2 * step, g);
+            }
+        }
+        if (!nans) return;
+        // NaN values that were left out above: counted for the rows that see them, in products of their own.
+        for (int b = first; b < last; b += step) {
+            const int id = pages_of(b);
+            const int key0 = b * ATTN_KEYS + 16 * g;
+            const bool here = valid(id) && key0 + 15 >= x.lo && key0 < x.hi;
+            S.load_v(C, head, b, id, true, vreg);
+            S.put_v(vreg);
+            hide_values(b, here, true);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                half8_t sees[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int key = key0 + 8 * u + j;
+                        sees[u][j] = here && key >= see_lo[rb] && key < see_hi[rb] ? (_Float16)1.f : (_Float16)0.f;
+                    }
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const u32x4_t z = S.value(d);
+                    float4_t n = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        n = W::mfma(W::widen((nan_bytes(z[2 * u]) >> 7) * 0x38u, (nan_bytes(z[2 * u + 1]) >> 7) * 0x38u),
+                                    sees[u], n);                                             // 0x38: one
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[d][rb][i] = n[i] > 0.f ? __builtin_nanf("") : o[d][rb][i];
+                }
             }
         }
     }
@@ -589,7 +689,9 @@ struct AttnWave {
 template <int DIM, int RB>
 struct AttnSize {
     static constexpr int ROWS = 16 * RB, PITCH = DIM + 4;
-    static constexpr int LDS = ATTN_WAVES * ROWS * (PITCH + 2) * 4;
+    static constexpr int JOIN = ATTN_WAVES * ROWS * (PITCH + 2) * 4, STAGE = ATTN_WAVES * AttnStage<DIM>::BYTES;
+    static constexpr int LDS = JOIN > STAGE ? JOIN : STAGE;       // the blocks of the waves, then their sums
+    static constexpr int WAVES_EU = RB <= 2 && DIM <= 128 ? 2 : 1;
     static constexpr int PART = ROWS * (DIM + 2);                 // floats of a partial result: rows of sums, then m and l
 };
 
@@ -638,9 +740,9 @@ __device__ __forceinline__ void clear_rows(const AttnArgs& A) {
 // second where it goes on behind it.  Without a place for partial results a workgroup
 // has a tile: blockIdx.x is the tile (the last, longest ones first), blockIdx.y the head.
 template <int DIM, bool BF16, int RB>
-__global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_kernel(AttnArgs A) {
+__global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) void fp8_attention_kernel(AttnArgs A) {
     typedef AttnSize<DIM, RB> Z;
-    extern __shared__ float lds[];
+    extern __shared__ __attribute__((aligned(16))) float lds[];
     __shared__ int64_t scan[ATTN_WAVES];
     __shared__ int64_t found[2];
     const CacheView& C = A.c;
@@ -684,6 +786,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_kernel(AttnArgs
         n = blocks_of(x);
         u1 = n;
     }
+    const AttnStage<DIM> S(C, reinterpret_cast<char*>(lds) + wave * AttnStage<DIM>::BYTES);
     float* sums = lds;                                          // [wave][row][PITCH]
     float* ml = lds + ATTN_WAVES * Z::ROWS * Z::PITCH;          // [wave][row][2]
     for (;;) {
@@ -692,7 +795,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_kernel(AttnArgs
         const int b0 = x.lo / ATTN_KEYS + done;
         AttnWave<DIM, BF16, RB> W;
         W.clear();
-        W.run(A, q, x, s, head, b0 + wave, min(b0 + here, (x.hi + ATTN_KEYS - 1) / ATTN_KEYS), ATTN_WAVES);
+        W.run(A, S, q, x, s, head, b0 + wave, min(b0 + here, (x.hi + ATTN_KEYS - 1) / ATTN_KEYS), ATTN_WAVES);
         __syncthreads();
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
@@ -700,10 +803,8 @@ __global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_kernel(AttnArgs
             float l = W.l[rb];
             l += __shfl_xor(l, 16);
             l += __shfl_xor(l, 32);
-            if (g == 0) {
-                ml[(wave * Z::ROWS + row) * 2] = W.m[rb];
-                ml[(wave * Z::ROWS + row) * 2 + 1] = l;
-            }
+            ml[(wave * Z::ROWS + row) * 2] = W.m[rb];           // by four lanes alike: no branch while the sums are live
+            ml[(wave * Z::ROWS + row) * 2 + 1] = l;
             const int back = (int)W.c[rb] - ATTN_HEADROOM;
 #pragma unroll
             for (int d = 0; d < DIM / 16; ++d) {
@@ -750,6 +851,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_kernel(AttnArgs
         }
         u += here;
         if (u >= u1) break;
+        __syncthreads();                                        // the sums' places hold blocks again
         done = 0;
         if (++t == tiles_of(A, q, Z::ROWS)) {
             t = 0;

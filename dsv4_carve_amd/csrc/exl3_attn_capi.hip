@@ -115,7 +115,7 @@ int exl3_fp8_attention(const void* q, int kind, int64_t q_token, int64_t q_head,
                 const_cast<float*>(v_scale), table, table_stride, lengths, starts, (int)seqs, (int)tokens, (int)kv_heads,
                 (int)dim, log2_of(page_size), (int)width, (int)pages},
                static_cast<const uint16_t*>(q), q_token, q_head, (int)heads, (int)(heads / kv_heads),
-               scale * 1.4426950408889634f, (int)window, sinks, static_cast<uint16_t*>(out), lse,
+               std::fabs(scale) * 1.4426950408889634f, scale < 0.f, (int)window, sinks, static_cast<uint16_t*>(out), lse,
                P.shares ? static_cast<float*>(scratch) : nullptr, ATTN_WAVES, clear != 0};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const bool bf16 = kind == OUT_BF16;
