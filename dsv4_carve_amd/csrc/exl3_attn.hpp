@@ -82,26 +82,39 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t (&lds)[WAVES], 
     return before + sum - v;
 }
 
-// The sequence that unit `at` of all sequences' units lies in, by a scan over the
-// sequences; count(s) units each.  Returns the total; found[0] is -1 where `at` is
-// behind it, found[1] the unit within the sequence.
-template <int WAVES, typename Count>
-__device__ __forceinline__ int64_t find_seq(int seqs, int64_t at, int64_t (&lds)[WAVES], int64_t (&found)[2], Count&& count) {
-    int64_t sum = 0;
-    if (threadIdx.x == 0) found[0] = -1;
-    for (int s0 = 0; s0 < seqs; s0 += WAVES * 64) {
-        const int s = s0 + threadIdx.x;
-        const int64_t c = s < seqs ? count(s) : 0;
-        int64_t total;
-        const int64_t before = sum + block_scan<WAVES>(c, lds, total);
-        if (at >= before && at < before + c) {
+// The sequence that a unit of all sequences' units lies in, by a scan over the
+// sequences; count(s) units each.  The unit is at(total), total being all of them;
+// found[0] is -1 where it lies behind them, found[1] the unit within the sequence.
+template <int WAVES, typename Count, typename At>
+__device__ __forceinline__ void find_seq(int seqs, int64_t (&lds)[WAVES], int64_t (&found)[2], Count&& count, At&& at) {
+    constexpr int THREADS = WAVES * 64;
+    const int tid = threadIdx.x;
+    if (tid == 0) found[0] = -1;
+    const auto here = [&](int s, int64_t before, int64_t c, int64_t want) {
+        if (want >= before && want < before + c) {
             found[0] = s;
-            found[1] = at - before;
+            found[1] = want - before;
         }
-        sum += total;
+    };
+    int64_t total;
+    if (seqs <= THREADS) {
+        const int64_t c = tid < seqs ? count(tid) : 0, before = block_scan<WAVES>(c, lds, total);
+        here(tid, before, c, at(uniform(total)));
+    } else {
+        int64_t sum = 0;
+        for (int s0 = 0; s0 < seqs; s0 += THREADS) {
+            block_scan<WAVES>(s0 + tid < seqs ? count(s0 + tid) : 0, lds, total);
+            sum += total;
+        }
+        const int64_t want = at(uniform(sum));
+        sum = 0;
+        for (int s0 = 0; s0 < seqs; s0 += THREADS) {
+            const int64_t c = s0 + tid < seqs ? count(s0 + tid) : 0, before = sum + block_scan<WAVES>(c, lds, total);
+            here(s0 + tid, before, c, want);
+            sum += total;
+        }
     }
     __syncthreads();
-    return uniform(sum);
 }
 
 // ---------------------------------------------------------------- the write
@@ -162,7 +175,8 @@ __global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(App
     const bool values = blockIdx.z;
     int s = blockIdx.x, nth = 0;
     if (C.starts) {
-        find_seq<APPEND_WAVES>(C.seqs, blockIdx.x, lds, found, [&](int i) { return (int64_t)touched_pages(C, get_seq(C, i)); });
+        find_seq<APPEND_WAVES>(C.seqs, lds, found, [&](int i) { return (int64_t)touched_pages(C, get_seq(C, i)); },
+                               [](int64_t) { return (int64_t)blockIdx.x; });
         if (found[0] < 0) return;
         s = uniform((int)found[0]);
         nth = uniform((int)found[1]);
@@ -257,6 +271,13 @@ constexpr float ATTN_LOW = -3.402823466e+38f; // a row's reference before its fi
 constexpr float ATTN_SLACK = 6.f;             // how far a logit may pass the reference (log2) before sums are rescaled
 constexpr int ATTN_HEADROOM = 8;              // 16-bit weights are below 2^(SLACK + HEADROOM) < 65504
 
+// A tile that goes on behind the share of the workgroup that begins it.
+struct SharedTile {
+    int first, r0, rows, head;                // the sequence's first token; the tile's rows within it; the cache head
+    int last;                                 // the workgroup of its last unit; -1: there is no such tile
+    int unused[3];
+};
+
 struct AttnArgs {
     CacheView c;
     const uint16_t* q;
@@ -268,7 +289,8 @@ struct AttnArgs {
     const float* sinks;                       // [heads] or null
     uint16_t* out;                            // [tokens][heads][dim]
     float* lse;                               // [tokens][heads] or null
-    float* part;                              // partial results of shared items, or null: a workgroup an item
+    float* part;                              // partial results of shared tiles, or null: a workgroup a tile
+    SharedTile* shared;                       // a workgroup's shared tile
     int least;                                // units that a workgroup has at least
     bool clear;                               // rows that no sequence has are zeroed
 };
@@ -747,23 +769,25 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
     __shared__ int64_t found[2];
     const CacheView& C = A.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, g = lane >> 4;
-    int64_t u = 0, u1 = 0, total = 0;
+    int64_t u = 0, u1 = 0, share = 0;
     int s = 0, t = 0, head = 0, done = 0;                       // done: the tile's blocks before the share
     Seq q;
     Tile x;
     int n = 0;
     clear_rows(A);
     if (A.part) {
-        const auto count = [&](int i) { return units_of(A, get_seq(C, i), Z::ROWS); };
-        total = find_seq<ATTN_WAVES>(C.seqs, 0, scan, found, count);
-        const int64_t all = total * C.kv;
-        int64_t share = (all + gridDim.x - 1) / gridDim.x;
-        if (share < A.least) share = A.least;
-        u = share * blockIdx.x;
-        u1 = u + share < all ? u + share : all;
+        find_seq<ATTN_WAVES>(C.seqs, scan, found, [&](int i) { return units_of(A, get_seq(C, i), Z::ROWS); }, [&](int64_t total) {
+            const int64_t all = total * C.kv;
+            share = (all + gridDim.x - 1) / gridDim.x;
+            if (share < A.least) share = A.least;
+            u = share * blockIdx.x;
+            u1 = u + share < all ? u + share : all;
+            if (u >= u1) return (int64_t)-1;
+            head = (int)(u / total);
+            return u - head * total;
+        });
+        if (tid == 0) A.shared[blockIdx.x].last = -1;            // nothing to join, unless a tile goes on behind the share
         if (u >= u1) return;
-        head = (int)(u / total);
-        find_seq<ATTN_WAVES>(C.seqs, u - head * total, scan, found, count);
         s = uniform((int)found[0]);
         int64_t left = uniform(found[1]);
         q = get_seq(C, s);
@@ -776,7 +800,8 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
         done = (int)left;
     } else {
         const int64_t at = (int64_t)gridDim.x - 1 - blockIdx.x;
-        find_seq<ATTN_WAVES>(C.seqs, at, scan, found, [&](int i) { return (int64_t)tiles_of(A, get_seq(C, i), Z::ROWS); });
+        find_seq<ATTN_WAVES>(C.seqs, scan, found, [&](int i) { return (int64_t)tiles_of(A, get_seq(C, i), Z::ROWS); },
+                             [&](int64_t) { return at; });
         if (found[0] < 0) return;
         s = uniform((int)found[0]);
         t = uniform((int)found[1]);
@@ -816,6 +841,8 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
         }
         __syncthreads();
         const bool final = here == n;
+        if (!final && done == 0 && tid == 0)
+            A.shared[blockIdx.x] = SharedTile{q.first, x.r0, x.rows, head, (int)((u + n - 1) / share)};
         float* part = A.part + ((int64_t)blockIdx.x * 2 + (done == 0 ? 1 : 0)) * Z::PART;
         const int quads = C.dim / 4;
         for (int i = tid; i < x.rows * quads; i += ATTN_WAVES * 64) {
@@ -868,60 +895,62 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
     }
 }
 
-// The tiles that a border between two workgroups' shares divides, joined by the
-// workgroup of the first such border; blockIdx.y takes every gridDim.y-th row.
+// A tile that several workgroups share, joined: blockIdx.x is the workgroup that
+// begins it, blockIdx.y takes every gridDim.y-th row.  A row's threads are groups that
+// each take some of the partial results, four channels a thread; the groups' sums
+// meet in LDS.
 template <int DIM, bool BF16, int RB>
-__global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_join_kernel(AttnArgs A, int shares) {
+__global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_join_kernel(AttnArgs A) {
     typedef AttnSize<DIM, RB> Z;
-    __shared__ int64_t scan[ATTN_WAVES];
-    __shared__ int64_t found[2];
+    constexpr int QUADS = DIM / 4, GROUPS = ATTN_WAVES * 64 / QUADS;
+    __shared__ float4_t sums[GROUPS][QUADS];
+    __shared__ float ml[GROUPS][2];
     const CacheView& C = A.c;
-    const auto count = [&](int i) { return units_of(A, get_seq(C, i), Z::ROWS); };
-    const int64_t total = find_seq<ATTN_WAVES>(C.seqs, 0, scan, found, count);
-    const int64_t all = total * C.kv;
-    int64_t share = (all + shares - 1) / shares;
-    if (share < A.least) share = A.least;
-    const int64_t u = share * ((int64_t)blockIdx.x + 1);
-    if (u >= all) return;
-    const int head = (int)(u / total);
-    find_seq<ATTN_WAVES>(C.seqs, u - head * total, scan, found, count);
-    const int s = uniform((int)found[0]);
-    int64_t left = uniform(found[1]);
-    const Seq q = get_seq(C, s);
-    Tile x;
-    int n;
-    for (int t = 0;; ++t) {
-        x = get_tile(A, q, t, Z::ROWS);
-        n = blocks_of(x);
-        if (left < n) break;
-        left -= n;
-    }
-    if (left == 0 || left > share) return;                       // the tile begins here, or a border before this divides it
-    const int last = (int)((u - left + n - 1) / share);          // the workgroup of the tile's last unit
-    const int first = blockIdx.x;
-    const auto place = [&](int w) { return A.part + ((int64_t)w * 2 + (w == first ? 1 : 0)) * Z::PART; };
-    const int quads = C.dim / 4, rows = (x.rows - (int)blockIdx.y + (int)gridDim.y - 1) / (int)gridDim.y;
-    for (int i = threadIdx.x; i < rows * quads; i += ATTN_WAVES * 64) {
-        const int nth = i / quads, d = (i - nth * quads) * 4, row = nth * gridDim.y + blockIdx.y;
+    const SharedTile x = A.shared[blockIdx.x];
+    const int first = blockIdx.x, group = threadIdx.x / QUADS, d = (threadIdx.x - group * QUADS) * 4;
+    if (x.last < 0) return;
+    for (int row = blockIdx.y; row < x.rows; row += gridDim.y) {
         float m = ATTN_LOW, l = 0.f;
-        for (int w = first; w <= last; ++w) m = fmaxf(m, place(w)[Z::ROWS * DIM + 2 * row]);
         float4_t v = {0.f, 0.f, 0.f, 0.f};
-        for (int w = first; w <= last; ++w) {
-            const float* p = place(w);
-            const float f = __builtin_amdgcn_exp2f(p[Z::ROWS * DIM + 2 * row] - m);
-            l += f * p[Z::ROWS * DIM + 2 * row + 1];
-            const float4_t a = *reinterpret_cast<const float4_t*>(p + row * C.dim + d);
+        if (group < GROUPS && d < C.dim) {
+#pragma unroll 4
+            for (int w = first + group; w <= x.last; w += GROUPS) {
+                const float* p = A.part + ((int64_t)w * 2 + (w == first ? 1 : 0)) * Z::PART;
+                const float pm = p[Z::ROWS * DIM + 2 * row], pl = p[Z::ROWS * DIM + 2 * row + 1];
+                const float4_t a = *reinterpret_cast<const float4_t*>(p + row * C.dim + d);
+                const float m1 = fmaxf(m, pm), f = __builtin_amdgcn_exp2f(m - m1), g = __builtin_amdgcn_exp2f(pm - m1);
+                m = m1;
+                l = fmaf(g, pl, l * f);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = fmaf(f, a[j], v[j]);
+                for (int j = 0; j < 4; ++j) v[j] = fmaf(g, a[j], v[j] * f);
+            }
+            sums[group][d / 4] = v;
+            if (d == 0) {
+                ml[group][0] = m;
+                ml[group][1] = l;
+            }
         }
-        const int at = (x.r0 + row) / A.group, h = head * A.group + x.r0 + row - at * A.group;
-        const int64_t o = (int64_t)(q.first + at) * A.heads + h;
-        float lse;
-        const float f = finish_row(A, h, m, l, lse);
+        __syncthreads();
+        if (group == 0 && d < C.dim) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] *= f;
-        store_row4<BF16>(A.out + o * C.dim + d, v);
-        if (A.lse && d == 0) A.lse[o] = lse;
+            for (int i = 1; i < GROUPS; ++i) {
+                const float m1 = fmaxf(m, ml[i][0]), f = __builtin_amdgcn_exp2f(m - m1), g = __builtin_amdgcn_exp2f(ml[i][0] - m1);
+                m = m1;
+                l = fmaf(g, ml[i][1], l * f);
+                const float4_t a = sums[i][d / 4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = fmaf(g, a[j], v[j] * f);
+            }
+            const int at = (x.r0 + row) / A.group, h = x.head * A.group + x.r0 + row - at * A.group;
+            const int64_t o = (int64_t)(x.first + at) * A.heads + h;
+            float lse;
+            const float f = finish_row(A, h, m, l, lse);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] *= f;
+            store_row4<BF16>(A.out + o * C.dim + d, v);
+            if (A.lse && d == 0) A.lse[o] = lse;
+        }
+        __syncthreads();
     }
 }
 

@@ -36,14 +36,19 @@ static AttnPlan plan_attention(int64_t tokens, int64_t heads, int64_t kv_heads, 
     if (tiles * kv_heads < 2 * cus || P.rb == 1) {
         const int64_t most = cus * (P.rb == 4 ? 1 : 2), units = tiles * kv_heads * std::max<int64_t>(blocks, 1);
         P.shares = (unsigned)std::max<int64_t>(1, std::min(most, (units + ATTN_WAVES - 1) / ATTN_WAVES));
-        P.join_rows = 4;
+        P.join_rows = (unsigned)(P.shares > 4 * tiles * kv_heads ? 16 * P.rb : 4 * P.rb);
     }
     return P;
 }
 
+// Partial results, and what the workgroups say of them.
 static int64_t part_bytes(const AttnPlan& P, int64_t dim) {
     const int64_t padded = (dim + 63) / 64 * 64;
     return (int64_t)P.shares * 2 * 16 * P.rb * (padded + 2) * 4;
+}
+
+static int64_t attention_scratch(const AttnPlan& P, int64_t dim) {
+    return P.shares ? part_bytes(P, dim) + (int64_t)P.shares * (int64_t)sizeof(SharedTile) : 0;
 }
 
 static int64_t keys_of(int64_t width, int64_t page_size, int64_t tokens, int64_t window) {
@@ -86,7 +91,7 @@ int64_t exl3_fp8_attention_scratch_bytes(int64_t tokens, int64_t heads, int64_t 
         heads % kv_heads || heads > 65536 || dim < 16 || dim > 256 || dim % 16 || page_size < 16 || page_size > 256 ||
         width < 1 || width > INT32_MAX / page_size || window < 0)
         return fail("sizes out of range");
-    return part_bytes(plan_attention(tokens, heads, kv_heads, dim, seqs, keys_of(width, page_size, tokens, window)), dim);
+    return attention_scratch(plan_attention(tokens, heads, kv_heads, dim, seqs, keys_of(width, page_size, tokens, window)), dim);
 }
 
 int exl3_fp8_attention(const void* q, int kind, int64_t q_token, int64_t q_head, int64_t tokens, int64_t heads,
@@ -107,7 +112,7 @@ int exl3_fp8_attention(const void* q, int kind, int64_t q_token, int64_t q_head,
     if (window < 0 || window > INT32_MAX / 2) return fail("window must be in 0..2^30");
     if (!aligned16(q) || !aligned16(out) || q_token % 8 || q_head % 8) return fail("rows of q and out must be 16-byte aligned");
     const AttnPlan P = plan_attention(tokens, heads, kv_heads, dim, seqs, keys_of(width, page_size, tokens, window));
-    const int64_t need = part_bytes(P, dim);
+    const int64_t need = attention_scratch(P, dim);
     if (need && !scratch) return fail("null pointer");
     if (!aligned16(scratch)) return fail("scratch must be 16-byte aligned");
     if (scratch_bytes < need) return fail("scratch too small");
@@ -116,7 +121,8 @@ int exl3_fp8_attention(const void* q, int kind, int64_t q_token, int64_t q_head,
                 (int)dim, log2_of(page_size), (int)width, (int)pages},
                static_cast<const uint16_t*>(q), q_token, q_head, (int)heads, (int)(heads / kv_heads),
                std::fabs(scale) * 1.4426950408889634f, scale < 0.f, (int)window, sinks, static_cast<uint16_t*>(out), lse,
-               P.shares ? static_cast<float*>(scratch) : nullptr, ATTN_WAVES, clear != 0};
+               P.shares ? static_cast<float*>(scratch) : nullptr,
+               reinterpret_cast<SharedTile*>(static_cast<char*>(scratch) + part_bytes(P, dim)), ATTN_WAVES, clear != 0};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const bool bf16 = kind == OUT_BF16;
     if (dim <= 64) return launch_attention_64(A, P, bf16, s);

@@ -18,9 +18,10 @@ static int launch(const AttnArgs& A, const AttnPlan& P, hipStream_t s) {
     }
     if (P.shares) {
         hipLaunchKernelGGL(kernel, dim3(P.shares), dim3(ATTN_WAVES * 64), LDS, s, A);
-        if (check_launch() || P.shares == 1) return P.shares == 1 ? 0 : -1;
+        if (check_launch()) return -1;
+        if (P.shares == 1) return 0;
         hipLaunchKernelGGL((fp8_attention_join_kernel<DIM, BF16, RB>), dim3(P.shares - 1, P.join_rows), dim3(ATTN_WAVES * 64), 0,
-                           s, A, (int)P.shares);
+                           s, A);
     } else {
         hipLaunchKernelGGL(kernel, dim3(P.tiles, A.c.kv), dim3(ATTN_WAVES * 64), LDS, s, A);
     }
