@@ -59,62 +59,62 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
     return __builtin_bit_cast(int64_t, u32x2_t{(uint32_t)uniform((int)a[0]), (uint32_t)uniform((int)a[1])});
 }
 
-// Exclusive prefix sum of one value a thread over a workgroup of WAVES waves, and the total.
-template <int WAVES>
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t (&lds)[WAVES], int64_t& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t sum = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t up = __shfl_up(sum, d);
-        if (lane >= d) sum += up;
-    }
-    __syncthreads();
-    if (lane == 63) lds[wave] = sum;
-    __syncthreads();
-    int64_t before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        if (w < wave) before += lds[w];
-        total += lds[w];
-    }
-    return before + sum - v;
+// Inclusive prefix sums over the wave's lanes.
+__device__ __forceinline__ int64_t wave_scan(int64_t v) {
+    v += lane_of<0x111, 0xf>(v, (int64_t)0);        // row_shr:1, 2, 4, 8
+    v += lane_of<0x112, 0xf>(v, (int64_t)0);
+    v += lane_of<0x114, 0xf>(v, (int64_t)0);
+    v += lane_of<0x118, 0xf>(v, (int64_t)0);
+    v += lane_of<0x142, 0xa>(v, (int64_t)0);        // row_bcast:15, 31
+    v += lane_of<0x143, 0xc>(v, (int64_t)0);
+    return v;
 }
 
-// The sequence that a unit of all sequences' units lies in, by a scan over the
-// sequences; count(s) units each.  The unit is at(total), total being all of them;
-// found[0] is -1 where it lies behind them, found[1] the unit within the sequence.
-template <int WAVES, typename Count, typename At>
-__device__ __forceinline__ void find_seq(int seqs, int64_t (&lds)[WAVES], int64_t (&found)[2], Count&& count, At&& at) {
-    constexpr int THREADS = WAVES * 64;
-    const int tid = threadIdx.x;
-    if (tid == 0) found[0] = -1;
-    const auto here = [&](int s, int64_t before, int64_t c, int64_t want) {
-        if (want >= before && want < before + c) {
-            found[0] = s;
-            found[1] = want - before;
-        }
+// a / b, 0 <= a, 0 < b; in 32 bits where both fit.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+    return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// The sequence that a unit of all sequences' units lies in; count(q) units each.  The
+// unit is at(total), total being all of them; s is -1 where it lies behind them.  Every
+// wave looks by itself: up to 64 sequences are one load and one scan.
+struct Found {
+    int s;
+    int64_t unit;                // within the sequence
+    Seq q;
+};
+
+template <typename Count, typename At>
+__device__ __forceinline__ Found find_seq(const CacheView& C, Count&& count, At&& at) {
+    const int lane = threadIdx.x & 63;
+    const Seq none{0, 0, 0};
+    Found f{-1, 0, none};
+    const auto look = [&](int s0, const Seq& q, int64_t c, int64_t before, int64_t sum, int64_t want) {
+        before += sum - c;
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(want >= before && want < before + c);
+        if (!hit) return;
+        const int l = __builtin_ctzll(hit);
+        f.s = s0 + l;
+        f.unit = want - read_lane(before, l);
+        f.q = Seq{read_lane(q.first, l), read_lane(q.n, l), read_lane(q.len, l)};
     };
-    int64_t total;
-    if (seqs <= THREADS) {
-        const int64_t c = tid < seqs ? count(tid) : 0, before = block_scan<WAVES>(c, lds, total);
-        here(tid, before, c, at(uniform(total)));
+    if (C.seqs <= 64) {
+        const Seq q = lane < C.seqs ? get_seq(C, lane) : none;
+        const int64_t c = count(q), sum = wave_scan(c);
+        look(0, q, c, 0, sum, at(read_lane(sum, 63)));
     } else {
-        int64_t sum = 0;
-        for (int s0 = 0; s0 < seqs; s0 += THREADS) {
-            block_scan<WAVES>(s0 + tid < seqs ? count(s0 + tid) : 0, lds, total);
-            sum += total;
-        }
-        const int64_t want = at(uniform(sum));
-        sum = 0;
-        for (int s0 = 0; s0 < seqs; s0 += THREADS) {
-            const int64_t c = s0 + tid < seqs ? count(s0 + tid) : 0, before = sum + block_scan<WAVES>(c, lds, total);
-            here(s0 + tid, before, c, want);
-            sum += total;
+        int64_t c = 0;
+        for (int s = lane; s < C.seqs; s += 64) c += count(get_seq(C, s));
+        const int64_t want = at(read_lane(wave_scan(c), 63));
+        int64_t before = 0;
+        for (int s0 = 0; s0 < C.seqs && want >= before && f.s < 0; s0 += 64) {
+            const Seq q = s0 + lane < C.seqs ? get_seq(C, s0 + lane) : none;
+            const int64_t n = count(q), sum = wave_scan(n);
+            look(s0, q, n, before, sum, want);
+            before += read_lane(sum, 63);
         }
     }
-    __syncthreads();
+    return f;
 }
 
 // ---------------------------------------------------------------- the write
@@ -167,21 +167,22 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t u, float by) {
 // The inputs are read twice (the second time from cache).
 template <int K>
 __global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(AppendArgs A) {
-    __shared__ int64_t lds[APPEND_WAVES];
-    __shared__ int64_t found[2];
     __shared__ float most_of[APPEND_WAVES];
     const CacheView& C = A.c;
     const int tid = threadIdx.x, head = blockIdx.y;
     const bool values = blockIdx.z;
     int s = blockIdx.x, nth = 0;
+    Seq q;
     if (C.starts) {
-        find_seq<APPEND_WAVES>(C.seqs, lds, found, [&](int i) { return (int64_t)touched_pages(C, get_seq(C, i)); },
-                               [](int64_t) { return (int64_t)blockIdx.x; });
-        if (found[0] < 0) return;
-        s = uniform((int)found[0]);
-        nth = uniform((int)found[1]);
+        const Found f = find_seq(C, [&](const Seq& x) { return (int64_t)touched_pages(C, x); },
+                                 [](int64_t) { return (int64_t)blockIdx.x; });
+        if (f.s < 0) return;
+        s = f.s;
+        nth = (int)f.unit;
+        q = f.q;
+    } else {
+        q = get_seq(C, s);
     }
-    const Seq q = get_seq(C, s);
     const int page = 1 << C.page_shift, base = q.len - q.n, from = max(base, 0);
     if (q.len <= from) return;
     const int at = (from >> C.page_shift) + nth;                                  // the page's place in the sequence
@@ -765,8 +766,6 @@ template <int DIM, bool BF16, int RB>
 __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) void fp8_attention_kernel(AttnArgs A) {
     typedef AttnSize<DIM, RB> Z;
     extern __shared__ __attribute__((aligned(16))) float lds[];
-    __shared__ int64_t scan[ATTN_WAVES];
-    __shared__ int64_t found[2];
     const CacheView& C = A.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, g = lane >> 4;
     int64_t u = 0, u1 = 0, share = 0;
@@ -776,21 +775,21 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
     int n = 0;
     clear_rows(A);
     if (A.part) {
-        find_seq<ATTN_WAVES>(C.seqs, scan, found, [&](int i) { return units_of(A, get_seq(C, i), Z::ROWS); }, [&](int64_t total) {
+        const Found f = find_seq(C, [&](const Seq& x) { return units_of(A, x, Z::ROWS); }, [&](int64_t total) {
             const int64_t all = total * C.kv;
-            share = (all + gridDim.x - 1) / gridDim.x;
+            share = divide(all + gridDim.x - 1, gridDim.x);
             if (share < A.least) share = A.least;
             u = share * blockIdx.x;
             u1 = u + share < all ? u + share : all;
             if (u >= u1) return (int64_t)-1;
-            head = (int)(u / total);
+            head = (int)divide(u, total);
             return u - head * total;
         });
         if (tid == 0) A.shared[blockIdx.x].last = -1;            // nothing to join, unless a tile goes on behind the share
-        if (u >= u1) return;
-        s = uniform((int)found[0]);
-        int64_t left = uniform(found[1]);
-        q = get_seq(C, s);
+        if (f.s < 0) return;
+        s = f.s;
+        q = f.q;
+        int64_t left = f.unit;
         for (;; ++t) {
             x = get_tile(A, q, t, Z::ROWS);
             n = blocks_of(x);
@@ -800,13 +799,12 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
         done = (int)left;
     } else {
         const int64_t at = (int64_t)gridDim.x - 1 - blockIdx.x;
-        find_seq<ATTN_WAVES>(C.seqs, scan, found, [&](int i) { return (int64_t)tiles_of(A, get_seq(C, i), Z::ROWS); },
-                             [&](int64_t) { return at; });
-        if (found[0] < 0) return;
-        s = uniform((int)found[0]);
-        t = uniform((int)found[1]);
+        const Found f = find_seq(C, [&](const Seq& x) { return (int64_t)tiles_of(A, x, Z::ROWS); }, [&](int64_t) { return at; });
+        if (f.s < 0) return;
+        s = f.s;
+        q = f.q;
+        t = (int)f.unit;
         head = blockIdx.y;
-        q = get_seq(C, s);
         x = get_tile(A, q, t, Z::ROWS);
         n = blocks_of(x);
         u1 = n;
@@ -842,7 +840,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
         __syncthreads();
         const bool final = here == n;
         if (!final && done == 0 && tid == 0)
-            A.shared[blockIdx.x] = SharedTile{q.first, x.r0, x.rows, head, (int)((u + n - 1) / share)};
+            A.shared[blockIdx.x] = SharedTile{q.first, x.r0, x.rows, head, (int)divide(u + n - 1, share)};
         float* part = A.part + ((int64_t)blockIdx.x * 2 + (done == 0 ? 1 : 0)) * Z::PART;
         const int quads = C.dim / 4;
         for (int i = tid; i < x.rows * quads; i += ATTN_WAVES * 64) {
@@ -909,21 +907,44 @@ __global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_join_kernel(Att
     const SharedTile x = A.shared[blockIdx.x];
     const int first = blockIdx.x, group = threadIdx.x / QUADS, d = (threadIdx.x - group * QUADS) * 4;
     if (x.last < 0) return;
+    const auto take = [&](int w, int row, float& m, float& l, float4_t& v) {
+        const float* p = A.part + ((int64_t)w * 2 + (w == first ? 1 : 0)) * Z::PART;
+        const float pm = p[Z::ROWS * DIM + 2 * row], pl = p[Z::ROWS * DIM + 2 * row + 1];
+        const float4_t a = *reinterpret_cast<const float4_t*>(p + row * C.dim + d);
+        const float m1 = fmaxf(m, pm), f = __builtin_amdgcn_exp2f(m - m1), g = __builtin_amdgcn_exp2f(pm - m1);
+        m = m1;
+        l = fmaf(g, pl, l * f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = fmaf(g, a[j], v[j] * f);
+    };
+    const auto finish = [&](int row, float m, float l, float4_t v) {
+        const int at = (x.r0 + row) / A.group, h = x.head * A.group + x.r0 + row - at * A.group;
+        const int64_t o = (int64_t)(x.first + at) * A.heads + h;
+        float lse;
+        const float f = finish_row(A, h, m, l, lse);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] *= f;
+        store_row4<BF16>(A.out + o * C.dim + d, v);
+        if (A.lse && d == 0) A.lse[o] = lse;
+    };
+    if (x.last - first < 2 * GROUPS) {
+        // few partial results: a row a group
+        if (group >= GROUPS || d >= C.dim) return;
+        for (int row = blockIdx.y * GROUPS + group; row < x.rows; row += gridDim.y * GROUPS) {
+            float m = ATTN_LOW, l = 0.f;
+            float4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (int w = first; w <= x.last; ++w) take(w, row, m, l, v);
+            finish(row, m, l, v);
+        }
+        return;
+    }
     for (int row = blockIdx.y; row < x.rows; row += gridDim.y) {
         float m = ATTN_LOW, l = 0.f;
         float4_t v = {0.f, 0.f, 0.f, 0.f};
         if (group < GROUPS && d < C.dim) {
 #pragma unroll 4
-            for (int w = first + group; w <= x.last; w += GROUPS) {
-                const float* p = A.part + ((int64_t)w * 2 + (w == first ? 1 : 0)) * Z::PART;
-                const float pm = p[Z::ROWS * DIM + 2 * row], pl = p[Z::ROWS * DIM + 2 * row + 1];
-                const float4_t a = *reinterpret_cast<const float4_t*>(p + row * C.dim + d);
-                const float m1 = fmaxf(m, pm), f = __builtin_amdgcn_exp2f(m - m1), g = __builtin_amdgcn_exp2f(pm - m1);
-                m = m1;
-                l = fmaf(g, pl, l * f);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = fmaf(g, a[j], v[j] * f);
-            }
+            for (int w = first + group; w <= x.last; w += GROUPS) take(w, row, m, l, v);
             sums[group][d / 4] = v;
             if (d == 0) {
                 ml[group][0] = m;
@@ -941,14 +962,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_join_kernel(Att
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] = fmaf(g, a[j], v[j] * f);
             }
-            const int at = (x.r0 + row) / A.group, h = x.head * A.group + x.r0 + row - at * A.group;
-            const int64_t o = (int64_t)(x.first + at) * A.heads + h;
-            float lse;
-            const float f = finish_row(A, h, m, l, lse);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] *= f;
-            store_row4<BF16>(A.out + o * C.dim + d, v);
-            if (A.lse && d == 0) A.lse[o] = lse;
+            finish(row, m, l, v);
         }
         __syncthreads();
     }
