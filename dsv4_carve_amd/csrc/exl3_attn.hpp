@@ -292,6 +292,7 @@ struct AttnArgs {
     float* lse;                               // [tokens][heads] or null
     float* part;                              // partial results of shared tiles, or null: a workgroup a tile
     SharedTile* shared;                       // a workgroup's shared tile
+    int tiles;                                // tiles at most
     int least;                                // units that a workgroup has at least
     bool clear;                               // rows that no sequence has are zeroed
 };
@@ -755,13 +756,39 @@ __device__ __forceinline__ void clear_rows(const AttnArgs& A) {
     }
 }
 
+// Workgroups go to the XCDs in turn (workgroup b to XCD b % 8), and what one reads its
+// neighbours on the XCD find in L2: so an XCD's workgroups take neighbouring work.
+constexpr int XCDS = 8;
+
+// Workgroup b's place where each XCD's workgroups are next to each other.
+__device__ __forceinline__ int by_xcd(int b, int n) {
+    const int x = b % XCDS, each = n / XCDS, more = n % XCDS;
+    return x * each + min(x, more) + b / XCDS;
+}
+
+// A workgroup a tile: a head's tiles in turn on the XCDs that the head has, or an XCD's heads one after another.
+__device__ __forceinline__ void tile_by_xcd(int b, int tiles, int heads, int& tile, int& head) {
+    const int x = b % XCDS, i = b / XCDS;
+    if (heads < XCDS && XCDS % heads == 0) {
+        const int of = XCDS / heads;
+        head = x / of;
+        tile = i * of + x % of;
+    } else if (heads % XCDS == 0) {
+        head = x * (heads / XCDS) + i / tiles;
+        tile = i % tiles;
+    } else {
+        head = b / tiles;
+        tile = b % tiles;
+    }
+}
+
 // Units are (cache head, tile, block of keys), in this order; a workgroup has an
 // equal share of them, next to each other, whatever sequences they are of.  Its four
 // waves go through a tile's blocks in turn and join their sums in LDS.  A tile whose
 // blocks one workgroup has all is finished; of the others each workgroup leaves a
 // partial result: in its first place where the tile began before its share, in its
 // second where it goes on behind it.  Without a place for partial results a workgroup
-// has a tile: blockIdx.x is the tile (the last, longest ones first), blockIdx.y the head.
+// has a tile, the last, longest ones first.
 template <int DIM, bool BF16, int RB>
 __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) void fp8_attention_kernel(AttnArgs A) {
     typedef AttnSize<DIM, RB> Z;
@@ -773,19 +800,22 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
     Seq q;
     Tile x;
     int n = 0;
+    int me = blockIdx.x;
     clear_rows(A);
     if (A.part) {
         const Found f = find_seq(C, [&](const Seq& x) { return units_of(A, x, Z::ROWS); }, [&](int64_t total) {
             const int64_t all = total * C.kv;
             share = divide(all + gridDim.x - 1, gridDim.x);
             if (share < A.least) share = A.least;
-            u = share * blockIdx.x;
+            const int busy = (int)divide(all + share - 1, share);
+            if (me >= busy) return (int64_t)-1;
+            me = by_xcd(me, busy);
+            u = share * me;
             u1 = u + share < all ? u + share : all;
-            if (u >= u1) return (int64_t)-1;
             head = (int)divide(u, total);
             return u - head * total;
         });
-        if (tid == 0) A.shared[blockIdx.x].last = -1;            // nothing to join, unless a tile goes on behind the share
+        if (tid == 0) A.shared[me].last = -1;            // nothing to join, unless a tile goes on behind the share
         if (f.s < 0) return;
         s = f.s;
         q = f.q;
@@ -798,13 +828,15 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
         }
         done = (int)left;
     } else {
-        const int64_t at = (int64_t)gridDim.x - 1 - blockIdx.x;
+        int tile;
+        tile_by_xcd(blockIdx.x, A.tiles, C.kv, tile, head);
+        if (tile >= A.tiles || head >= C.kv) return;
+        const int64_t at = A.tiles - 1 - tile;
         const Found f = find_seq(C, [&](const Seq& x) { return (int64_t)tiles_of(A, x, Z::ROWS); }, [&](int64_t) { return at; });
         if (f.s < 0) return;
         s = f.s;
         q = f.q;
         t = (int)f.unit;
-        head = blockIdx.y;
         x = get_tile(A, q, t, Z::ROWS);
         n = blocks_of(x);
         u1 = n;
@@ -840,8 +872,8 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
         __syncthreads();
         const bool final = here == n;
         if (!final && done == 0 && tid == 0)
-            A.shared[blockIdx.x] = SharedTile{q.first, x.r0, x.rows, head, (int)divide(u + n - 1, share)};
-        float* part = A.part + ((int64_t)blockIdx.x * 2 + (done == 0 ? 1 : 0)) * Z::PART;
+            A.shared[me] = SharedTile{q.first, x.r0, x.rows, head, (int)divide(u + n - 1, share)};
+        float* part = A.part + ((int64_t)me * 2 + (done == 0 ? 1 : 0)) * Z::PART;
         const int quads = C.dim / 4;
         for (int i = tid; i < x.rows * quads; i += ATTN_WAVES * 64) {
             const int row = i / quads, d = (i - row * quads) * 4;

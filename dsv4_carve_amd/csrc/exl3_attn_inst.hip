@@ -23,7 +23,7 @@ static int launch(const AttnArgs& A, const AttnPlan& P, hipStream_t s) {
         hipLaunchKernelGGL((fp8_attention_join_kernel<DIM, BF16, RB>), dim3(P.shares - 1, P.join_rows), dim3(ATTN_WAVES * 64), 0,
                            s, A);
     } else {
-        hipLaunchKernelGGL(kernel, dim3(P.tiles, A.c.kv), dim3(ATTN_WAVES * 64), LDS, s, A);
+        hipLaunchKernelGGL(kernel, dim3((P.tiles + XCDS - 1) / XCDS * XCDS * A.c.kv), dim3(ATTN_WAVES * 64), LDS, s, A);
     }
     return check_launch();
 }
