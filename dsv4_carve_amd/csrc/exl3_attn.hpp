@@ -1,270 +1,12 @@
-// A paged cache of e4m3 keys and values with one power-of-two scale for each page
-// and head, the write into it, and causal attention over it.
-//
-//   k  [pages][kv][page][dim]   k_scale [pages][kv]
-//   v  [pages][kv][dim][page]   v_scale [pages][kv]      (a value's tokens are neighbours)
+// Causal attention over the 8-bit paged cache, with grouped heads.
 //
 //   s_ij = scale * q_i . k_j for the keys j that query i sees (j <= i, j > i - window)
 //   out_i = sum_j e^(s_ij) v_j / (sum_j e^(s_ij) + e^sink),  lse_i = log of that sum
-//
-// A power of two as the scale keeps a value's bits where the scale of a begun page
-// grows (but for those that fall below e4m3's normal range), and e4m3's relative
-// error does not depend on where in its range a value lies.
 #pragma once
 
-#include "exl3_fp8.hpp"
-#include "exl3_topk.hpp"
+#include "exl3_cache.hpp"
 
 namespace exl3 {
-
-struct CacheView {
-    uint8_t* k;
-    float* k_scale;
-    uint8_t* v;
-    float* v_scale;
-    const int* table;            // [seqs][width] pages
-    int64_t table_stride;
-    const int* lengths;          // [seqs], the new tokens counted
-    const int* starts;           // [seqs + 1] first token of each sequence, or null: one token each
-    int seqs, tokens, kv, dim, page_shift, width, pages;
-};
-
-// A sequence's tokens in a call and its length.  What a table, a length or a start
-// names past its range is cut to it: no index leaves a buffer.
-struct Seq {
-    int first, n, len;
-};
-
-__device__ __forceinline__ Seq get_seq(const CacheView& C, int s) {
-    Seq q;
-    if (C.starts) {
-        const int a = C.starts[s], b = C.starts[s + 1];
-        q.first = min(max(a, 0), C.tokens);
-        q.n = max(min(b, C.tokens) - q.first, 0);
-    } else {
-        q.first = s;
-        q.n = 1;
-    }
-    const int64_t room = (int64_t)C.width << C.page_shift;
-    const int len = max(C.lengths[s], 0);
-    q.len = (int64_t)len < room ? len : (int)room;
-    return q;
-}
-
-// A value that all lanes have alike, known as such to the compiler: control flow and
-// addresses that follow from it are scalar.
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-    const u32x2_t a = __builtin_bit_cast(u32x2_t, v);
-    return __builtin_bit_cast(int64_t, u32x2_t{(uint32_t)uniform((int)a[0]), (uint32_t)uniform((int)a[1])});
-}
-
-// Inclusive prefix sums over the wave's lanes.
-__device__ __forceinline__ int64_t wave_scan(int64_t v) {
-    v += lane_of<0x111, 0xf>(v, (int64_t)0);        // row_shr:1, 2, 4, 8
-    v += lane_of<0x112, 0xf>(v, (int64_t)0);
-    v += lane_of<0x114, 0xf>(v, (int64_t)0);
-    v += lane_of<0x118, 0xf>(v, (int64_t)0);
-    v += lane_of<0x142, 0xa>(v, (int64_t)0);        // row_bcast:15, 31
-    v += lane_of<0x143, 0xc>(v, (int64_t)0);
-    return v;
-}
-
-// a / b, 0 <= a, 0 < b; in 32 bits where both fit.
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
-    return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
-}
-
-// The sequence that a unit of all sequences' units lies in; count(q) units each.  The
-// unit is at(total), total being all of them; s is -1 where it lies behind them.  Every
-// wave looks by itself: up to 64 sequences are one load and one scan.
-struct Found {
-    int s;
-    int64_t unit;                // within the sequence
-    Seq q;
-};
-
-template <typename Count, typename At>
-__device__ __forceinline__ Found find_seq(const CacheView& C, Count&& count, At&& at) {
-    const int lane = threadIdx.x & 63;
-    const Seq none{0, 0, 0};
-    Found f{-1, 0, none};
-    const auto look = [&](int s0, const Seq& q, int64_t c, int64_t before, int64_t sum, int64_t want) {
-        before += sum - c;
-        const uint64_t hit = __builtin_amdgcn_ballot_w64(want >= before && want < before + c);
-        if (!hit) return;
-        const int l = __builtin_ctzll(hit);
-        f.s = s0 + l;
-        f.unit = want - read_lane(before, l);
-        f.q = Seq{read_lane(q.first, l), read_lane(q.n, l), read_lane(q.len, l)};
-    };
-    if (C.seqs <= 64) {
-        const Seq q = lane < C.seqs ? get_seq(C, lane) : none;
-        const int64_t c = count(q), sum = wave_scan(c);
-        look(0, q, c, 0, sum, at(read_lane(sum, 63)));
-    } else {
-        int64_t c = 0;
-        for (int s = lane; s < C.seqs; s += 64) c += count(get_seq(C, s));
-        const int64_t want = at(read_lane(wave_scan(c), 63));
-        int64_t before = 0;
-        for (int s0 = 0; s0 < C.seqs && want >= before && f.s < 0; s0 += 64) {
-            const Seq q = s0 + lane < C.seqs ? get_seq(C, s0 + lane) : none;
-            const int64_t n = count(q), sum = wave_scan(n);
-            look(s0, q, n, before, sum, want);
-            before += read_lane(sum, 63);
-        }
-    }
-    return f;
-}
-
-// ---------------------------------------------------------------- the write
-
-constexpr int APPEND_WAVES = 4;
-
-struct AppendArgs {
-    CacheView c;
-    const void* k;
-    const void* v;
-    int64_t k_token, k_head, v_token, v_head;          // strides in values
-};
-
-// The pages that a sequence's new tokens lie in.
-__device__ __forceinline__ int touched_pages(const CacheView& C, const Seq& q) {
-    const int from = max(q.len - q.n, 0);
-    return q.len > from ? ((q.len - 1) >> C.page_shift) - (from >> C.page_shift) + 1 : 0;
-}
-
-// Eight neighbouring values (16-byte aligned) as fp32; an infinity as a NaN.
-template <int K>
-__device__ __forceinline__ void load8_finite(const void* p, int64_t at, float (&v)[8]) {
-    if constexpr (K == OUT_F32) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float4_t f = reinterpret_cast<const float4_t*>(static_cast<const float*>(p) + at)[i];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * i + j] = f[j];
-        }
-    } else {
-        const u32x4_t u = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + at);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[2 * j] = K == OUT_BF16 ? __uint_as_float(u[j] << 16) : f16_bits_to_f32((uint16_t)u[j]);
-            v[2 * j + 1] = K == OUT_BF16 ? __uint_as_float(u[j] & 0xffff0000u) : f16_bits_to_f32((uint16_t)(u[j] >> 16));
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fabsf(v[j]) == __builtin_inff() ? __builtin_nanf("") : v[j];
-}
-
-// Four codes times a power of two, rounded to e4m3 again.
-__device__ __forceinline__ uint32_t rescale4(uint32_t u, float by) {
-    return pack_e4m3(__builtin_amdgcn_cvt_f32_fp8((int)u, 0) * by, __builtin_amdgcn_cvt_f32_fp8((int)u, 1) * by,
-                     __builtin_amdgcn_cvt_f32_fp8((int)u, 2) * by, __builtin_amdgcn_cvt_f32_fp8((int)u, 3) * by);
-}
-
-// A workgroup has one page of one head, of the keys or of the values: the new
-// tokens' largest magnitude, the scale, the old codes where it grew, the new ones.
-// The inputs are read twice (the second time from cache).
-template <int K>
-__global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(AppendArgs A) {
-    __shared__ float most_of[APPEND_WAVES];
-    const CacheView& C = A.c;
-    const int tid = threadIdx.x, head = blockIdx.y;
-    const bool values = blockIdx.z;
-    int s = blockIdx.x, nth = 0;
-    Seq q;
-    if (C.starts) {
-        const Found f = find_seq(C, [&](const Seq& x) { return (int64_t)touched_pages(C, x); },
-                                 [](int64_t) { return (int64_t)blockIdx.x; });
-        if (f.s < 0) return;
-        s = f.s;
-        nth = (int)f.unit;
-        q = f.q;
-    } else {
-        q = get_seq(C, s);
-    }
-    const int page = 1 << C.page_shift, base = q.len - q.n, from = max(base, 0);
-    if (q.len <= from) return;
-    const int at = (from >> C.page_shift) + nth;                                  // the page's place in the sequence
-    const int id = C.table[s * C.table_stride + at];
-    if ((unsigned)id >= (unsigned)C.pages) return;
-    const int lo = max(from - (at << C.page_shift), 0), hi = min(q.len - (at << C.page_shift), page);
-    const int64_t token = q.first + (at << C.page_shift) - base;                  // the token of the page's place 0
-    const int64_t stride = values ? A.v_token : A.k_token;
-    const int64_t in0 = token * stride + head * (values ? A.v_head : A.k_head);
-    const void* in = values ? A.v : A.k;
-    const int64_t block = (int64_t)id * C.kv + head;
-    uint8_t* code = (values ? C.v : C.k) + (block << C.page_shift) * C.dim;
-    float* scale = (values ? C.v_scale : C.k_scale) + block;
-
-    const int per = C.dim >> 3;                                                   // chunks of eight a token
-    float most = 0.f;
-    float x[8];
-    for (int i = tid; i < (hi - lo) * per; i += APPEND_WAVES * 64) {
-        const int t = i / per;
-        load8_finite<K>(in, in0 + (lo + t) * stride + (i - t * per) * 8, x);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
-    }
-    most = wave_max(most, 0.f);
-    if ((tid & 63) == 0) most_of[tid >> 6] = most;
-    const float before = lo ? *scale : 0.f;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < APPEND_WAVES; ++w) most = fmaxf(most, most_of[w]);
-    const float now = fmaxf(QuantGroup(most, true).scale, before);
-    const float inverse = 1.0f / now, by = before / now;
-    const bool grew = lo && by != 1.0f;
-    if (!values) {
-        if (grew)
-            for (int i = tid; i < lo * C.dim / 16; i += APPEND_WAVES * 64) {
-                u32x4_t u = reinterpret_cast<u32x4_t*>(code)[i];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) u[j] = rescale4(u[j], by);
-                reinterpret_cast<u32x4_t*>(code)[i] = u;
-            }
-        for (int i = tid; i < (hi - lo) * per; i += APPEND_WAVES * 64) {
-            const int t = i / per, d = (i - t * per) * 8;
-            load8_finite<K>(in, in0 + (lo + t) * stride + d, x);
-            *reinterpret_cast<u32x2_t*>(code + (lo + t) * C.dim + d) =
-                u32x2_t{pack_e4m3(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse),
-                        pack_e4m3(x[4] * inverse, x[5] * inverse, x[6] * inverse, x[7] * inverse)};
-        }
-    } else {
-        // 16 tokens of one value's channel at once; what is outside [lo, hi) goes back as it was, or rescaled below lo
-        const int first = grew ? 0 : lo >> 4, groups = ((hi + 15) >> 4) - first;
-        for (int i = tid; i < groups * C.dim; i += APPEND_WAVES * 64) {
-            const int b = i / C.dim, d = i - b * C.dim, t0 = (first + b) * 16;
-            u32x4_t* p = reinterpret_cast<u32x4_t*>(code + ((int64_t)d << C.page_shift) + t0);
-            u32x4_t u = {0, 0, 0, 0};
-            if (t0 < lo || t0 + 16 > hi) u = *p;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t moved = grew ? rescale4(u[j], by) : u[j];
-                float y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int t = t0 + 4 * j + e;
-                    const float f = t >= lo && t < hi ? load_kind<K>(in, in0 + t * stride + d) : 0.f;
-                    y[e] = (fabsf(f) == __builtin_inff() ? __builtin_nanf("") : f) * inverse;
-                }
-                const uint32_t made = pack_e4m3(y[0], y[1], y[2], y[3]);
-                uint32_t r = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int t = t0 + 4 * j + e;
-                    const uint32_t m = 0xffu << (8 * e);
-                    r |= m & (t < lo ? moved : t < hi ? made : u[j]);
-                }
-                u[j] = r;
-            }
-            *p = u;
-        }
-    }
-    if (tid == 0) *scale = now;
-}
-
-// ---------------------------------------------------------------- attention
 
 constexpr int ATTN_WAVES = 4;
 constexpr int ATTN_KEYS = 64;                 // keys of a block
@@ -359,13 +101,258 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t u) {       // 0x80 in eac
 // less counts as nothing beside the row's largest.)  The denominator is the sum of w
 // 2^-k.  Sums are fp32.  A 16-bit weight has 11 bits, three more than a bf16 result;
 // for an fp16 result the rest of the weight goes through the product as well (FINE).
-//
+template <int DIM, bool BF16, int RB>
+struct AttnRows {
+    static constexpr bool FINE = !BF16;
+    static constexpr int ROWS = 16 * RB, KC = DIM / 64, DT = DIM / 16;
+    typedef Half16<BF16> H;
+    typedef Half16<false> W;
+
+    typename H::vec8 qf[RB][KC][2];
+    int see_lo[RB], see_hi[RB];
+    float4_t o[DT][RB];
+    float m[RB], top[RB], c[RB], l[RB];
+
+    // The rows from r0 on of sequence q and a cache head, `rows` of them (one at least).
+    __device__ __forceinline__ void begin(const AttnArgs& A, const Seq& q, int r0, int rows, int head) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, base = q.len - q.n;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const int row = 16 * rb + r;
+            const bool in = row < rows;
+            const int of = r0 + (in ? row : 0), at = of / A.group, hg = of - at * A.group;
+            const uint16_t* p = A.q + (int64_t)(q.first + at) * A.q_token + (int64_t)(head * A.group + hg) * A.q_head;
+#pragma unroll
+            for (int k = 0; k < KC; ++k)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int d = 64 * k + 16 * g + 8 * u;
+                    const bool is = in && d < A.c.dim;
+                    const u32x4_t z = *reinterpret_cast<const u32x4_t*>(p + (d < A.c.dim ? d : 0));
+                    u32x4_t v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = is ? A.negative ? z[i] ^ 0x80008000u : z[i] : 0u;
+                    qf[rb][k][u] = __builtin_bit_cast(typename H::vec8, v);
+                }
+            see_hi[rb] = in ? min(base + at + 1, q.len) : 0;
+            see_lo[rb] = in && A.window ? base + at + 1 - A.window : 0;
+            m[rb] = top[rb] = ATTN_LOW;
+            c[rb] = l[rb] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d][rb] = float4_t{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+
+    // What no row of [lo, hi) sees may hold anything: its bytes become zeros (a weight of 0 would leave a NaN one).
+    static __device__ __forceinline__ void keep_bytes(uint32_t (&keep)[4], bool here, int key0, int lo, int hi) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            keep[j] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int key = key0 + 4 * j + e;
+                if (here && key >= lo && key < hi) keep[j] |= 0xffu << (8 * e);
+            }
+        }
+    }
+
+    // A block of keys, key0 = its first plus 16 (lane / 16).  key(t, k): 16 bytes of key 16 (lane % 16 / 4) + 4 t + lane % 4
+    // from channel 64 k + 16 (lane / 16) on; value(d): 16 tokens, from key0 on, of channel 16 d + lane % 16.  ks, vs: the
+    // scales of the lane's 16 keys.  MASKED: not every row sees it whole; the lane's keys are in a page (`here`) and the rows
+    // see [lo, hi) at most.  Returns whether a value that some rows see is a NaN: it is left out (counted by add_nans).
+    template <bool MASKED, typename K, typename V>
+    __device__ __forceinline__ bool step(const AttnArgs& A, float ks, float vs, bool here, int key0, int lo, int hi, K&& key,
+                                         V&& value) {
+        float4_t p[4][RB];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) p[t][rb] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const u32x4_t z = key(t, k);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const typename H::vec8 w = H::widen(z[2 * u], z[2 * u + 1]);
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) p[t][rb] = H::mfma(w, qf[rb][k][u], p[t][rb]);
+                }
+            }
+        float kc = fmaxf(ks * A.qk_scale, 0x1p-126f);
+        uint32_t keep[4];
+        if constexpr (MASKED) {
+            here = here && key0 + 15 >= lo && key0 < hi;
+            kc = here ? kc : 1.f;
+            vs = here ? vs : 1.f;
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const int from = here ? see_lo[rb] - key0 : 16, n = see_hi[rb] - key0;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = 4 * t + i;
+                        p[t][rb][i] = at >= from && at < n ? p[t][rb][i] : -__builtin_inff();
+                    }
+            }
+            keep_bytes(keep, here, key0, lo, hi);
+        }
+        const float lv = __builtin_amdgcn_logf(vs);
+        bool grew = false;
+        float most[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            float a = p[0][rb][0];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (t + i) a = fmaxf(a, p[t][rb][i]);
+            most[rb] = a * kc;
+            grew |= most[rb] > m[rb] + ATTN_SLACK || most[rb] + lv > top[rb] + ATTN_SLACK;
+        }
+        if (__builtin_amdgcn_ballot_w64(grew)) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const float m1 = fmaxf(m[rb], xor_max(most[rb])), top1 = fmaxf(top[rb], xor_max(most[rb] + lv));
+                const float c1 = ceilf(top1 - m1);
+                const float fl = __builtin_amdgcn_exp2f(m[rb] - m1);
+                const float fo = __builtin_amdgcn_exp2f(m[rb] - m1 + (c[rb] - c1));
+                m[rb] = m1;
+                top[rb] = top1;
+                c[rb] = c1;
+                l[rb] *= fl;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[d][rb][i] *= fo;
+            }
+        }
+        half8_t big[RB][2], rest[RB][2];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const float k = fmaxf(lv + (ATTN_HEADROOM - c[rb]), -64.f), add = k - m[rb];
+            float sum = 0.f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(p[t][rb][i], kc, add));
+                    sum += w;
+                    const _Float16 h = (_Float16)w;
+                    big[rb][t >> 1][4 * (t & 1) + i] = h;
+                    if constexpr (FINE) rest[rb][t >> 1][4 * (t & 1) + i] = (_Float16)(w - (float)h);
+                }
+            l[rb] = fmaf(sum, __builtin_amdgcn_exp2f(-k), l[rb]);
+        }
+        uint32_t nan = 0;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            u32x4_t z = value(d);
+            if constexpr (MASKED) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    z[j] &= keep[j];
+                    const uint32_t bad = nan_bytes(z[j]);
+                    nan |= bad;
+                    z[j] &= ~((bad >> 7) * 0xffu);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const half8_t v = W::widen(z[2 * u], z[2 * u + 1]);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    o[d][rb] = W::mfma(v, big[rb][u], o[d][rb]);
+                    if constexpr (FINE) o[d][rb] = W::mfma(v, rest[rb][u], o[d][rb]);
+                }
+            }
+        }
+        return MASKED && __builtin_amdgcn_ballot_w64(nan != 0) != 0;
+    }
+
+    // The NaN values of a masked block, counted for the rows that see them in products of their own.
+    template <typename V>
+    __device__ __forceinline__ void add_nans(bool here, int key0, int lo, int hi, V&& value) {
+        uint32_t keep[4];
+        here = here && key0 + 15 >= lo && key0 < hi;
+        keep_bytes(keep, here, key0, lo, hi);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            half8_t sees[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int at = key0 + 8 * u + j;
+                    sees[u][j] = here && at >= see_lo[rb] && at < see_hi[rb] ? (_Float16)1.f : (_Float16)0.f;
+                }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const u32x4_t z = value(d);
+                float4_t n = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    n = W::mfma(W::widen((nan_bytes(z[2 * u] & keep[2 * u]) >> 7) * 0x38u,                // 0x38: one
+                                         (nan_bytes(z[2 * u + 1] & keep[2 * u + 1]) >> 7) * 0x38u), sees[u], n);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][rb][i] = n[i] > 0.f ? __builtin_nanf("") : o[d][rb][i];
+            }
+        }
+    }
+
+    // A row's sum over the lanes that share it, and what brings its o to the unit of that sum.
+    __device__ __forceinline__ float row_sum(int rb) const {
+        float a = l[rb];
+        a += __shfl_xor(a, 16);
+        return a + __shfl_xor(a, 32);
+    }
+    __device__ __forceinline__ int back(int rb) const { return (int)c[rb] - ATTN_HEADROOM; }
+};
+
+// A sequence's pages and their scales for one cache head.
+struct Pages {
+    const int* table;
+    int pages;
+
+    __device__ __forceinline__ Pages(const CacheView& C, const Seq& q, int s)
+        : table(C.table + s * C.table_stride), pages((q.len + (1 << C.page_shift) - 1) >> C.page_shift) {}
+
+    // The page of the 16 keys from 64 b + 16 (lane / 16) on, -1 behind the sequence's end.
+    __device__ __forceinline__ int of(const CacheView& C, int b) const {
+        const int i = (b * ATTN_KEYS + (threadIdx.x & 48)) >> C.page_shift, id = table[min(i, pages - 1)];
+        return i < pages ? id : -1;
+    }
+};
+
+__device__ __forceinline__ bool valid_page(const CacheView& C, int id) { return (unsigned)id < (unsigned)C.pages; }
+__device__ __forceinline__ float scale_of(const CacheView& C, const float* p, int id, int head) {
+    return p[(int64_t)(valid_page(C, id) ? id : 0) * C.kv + head];
+}
+
+// Whether some row of a tile does not see a block whole.
+__device__ __forceinline__ bool masked_block(const CacheView& C, const Tile& x, int b, int id) {
+    return b * ATTN_KEYS < x.full_lo || (b + 1) * ATTN_KEYS > x.full_hi || __builtin_amdgcn_ballot_w64(valid_page(C, id)) != ~0ull;
+}
+
+// Bytes of a page and head from `at` on, as a buffer that ends with the page; none where ids' lane group g names no
+// page, or without `on`: what lies outside a buffer is not read and comes back as zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_part(const CacheView& C, const uint8_t* p, int head, int ids, int g, int at,
+                                                            bool on) {
+    const int id = __builtin_amdgcn_readlane(ids, 16 * g);
+    const bool is = on && valid_page(C, id);
+    const uint32_t bytes = (uint32_t)C.dim << C.page_shift;                   // below 2^16, and 1024 heads of it below 2^32
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(p) + (uint64_t)(uint32_t)(is ? id : 0) * ((uint32_t)C.kv * bytes) + (head * bytes + at), 0,
+        is ? bytes - at : 0, 0x27000);
+}
+
 // Memory wants neighbouring lanes on neighbouring bytes, the products lanes of
 // different keys and channels: a wave's loads go by whole rows (16 bytes a lane) and are
 // turned in LDS, in a place of its own, so that no barrier is needed.  Chunks of 16
 // bytes are XORed with their row: neither side meets a bank twice in eight lanes.
-// Loads are of buffers that end with the page: what lies outside is not read and comes
-// back as zeros, so a call's end and a page that is none need no branch.
 template <int DIM>
 struct AttnStage {
     static constexpr int SUB = DIM % 128 == 0 ? 128 : 64, CS = SUB / 16, SUBS = DIM / SUB, KEYS = 64 / CS;
@@ -398,22 +385,11 @@ struct AttnStage {
         v_read = K_BYTES + r * 64 + ((g ^ (r >> 1 & 3)) << 4);
     }
 
-    // Bytes of a page and head from `at` on; none where ids' lane group g names no page, or without `on`.
-    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t part(const CacheView& C, const uint8_t* p, int head, int ids, int g,
-                                                                  int at, bool on) {
-        const int id = __builtin_amdgcn_readlane(ids, 16 * g);
-        const bool is = on && (unsigned)id < (unsigned)C.pages;
-        const uint32_t bytes = (uint32_t)C.dim << C.page_shift;                   // below 2^16, and 1024 heads of it below 2^32
-        return __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(p) + (uint64_t)(uint32_t)(is ? id : 0) * ((uint32_t)C.kv * bytes) + (head * bytes + at), 0,
-            is ? bytes - at : 0, 0x27000);
-    }
-
     __device__ __forceinline__ void load_k(const CacheView& C, int head, int b, int ids, bool on, u32x4_t (&z)[LOADS]) const {
         const int mask = (1 << C.page_shift) - 1;
         __amdgpu_buffer_rsrc_t p[4];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) p[g] = part(C, C.k, head, ids, g, ((b * ATTN_KEYS + 16 * g) & mask) * C.dim, on);
+        for (int g = 0; g < 4; ++g) p[g] = page_part(C, C.k, head, ids, g, ((b * ATTN_KEYS + 16 * g) & mask) * C.dim, on);
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
             const int key = j / SUBS * KEYS;
@@ -427,7 +403,7 @@ struct AttnStage {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int g = (i & ((1 << (2 - lg)) - 1)) << lg;
-            p[i] = part(C, C.v, head, ids, g, (b * ATTN_KEYS + 16 * g) & mask, on);
+            p[i] = page_part(C, C.v, head, ids, g, (b * ATTN_KEYS + 16 * g) & mask, on);
         }
 #pragma unroll
         for (int j = 0; j < LOADS; ++j)
@@ -458,264 +434,64 @@ struct AttnStage {
         order();
     }
 
-    // 16 values of key 16 (lane % 16 / 4) + 4 t + lane % 4, from 64 k + 16 (lane / 16) on
     __device__ __forceinline__ u32x4_t key(int t, int k) const {
         return *reinterpret_cast<const u32x4_t*>(lds + k_read[k & 1] + k / 2 * 128 + 4 * t * DIM);
     }
-
-    // 16 tokens, from 16 (lane / 16) on, of channel 16 d + lane % 16
-    __device__ __forceinline__ u32x4_t& value(int d) const { return *reinterpret_cast<u32x4_t*>(lds + v_read + d * 1024); }
+    __device__ __forceinline__ u32x4_t value(int d) const { return *reinterpret_cast<const u32x4_t*>(lds + v_read + d * 1024); }
 };
 
+// Blocks first, first + step, ... < last of a tile's keys for one wave.  No branch divides lanes in here: the compiler may
+// leave them apart in the loop around the products, and may place copies of other lanes' registers before they are back.
 template <int DIM, bool BF16, int RB>
-struct AttnWave {
-    static constexpr bool FINE = !BF16;
-    static constexpr int KC = DIM / 64, DT = DIM / 16;
-    typedef Half16<BF16> H;
-    typedef Half16<false> W;
-
-    float4_t o[DT][RB];
-    float m[RB], top[RB], c[RB], l[RB];
-
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            m[rb] = top[rb] = ATTN_LOW;
-            c[rb] = l[rb] = 0.f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) o[d][rb] = float4_t{0.f, 0.f, 0.f, 0.f};
-        }
+__device__ __forceinline__ void attend(const AttnArgs& A, const AttnStage<DIM>& S, AttnRows<DIM, BF16, RB>& R, const Seq& q,
+                                       const Tile& x, int s, int head, int first, int last, int step) {
+    constexpr int DT = DIM / 16;
+    if (first >= last) return;
+    const CacheView& C = A.c;
+    const int g16 = threadIdx.x & 48;
+    const Pages P(C, q, s);
+    const auto key = [&](int t, int k) { return S.key(t, k); };
+    const auto value = [&](int d) { return S.value(d); };
+    u32x4_t kreg[DT], vreg[DT];
+    int ids = P.of(C, first), next = P.of(C, min(first + step, last - 1));    // two blocks ahead: loads come back in order
+    S.load_k(C, head, first, ids, true, kreg);
+    float ks = scale_of(C, C.k_scale, ids, head), vs = scale_of(C, C.v_scale, ids, head);
+    S.load_v(C, head, first, ids, true, vreg);
+    bool nans = false;
+    for (int b = first; b < last; b += step) {
+        const int id = ids;
+        const float ks_now = ks, vs_now = vs;
+        const int after = P.of(C, min(b + 2 * step, last - 1));
+        const bool more = b + step < last;
+        S.put_k(kreg);
+        S.load_k(C, head, b + step, next, more, kreg);
+        ks = scale_of(C, C.k_scale, next, head);
+        vs = scale_of(C, C.v_scale, next, head);
+        S.put_v(vreg);
+        S.load_v(C, head, b + step, next, more, vreg);
+        ids = next;
+        next = after;
+        const int key0 = b * ATTN_KEYS + g16;
+        if (masked_block(C, x, b, id))
+            nans |= R.template step<true>(A, ks_now, vs_now, valid_page(C, id), key0, x.lo, x.hi, key, value);
+        else
+            R.template step<false>(A, ks_now, vs_now, true, key0, 0, 0, key, value);
     }
-
-    // Blocks first, first + step, ... < last of the tile's keys.  No branch divides lanes in here: the compiler may leave
-    // them apart in the loop around the products, and may place copies of other lanes' registers before they are back.
-    __device__ __forceinline__ void run(const AttnArgs& A, const AttnStage<DIM>& S, const Seq& q, const Tile& x, int s, int head,
-                                        int first, int last, int step) {
-        if (first >= last) return;
-        const CacheView& C = A.c;
-        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-        const int base = q.len - q.n;
-        typename H::vec8 qf[RB][KC][2];
-        int see_lo[RB], see_hi[RB];
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            const int row = 16 * rb + r;
-            const bool in = row < x.rows;
-            const int of = x.r0 + (in ? row : 0), at = of / A.group, hg = of - at * A.group;
-            const uint16_t* p = A.q + (int64_t)(q.first + at) * A.q_token + (int64_t)(head * A.group + hg) * A.q_head;
-#pragma unroll
-            for (int k = 0; k < KC; ++k)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int d = 64 * k + 16 * g + 8 * u;
-                    const bool is = in && d < C.dim;
-                    const u32x4_t z = *reinterpret_cast<const u32x4_t*>(p + (d < C.dim ? d : 0));
-                    u32x4_t v;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = is ? A.negative ? z[i] ^ 0x80008000u : z[i] : 0u;
-                    qf[rb][k][u] = __builtin_bit_cast(typename H::vec8, v);
-                }
-            see_hi[rb] = in ? min(base + at + 1, q.len) : 0;
-            see_lo[rb] = in && A.window ? base + at + 1 - A.window : 0;
-        }
-        const int* table = C.table + s * C.table_stride;
-        const int pages = (q.len + (1 << C.page_shift) - 1) >> C.page_shift;
-        // The page of lane group g's 16 keys.
-        const auto pages_of = [&](int b) {
-            const int i = (min(b, last - 1) * ATTN_KEYS + 16 * g) >> C.page_shift, id = table[min(i, pages - 1)];
-            return i < pages ? id : -1;
-        };
-        const auto valid = [&](int id) { return (unsigned)id < (unsigned)C.pages; };
-        const auto scale_of = [&](const float* p, int id) { return p[(int64_t)(valid(id) ? id : 0) * C.kv + head]; };
-        // In a block that not every row sees whole, what no row sees may hold anything: its bytes become zeros (a weight of 0
-        // would leave a NaN one).  A NaN that only some rows see becomes a zero too, and `nans` has it counted later.
-        bool nans = false;
-        const auto hide_values = [&](int b, bool here, bool keep_nans) {
-            const int key0 = b * ATTN_KEYS + 16 * g;
-            uint32_t keep[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                keep[j] = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int key = key0 + 4 * j + e;
-                    if (here && key >= x.lo && key < x.hi) keep[j] |= 0xffu << (8 * e);
-                }
-            }
-            uint32_t nan = 0;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                u32x4_t v = S.value(d);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[j] &= keep[j];
-                    const uint32_t bad = nan_bytes(v[j]);
-                    nan |= bad;
-                    if (!keep_nans) v[j] &= ~((bad >> 7) * 0xffu);
-                }
-                S.value(d) = v;
-            }
-            S.order();
-            nans |= __builtin_amdgcn_ballot_w64(nan != 0) != 0;
-        };
-
-        u32x4_t kreg[DT], vreg[DT];
-        int ids = pages_of(first), next = pages_of(first + step);  // asked for two blocks ahead: loads come back in order
-        S.load_k(C, head, first, ids, true, kreg);
-        float ks = scale_of(C.k_scale, ids), vs = scale_of(C.v_scale, ids);
-        S.load_v(C, head, first, ids, true, vreg);
-        for (int b = first; b < last; b += step) {
-            const int id_here = ids;
-            float kc = fmaxf(ks * A.qk_scale, 0x1p-126f), vscale = vs;
-            const int after = pages_of(b + 2 * step);
-            const bool more = b + step < last;
-            S.put_k(kreg);
-            S.load_k(C, head, b + step, next, more, kreg);
-            ks = scale_of(C.k_scale, next);
-            vs = scale_of(C.v_scale, next);
-            float4_t p[4][RB];
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) p[t][rb] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < KC; ++k)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const u32x4_t z = S.key(t, k);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const typename H::vec8 key = H::widen(z[2 * u], z[2 * u + 1]);
-#pragma unroll
-                        for (int rb = 0; rb < RB; ++rb) p[t][rb] = H::mfma(key, qf[rb][k][u], p[t][rb]);
-                    }
-                }
-            S.put_v(vreg);
-            S.load_v(C, head, b + step, next, more, vreg);
-            ids = next;
-            next = after;
-            if (b * ATTN_KEYS < x.full_lo || (b + 1) * ATTN_KEYS > x.full_hi ||
-                __builtin_amdgcn_ballot_w64(valid(id_here)) != ~0ull) {
-                const int key0 = b * ATTN_KEYS + 16 * g;
-                const bool here = valid(id_here) && key0 + 15 >= x.lo && key0 < x.hi;
-                kc = here ? kc : 1.f;
-                vscale = here ? vscale : 1.f;
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    const int lo = here ? see_lo[rb] - key0 : 16, n = see_hi[rb] - key0;
-#pragma unroll
-                    for (int t = 0; t < 4; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int key = 4 * t + i;
-                            p[t][rb][i] = key >= lo && key < n ? p[t][rb][i] : -__builtin_inff();
-                        }
-                }
-                hide_values(b, here, false);
-            }
-            const float lv = __builtin_amdgcn_logf(vscale);
-            bool grew = false;
-            float most[RB];
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-                float a = p[0][rb][0];
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (t + i) a = fmaxf(a, p[t][rb][i]);
-                most[rb] = a * kc;
-                grew |= most[rb] > m[rb] + ATTN_SLACK || most[rb] + lv > top[rb] + ATTN_SLACK;
-            }
-            if (__builtin_amdgcn_ballot_w64(grew)) {
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    const float m1 = fmaxf(m[rb], xor_max(most[rb])), top1 = fmaxf(top[rb], xor_max(most[rb] + lv));
-                    const float c1 = ceilf(top1 - m1);
-                    const float fl = __builtin_amdgcn_exp2f(m[rb] - m1);
-                    const float fo = __builtin_amdgcn_exp2f(m[rb] - m1 + (c[rb] - c1));
-                    m[rb] = m1;
-                    top[rb] = top1;
-                    c[rb] = c1;
-                    l[rb] *= fl;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[d][rb][i] *= fo;
-                }
-            }
-            half8_t hi[RB][2], lo[RB][2];
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-                const float k = fmaxf(lv + (ATTN_HEADROOM - c[rb]), -64.f), add = k - m[rb];
-                float sum = 0.f;
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float w = __builtin_amdgcn_exp2f(fmaf(p[t][rb][i], kc, add));
-                        sum += w;
-                        const _Float16 h = (_Float16)w;
-                        hi[rb][t >> 1][4 * (t & 1) + i] = h;
-                        if constexpr (FINE) lo[rb][t >> 1][4 * (t & 1) + i] = (_Float16)(w - (float)h);
-                    }
-                l[rb] = fmaf(sum, __builtin_amdgcn_exp2f(-k), l[rb]);
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const u32x4_t z = S.value(d);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const half8_t v = W::widen(z[2 * u], z[2 * u + 1]);
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) {
-                        o[d][rb] = W::mfma(v, hi[rb][u], o[d][rb]);
-                        if constexpr (FINE) o[d][rb] = W::mfma(v, lo[rb][u], o[d][rb]);
-                    }
-                }
-            }
-        }
-        if (!nans) return;
-        // NaN values that were left out above: counted for the rows that see them, in products of their own.
-        for (int b = first; b < last; b += step) {
-            const int id = pages_of(b);
-            const int key0 = b * ATTN_KEYS + 16 * g;
-            const bool here = valid(id) && key0 + 15 >= x.lo && key0 < x.hi;
-            S.load_v(C, head, b, id, true, vreg);
-            S.put_v(vreg);
-            hide_values(b, here, true);
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-                half8_t sees[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int key = key0 + 8 * u + j;
-                        sees[u][j] = here && key >= see_lo[rb] && key < see_hi[rb] ? (_Float16)1.f : (_Float16)0.f;
-                    }
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const u32x4_t z = S.value(d);
-                    float4_t n = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        n = W::mfma(W::widen((nan_bytes(z[2 * u]) >> 7) * 0x38u, (nan_bytes(z[2 * u + 1]) >> 7) * 0x38u),
-                                    sees[u], n);                                             // 0x38: one
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[d][rb][i] = n[i] > 0.f ? __builtin_nanf("") : o[d][rb][i];
-                }
-            }
-        }
+    if (!nans) return;
+    for (int b = first; b < last; b += step) {
+        const int id = P.of(C, b);
+        S.load_v(C, head, b, id, true, vreg);
+        S.put_v(vreg);
+        R.add_nans(valid_page(C, id), b * ATTN_KEYS + g16, x.lo, x.hi, value);
     }
-};
+}
 
 template <int DIM, int RB>
 struct AttnSize {
     static constexpr int ROWS = 16 * RB, PITCH = DIM + 4;
     static constexpr int JOIN = ATTN_WAVES * ROWS * (PITCH + 2) * 4, STAGE = ATTN_WAVES * AttnStage<DIM>::BYTES;
     static constexpr int LDS = JOIN > STAGE ? JOIN : STAGE;       // the blocks of the waves, then their sums
-    static constexpr int WAVES_EU = RB <= 2 && DIM <= 128 ? 2 : 1;
+    static constexpr int WAVES_EU = DIM <= 128 ? 2 : 1;
     static constexpr int PART = ROWS * (DIM + 2);                 // floats of a partial result: rows of sums, then m and l
 };
 
@@ -783,134 +559,89 @@ __device__ __forceinline__ void tile_by_xcd(int b, int tiles, int heads, int& ti
 }
 
 // Units are (cache head, tile, block of keys), in this order; a workgroup has an
-// equal share of them, next to each other, whatever sequences they are of.  Its four
-// waves go through a tile's blocks in turn and join their sums in LDS.  A tile whose
+// equal share of them, next to each other, whatever sequences they are of.  A tile whose
 // blocks one workgroup has all is finished; of the others each workgroup leaves a
 // partial result: in its first place where the tile began before its share, in its
 // second where it goes on behind it.  Without a place for partial results a workgroup
 // has a tile, the last, longest ones first.
-template <int DIM, bool BF16, int RB>
-__global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) void fp8_attention_kernel(AttnArgs A) {
-    typedef AttnSize<DIM, RB> Z;
-    extern __shared__ __attribute__((aligned(16))) float lds[];
-    const CacheView& C = A.c;
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, g = lane >> 4;
-    int64_t u = 0, u1 = 0, share = 0;
-    int s = 0, t = 0, head = 0, done = 0;                       // done: the tile's blocks before the share
+template <int ROWS>
+struct Work {
+    int64_t u, u1, share;        // units: the next, the end of the workgroup's, how many a workgroup has
+    int me, s, t, head;
+    int done, n, here;           // of the tile: blocks before the next unit, all of them, those of this workgroup
     Seq q;
     Tile x;
-    int n = 0;
-    int me = blockIdx.x;
-    clear_rows(A);
-    if (A.part) {
-        const Found f = find_seq(C, [&](const Seq& x) { return units_of(A, x, Z::ROWS); }, [&](int64_t total) {
-            const int64_t all = total * C.kv;
-            share = divide(all + gridDim.x - 1, gridDim.x);
-            if (share < A.least) share = A.least;
-            const int busy = (int)divide(all + share - 1, share);
-            if (me >= busy) return (int64_t)-1;
-            me = by_xcd(me, busy);
-            u = share * me;
-            u1 = u + share < all ? u + share : all;
-            head = (int)divide(u, total);
-            return u - head * total;
-        });
-        if (tid == 0) A.shared[me].last = -1;            // nothing to join, unless a tile goes on behind the share
-        if (f.s < 0) return;
-        s = f.s;
-        q = f.q;
-        int64_t left = f.unit;
-        for (;; ++t) {
-            x = get_tile(A, q, t, Z::ROWS);
+
+    // False if there is nothing for this workgroup.
+    __device__ __forceinline__ bool find(const AttnArgs& A) {
+        const CacheView& C = A.c;
+        u = u1 = share = 0;
+        me = blockIdx.x;
+        t = head = done = 0;
+        if (A.part) {
+            const Found f = find_seq(C, [&](const Seq& x) { return units_of(A, x, ROWS); }, [&](int64_t total) {
+                const int64_t all = total * C.kv;
+                share = divide(all + gridDim.x - 1, gridDim.x);
+                if (share < A.least) share = A.least;
+                const int busy = (int)divide(all + share - 1, share);
+                if (me >= busy) return (int64_t)-1;
+                me = by_xcd(me, busy);
+                u = share * me;
+                u1 = u + share < all ? u + share : all;
+                head = (int)divide(u, total);
+                return u - head * total;
+            });
+            if (threadIdx.x == 0) A.shared[me].last = -1;        // nothing to join, unless a tile goes on behind the share
+            if (f.s < 0) return false;
+            s = f.s;
+            q = f.q;
+            int64_t left = f.unit;
+            for (;; ++t) {
+                x = get_tile(A, q, t, ROWS);
+                n = blocks_of(x);
+                if (left < n) break;
+                left -= n;
+            }
+            done = (int)left;
+        } else {
+            int tile;
+            tile_by_xcd(blockIdx.x, A.tiles, C.kv, tile, head);
+            if (tile >= A.tiles || head >= C.kv) return false;
+            const int64_t at = A.tiles - 1 - tile;
+            const Found f = find_seq(C, [&](const Seq& x) { return (int64_t)tiles_of(A, x, ROWS); }, [&](int64_t) { return at; });
+            if (f.s < 0) return false;
+            s = f.s;
+            q = f.q;
+            t = (int)f.unit;
+            x = get_tile(A, q, t, ROWS);
             n = blocks_of(x);
-            if (left < n) break;
-            left -= n;
+            u1 = n;
         }
-        done = (int)left;
-    } else {
-        int tile;
-        tile_by_xcd(blockIdx.x, A.tiles, C.kv, tile, head);
-        if (tile >= A.tiles || head >= C.kv) return;
-        const int64_t at = A.tiles - 1 - tile;
-        const Found f = find_seq(C, [&](const Seq& x) { return (int64_t)tiles_of(A, x, Z::ROWS); }, [&](int64_t) { return at; });
-        if (f.s < 0) return;
-        s = f.s;
-        q = f.q;
-        t = (int)f.unit;
-        x = get_tile(A, q, t, Z::ROWS);
-        n = blocks_of(x);
-        u1 = n;
+        measure();
+        return true;
     }
-    const AttnStage<DIM> S(C, reinterpret_cast<char*>(lds) + wave * AttnStage<DIM>::BYTES);
-    float* sums = lds;                                          // [wave][row][PITCH]
-    float* ml = lds + ATTN_WAVES * Z::ROWS * Z::PITCH;          // [wave][row][2]
-    for (;;) {
+
+    __device__ __forceinline__ void measure() {
         const int64_t want = u1 - u;
-        const int here = (int)(n - done < want ? n - done : want);
-        const int b0 = x.lo / ATTN_KEYS + done;
-        AttnWave<DIM, BF16, RB> W;
-        W.clear();
-        W.run(A, S, q, x, s, head, b0 + wave, min(b0 + here, (x.hi + ATTN_KEYS - 1) / ATTN_KEYS), ATTN_WAVES);
-        __syncthreads();
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            const int row = 16 * rb + r;
-            float l = W.l[rb];
-            l += __shfl_xor(l, 16);
-            l += __shfl_xor(l, 32);
-            ml[(wave * Z::ROWS + row) * 2] = W.m[rb];           // by four lanes alike: no branch while the sums are live
-            ml[(wave * Z::ROWS + row) * 2 + 1] = l;
-            const int back = (int)W.c[rb] - ATTN_HEADROOM;
-#pragma unroll
-            for (int d = 0; d < DIM / 16; ++d) {
-                float4_t v;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = ldexpf(W.o[d][rb][i], back);
-                *reinterpret_cast<float4_t*>(sums + (wave * Z::ROWS + row) * Z::PITCH + 16 * d + 4 * g) = v;
-            }
-        }
-        __syncthreads();
-        const bool final = here == n;
-        if (!final && done == 0 && tid == 0)
-            A.shared[me] = SharedTile{q.first, x.r0, x.rows, head, (int)divide(u + n - 1, share)};
-        float* part = A.part + ((int64_t)me * 2 + (done == 0 ? 1 : 0)) * Z::PART;
-        const int quads = C.dim / 4;
-        for (int i = tid; i < x.rows * quads; i += ATTN_WAVES * 64) {
-            const int row = i / quads, d = (i - row * quads) * 4;
-            float m = ATTN_LOW, l = 0.f;
-#pragma unroll
-            for (int w = 0; w < ATTN_WAVES; ++w) m = fmaxf(m, ml[(w * Z::ROWS + row) * 2]);
-            float4_t v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < ATTN_WAVES; ++w) {
-                const float f = __builtin_amdgcn_exp2f(ml[(w * Z::ROWS + row) * 2] - m);
-                l += f * ml[(w * Z::ROWS + row) * 2 + 1];
-                const float4_t a = *reinterpret_cast<const float4_t*>(sums + (w * Z::ROWS + row) * Z::PITCH + d);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = fmaf(f, a[j], v[j]);
-            }
-            if (final) {
-                const int at = (x.r0 + row) / A.group, h = head * A.group + x.r0 + row - at * A.group;
-                const int64_t o = (int64_t)(q.first + at) * A.heads + h;
-                float lse;
-                const float f = finish_row(A, h, m, l, lse);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] *= f;
-                store_row4<BF16>(A.out + o * C.dim + d, v);
-                if (A.lse && d == 0) A.lse[o] = lse;
-            } else {
-                *reinterpret_cast<float4_t*>(part + row * C.dim + d) = v;
-                if (d == 0) {
-                    part[Z::ROWS * DIM + 2 * row] = m;
-                    part[Z::ROWS * DIM + 2 * row + 1] = l;
-                }
-            }
-        }
+        here = (int)(n - done < want ? n - done : want);
+    }
+    __device__ __forceinline__ int first() const { return x.lo / ATTN_KEYS + done; }
+    __device__ __forceinline__ int last() const { return min(first() + here, (x.hi + ATTN_KEYS - 1) / ATTN_KEYS); }
+    __device__ __forceinline__ bool whole() const { return here == n; }
+
+    // Where a partial result goes, of `size` floats each; tells the join of a tile that begins here.
+    __device__ __forceinline__ float* part(const AttnArgs& A, int size) const {
+        if (done == 0 && threadIdx.x == 0) A.shared[me] = SharedTile{q.first, x.r0, x.rows, head, (int)divide(u + n - 1, share)};
+        return A.part + ((int64_t)me * 2 + (done == 0 ? 1 : 0)) * size;
+    }
+
+    // The next tile of the workgroup's units; false behind the last.
+    __device__ __forceinline__ bool next(const AttnArgs& A) {
+        const CacheView& C = A.c;
         u += here;
-        if (u >= u1) break;
-        __syncthreads();                                        // the sums' places hold blocks again
+        if (u >= u1) return false;
         done = 0;
-        if (++t == tiles_of(A, q, Z::ROWS)) {
+        if (++t == tiles_of(A, q, ROWS)) {
             t = 0;
             do {
                 if (++s == C.seqs) {
@@ -920,8 +651,275 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
                 q = get_seq(C, s);
             } while (q.n == 0);
         }
-        x = get_tile(A, q, t, Z::ROWS);
+        x = get_tile(A, q, t, ROWS);
         n = blocks_of(x);
+        measure();
+        return true;
+    }
+};
+
+// Few rows a sequence: the four waves of a workgroup go through a tile's blocks in
+// turn, each with a place of its own in LDS, and join their sums there.
+template <int DIM, bool BF16, int RB>
+__global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) void fp8_attention_kernel(AttnArgs A) {
+    typedef AttnSize<DIM, RB> Z;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const CacheView& C = A.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, g = lane >> 4;
+    clear_rows(A);
+    Work<Z::ROWS> w;
+    if (!w.find(A)) return;
+    const AttnStage<DIM> S(C, reinterpret_cast<char*>(lds) + wave * AttnStage<DIM>::BYTES);
+    float* sums = lds;                                          // [wave][row][PITCH]
+    float* ml = lds + ATTN_WAVES * Z::ROWS * Z::PITCH;          // [wave][row][2]
+    for (;;) {
+        {
+            AttnRows<DIM, BF16, RB> R;
+            R.begin(A, w.q, w.x.r0, w.x.rows, w.head);
+            attend(A, S, R, w.q, w.x, w.s, w.head, w.first() + wave, w.last(), ATTN_WAVES);
+            __syncthreads();
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const int row = 16 * rb + r;
+                const float l = R.row_sum(rb);
+                ml[(wave * Z::ROWS + row) * 2] = R.m[rb];       // by four lanes alike: no branch while the sums are live
+                ml[(wave * Z::ROWS + row) * 2 + 1] = l;
+#pragma unroll
+                for (int d = 0; d < DIM / 16; ++d) {
+                    float4_t v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = ldexpf(R.o[d][rb][i], R.back(rb));
+                    *reinterpret_cast<float4_t*>(sums + (wave * Z::ROWS + row) * Z::PITCH + 16 * d + 4 * g) = v;
+                }
+            }
+        }
+        __syncthreads();
+        float* part = w.whole() ? nullptr : w.part(A, Z::PART);
+        const int quads = C.dim / 4;
+        for (int i = tid; i < w.x.rows * quads; i += ATTN_WAVES * 64) {
+            const int row = i / quads, d = (i - row * quads) * 4;
+            float m = ATTN_LOW, l = 0.f;
+#pragma unroll
+            for (int j = 0; j < ATTN_WAVES; ++j) m = fmaxf(m, ml[(j * Z::ROWS + row) * 2]);
+            float4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < ATTN_WAVES; ++j) {
+                const float f = __builtin_amdgcn_exp2f(ml[(j * Z::ROWS + row) * 2] - m);
+                l += f * ml[(j * Z::ROWS + row) * 2 + 1];
+                const float4_t a = *reinterpret_cast<const float4_t*>(sums + (j * Z::ROWS + row) * Z::PITCH + d);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = fmaf(f, a[e], v[e]);
+            }
+            if (!part) {
+                const int at = (w.x.r0 + row) / A.group, h = w.head * A.group + w.x.r0 + row - at * A.group;
+                const int64_t o = (int64_t)(w.q.first + at) * A.heads + h;
+                float lse;
+                const float f = finish_row(A, h, m, l, lse);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] *= f;
+                store_row4<BF16>(A.out + o * C.dim + d, v);
+                if (A.lse && d == 0) A.lse[o] = lse;
+            } else {
+                *reinterpret_cast<float4_t*>(part + row * DIM + d) = v;
+                if (d == 0) {
+                    part[Z::ROWS * DIM + 2 * row] = m;
+                    part[Z::ROWS * DIM + 2 * row + 1] = l;
+                }
+            }
+        }
+        if (!w.next(A)) break;
+        __syncthreads();                                        // the sums' places hold blocks again
+    }
+}
+
+// ---------------------------------------------------------------- many rows
+
+// Keys and values of a block for a whole workgroup, straight from memory to LDS, in
+// two places that take turns.  A load's 64 chunks of 16 bytes lie in LDS in the order
+// of the lanes, so it is the lane's chunk in memory that is XORed with its row.
+//   keys    [DIM / SUB][64][SUB bytes]
+//   values  [pieces][DIM][16 << lg bytes]: the tokens of a page, 64 at most
+template <int DIM>
+struct AttnShare {
+    static constexpr int SUB = DIM % 128 == 0 ? 128 : 64, CS = SUB / 16, KEYS = 64 / CS;
+    static constexpr int LOADS = DIM / 16 / ATTN_WAVES;       // of a wave, for the keys or the values
+    static constexpr int K_BYTES = ATTN_KEYS * DIM, BYTES = 2 * K_BYTES;
+
+    char* lds;
+    int k_read[2], v_read;
+    uint32_t k_off[2], k_lim, v_off;
+    int lg, wave;
+
+    __device__ __forceinline__ AttnShare(const CacheView& C, char* lds_, int wave_) : lds(lds_), wave(wave_) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+        const int key = lane / CS, place = lane % CS;
+        const int sw = SUB == 128 ? key & 3 : (key >> 1) & 1;
+        k_off[0] = (place ^ sw) << 4;                         // within the row; keys 16 .. 31 and 48 .. 63 have another bit
+        k_off[1] = k_off[0] ^ (SUB == 128 ? 64 : 32);
+        k_lim = key * C.dim;
+        const int sr = SUB == 128 ? (r & 3) | (r >> 2 & 1) << 2 : (r >> 1 & 1) | (r >> 2 & 1) << 1;
+        const int row = (16 * (r >> 2) + (r & 3)) * SUB;
+        k_read[0] = row + ((g ^ sr) << 4);
+        k_read[1] = SUB == 128 ? row + (((4 + g) ^ sr) << 4) : k_read[0] + ATTN_KEYS * SUB;
+        lg = min(C.page_shift, 6) - 4;
+        // a row of `1 << lg` chunks; eight lanes meet every bank once
+        const int channel = lane >> lg, mask = (1 << lg) - 1;
+        const auto swap = [&](int c) { return lg == 2 ? c >> 1 & 3 : lg == 1 ? c >> 2 & 1 : 0; };
+        v_off = (channel << C.page_shift) + (((lane & mask) ^ swap(channel)) << 4);
+        v_read = K_BYTES + ((((g >> lg) * DIM + r) << lg) + ((g & mask) ^ swap(r))) * 16;
+    }
+
+    __device__ __forceinline__ static void to_lds(__amdgpu_buffer_rsrc_t p, char* to, uint32_t at) { load_to_lds(p, to, at, 0); }
+
+    // This wave's loads of block b.
+    __device__ __forceinline__ void load(const CacheView& C, int head, int b, int ids, bool on, int place) const {
+        const int mask = (1 << C.page_shift) - 1;
+        char* to = lds + place * BYTES;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int j = i * ATTN_WAVES + wave;              // LDS chunks 64 j ..: 64 / KEYS loads a piece of SUB channels
+            const int sub = j / (ATTN_KEYS / KEYS), key = j % (ATTN_KEYS / KEYS) * KEYS;
+            const __amdgpu_buffer_rsrc_t p = page_part(C, C.k, head, ids, key >> 4, ((b * ATTN_KEYS + key) & mask) * C.dim, on);
+            const uint32_t c = sub * SUB + k_off[key >> 4 & 1];
+            to_lds(p, to + j * 1024, c < (uint32_t)C.dim ? k_lim + c : OUTSIDE);             // behind the row's end: zeros
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int j = i * ATTN_WAVES + wave;              // LDS chunks 64 j ..: (DIM << lg) / 64 loads a piece
+            const int each = (DIM << lg) / 64, piece = lg == 2 ? 0 : j / each, channel = (j - piece * each) << (6 - lg);
+            const int g = piece << lg;
+            const __amdgpu_buffer_rsrc_t p = page_part(C, C.v, head, ids, g, (b * ATTN_KEYS + 16 * g) & mask, on);
+            to_lds(p, to + K_BYTES + j * 1024, v_off + (channel << C.page_shift));           // behind the last channel: zeros
+        }
+    }
+
+    __device__ __forceinline__ u32x4_t key(int place, int t, int k) const {
+        return *reinterpret_cast<const u32x4_t*>(lds + place * BYTES + k_read[k & 1] +
+                                                 k / 2 * (ATTN_KEYS * 128) + 4 * t * SUB);
+    }
+    __device__ __forceinline__ u32x4_t value(int place, int d) const {
+        return *reinterpret_cast<const u32x4_t*>(lds + place * BYTES + v_read + (d << (8 + lg)));
+    }
+};
+
+template <int DIM, int RB>
+struct ShareSize {
+    static constexpr int ROWS = ATTN_WAVES * 16 * RB;
+    static constexpr int LDS = 2 * AttnShare<DIM>::BYTES;
+    static constexpr int WAVES_EU = DIM <= 128 ? 2 : 1;
+    static constexpr int PART = ROWS * (DIM + 2);
+    static_assert(LDS >= ROWS * DIM * 2, "a tile's results go through the blocks' places");
+};
+
+// Many rows a sequence: each wave has rows of its own, all go through a tile's blocks
+// together, with one barrier a block; the next block is on its way meanwhile.
+template <int DIM, bool BF16, int RB>
+__global__ __launch_bounds__(ATTN_WAVES * 64, (ShareSize<DIM, RB>::WAVES_EU)) void fp8_attention_rows_kernel(AttnArgs A) {
+    typedef ShareSize<DIM, RB> Z;
+    constexpr int OWN = 16 * RB;
+    extern __shared__ __attribute__((aligned(16))) char share_lds[];
+    const CacheView& C = A.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, g = lane >> 4;
+    clear_rows(A);
+    Work<Z::ROWS> w;
+    if (!w.find(A)) return;
+    const AttnShare<DIM> S(C, share_lds, wave);
+    for (;;) {
+        const int first = w.first(), last = w.last();
+        // this wave's rows; a wave without any takes the first one's, and stores nothing
+        const int rows = w.x.rows - wave * OWN;
+        const Tile x = get_tile(A, w.q, w.t * ATTN_WAVES + (rows > 0 ? wave : 0), OWN);
+        AttnRows<DIM, BF16, RB> R;
+        R.begin(A, w.q, x.r0, x.rows, w.head);
+        const Pages P(C, w.q, w.s);
+        bool nans = false;
+        if (first < last) {
+            int ids = P.of(C, first), next = P.of(C, min(first + 1, last - 1));
+            float ks = scale_of(C, C.k_scale, ids, w.head), vs = scale_of(C, C.v_scale, ids, w.head);
+            S.load(C, w.head, first, ids, true, 0);
+            for (int b = first; b < last; ++b) {
+                const int place = (b - first) & 1, id = ids;
+                const float ks_now = ks, vs_now = vs;
+                const int after = P.of(C, min(b + 2, last - 1));
+                wait_loads();
+                bare_barrier();                                 // block b is there, and nobody reads the other place
+                ids = next;
+                next = after;
+                ks = scale_of(C, C.k_scale, ids, w.head);
+                vs = scale_of(C, C.v_scale, ids, w.head);
+                S.load(C, w.head, b + 1, ids, b + 1 < last, place ^ 1);
+                const int key0 = b * ATTN_KEYS + (lane & 48);
+                const auto key = [&](int t, int k) { return S.key(place, t, k); };
+                const auto value = [&](int d) { return S.value(place, d); };
+                if (rows > 0 && b * ATTN_KEYS < x.hi && (b + 1) * ATTN_KEYS > x.lo) {
+                    if (masked_block(C, x, b, id))
+                        nans |= R.template step<true>(A, ks_now, vs_now, valid_page(C, id), key0, x.lo, x.hi, key, value);
+                    else
+                        R.template step<false>(A, ks_now, vs_now, true, key0, 0, 0, key, value);
+                }
+            }
+            wait_loads();                                       // a load of nothing writes zeros
+            if (__syncthreads_or(nans)) {
+                for (int b = first; b < last; ++b) {
+                    const int id = P.of(C, b);
+                    S.load(C, w.head, b, id, true, 0);
+                    wait_loads();
+                    bare_barrier();
+                    R.add_nans(valid_page(C, id), b * ATTN_KEYS + (lane & 48), x.lo, x.hi, [&](int d) { return S.value(0, d); });
+                    wait_loads();
+                    bare_barrier();
+                }
+            }
+        }
+        float lse[RB];
+        if (w.whole()) {
+            // through LDS: rows leave it 16 bytes a lane
+            uint16_t* out = reinterpret_cast<uint16_t*>(share_lds) + wave * OWN * DIM;
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const int row = 16 * rb + r, of = x.r0 + min(row, x.rows - 1), at = of / A.group;
+                const float f = finish_row(A, w.head * A.group + of - at * A.group, R.m[rb], R.row_sum(rb), lse[rb]);
+#pragma unroll
+                for (int d = 0; d < DIM / 16; ++d) {
+                    float4_t v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = ldexpf(R.o[d][rb][i], R.back(rb)) * f;
+                    store_row4<BF16>(out + row * DIM + 16 * d + 4 * g, v);
+                }
+            }
+            asm volatile("" ::: "memory");
+            const int chunks = C.dim / 8;
+            for (int i = lane; i < (rows > 0 ? x.rows : 0) * chunks; i += 64) {
+                const int row = i / chunks, d = (i - row * chunks) * 8, of = x.r0 + row, at = of / A.group;
+                const int64_t o = (int64_t)(w.q.first + at) * A.heads + w.head * A.group + of - at * A.group;
+                *reinterpret_cast<u32x4_t*>(A.out + o * C.dim + d) = *reinterpret_cast<const u32x4_t*>(out + row * DIM + d);
+            }
+            if (A.lse && rows > 0 && g == 0) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    const int row = 16 * rb + r, of = x.r0 + row, at = of / A.group;
+                    if (row < x.rows)
+                        A.lse[(int64_t)(w.q.first + at) * A.heads + w.head * A.group + of - at * A.group] = lse[rb];
+                }
+            }
+        } else {
+            float* part = w.part(A, Z::PART);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const int row = wave * OWN + 16 * rb + r;      // rows behind the last have room too
+#pragma unroll
+                for (int d = 0; d < DIM / 16; ++d) {
+                    float4_t v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = ldexpf(R.o[d][rb][i], R.back(rb));
+                    *reinterpret_cast<float4_t*>(part + row * DIM + 16 * d + 4 * g) = v;
+                }
+                part[Z::ROWS * DIM + 2 * row] = R.m[rb];
+                part[Z::ROWS * DIM + 2 * row + 1] = R.row_sum(rb);
+            }
+        }
+        if (!w.next(A)) break;
+        __syncthreads();                                        // the results' places hold blocks again
     }
 }
 
@@ -929,10 +927,9 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
 // begins it, blockIdx.y takes every gridDim.y-th row.  A row's threads are groups that
 // each take some of the partial results, four channels a thread; the groups' sums
 // meet in LDS.
-template <int DIM, bool BF16, int RB>
+template <int DIM, bool BF16, int ROWS>
 __global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_join_kernel(AttnArgs A) {
-    typedef AttnSize<DIM, RB> Z;
-    constexpr int QUADS = DIM / 4, GROUPS = ATTN_WAVES * 64 / QUADS;
+    constexpr int PART = ROWS * (DIM + 2), QUADS = DIM / 4, GROUPS = ATTN_WAVES * 64 / QUADS;
     __shared__ float4_t sums[GROUPS][QUADS];
     __shared__ float ml[GROUPS][2];
     const CacheView& C = A.c;
@@ -940,9 +937,9 @@ __global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_join_kernel(Att
     const int first = blockIdx.x, group = threadIdx.x / QUADS, d = (threadIdx.x - group * QUADS) * 4;
     if (x.last < 0) return;
     const auto take = [&](int w, int row, float& m, float& l, float4_t& v) {
-        const float* p = A.part + ((int64_t)w * 2 + (w == first ? 1 : 0)) * Z::PART;
-        const float pm = p[Z::ROWS * DIM + 2 * row], pl = p[Z::ROWS * DIM + 2 * row + 1];
-        const float4_t a = *reinterpret_cast<const float4_t*>(p + row * C.dim + d);
+        const float* p = A.part + ((int64_t)w * 2 + (w == first ? 1 : 0)) * PART;
+        const float pm = p[ROWS * DIM + 2 * row], pl = p[ROWS * DIM + 2 * row + 1];
+        const float4_t a = *reinterpret_cast<const float4_t*>(p + row * DIM + d);
         const float m1 = fmaxf(m, pm), f = __builtin_amdgcn_exp2f(m - m1), g = __builtin_amdgcn_exp2f(pm - m1);
         m = m1;
         l = fmaf(g, pl, l * f);

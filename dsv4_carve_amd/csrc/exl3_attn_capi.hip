@@ -30,13 +30,14 @@ static int log2_of(int64_t v) { return 63 - __builtin_clzll((unsigned long long)
 static AttnPlan plan_attention(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t keys) {
     const int64_t group = heads / kv_heads, rows = (tokens + seqs - 1) / seqs * group, cus = device_cus();
     AttnPlan P{};
-    P.rb = rows <= 16 ? 1 : rows <= 32 || dim > 128 ? 2 : 4;
-    const int64_t tiles = tokens * group / (16 * P.rb) + std::min(seqs, tokens), blocks = (keys + ATTN_KEYS - 1) / ATTN_KEYS;
+    P.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : ATTN_MANY;
+    const int64_t tiles = tokens * group / P.rows + std::min(seqs, tokens), blocks = (keys + ATTN_KEYS - 1) / ATTN_KEYS;
     P.tiles = (unsigned)tiles;
-    if (tiles * kv_heads < 2 * cus || P.rb == 1) {
-        const int64_t most = cus * (P.rb == 4 ? 1 : 2), units = tiles * kv_heads * std::max<int64_t>(blocks, 1);
-        P.shares = (unsigned)std::max<int64_t>(1, std::min(most, (units + ATTN_WAVES - 1) / ATTN_WAVES));
-        P.join_rows = (unsigned)(P.shares > 4 * tiles * kv_heads ? 16 * P.rb : 4 * P.rb);
+    if (tiles * kv_heads < 2 * cus || P.rows < ATTN_MANY) {
+        const int64_t each = P.rows < ATTN_MANY ? ATTN_WAVES : 1, units = tiles * kv_heads * std::max<int64_t>(blocks, 1);
+        P.shares = (unsigned)std::max<int64_t>(1, std::min(2 * cus, (units + each - 1) / each));
+        P.least = (int)each;
+        P.join_rows = (unsigned)(P.shares > 4 * tiles * kv_heads ? P.rows : P.rows / 4);
     }
     return P;
 }
@@ -44,7 +45,7 @@ static AttnPlan plan_attention(int64_t tokens, int64_t heads, int64_t kv_heads, 
 // Partial results, and what the workgroups say of them.
 static int64_t part_bytes(const AttnPlan& P, int64_t dim) {
     const int64_t padded = (dim + 63) / 64 * 64;
-    return (int64_t)P.shares * 2 * 16 * P.rb * (padded + 2) * 4;
+    return (int64_t)P.shares * 2 * P.rows * (padded + 2) * 4;
 }
 
 static int64_t attention_scratch(const AttnPlan& P, int64_t dim) {
@@ -122,7 +123,7 @@ int exl3_fp8_attention(const void* q, int kind, int64_t q_token, int64_t q_head,
                static_cast<const uint16_t*>(q), q_token, q_head, (int)heads, (int)(heads / kv_heads),
                std::fabs(scale) * 1.4426950408889634f, scale < 0.f, (int)window, sinks, static_cast<uint16_t*>(out), lse,
                P.shares ? static_cast<float*>(scratch) : nullptr,
-               reinterpret_cast<SharedTile*>(static_cast<char*>(scratch) + part_bytes(P, dim)), (int)P.tiles, ATTN_WAVES, clear != 0};
+               reinterpret_cast<SharedTile*>(static_cast<char*>(scratch) + part_bytes(P, dim)), (int)P.tiles, P.least, clear != 0};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const bool bf16 = kind == OUT_BF16;
     if (dim <= 64) return launch_attention_64(A, P, bf16, s);

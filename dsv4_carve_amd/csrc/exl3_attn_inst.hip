@@ -3,11 +3,8 @@
 
 namespace exl3 {
 
-template <int DIM, bool BF16, int RB>
-static int launch(const AttnArgs& A, const AttnPlan& P, hipStream_t s) {
-    const auto kernel = fp8_attention_kernel<DIM, BF16, RB>;
-    constexpr int LDS = AttnSize<DIM, RB>::LDS;
-    static std::atomic<uint64_t> ready{0};           // devices that know of the LDS size
+template <int DIM, bool BF16, int ROWS, int LDS>
+static int launch(void (*kernel)(AttnArgs), const AttnArgs& A, const AttnPlan& P, std::atomic<uint64_t>& ready, hipStream_t s) {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= MAX_DEVICES) return fail("no HIP device");
     if (!(ready.load() >> dev & 1)) {
@@ -16,24 +13,29 @@ static int launch(const AttnArgs& A, const AttnPlan& P, hipStream_t s) {
             return fail("the device does not give the kernel its LDS");
         ready.fetch_or(1ull << dev);
     }
-    if (P.shares) {
-        hipLaunchKernelGGL(kernel, dim3(P.shares), dim3(ATTN_WAVES * 64), LDS, s, A);
-        if (check_launch()) return -1;
-        if (P.shares == 1) return 0;
-        hipLaunchKernelGGL((fp8_attention_join_kernel<DIM, BF16, RB>), dim3(P.shares - 1, P.join_rows), dim3(ATTN_WAVES * 64), 0,
-                           s, A);
-    } else {
-        hipLaunchKernelGGL(kernel, dim3((P.tiles + XCDS - 1) / XCDS * XCDS * A.c.kv), dim3(ATTN_WAVES * 64), LDS, s, A);
-    }
+    const unsigned grid = P.shares ? P.shares : (P.tiles + XCDS - 1) / XCDS * XCDS * A.c.kv;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(ATTN_WAVES * 64), LDS, s, A);
+    if (check_launch()) return -1;
+    if (P.shares < 2) return 0;
+    hipLaunchKernelGGL((fp8_attention_join_kernel<DIM, BF16, ROWS>), dim3(P.shares - 1, P.join_rows), dim3(ATTN_WAVES * 64), 0, s, A);
     return check_launch();
+}
+
+template <int DIM, bool BF16, int RB>
+static int launch_few(const AttnArgs& A, const AttnPlan& P, hipStream_t s) {
+    static std::atomic<uint64_t> ready{0};           // devices that know of the LDS size
+    typedef AttnSize<DIM, RB> Z;
+    return launch<DIM, BF16, Z::ROWS, Z::LDS>(fp8_attention_kernel<DIM, BF16, RB>, A, P, ready, s);
 }
 
 template <int DIM, bool BF16>
 static int launch(const AttnArgs& A, const AttnPlan& P, hipStream_t s) {
-    if (P.rb == 1) return launch<DIM, BF16, 1>(A, P, s);
-    if constexpr (DIM <= 128)
-        if (P.rb == 4) return launch<DIM, BF16, 4>(A, P, s);
-    return launch<DIM, BF16, 2>(A, P, s);
+    if (P.rows == 16) return launch_few<DIM, BF16, 1>(A, P, s);
+    if (P.rows == 32) return launch_few<DIM, BF16, 2>(A, P, s);
+    static std::atomic<uint64_t> ready{0};
+    typedef ShareSize<DIM, 2> Z;
+    static_assert(Z::ROWS == ATTN_MANY, "rows of a tile");
+    return launch<DIM, BF16, Z::ROWS, Z::LDS>(fp8_attention_rows_kernel<DIM, BF16, 2>, A, P, ready, s);
 }
 
 #define EXL3_ATTN_CAT_(a, b) a##b

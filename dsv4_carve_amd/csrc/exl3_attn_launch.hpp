@@ -7,10 +7,13 @@
 
 namespace exl3 {
 
+constexpr int ATTN_MANY = 128;
+
 struct AttnPlan {
-    int rb;                      // 16 rb rows a tile
+    int rows;                    // of a tile: 16, 32 or ATTN_MANY
     unsigned shares;             // workgroups that share the work, or 0: a workgroup a tile
     unsigned tiles;              // tiles at most, for a workgroup a tile
+    int least;                   // units that a workgroup has at least
     unsigned join_rows;          // workgroups that join the rows of a tile
 };
 

@@ -1,0 +1,264 @@
+// A paged cache of e4m3 keys and values with one power-of-two scale for each page
+// and head, and the write into it.
+//
+//   k  [pages][kv][page][dim]   k_scale [pages][kv]
+//   v  [pages][kv][dim][page]   v_scale [pages][kv]      (a value's tokens are neighbours)
+//
+// A power of two as the scale keeps a value's bits where the scale of a begun page
+// grows (but for those that fall below e4m3's normal range), and e4m3's relative
+// error does not depend on where in its range a value lies.
+#pragma once
+
+#include "exl3_fp8.hpp"
+#include "exl3_topk.hpp"
+
+namespace exl3 {
+
+struct CacheView {
+    uint8_t* k;
+    float* k_scale;
+    uint8_t* v;
+    float* v_scale;
+    const int* table;            // [seqs][width] pages
+    int64_t table_stride;
+    const int* lengths;          // [seqs], the new tokens counted
+    const int* starts;           // [seqs + 1] first token of each sequence, or null: one token each
+    int seqs, tokens, kv, dim, page_shift, width, pages;
+};
+
+// A sequence's tokens in a call and its length.  What a table, a length or a start
+// names past its range is cut to it: no index leaves a buffer.
+struct Seq {
+    int first, n, len;
+};
+
+__device__ __forceinline__ Seq get_seq(const CacheView& C, int s) {
+    Seq q;
+    if (C.starts) {
+        const int a = C.starts[s], b = C.starts[s + 1];
+        q.first = min(max(a, 0), C.tokens);
+        q.n = max(min(b, C.tokens) - q.first, 0);
+    } else {
+        q.first = s;
+        q.n = 1;
+    }
+    const int64_t room = (int64_t)C.width << C.page_shift;
+    const int len = max(C.lengths[s], 0);
+    q.len = (int64_t)len < room ? len : (int)room;
+    return q;
+}
+
+// A value that all lanes have alike, known as such to the compiler: control flow and
+// addresses that follow from it are scalar.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const u32x2_t a = __builtin_bit_cast(u32x2_t, v);
+    return __builtin_bit_cast(int64_t, u32x2_t{(uint32_t)uniform((int)a[0]), (uint32_t)uniform((int)a[1])});
+}
+
+// Inclusive prefix sums over the wave's lanes.
+__device__ __forceinline__ int64_t wave_scan(int64_t v) {
+    v += lane_of<0x111, 0xf>(v, (int64_t)0);        // row_shr:1, 2, 4, 8
+    v += lane_of<0x112, 0xf>(v, (int64_t)0);
+    v += lane_of<0x114, 0xf>(v, (int64_t)0);
+    v += lane_of<0x118, 0xf>(v, (int64_t)0);
+    v += lane_of<0x142, 0xa>(v, (int64_t)0);        // row_bcast:15, 31
+    v += lane_of<0x143, 0xc>(v, (int64_t)0);
+    return v;
+}
+
+// a / b, 0 <= a, 0 < b; in 32 bits where both fit.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+    return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// The sequence that a unit of all sequences' units lies in; count(q) units each.  The
+// unit is at(total), total being all of them; s is -1 where it lies behind them.  Every
+// wave looks by itself: up to 64 sequences are one load and one scan.
+struct Found {
+    int s;
+    int64_t unit;                // within the sequence
+    Seq q;
+};
+
+template <typename Count, typename At>
+__device__ __forceinline__ Found find_seq(const CacheView& C, Count&& count, At&& at) {
+    const int lane = threadIdx.x & 63;
+    const Seq none{0, 0, 0};
+    Found f{-1, 0, none};
+    const auto look = [&](int s0, const Seq& q, int64_t c, int64_t before, int64_t sum, int64_t want) {
+        before += sum - c;
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(want >= before && want < before + c);
+        if (!hit) return;
+        const int l = __builtin_ctzll(hit);
+        f.s = s0 + l;
+        f.unit = want - read_lane(before, l);
+        f.q = Seq{read_lane(q.first, l), read_lane(q.n, l), read_lane(q.len, l)};
+    };
+    if (C.seqs <= 64) {
+        const Seq q = lane < C.seqs ? get_seq(C, lane) : none;
+        const int64_t c = count(q), sum = wave_scan(c);
+        look(0, q, c, 0, sum, at(read_lane(sum, 63)));
+    } else {
+        int64_t c = 0;
+        for (int s = lane; s < C.seqs; s += 64) c += count(get_seq(C, s));
+        const int64_t want = at(read_lane(wave_scan(c), 63));
+        int64_t before = 0;
+        for (int s0 = 0; s0 < C.seqs && want >= before && f.s < 0; s0 += 64) {
+            const Seq q = s0 + lane < C.seqs ? get_seq(C, s0 + lane) : none;
+            const int64_t n = count(q), sum = wave_scan(n);
+            look(s0, q, n, before, sum, want);
+            before += read_lane(sum, 63);
+        }
+    }
+    return f;
+}
+
+// ---------------------------------------------------------------- the write
+
+constexpr int APPEND_WAVES = 4;
+
+struct AppendArgs {
+    CacheView c;
+    const void* k;
+    const void* v;
+    int64_t k_token, k_head, v_token, v_head;          // strides in values
+};
+
+// The pages that a sequence's new tokens lie in.
+__device__ __forceinline__ int touched_pages(const CacheView& C, const Seq& q) {
+    const int from = max(q.len - q.n, 0);
+    return q.len > from ? ((q.len - 1) >> C.page_shift) - (from >> C.page_shift) + 1 : 0;
+}
+
+// Eight neighbouring values (16-byte aligned) as fp32; an infinity as a NaN.
+template <int K>
+__device__ __forceinline__ void load8_finite(const void* p, int64_t at, float (&v)[8]) {
+    if constexpr (K == OUT_F32) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float4_t f = reinterpret_cast<const float4_t*>(static_cast<const float*>(p) + at)[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * i + j] = f[j];
+        }
+    } else {
+        const u32x4_t u = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[2 * j] = K == OUT_BF16 ? __uint_as_float(u[j] << 16) : f16_bits_to_f32((uint16_t)u[j]);
+            v[2 * j + 1] = K == OUT_BF16 ? __uint_as_float(u[j] & 0xffff0000u) : f16_bits_to_f32((uint16_t)(u[j] >> 16));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = fabsf(v[j]) == __builtin_inff() ? __builtin_nanf("") : v[j];
+}
+
+// Four codes times a power of two, rounded to e4m3 again.
+__device__ __forceinline__ uint32_t rescale4(uint32_t u, float by) {
+    return pack_e4m3(__builtin_amdgcn_cvt_f32_fp8((int)u, 0) * by, __builtin_amdgcn_cvt_f32_fp8((int)u, 1) * by,
+                     __builtin_amdgcn_cvt_f32_fp8((int)u, 2) * by, __builtin_amdgcn_cvt_f32_fp8((int)u, 3) * by);
+}
+
+// A workgroup has one page of one head, of the keys or of the values: the new
+// tokens' largest magnitude, the scale, the old codes where it grew, the new ones.
+// The inputs are read twice (the second time from cache).
+template <int K>
+__global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(AppendArgs A) {
+    __shared__ float most_of[APPEND_WAVES];
+    const CacheView& C = A.c;
+    const int tid = threadIdx.x, head = blockIdx.y;
+    const bool values = blockIdx.z;
+    int s = blockIdx.x, nth = 0;
+    Seq q;
+    if (C.starts) {
+        const Found f = find_seq(C, [&](const Seq& x) { return (int64_t)touched_pages(C, x); },
+                                 [](int64_t) { return (int64_t)blockIdx.x; });
+        if (f.s < 0) return;
+        s = f.s;
+        nth = (int)f.unit;
+        q = f.q;
+    } else {
+        q = get_seq(C, s);
+    }
+    const int page = 1 << C.page_shift, base = q.len - q.n, from = max(base, 0);
+    if (q.len <= from) return;
+    const int at = (from >> C.page_shift) + nth;                                  // the page's place in the sequence
+    const int id = C.table[s * C.table_stride + at];
+    if ((unsigned)id >= (unsigned)C.pages) return;
+    const int lo = max(from - (at << C.page_shift), 0), hi = min(q.len - (at << C.page_shift), page);
+    const int64_t token = q.first + (at << C.page_shift) - base;                  // the token of the page's place 0
+    const int64_t stride = values ? A.v_token : A.k_token;
+    const int64_t in0 = token * stride + head * (values ? A.v_head : A.k_head);
+    const void* in = values ? A.v : A.k;
+    const int64_t block = (int64_t)id * C.kv + head;
+    uint8_t* code = (values ? C.v : C.k) + (block << C.page_shift) * C.dim;
+    float* scale = (values ? C.v_scale : C.k_scale) + block;
+
+    const int per = C.dim >> 3;                                                   // chunks of eight a token
+    float most = 0.f;
+    float x[8];
+    for (int i = tid; i < (hi - lo) * per; i += APPEND_WAVES * 64) {
+        const int t = i / per;
+        load8_finite<K>(in, in0 + (lo + t) * stride + (i - t * per) * 8, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+    }
+    most = wave_max(most, 0.f);
+    if ((tid & 63) == 0) most_of[tid >> 6] = most;
+    const float before = lo ? *scale : 0.f;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < APPEND_WAVES; ++w) most = fmaxf(most, most_of[w]);
+    const float now = fmaxf(QuantGroup(most, true).scale, before);
+    const float inverse = 1.0f / now, by = before / now;
+    const bool grew = lo && by != 1.0f;
+    if (!values) {
+        if (grew)
+            for (int i = tid; i < lo * C.dim / 16; i += APPEND_WAVES * 64) {
+                u32x4_t u = reinterpret_cast<u32x4_t*>(code)[i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) u[j] = rescale4(u[j], by);
+                reinterpret_cast<u32x4_t*>(code)[i] = u;
+            }
+        for (int i = tid; i < (hi - lo) * per; i += APPEND_WAVES * 64) {
+            const int t = i / per, d = (i - t * per) * 8;
+            load8_finite<K>(in, in0 + (lo + t) * stride + d, x);
+            *reinterpret_cast<u32x2_t*>(code + (lo + t) * C.dim + d) =
+                u32x2_t{pack_e4m3(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse),
+                        pack_e4m3(x[4] * inverse, x[5] * inverse, x[6] * inverse, x[7] * inverse)};
+        }
+    } else {
+        // 16 tokens of one value's channel at once; what is outside [lo, hi) goes back as it was, or rescaled below lo
+        const int first = grew ? 0 : lo >> 4, groups = ((hi + 15) >> 4) - first;
+        for (int i = tid; i < groups * C.dim; i += APPEND_WAVES * 64) {
+            const int b = i / C.dim, d = i - b * C.dim, t0 = (first + b) * 16;
+            u32x4_t* p = reinterpret_cast<u32x4_t*>(code + ((int64_t)d << C.page_shift) + t0);
+            u32x4_t u = {0, 0, 0, 0};
+            if (t0 < lo || t0 + 16 > hi) u = *p;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t moved = grew ? rescale4(u[j], by) : u[j];
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int t = t0 + 4 * j + e;
+                    const float f = t >= lo && t < hi ? load_kind<K>(in, in0 + t * stride + d) : 0.f;
+                    y[e] = (fabsf(f) == __builtin_inff() ? __builtin_nanf("") : f) * inverse;
+                }
+                const uint32_t made = pack_e4m3(y[0], y[1], y[2], y[3]);
+                uint32_t r = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int t = t0 + 4 * j + e;
+                    const uint32_t m = 0xffu << (8 * e);
+                    r |= m & (t < lo ? moved : t < hi ? made : u[j]);
+                }
+                u[j] = r;
+            }
+            *p = u;
+        }
+    }
+    if (tid == 0) *scale = now;
+}
+
+}  // namespace exl3
