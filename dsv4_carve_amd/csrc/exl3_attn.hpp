@@ -168,18 +168,27 @@ struct AttnRows {
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) p[t][rb] = float4_t{0.f, 0.f, 0.f, 0.f};
+        // Two reads from LDS are on their way while the last two are multiplied: piece n of the keys is t = 2 n % 4 and the
+        // next, k = n / 2; the values' follow.
+        u32x4_t z[2][2];
+        const auto read_key = [&](int n, int i) { return key(2 * n % 4 + i, n / 2); };
 #pragma unroll
-        for (int k = 0; k < KC; ++k)
+        for (int i = 0; i < 2; ++i) z[0][i] = read_key(0, i);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const u32x4_t z = key(t, k);
+        for (int n = 0; n < 2 * KC; ++n) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const typename H::vec8 w = H::widen(z[2 * u], z[2 * u + 1]);
+            for (int i = 0; i < 2; ++i) z[(n + 1) & 1][i] = n + 1 < 2 * KC ? read_key(n + 1, i) : value(i);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) p[t][rb] = H::mfma(w, qf[rb][k][u], p[t][rb]);
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const typename H::vec8 w = H::widen(z[n & 1][i][2 * u], z[n & 1][i][2 * u + 1]);
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) p[2 * n % 4 + i][rb] = H::mfma(w, qf[rb][n / 2][u], p[2 * n % 4 + i][rb]);
                 }
-            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
         float kc = fmaxf(ks * A.qk_scale, 0x1p-126f);
         uint32_t keep[4];
         if constexpr (MASKED) {
@@ -246,29 +255,41 @@ struct AttnRows {
                     if constexpr (FINE) rest[rb][t >> 1][4 * (t & 1) + i] = (_Float16)(w - (float)h);
                 }
             l[rb] = fmaf(sum, __builtin_amdgcn_exp2f(-k), l[rb]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         uint32_t nan = 0;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            u32x4_t z = value(d);
+        for (int n = 0; n < DT / 2; ++n) {
+            u32x4_t (&v)[2] = z[n & 1];
+            if (n + 1 < DT / 2) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) z[(n + 1) & 1][i] = value(2 * n + 2 + i);
+            }
+            __builtin_amdgcn_sched_barrier(0);
             if constexpr (MASKED) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    z[j] &= keep[j];
-                    const uint32_t bad = nan_bytes(z[j]);
-                    nan |= bad;
-                    z[j] &= ~((bad >> 7) * 0xffu);
-                }
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        v[i][j] &= keep[j];
+                        const uint32_t bad = nan_bytes(v[i][j]);
+                        nan |= bad;
+                        v[i][j] &= ~((bad >> 7) * 0xffu);
+                    }
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const half8_t v = W::widen(z[2 * u], z[2 * u + 1]);
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    o[d][rb] = W::mfma(v, big[rb][u], o[d][rb]);
-                    if constexpr (FINE) o[d][rb] = W::mfma(v, rest[rb][u], o[d][rb]);
+                for (int i = 0; i < 2; ++i) {
+                    const half8_t w = W::widen(v[i][2 * u], v[i][2 * u + 1]);
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) o[2 * n + i][rb] = W::mfma(w, big[rb][u], o[2 * n + i][rb]);
+                    if constexpr (FINE) {
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) o[2 * n + i][rb] = W::mfma(w, rest[rb][u], o[2 * n + i][rb]);
+                    }
                 }
-            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         return MASKED && __builtin_amdgcn_ballot_w64(nan != 0) != 0;
     }
@@ -312,7 +333,15 @@ struct AttnRows {
     __device__ __forceinline__ int back(int rb) const { return (int)c[rb] - ATTN_HEADROOM; }
 };
 
-// A sequence's pages and their scales for one cache head.
+// v in another register: the one that it came in is free for the next load.
+template <typename T>
+__device__ __forceinline__ T moved(T v) {
+    T r;
+    asm volatile("v_mov_b32 %0, %1" : "=v"(r) : "v"(v));
+    return r;
+}
+
+// A sequence's pages for one cache head.
 struct Pages {
     const int* table;
     int pages;
@@ -320,11 +349,11 @@ struct Pages {
     __device__ __forceinline__ Pages(const CacheView& C, const Seq& q, int s)
         : table(C.table + s * C.table_stride), pages((q.len + (1 << C.page_shift) - 1) >> C.page_shift) {}
 
-    // The page of the 16 keys from 64 b + 16 (lane / 16) on, -1 behind the sequence's end.
-    __device__ __forceinline__ int of(const CacheView& C, int b) const {
-        const int i = (b * ATTN_KEYS + (threadIdx.x & 48)) >> C.page_shift, id = table[min(i, pages - 1)];
-        return i < pages ? id : -1;
-    }
+    // The page of the 16 keys from 64 b + 16 (lane / 16) on, -1 behind the sequence's end; raw: as the table has it.
+    __device__ __forceinline__ int index(const CacheView& C, int b) const { return (b * ATTN_KEYS + (threadIdx.x & 48)) >> C.page_shift; }
+    __device__ __forceinline__ int raw(const CacheView& C, int b) const { return table[min(index(C, b), pages - 1)]; }
+    __device__ __forceinline__ int of(const CacheView& C, int b, int raw) const { return index(C, b) < pages ? raw : -1; }
+    __device__ __forceinline__ int of(const CacheView& C, int b) const { return of(C, b, raw(C, b)); }
 };
 
 __device__ __forceinline__ bool valid_page(const CacheView& C, int id) { return (unsigned)id < (unsigned)C.pages; }
@@ -747,16 +776,16 @@ struct AttnShare {
 
     char* lds;
     int k_read[2], v_read;
-    uint32_t k_off[2], k_lim, v_off;
+    uint32_t k_off, k_row, v_off;
     int lg, wave;
 
     __device__ __forceinline__ AttnShare(const CacheView& C, char* lds_, int wave_) : lds(lds_), wave(wave_) {
         const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
         const int key = lane / CS, place = lane % CS;
         const int sw = SUB == 128 ? key & 3 : (key >> 1) & 1;
-        k_off[0] = (place ^ sw) << 4;                         // within the row; keys 16 .. 31 and 48 .. 63 have another bit
-        k_off[1] = k_off[0] ^ (SUB == 128 ? 64 : 32);
-        k_lim = key * C.dim;
+        // within the row; keys 16 .. 31 and 48 .. 63 have another bit, and a wave's loads are all of such keys or all of others
+        k_off = ((place ^ sw) << 4) ^ ((wave * KEYS >> 4 & 1) ? SUB / 2 : 0);
+        k_row = key * C.dim;
         const int sr = SUB == 128 ? (r & 3) | (r >> 2 & 1) << 2 : (r >> 1 & 1) | (r >> 2 & 1) << 1;
         const int row = (16 * (r >> 2) + (r & 3)) * SUB;
         k_read[0] = row + ((g ^ sr) << 4);
@@ -778,10 +807,10 @@ struct AttnShare {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int j = i * ATTN_WAVES + wave;              // LDS chunks 64 j ..: 64 / KEYS loads a piece of SUB channels
-            const int sub = j / (ATTN_KEYS / KEYS), key = j % (ATTN_KEYS / KEYS) * KEYS;
+            const int sub = i * ATTN_WAVES / (ATTN_KEYS / KEYS), key = (j - sub * (ATTN_KEYS / KEYS)) * KEYS;
             const __amdgpu_buffer_rsrc_t p = page_part(C, C.k, head, ids, key >> 4, ((b * ATTN_KEYS + key) & mask) * C.dim, on);
-            const uint32_t c = sub * SUB + k_off[key >> 4 & 1];
-            to_lds(p, to + j * 1024, c < (uint32_t)C.dim ? k_lim + c : OUTSIDE);             // behind the row's end: zeros
+            const uint32_t c = sub * SUB + k_off;
+            to_lds(p, to + j * 1024, c < (uint32_t)C.dim ? k_row + c : OUTSIDE);             // behind the row's end: zeros
         }
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
@@ -834,29 +863,44 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (ShareSize<DIM, RB>::WAVES_EU)) vo
         const Pages P(C, w.q, w.s);
         bool nans = false;
         if (first < last) {
-            int ids = P.of(C, first), next = P.of(C, min(first + 1, last - 1));
+            // What a block needs is asked for a whole block before, so that the wait at its beginning is for all of it alike.
+            int raw = P.raw(C, first);
+            int ids = P.of(C, first, raw);
             float ks = scale_of(C, C.k_scale, ids, w.head), vs = scale_of(C, C.v_scale, ids, w.head);
             S.load(C, w.head, first, ids, true, 0);
-            for (int b = first; b < last; ++b) {
-                const int place = (b - first) & 1, id = ids;
-                const float ks_now = ks, vs_now = vs;
-                const int after = P.of(C, min(b + 2, last - 1));
+            raw = P.raw(C, min(first + 1, last - 1));
+            int id, key0, place;
+            float ks_now, vs_now;
+            // Block b begins; 0: these rows see nothing of it, 1: all of them see it whole, 2: some do not.
+            const auto top = [&](int b) {
+                place = (b - first) & 1;
+                id = ids;
+                key0 = b * ATTN_KEYS + (lane & 48);
                 wait_loads();
                 bare_barrier();                                 // block b is there, and nobody reads the other place
-                ids = next;
-                next = after;
+                ks_now = moved(ks);
+                vs_now = moved(vs);
+                ids = P.of(C, b + 1, moved(raw));
+                raw = P.raw(C, min(b + 2, last - 1));
                 ks = scale_of(C, C.k_scale, ids, w.head);
                 vs = scale_of(C, C.v_scale, ids, w.head);
                 S.load(C, w.head, b + 1, ids, b + 1 < last, place ^ 1);
-                const int key0 = b * ATTN_KEYS + (lane & 48);
-                const auto key = [&](int t, int k) { return S.key(place, t, k); };
-                const auto value = [&](int d) { return S.value(place, d); };
-                if (rows > 0 && b * ATTN_KEYS < x.hi && (b + 1) * ATTN_KEYS > x.lo) {
-                    if (masked_block(C, x, b, id))
-                        nans |= R.template step<true>(A, ks_now, vs_now, valid_page(C, id), key0, x.lo, x.hi, key, value);
-                    else
-                        R.template step<false>(A, ks_now, vs_now, true, key0, 0, 0, key, value);
+                if (uniform((int)(rows <= 0 || b * ATTN_KEYS >= x.hi || (b + 1) * ATTN_KEYS <= x.lo))) return 0;
+                return uniform(masked_block(C, x, b, id) ? 2 : 1);
+            };
+            const auto key = [&](int t, int k) { return S.key(place, t, k); };
+            const auto value = [&](int d) { return S.value(place, d); };
+            // blocks that are seen whole have a loop of their own
+            int b = first;
+            for (int mode = top(b);;) {
+                while (mode == 1) {
+                    R.template step<false>(A, ks_now, vs_now, true, key0, 0, 0, key, value);
+                    mode = ++b < last ? top(b) : -1;
                 }
+                if (mode < 0) break;
+                if (mode == 2) nans |= R.template step<true>(A, ks_now, vs_now, valid_page(C, id), key0, x.lo, x.hi, key, value);
+                if (++b == last) break;
+                mode = top(b);
             }
             wait_loads();                                       // a load of nothing writes zeros
             if (__syncthreads_or(nans)) {
