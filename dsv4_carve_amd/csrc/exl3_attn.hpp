@@ -158,10 +158,10 @@ struct AttnRows {
 
     // A block of keys, key0 = its first plus 16 (lane / 16).  key(t, k): 16 bytes of key 16 (lane % 16 / 4) + 4 t + lane % 4
     // from channel 64 k + 16 (lane / 16) on; value(d): 16 tokens, from key0 on, of channel 16 d + lane % 16.  ks, vs: the
-    // scales of the lane's 16 keys.  MASKED: not every row sees it whole; the lane's keys are in a page (`here`) and the rows
+    // scales of the lane's 16 keys.  masked: not every row sees it whole; the lane's keys are in a page (`here`) and the rows
     // see [lo, hi) at most.  Returns whether a value that some rows see is a NaN: it is left out (counted by add_nans).
-    template <bool MASKED, typename K, typename V>
-    __device__ __forceinline__ bool step(const AttnArgs& A, float ks, float vs, bool here, int key0, int lo, int hi, K&& key,
+    template <typename K, typename V>
+    __device__ __forceinline__ bool step(const AttnArgs& A, bool masked, float ks, float vs, bool here, int key0, int lo, int hi, K&& key,
                                          V&& value) {
         float4_t p[4][RB];
 #pragma unroll
@@ -190,8 +190,8 @@ struct AttnRows {
             __builtin_amdgcn_sched_barrier(0);
         }
         float kc = fmaxf(ks * A.qk_scale, 0x1p-126f);
-        uint32_t keep[4];
-        if constexpr (MASKED) {
+        uint32_t keep[4] = {};
+        if (masked) {
             here = here && key0 + 15 >= lo && key0 < hi;
             kc = here ? kc : 1.f;
             vs = here ? vs : 1.f;
@@ -266,7 +266,7 @@ struct AttnRows {
                 for (int i = 0; i < 2; ++i) z[(n + 1) & 1][i] = value(2 * n + 2 + i);
             }
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (MASKED) {
+            if (masked) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -291,7 +291,7 @@ struct AttnRows {
                 }
             __builtin_amdgcn_sched_barrier(0);
         }
-        return MASKED && __builtin_amdgcn_ballot_w64(nan != 0) != 0;
+        return masked && __builtin_amdgcn_ballot_w64(nan != 0) != 0;
     }
 
     // The NaN values of a masked block, counted for the rows that see them in products of their own.
@@ -482,29 +482,26 @@ __device__ __forceinline__ void attend(const AttnArgs& A, const AttnStage<DIM>& 
     const auto key = [&](int t, int k) { return S.key(t, k); };
     const auto value = [&](int d) { return S.value(d); };
     u32x4_t kreg[DT], vreg[DT];
-    int ids = P.of(C, first), next = P.of(C, min(first + step, last - 1));    // two blocks ahead: loads come back in order
+    int ids = P.of(C, first), raw = P.raw(C, min(first + step, last - 1));    // two blocks ahead: loads come back in order
     S.load_k(C, head, first, ids, true, kreg);
     float ks = scale_of(C, C.k_scale, ids, head), vs = scale_of(C, C.v_scale, ids, head);
     S.load_v(C, head, first, ids, true, vreg);
     bool nans = false;
     for (int b = first; b < last; b += step) {
-        const int id = ids;
-        const float ks_now = ks, vs_now = vs;
-        const int after = P.of(C, min(b + 2 * step, last - 1));
         const bool more = b + step < last;
+        const int id = ids;
+        ids = P.of(C, min(b + step, last - 1), moved(raw));
+        raw = P.raw(C, min(b + 2 * step, last - 1));
         S.put_k(kreg);
-        S.load_k(C, head, b + step, next, more, kreg);
-        ks = scale_of(C, C.k_scale, next, head);
-        vs = scale_of(C, C.v_scale, next, head);
+        const float ks_now = moved(ks), vs_now = moved(vs);
+        S.load_k(C, head, b + step, ids, more, kreg);
+        ks = scale_of(C, C.k_scale, ids, head);
+        vs = scale_of(C, C.v_scale, ids, head);
         S.put_v(vreg);
-        S.load_v(C, head, b + step, next, more, vreg);
-        ids = next;
-        next = after;
-        const int key0 = b * ATTN_KEYS + g16;
-        if (masked_block(C, x, b, id))
-            nans |= R.template step<true>(A, ks_now, vs_now, valid_page(C, id), key0, x.lo, x.hi, key, value);
-        else
-            R.template step<false>(A, ks_now, vs_now, true, key0, 0, 0, key, value);
+        S.load_v(C, head, b + step, ids, more, vreg);
+        // one step for both kinds of blocks: with one each, the compiler keeps the sums twice
+        const bool masked = uniform((int)masked_block(C, x, b, id)) != 0;
+        nans |= R.step(A, masked, ks_now, vs_now, !masked || valid_page(C, id), b * ATTN_KEYS + g16, x.lo, x.hi, key, value);
     }
     if (!nans) return;
     for (int b = first; b < last; b += step) {
@@ -894,11 +891,11 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (ShareSize<DIM, RB>::WAVES_EU)) vo
             int b = first;
             for (int mode = top(b);;) {
                 while (mode == 1) {
-                    R.template step<false>(A, ks_now, vs_now, true, key0, 0, 0, key, value);
+                    R.step(A, false, ks_now, vs_now, true, key0, 0, 0, key, value);
                     mode = ++b < last ? top(b) : -1;
                 }
                 if (mode < 0) break;
-                if (mode == 2) nans |= R.template step<true>(A, ks_now, vs_now, valid_page(C, id), key0, x.lo, x.hi, key, value);
+                if (mode == 2) nans |= R.step(A, true, ks_now, vs_now, valid_page(C, id), key0, x.lo, x.hi, key, value);
                 if (++b == last) break;
                 mode = top(b);
             }
@@ -922,13 +919,14 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (ShareSize<DIM, RB>::WAVES_EU)) vo
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 const int row = 16 * rb + r, of = x.r0 + min(row, x.rows - 1), at = of / A.group;
+                const int swap = (row & 7) << 3;                // chunks of 16 bytes XORed with their row, for the banks
                 const float f = finish_row(A, w.head * A.group + of - at * A.group, R.m[rb], R.row_sum(rb), lse[rb]);
 #pragma unroll
                 for (int d = 0; d < DIM / 16; ++d) {
                     float4_t v;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[i] = ldexpf(R.o[d][rb][i], R.back(rb)) * f;
-                    store_row4<BF16>(out + row * DIM + 16 * d + 4 * g, v);
+                    store_row4<BF16>(out + row * DIM + (16 * d + 4 * g ^ swap), v);
                 }
             }
             asm volatile("" ::: "memory");
@@ -936,7 +934,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (ShareSize<DIM, RB>::WAVES_EU)) vo
             for (int i = lane; i < (rows > 0 ? x.rows : 0) * chunks; i += 64) {
                 const int row = i / chunks, d = (i - row * chunks) * 8, of = x.r0 + row, at = of / A.group;
                 const int64_t o = (int64_t)(w.q.first + at) * A.heads + w.head * A.group + of - at * A.group;
-                *reinterpret_cast<u32x4_t*>(A.out + o * C.dim + d) = *reinterpret_cast<const u32x4_t*>(out + row * DIM + d);
+                *reinterpret_cast<u32x4_t*>(A.out + o * C.dim + d) = *reinterpret_cast<const u32x4_t*>(out + row * DIM + (d ^ (row & 7) << 3));
             }
             if (A.lse && rows > 0 && g == 0) {
 #pragma unroll
