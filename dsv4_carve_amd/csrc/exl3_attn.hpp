@@ -36,6 +36,7 @@ struct AttnArgs {
     SharedTile* shared;                       // a workgroup's shared tile
     int tiles;                                // tiles at most
     int least;                                // units that a workgroup has at least
+    int most;                                 // workgroups that the units are divided over at most
     bool clear;                               // rows that no sequence has are zeroed
 };
 
@@ -71,10 +72,14 @@ __device__ __forceinline__ int blocks_of(const Tile& x) {
     return max((x.hi + ATTN_KEYS - 1) / ATTN_KEYS - x.lo / ATTN_KEYS, 1);
 }
 
-__device__ __forceinline__ int64_t units_of(const AttnArgs& A, const Seq& q, int ROWS) {
+// Pieces of `each` blocks that the tiles of a sequence make.
+__device__ __forceinline__ int64_t units_of(const AttnArgs& A, const Seq& q, int ROWS, int64_t each) {
     const int tiles = tiles_of(A, q, ROWS);
     int64_t n = 0;
-    for (int t = 0; t < tiles; ++t) n += blocks_of(get_tile(A, q, t, ROWS));
+    for (int t = 0; t < tiles; ++t) {
+        const int blocks = blocks_of(get_tile(A, q, t, ROWS));
+        n += each == 1 ? blocks : divide(blocks + each - 1, each);
+    }
     return n;
 }
 
@@ -585,11 +590,14 @@ __device__ __forceinline__ void tile_by_xcd(int b, int tiles, int heads, int& ti
 }
 
 // Units are (cache head, tile, block of keys), in this order; a workgroup has an
-// equal share of them, next to each other, whatever sequences they are of.  A tile whose
-// blocks one workgroup has all is finished; of the others each workgroup leaves a
-// partial result: in its first place where the tile began before its share, in its
-// second where it goes on behind it.  Without a place for partial results a workgroup
-// has a tile, the last, longest ones first.
+// equal share of them, next to each other, whatever sequences they are of.  Where the
+// shares are hardly larger then, a share is of one tile: a second one costs a workgroup
+// what about four units a wave do (16 sequences of 5 tokens, window 1024: 24.9 -> 21.1 us;
+// 24 sequences of 1 token: 25.8 -> 20.7).  A tile whose blocks one workgroup has all is
+// finished; of the others each workgroup leaves a partial result: in its first place
+// where the tile began before its share, in its second where it goes on behind it.
+// Without a place for partial results a workgroup has a tile, the last, longest ones
+// first.
 template <int ROWS>
 struct Work {
     int64_t u, u1, share;        // units: the next, the end of the workgroup's, how many a workgroup has
@@ -605,17 +613,43 @@ struct Work {
         me = blockIdx.x;
         t = head = done = 0;
         if (A.part) {
-            const Found f = find_seq(C, [&](const Seq& x) { return units_of(A, x, ROWS); }, [&](int64_t total) {
-                const int64_t all = total * C.kv;
-                share = divide(all + gridDim.x - 1, gridDim.x);
-                if (share < A.least) share = A.least;
-                const int busy = (int)divide(all + share - 1, share);
+            int64_t all = 0, mine = 0, piece = 0;                 // units; tiles of this lane's sequences
+            int pieces = -1;                                      // a share is of one tile; -1: not known yet
+            const Found f = find_seq(C, [&](const Seq& x) {
+                if (pieces < 0) mine += tiles_of(A, x, ROWS);
+                return units_of(A, x, ROWS, pieces > 0 ? share : 1);
+            }, [&](int64_t total) {
+                int64_t busy;
+                if (pieces < 0) {
+                    // (starts that decrease may make more units than the launch was bounded for)
+                    const int64_t wgs = min(A.most, (int)gridDim.x), tiles = (C.seqs == 1 ? mine : read_lane(wave_scan(mine), 63)) * C.kv;
+                    all = total * C.kv;
+                    share = piece = A.least;
+                    pieces = 1;
+                    if (all > (wgs - tiles) * piece) {
+                        share = max(share, divide(all + wgs - 1, wgs));
+                        // no more than wgs pieces have this length, or the rest of a tile
+                        if (wgs > tiles) piece = max(piece, divide(all + wgs - tiles - 1, wgs - tiles));
+                        pieces = wgs > tiles && piece <= share + 4 * A.least;
+                    }
+                    if (pieces) return COUNT_AGAIN;
+                }
+                if (pieces) {
+                    busy = total * C.kv;
+                    if (busy > min(A.most, (int)gridDim.x)) {
+                        share = piece;                            // those of the shares' length are too many
+                        return COUNT_AGAIN;
+                    }
+                } else {
+                    busy = divide(all + share - 1, share);
+                }
                 if (me >= busy) return (int64_t)-1;
-                me = by_xcd(me, busy);
+                me = by_xcd(me, (int)busy);
                 u = share * me;
                 u1 = u + share < all ? u + share : all;
-                head = (int)divide(u, total);
-                return u - head * total;
+                const int64_t at = pieces ? me : u;
+                head = (int)divide(at, total);
+                return at - head * total;
             });
             if (threadIdx.x == 0) A.shared[me].last = -1;        // nothing to join, unless a tile goes on behind the share
             if (f.s < 0) return false;
@@ -625,8 +659,13 @@ struct Work {
             for (;; ++t) {
                 x = get_tile(A, q, t, ROWS);
                 n = blocks_of(x);
-                if (left < n) break;
-                left -= n;
+                const int64_t units = pieces ? divide(n + share - 1, share) : n;
+                if (left < units) break;
+                left -= units;
+            }
+            if (pieces) {
+                left *= share;
+                u1 = u + min(share, n - left);
             }
             done = (int)left;
         } else {

@@ -35,9 +35,10 @@ static AttnPlan plan_attention(int64_t tokens, int64_t heads, int64_t kv_heads, 
     P.tiles = (unsigned)tiles;
     if (tiles * kv_heads < 2 * cus || P.rows < ATTN_MANY) {
         const int64_t each = P.rows < ATTN_MANY ? ATTN_WAVES : 1, units = tiles * kv_heads * std::max<int64_t>(blocks, 1);
-        P.shares = (unsigned)std::max<int64_t>(1, std::min(2 * cus, (units + each - 1) / each));
+        P.shares = (unsigned)std::max<int64_t>(1, std::min(2 * cus, (units + each - 1) / each + tiles * kv_heads));
         P.least = (int)each;
-        P.join_rows = (unsigned)(P.shares > 4 * tiles * kv_heads ? P.rows : P.rows / 4);
+        P.most = (int)(2 * cus);
+        P.join_rows = (unsigned)(P.shares > 5 * tiles * kv_heads ? P.rows : P.rows / 4);
     }
     return P;
 }
@@ -123,7 +124,7 @@ int exl3_fp8_attention(const void* q, int kind, int64_t q_token, int64_t q_head,
                static_cast<const uint16_t*>(q), q_token, q_head, (int)heads, (int)(heads / kv_heads),
                std::fabs(scale) * 1.4426950408889634f, scale < 0.f, (int)window, sinks, static_cast<uint16_t*>(out), lse,
                P.shares ? static_cast<float*>(scratch) : nullptr,
-               reinterpret_cast<SharedTile*>(static_cast<char*>(scratch) + part_bytes(P, dim)), (int)P.tiles, P.least, clear != 0};
+               reinterpret_cast<SharedTile*>(static_cast<char*>(scratch) + part_bytes(P, dim)), (int)P.tiles, P.least, P.most, clear != 0};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const bool bf16 = kind == OUT_BF16;
     if (dim <= 64) return launch_attention_64(A, P, bf16, s);

@@ -11,9 +11,10 @@ constexpr int ATTN_MANY = 128;
 
 struct AttnPlan {
     int rows;                    // of a tile: 16, 32 or ATTN_MANY
-    unsigned shares;             // workgroups that share the work, or 0: a workgroup a tile
+    unsigned shares;             // workgroups of a launch that share the work, or 0: a workgroup a tile
     unsigned tiles;              // tiles at most, for a workgroup a tile
     int least;                   // units that a workgroup has at least
+    int most;                    // workgroups that have units at most: whatever bounds the launch, the sums are divided alike
     unsigned join_rows;          // workgroups that join the rows of a tile
 };
 

@@ -67,14 +67,28 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v) {
     return v;
 }
 
-// a / b, 0 <= a, 0 < b; in 32 bits where both fit.
+// a / b, 0 <= a, 0 < b; in 32 bits where both fit, and else bit by bit: a short call
+// spends much of its time on fetching its instructions, and these are few.
 __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
-    return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+    if (((uint64_t)(a | b) >> 32) == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
+    uint64_t r = 0, x = (uint64_t)a;
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i) {
+        r = r << 1 | x >> 63;
+        x <<= 1;
+        if (r >= (uint64_t)b) {
+            r -= (uint64_t)b;
+            x |= 1;
+        }
+    }
+    return (int64_t)x;
 }
 
 // The sequence that a unit of all sequences' units lies in; count(q) units each.  The
-// unit is at(total), total being all of them; s is -1 where it lies behind them.  Every
-// wave looks by itself: up to 64 sequences are one load and one scan.
+// unit is at(total), total being all of them, or COUNT_AGAIN, where at has changed what a
+// unit is; s is -1 where it lies behind them.  Every wave looks by itself: up to 64
+// sequences are one load and one scan, one sequence is not divided over lanes.
+constexpr int64_t COUNT_AGAIN = -2;
 struct Found {
     int s;
     int64_t unit;                // within the sequence
@@ -95,14 +109,30 @@ __device__ __forceinline__ Found find_seq(const CacheView& C, Count&& count, At&
         f.unit = want - read_lane(before, l);
         f.q = Seq{read_lane(q.first, l), read_lane(q.n, l), read_lane(q.len, l)};
     };
-    if (C.seqs <= 64) {
+    if (C.seqs == 1) {
+        f.q = get_seq(C, 0);
+        for (;;) {
+            const int64_t c = uniform(count(f.q)), want = at(c);
+            if (want == COUNT_AGAIN) continue;
+            if (want >= 0 && want < c) f.s = 0;
+            f.unit = want;
+            break;
+        }
+    } else if (C.seqs <= 64) {
         const Seq q = lane < C.seqs ? get_seq(C, lane) : none;
-        const int64_t c = count(q), sum = wave_scan(c);
-        look(0, q, c, 0, sum, at(read_lane(sum, 63)));
+        for (;;) {
+            const int64_t c = count(q), sum = wave_scan(c), want = at(read_lane(sum, 63));
+            if (want == COUNT_AGAIN) continue;
+            look(0, q, c, 0, sum, want);
+            break;
+        }
     } else {
-        int64_t c = 0;
-        for (int s = lane; s < C.seqs; s += 64) c += count(get_seq(C, s));
-        const int64_t want = at(read_lane(wave_scan(c), 63));
+        int64_t want;
+        do {
+            int64_t c = 0;
+            for (int s = lane; s < C.seqs; s += 64) c += count(get_seq(C, s));
+            want = at(read_lane(wave_scan(c), 63));
+        } while (want == COUNT_AGAIN);
         int64_t before = 0;
         for (int s0 = 0; s0 < C.seqs && want >= before && f.s < 0; s0 += 64) {
             const Seq q = s0 + lane < C.seqs ? get_seq(C, s0 + lane) : none;
