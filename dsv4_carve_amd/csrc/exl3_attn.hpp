@@ -245,21 +245,30 @@ struct AttnRows {
             }
         }
         half8_t big[RB][2], rest[RB][2];
+        float minus = -1.f;
+        asm("" : "+s"(minus));                                  // unknown: a mixed fma reads the 16-bit weight as it is
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             const float k = fmaxf(lv + (ATTN_HEADROOM - c[rb]), -64.f), add = k - m[rb];
-            float sum = 0.f;
+            float sum[4];                                       // four chains of additions
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(p[t][rb][i], kc, add));
-                    sum += w;
-                    const _Float16 h = (_Float16)w;
-                    big[rb][t >> 1][4 * (t & 1) + i] = h;
-                    if constexpr (FINE) rest[rb][t >> 1][4 * (t & 1) + i] = (_Float16)(w - (float)h);
+                for (int i = 0; i < 4; i += 2) {
+                    const float w0 = __builtin_amdgcn_exp2f(fmaf(p[t][rb][i], kc, add));
+                    const float w1 = __builtin_amdgcn_exp2f(fmaf(p[t][rb][i + 1], kc, add));
+                    sum[i] = t ? sum[i] + w0 : w0;
+                    sum[i + 1] = t ? sum[i + 1] + w1 : w1;
+                    const int at = 4 * (t & 1) + i;
+                    big[rb][t >> 1][at] = (_Float16)w0;
+                    big[rb][t >> 1][at + 1] = (_Float16)w1;
+                    if constexpr (FINE) {
+                        rest[rb][t >> 1][at] = (_Float16)fmaf((float)big[rb][t >> 1][at], minus, w0);
+                        rest[rb][t >> 1][at + 1] = (_Float16)fmaf((float)big[rb][t >> 1][at + 1], minus, w1);
+                    }
                 }
-            l[rb] = fmaf(sum, __builtin_amdgcn_exp2f(-k), l[rb]);
+            l[rb] = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), __builtin_amdgcn_exp2f(-k), l[rb]);
+            asm volatile("" : "+v"(l[rb]));                     // now: the weights would be kept until behind the products
             __builtin_amdgcn_sched_barrier(0);
         }
         uint32_t nan = 0;
@@ -806,22 +815,25 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
 //   values  [pieces][DIM][16 << lg bytes]: the tokens of a page, 64 at most
 template <int DIM>
 struct AttnShare {
-    static constexpr int SUB = DIM % 128 == 0 ? 128 : 64, CS = SUB / 16, KEYS = 64 / CS;
+    static constexpr int SUB = DIM % 128 == 0 ? 128 : 64, CS = SUB / 16, SUBS = DIM / SUB, KEYS = 64 / CS;
     static constexpr int LOADS = DIM / 16 / ATTN_WAVES;       // of a wave, for the keys or the values
     static constexpr int K_BYTES = ATTN_KEYS * DIM, BYTES = 2 * K_BYTES;
 
     char* lds;
     int k_read[2], v_read;
-    uint32_t k_off, k_row, v_off;
+    uint32_t k_off[SUBS], v_off;
     int lg, wave;
 
     __device__ __forceinline__ AttnShare(const CacheView& C, char* lds_, int wave_) : lds(lds_), wave(wave_) {
         const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
         const int key = lane / CS, place = lane % CS;
         const int sw = SUB == 128 ? key & 3 : (key >> 1) & 1;
-        // within the row; keys 16 .. 31 and 48 .. 63 have another bit, and a wave's loads are all of such keys or all of others
-        k_off = ((place ^ sw) << 4) ^ ((wave * KEYS >> 4 & 1) ? SUB / 2 : 0);
-        k_row = key * C.dim;
+#pragma unroll
+        for (int i = 0; i < SUBS; ++i) {
+            // keys 16 .. 31 and 48 .. 63 have another bit
+            const int c = i * SUB + ((((place ^ sw) << 4)) ^ ((wave & 1) ? SUB / 2 : 0));
+            k_off[i] = c < C.dim ? key * C.dim + c : OUTSIDE;  // behind the row's end: zeros
+        }
         const int sr = SUB == 128 ? (r & 3) | (r >> 2 & 1) << 2 : (r >> 1 & 1) | (r >> 2 & 1) << 1;
         const int row = (16 * (r >> 2) + (r & 3)) * SUB;
         k_read[0] = row + ((g ^ sr) << 4);
@@ -830,32 +842,31 @@ struct AttnShare {
         // a row of `1 << lg` chunks; eight lanes meet every bank once
         const int channel = lane >> lg, mask = (1 << lg) - 1;
         const auto swap = [&](int c) { return lg == 2 ? c >> 1 & 3 : lg == 1 ? c >> 2 & 1 : 0; };
-        v_off = (channel << C.page_shift) + (((lane & mask) ^ swap(channel)) << 4);
+        v_off = ((channel + (wave & mask) * (DIM >> lg)) << C.page_shift) + (((lane & mask) ^ swap(channel)) << 4);
         v_read = K_BYTES + ((((g >> lg) * DIM + r) << lg) + ((g & mask) ^ swap(r))) * 16;
     }
 
-    __device__ __forceinline__ static void to_lds(__amdgpu_buffer_rsrc_t p, char* to, uint32_t at) { load_to_lds(p, to, at, 0); }
-
-    // This wave's loads of block b.
+    // This wave's loads of block b: keys 16 wave .. 16 wave + 15, and its part of the piece of values that they are in. One
+    // page has them all.
     __device__ __forceinline__ void load(const CacheView& C, int head, int b, int ids, bool on, int place) const {
-        const int mask = (1 << C.page_shift) - 1;
-        char* to = lds + place * BYTES;
+        const int mask = (1 << C.page_shift) - 1, at = b * ATTN_KEYS;
+        const int id = __builtin_amdgcn_readlane(ids, 16 * wave);
+        const bool is = on && valid_page(C, id);
+        const uint32_t bytes = (uint32_t)C.dim << C.page_shift;
+        const uint64_t page = (uint64_t)(uint32_t)(is ? id : 0) * ((uint32_t)C.kv * bytes) + head * bytes;
+        const uint32_t k_at = ((at + 16 * wave) & mask) * C.dim, v_at = (at + (wave >> lg << lg) * 16) & mask;
+        const __amdgpu_buffer_rsrc_t k = __builtin_amdgcn_make_buffer_rsrc(C.k + page + k_at, 0, is ? bytes - k_at : 0, 0x27000);
+        const __amdgpu_buffer_rsrc_t v = __builtin_amdgcn_make_buffer_rsrc(C.v + page + v_at, 0, is ? bytes - v_at : 0, 0x27000);
+        char* to = lds + place * BYTES + wave * (16 * SUB);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int j = i * ATTN_WAVES + wave;              // LDS chunks 64 j ..: 64 / KEYS loads a piece of SUB channels
-            const int sub = i * ATTN_WAVES / (ATTN_KEYS / KEYS), key = (j - sub * (ATTN_KEYS / KEYS)) * KEYS;
-            const __amdgpu_buffer_rsrc_t p = page_part(C, C.k, head, ids, key >> 4, ((b * ATTN_KEYS + key) & mask) * C.dim, on);
-            const uint32_t c = sub * SUB + k_off;
-            to_lds(p, to + j * 1024, c < (uint32_t)C.dim ? k_row + c : OUTSIDE);             // behind the row's end: zeros
+            const int sub = i * KEYS / 16, key = i * KEYS % 16;
+            load_to_lds(k, to + (sub * ATTN_KEYS + key) * SUB, k_off[sub], key * C.dim);
         }
+        to = lds + place * BYTES + K_BYTES + wave * (LOADS * 1024);
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int j = i * ATTN_WAVES + wave;              // LDS chunks 64 j ..: (DIM << lg) / 64 loads a piece
-            const int each = (DIM << lg) / 64, piece = lg == 2 ? 0 : j / each, channel = (j - piece * each) << (6 - lg);
-            const int g = piece << lg;
-            const __amdgpu_buffer_rsrc_t p = page_part(C, C.v, head, ids, g, (b * ATTN_KEYS + 16 * g) & mask, on);
-            to_lds(p, to + K_BYTES + j * 1024, v_off + (channel << C.page_shift));           // behind the last channel: zeros
-        }
+        for (int i = 0; i < LOADS; ++i)                       // behind the last channel: zeros
+            load_to_lds(v, to + i * 1024, v_off + (i << (6 - lg + C.page_shift)), 0);
     }
 
     __device__ __forceinline__ u32x4_t key(int place, int t, int k) const {
