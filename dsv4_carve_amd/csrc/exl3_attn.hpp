@@ -224,6 +224,9 @@ struct AttnRows {
         const auto read_key = [&](int n, int i) { return PARTS ? key(n % 4, n / 4 * 2 + i) : key(2 * n % 4 + i, n / 2); };
 #pragma unroll
         for (int i = 0; i < 2; ++i) z[0][i] = read_key(0, i);
+        // Products first: the other waves' other work goes on beside them (a chunk of 512 tokens, 16384 keys: 174.8 -> 167 us;
+        // the other way round 170).
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int n = 0; n < 2 * KC; ++n) {
 #pragma unroll
@@ -250,6 +253,7 @@ struct AttnRows {
                 }
             __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
         float kc[RB];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) kc[rb] = __builtin_amdgcn_fmed3f(ks * A.qk_scale * unit[rb], 0x1p-126f, 0x1.fffffep127f);
@@ -330,6 +334,7 @@ struct AttnRows {
             __builtin_amdgcn_sched_barrier(0);
         }
         uint32_t nan = 0;
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int n = 0; n < DT / 2; ++n) {
             u32x4_t (&v)[2] = z[n & 1];
@@ -363,6 +368,7 @@ struct AttnRows {
                 }
             __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
         return masked && __builtin_amdgcn_ballot_w64(nan != 0) != 0;
     }
 
