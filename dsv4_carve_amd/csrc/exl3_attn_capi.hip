@@ -57,6 +57,21 @@ static int64_t keys_of(int64_t width, int64_t page_size, int64_t tokens, int64_t
     return window ? std::min(width * page_size, window + tokens + 2 * ATTN_KEYS) : width * page_size;
 }
 
+template <int K>
+static int launch_append(const AppendArgs& A, dim3 grid, hipStream_t s) {
+    static std::atomic<uint64_t> ready{0};           // devices that know of the LDS size
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= MAX_DEVICES) return fail("no HIP device");
+    if (!(ready.load() >> dev & 1)) {
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(fp8_cache_append_kernel<K>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, append_lds(256, 256)) != hipSuccess)
+            return fail("the device does not give the kernel its LDS");
+        ready.fetch_or(1ull << dev);
+    }
+    hipLaunchKernelGGL(fp8_cache_append_kernel<K>, grid, dim3(APPEND_WAVES * 64), append_lds(1 << A.c.page_shift, A.c.dim), s, A);
+    return check_launch();
+}
+
 extern "C" {
 
 int exl3_fp8_cache_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
@@ -78,12 +93,11 @@ int exl3_fp8_cache_append(const void* k, int64_t k_token, int64_t k_head, const 
                        k, v, k_token, k_head, v_token, v_head};
     // pages that may be touched: each sequence's first and last one, and those that its tokens fill
     const int64_t bound = starts ? std::min(tokens, tokens / page_size + 2 * seqs) : tokens;
-    const auto kernel = kind == OUT_F16    ? fp8_cache_append_kernel<OUT_F16>
-                        : kind == OUT_BF16 ? fp8_cache_append_kernel<OUT_BF16>
-                                           : fp8_cache_append_kernel<OUT_F32>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)bound, (unsigned)kv_heads, 2), dim3(APPEND_WAVES * 64), 0,
-                       reinterpret_cast<hipStream_t>(stream), A);
-    return check_launch();
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const dim3 grid((unsigned)bound, (unsigned)kv_heads, 2);
+    if (kind == OUT_F16) return launch_append<OUT_F16>(A, grid, s);
+    if (kind == OUT_BF16) return launch_append<OUT_BF16>(A, grid, s);
+    return launch_append<OUT_F32>(A, grid, s);
 }
 
 int64_t exl3_fp8_attention_scratch_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs,

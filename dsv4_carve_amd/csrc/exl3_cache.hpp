@@ -161,27 +161,27 @@ __device__ __forceinline__ int touched_pages(const CacheView& C, const Seq& q) {
     return q.len > from ? ((q.len - 1) >> C.page_shift) - (from >> C.page_shift) + 1 : 0;
 }
 
-// Eight neighbouring values (16-byte aligned) as fp32; an infinity as a NaN.
+// Eight neighbouring values (16-byte aligned), as they are in memory.
 template <int K>
-__device__ __forceinline__ void load8_finite(const void* p, int64_t at, float (&v)[8]) {
-    if constexpr (K == OUT_F32) {
+struct Eight {
+    u32x4_t u[K == OUT_F32 ? 2 : 1];
+
+    __device__ __forceinline__ void load(const void* p, int64_t at) {
+        const u32x4_t* from = reinterpret_cast<const u32x4_t*>(static_cast<const char*>(p) + at * (K == OUT_F32 ? 4 : 2));
+        u[0] = from[0];
+        if constexpr (K == OUT_F32) u[1] = from[1];
+    }
+    // as fp32, an infinity as a NaN
+    __device__ __forceinline__ void finite(float (&v)[8]) const {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float4_t f = reinterpret_cast<const float4_t*>(static_cast<const float*>(p) + at)[i];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * i + j] = f[j];
-        }
-    } else {
-        const u32x4_t u = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + at);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[2 * j] = K == OUT_BF16 ? __uint_as_float(u[j] << 16) : f16_bits_to_f32((uint16_t)u[j]);
-            v[2 * j + 1] = K == OUT_BF16 ? __uint_as_float(u[j] & 0xffff0000u) : f16_bits_to_f32((uint16_t)(u[j] >> 16));
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (K == OUT_F32) v[j] = __uint_as_float(u[j / 4][j % 4]);
+            else if constexpr (K == OUT_BF16) v[j] = __uint_as_float(j & 1 ? u[0][j / 2] & 0xffff0000u : u[0][j / 2] << 16);
+            else v[j] = f16_bits_to_f32((uint16_t)(u[0][j / 2] >> (16 * (j & 1))));
+            v[j] = fabsf(v[j]) == __builtin_inff() ? __builtin_nanf("") : v[j];
         }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fabsf(v[j]) == __builtin_inff() ? __builtin_nanf("") : v[j];
-}
+};
 
 // Four codes times a power of two, rounded to e4m3 again.
 __device__ __forceinline__ uint32_t rescale4(uint32_t u, float by) {
@@ -189,11 +189,29 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t u, float by) {
                      __builtin_amdgcn_cvt_f32_fp8((int)u, 2) * by, __builtin_amdgcn_cvt_f32_fp8((int)u, 3) * by);
 }
 
+// Byte c of each of four words, as one word each.
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    w[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    w[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    w[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+    w[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+
 // A workgroup has one page of one head, of the keys or of the values: the new
 // tokens' largest magnitude, the scale, the old codes where it grew, the new ones.
-// The inputs are read twice (the second time from cache).
+// The inputs stay in registers in between, the first APPEND_HOLD * 256 chunks of eight
+// (64 tokens of 256, 128 of 128); what a page has more is read twice.  A value's codes
+// are turned in LDS: tokens of a channel are neighbours in the cache.
+constexpr int APPEND_HOLD = 8;
+
+inline int append_lds(int page, int dim) { return page * (dim + 4); }
+
 template <int K>
 __global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(AppendArgs A) {
+    constexpr int THREADS = APPEND_WAVES * 64;
+    extern __shared__ __attribute__((aligned(16))) char append_codes[];           // values: [page][dim + 4]
     __shared__ float most_of[APPEND_WAVES];
     const CacheView& C = A.c;
     const int tid = threadIdx.x, head = blockIdx.y;
@@ -224,68 +242,128 @@ __global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(App
     uint8_t* code = (values ? C.v : C.k) + (block << C.page_shift) * C.dim;
     float* scale = (values ? C.v_scale : C.k_scale) + block;
 
-    const int per = C.dim >> 3;                                                   // chunks of eight a token
+    const int per = C.dim >> 3, chunks = (hi - lo) * per;                         // chunks of eight, of a token and new
+    const float each = __builtin_amdgcn_rcpf((float)per);                         // i / per: i is below 2^13, per 32 at most
+    const auto where = [&](int i, int& t, int& d) {
+        t = (int)(((float)i + 0.5f) * each);
+        d = (i - t * per) * 8;
+        t += lo;
+        return in0 + t * stride + d;
+    };
+    Eight<K> held[APPEND_HOLD];
+    int t, d;
+#pragma unroll
+    for (int c = 0; c < APPEND_HOLD; ++c) {
+        if (c * THREADS >= chunks) break;
+        if (tid + c * THREADS < chunks) held[c].load(in, where(tid + c * THREADS, t, d));
+    }
+    const float before = lo ? *scale : 0.f;
+    // values: 16 tokens of four channels are a thread's; what is outside [lo, hi) goes back as it was, or rescaled below lo
+    const int lg = C.page_shift - 4, last = (hi + 15) >> 4, fours = values ? C.dim / 4 << lg : 0;
+    const auto row = [&](int i, int e) {
+        return reinterpret_cast<u32x4_t*>(code + ((int64_t)((i >> lg << 2) + e) << C.page_shift) + (i & ((1 << lg) - 1)) * 16);
+    };
+    const auto outside = [&](int i) {
+        const int t0 = (i & ((1 << lg) - 1)) * 16;
+        return t0 < hi && (t0 < lo || t0 + 16 > hi);
+    };
+    u32x4_t old[4];
+    if (tid < fours && outside(tid)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) old[e] = *row(tid, e);
+    }
     float most = 0.f;
     float x[8];
-    for (int i = tid; i < (hi - lo) * per; i += APPEND_WAVES * 64) {
-        const int t = i / per;
-        load8_finite<K>(in, in0 + (lo + t) * stride + (i - t * per) * 8, x);
+    const auto largest = [&](const Eight<K>& v) {
+        v.finite(x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+    };
+#pragma unroll
+    for (int c = 0; c < APPEND_HOLD; ++c) {
+        if (c * THREADS >= chunks) break;
+        if (tid + c * THREADS < chunks) largest(held[c]);
+    }
+    for (int i = tid + APPEND_HOLD * THREADS; i < chunks; i += THREADS) {
+        Eight<K> v;
+        v.load(in, where(i, t, d));
+        largest(v);
     }
     most = wave_max(most, 0.f);
     if ((tid & 63) == 0) most_of[tid >> 6] = most;
-    const float before = lo ? *scale : 0.f;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < APPEND_WAVES; ++w) most = fmaxf(most, most_of[w]);
     const float now = fmaxf(QuantGroup(most, true).scale, before);
     const float inverse = 1.0f / now, by = before / now;
     const bool grew = lo && by != 1.0f;
+    const auto put = [&](int i, const Eight<K>& v) {
+        where(i, t, d);
+        v.finite(x);
+        const uint32_t a = pack_e4m3(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse);
+        const uint32_t b = pack_e4m3(x[4] * inverse, x[5] * inverse, x[6] * inverse, x[7] * inverse);
+        if (values) {
+            uint32_t* to = reinterpret_cast<uint32_t*>(append_codes + t * (C.dim + 4) + d);
+            to[0] = a;
+            to[1] = b;
+        } else {
+            *reinterpret_cast<u32x2_t*>(code + t * C.dim + d) = u32x2_t{a, b};
+        }
+    };
+#pragma unroll
+    for (int c = 0; c < APPEND_HOLD; ++c) {
+        if (c * THREADS >= chunks) break;
+        if (tid + c * THREADS < chunks) put(tid + c * THREADS, held[c]);
+    }
+    for (int i = tid + APPEND_HOLD * THREADS; i < chunks; i += THREADS) {
+        Eight<K> v;
+        where(i, t, d);
+        v.load(in, in0 + t * stride + d);
+        put(i, v);
+    }
     if (!values) {
         if (grew)
-            for (int i = tid; i < lo * C.dim / 16; i += APPEND_WAVES * 64) {
+            for (int i = tid; i < lo * C.dim / 16; i += THREADS) {
                 u32x4_t u = reinterpret_cast<u32x4_t*>(code)[i];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) u[j] = rescale4(u[j], by);
                 reinterpret_cast<u32x4_t*>(code)[i] = u;
             }
-        for (int i = tid; i < (hi - lo) * per; i += APPEND_WAVES * 64) {
-            const int t = i / per, d = (i - t * per) * 8;
-            load8_finite<K>(in, in0 + (lo + t) * stride + d, x);
-            *reinterpret_cast<u32x2_t*>(code + (lo + t) * C.dim + d) =
-                u32x2_t{pack_e4m3(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse),
-                        pack_e4m3(x[4] * inverse, x[5] * inverse, x[6] * inverse, x[7] * inverse)};
-        }
     } else {
-        // 16 tokens of one value's channel at once; what is outside [lo, hi) goes back as it was, or rescaled below lo
-        const int first = grew ? 0 : lo >> 4, groups = ((hi + 15) >> 4) - first;
-        for (int i = tid; i < groups * C.dim; i += APPEND_WAVES * 64) {
-            const int b = i / C.dim, d = i - b * C.dim, t0 = (first + b) * 16;
-            u32x4_t* p = reinterpret_cast<u32x4_t*>(code + ((int64_t)d << C.page_shift) + t0);
-            u32x4_t u = {0, 0, 0, 0};
-            if (t0 < lo || t0 + 16 > hi) u = *p;
+        __syncthreads();
+        const int first = grew ? 0 : lo >> 4;
+        for (int i = tid; i < fours; i += THREADS) {
+            const int group = i & ((1 << lg) - 1), d = i >> lg << 2, t0 = group * 16;
+            if (group < first || group >= last) continue;
+            u32x4_t made[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t moved = grew ? rescale4(u[j], by) : u[j];
-                float y[4];
+                uint32_t w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int t = t0 + 4 * j + e;
-                    const float f = t >= lo && t < hi ? load_kind<K>(in, in0 + t * stride + d) : 0.f;
-                    y[e] = (fabsf(f) == __builtin_inff() ? __builtin_nanf("") : f) * inverse;
-                }
-                const uint32_t made = pack_e4m3(y[0], y[1], y[2], y[3]);
-                uint32_t r = 0;
+                for (int e = 0; e < 4; ++e)
+                    w[e] = *reinterpret_cast<const uint32_t*>(append_codes + (t0 + 4 * j + e) * (C.dim + 4) + d);
+                transpose4(w);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int t = t0 + 4 * j + e;
-                    const uint32_t m = 0xffu << (8 * e);
-                    r |= m & (t < lo ? moved : t < hi ? made : u[j]);
-                }
-                u[j] = r;
+                for (int e = 0; e < 4; ++e) made[e][j] = w[e];
             }
-            *p = u;
+            if (outside(i)) {
+                if (i != tid) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) old[e] = *row(i, e);
+                }
+                const auto bytes_before = [&](int t) { return (uint32_t)((1ull << (8 * min(max(t, 0), 4))) - 1); };
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t below = bytes_before(lo - t0 - 4 * j), fresh = bytes_before(hi - t0 - 4 * j) & ~below;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t u = old[e][j], moved = grew ? rescale4(u, by) : u;
+                        made[e][j] = (made[e][j] & fresh) | (moved & below) | (u & ~(fresh | below));
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *row(i, e) = made[e];
         }
     }
     if (tid == 0) *scale = now;
