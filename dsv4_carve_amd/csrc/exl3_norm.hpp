@@ -7,7 +7,9 @@
 // y / a is (h w) / max|h w|: r cancels, and quotients of few-bit values that lie on
 // a rounding border of e4m3 stay on it.  Everything between the inputs and the
 // roundings is 64-bit: a quotient in fp32 rounds about one value in 2^18 to the
-// other side of a border, and the arithmetic hides behind memory.
+// other side of a border.  Most values are nowhere near one, though: an fp32 quotient
+// whose both neighbours at its error's distance have the same code has that code, and
+// only a wave that holds another value divides in 64 bits (SURE).
 #pragma once
 
 #include "exl3_fp8.hpp"
@@ -45,16 +47,17 @@ __device__ __forceinline__ float to_odd(double v) {
 
 // What a group's largest |h w| makes of its values g = h w.
 struct NormGroup {
-    double mul, b, rb;
+    double mul, b;
     float scale;
+    bool small;
 
-    // most: the group's largest |g| (NaN left out); r: the row's factor; sum: the row's sum of squares
+    // most: the group's largest |g| (NaN left out); r: the row's factor
     __device__ __forceinline__ NormGroup(double most, double r, bool finite, bool pow2) {
         constexpr double LEAST = 448.0 * 0x1p-126;
         const double top = most * r;
-        const bool small = !(top > LEAST) || !finite;
+        small = !(top > LEAST) || !finite;
         const double a = small ? LEAST : top;
-        b = rb = 1.0;
+        b = 1.0;
         if (pow2) {
             const uint64_t bits = __builtin_bit_cast(uint64_t, a);
             const int e = (int)(bits >> 52) - 1023 - 8 + ((bits & 0xfffffffffffffull) > 0xc000000000000ull ? 1 : 0);
@@ -64,18 +67,34 @@ struct NormGroup {
             scale = (float)(a / 448.0);
             mul = small ? r * 0x1p126 : 448.0;
             b = small ? 1.0 : most;
-            rb = 1.0 / b;
         }
         if (!finite) mul = r;                                      // 0 for finite values, NaN for the others
     }
+};
 
-    // a group's scale and its values' quotients, correctly rounded (one correction of the remainder)
+// A group's values over its scale, correctly rounded (one correction of the remainder).
+struct NormDivide {
+    double mul, b, rb;
+
+    __device__ __forceinline__ explicit NormDivide(const NormGroup& g) : mul(g.mul), b(g.b), rb(1.0 / g.b) {}
     __device__ __forceinline__ double operator()(double g) const {
         const double n = g * mul;
         const double q = n * rb;
         return fma(fma(-q, b, n), rb, q);
     }
 };
+
+// Bound of an fp32 quotient's relative error, in halves of a last bit: 1 of g, 1 of the largest, 2 of its reciprocal, 1
+// of that times 448, 1 of the product and 1 of the neighbour make 7 of these 8.
+constexpr float SURE = 0x1p-21f;
+
+// 1 / sqrt(x), to the last bit or two: two steps of Newton's from the hardware's estimate.
+__device__ __forceinline__ double inverse_root(double x) {
+    const double y = __builtin_amdgcn_rsq(x), half = 0.5 * x;
+    double z = fma(y, fma(-half * y, y, 0.5), y);
+    z = fma(z, fma(-half * z, z, 0.5), z);
+    return x > 0.0 && x < __builtin_inf() ? z : y;
+}
 
 template <int N>
 __device__ __forceinline__ void store_kind(void* p, int kind, int64_t at, const double (&v)[N]) {
@@ -89,11 +108,11 @@ __device__ __forceinline__ void store_kind(void* p, int kind, int64_t at, const 
 
 // Sixteen neighbouring values, 16-byte aligned.
 template <int KIND>
-__device__ __forceinline__ void store16(void* p, int64_t at, const double (&v)[16]) {
+__device__ __forceinline__ void store16(void* p, int64_t at, const float (&v)[16]) {
     if constexpr (KIND == OUT_F32) {
         float4_t* o = reinterpret_cast<float4_t*>(static_cast<float*>(p) + at);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = float4_t{(float)v[4 * i], (float)v[4 * i + 1], (float)v[4 * i + 2], (float)v[4 * i + 3]};
+        for (int i = 0; i < 4; ++i) o[i] = float4_t{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
     } else {
         u32x4_t* o = reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p) + at);
 #pragma unroll
@@ -101,7 +120,7 @@ __device__ __forceinline__ void store16(void* p, int64_t at, const double (&v)[1
             u32x4_t u;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float a = (float)v[8 * i + 2 * j], b = (float)v[8 * i + 2 * j + 1];
+                const float a = v[8 * i + 2 * j], b = v[8 * i + 2 * j + 1];
                 u[j] = KIND == OUT_BF16 ? pack_bf16(a, b) : f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16;
             }
             o[i] = u;
@@ -163,44 +182,67 @@ __global__ __launch_bounds__(256) void fp8_norm_kernel(NormArgs A) {
 #pragma unroll
         for (int i = 1; i < WAVES; ++i) sum += part[first + i];
     }
-    const double r = 1.0 / sqrt(fma(sum, A.inverse_k, A.eps));
+    const double r = inverse_root(fma(sum, A.inverse_k, A.eps));
     const bool finite = sum < __builtin_inf() && r < __builtin_inf();
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
         const int i = (c * WAVES * 64 + t) * 16;
         const bool in = i < k;
-        double g[16];
         double most = 0.0;
-        float w[16];
+        float w[16] = {}, g[16] = {};                                   // g: h w in 32 bits
         if (in) {
             load16_any(A.weight, A.weight_kind, i, w);
             if constexpr (R != NO_RESIDUAL) {
-                double h[16];
+                float h[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) h[j] = value(c, j);
+                for (int j = 0; j < 16; ++j) h[j] = h0[c][j] + h1[c][j];
                 store16<R>(A.sum, at + i, h);
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                g[j] = value(c, j) * (double)w[j];
-                most = fmax(most, fabs(g[j]));
+                const double v = value(c, j) * (double)w[j];
+                most = fmax(most, fabs(v));
+                g[j] = (float)v;
             }
         }
         most = fmax(most, __shfl_xor(most, 1));
         most = fmax(most, __shfl_xor(most, 2));
         most = fmax(most, __shfl_xor(most, 4));
-        if (!in) continue;
         const NormGroup group(most, r, finite, A.pow2);
-        if ((lane & 7) == 0) A.scale[row * A.groups + (i >> 7)] = group.scale;
-        u32x4_t out;
+        u32x4_t out = {0, 0, 0, 0}, differ = {0, 0, 0, 0};
+        if (in) {
+            if ((lane & 7) == 0) A.scale[row * A.groups + (i >> 7)] = group.scale;
+            const bool plain = finite && !group.small && most > 0x1p-100 && most < 0x1p100;
+            const float by = A.pow2 ? (float)group.mul : 448.f * __builtin_amdgcn_rcpf((float)most);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            out[j] = pack_e4m3(to_odd(group(g[4 * j])), to_odd(group(g[4 * j + 1])), to_odd(group(g[4 * j + 2])),
-                               to_odd(group(g[4 * j + 3])));
+            for (int j = 0; j < 4; ++j) {
+                float lo[4], hi[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float q = g[4 * j + e] * by;
+                    lo[e] = q * (1.f - SURE);
+                    hi[e] = q * (1.f + SURE);
+                }
+                out[j] = pack_e4m3(lo[0], lo[1], lo[2], lo[3]);
+                differ[j] = plain ? out[j] ^ pack_e4m3(hi[0], hi[1], hi[2], hi[3]) : ~0u;
+            }
+        }
+        if (__builtin_amdgcn_ballot_w64((differ[0] | differ[1] | differ[2] | differ[3]) != 0)) {
+            const NormDivide divide(group);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (!__builtin_amdgcn_ballot_w64(differ[j] != 0)) continue;
+                float q[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[e] = to_odd(divide(value(c, 4 * j + e) * (double)w[4 * j + e]));
+                out[j] = pack_e4m3(q[0], q[1], q[2], q[3]);
+            }
+        }
+        if (!in) continue;
         *reinterpret_cast<u32x4_t*>(A.q + at + i) = out;
         if (A.normed) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) g[j] *= r;
+            for (int j = 0; j < 16; ++j) g[j] = (float)(value(c, j) * (double)w[j] * r);
             with_kind(A.normed_kind, [&](auto kind) { store16<decltype(kind)::value>(A.normed, at + i, g); });
         }
     }
@@ -227,7 +269,7 @@ __global__ __launch_bounds__(256) void fp8_norm_any_kernel(NormArgs A) {
     if (lane == 0) part[wave] = sum;
     __syncthreads();
     sum = part[0] + part[1] + part[2] + part[3];
-    const double r = 1.0 / sqrt(fma(sum, A.inverse_k, A.eps));
+    const double r = inverse_root(fma(sum, A.inverse_k, A.eps));
     const bool finite = sum < __builtin_inf() && r < __builtin_inf();
     for (int b = wave; b < A.groups; b += 4) {
         double g[2] = {0.0, 0.0};
@@ -249,7 +291,8 @@ __global__ __launch_bounds__(256) void fp8_norm_any_kernel(NormArgs A) {
         most = wave_max(most, 0.0);
         const NormGroup group(most, r, finite, A.pow2);
         if (lane == 0) A.scale[row * A.groups + b] = group.scale;
-        const uint32_t u = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(to_odd(group(g[0])), to_odd(group(g[1])), 0, false);
+        const NormDivide divide(group);
+        const uint32_t u = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(to_odd(divide(g[0])), to_odd(divide(g[1])), 0, false);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int i = b * FP8_BLOCK + j * 64 + lane;
