@@ -709,7 +709,7 @@ struct Work {
                 }
                 if (pieces) {
                     busy = total * C.kv;
-                    if (busy > min(A.most, (int)gridDim.x)) {
+                    if (busy > min(A.most, (int)gridDim.x) && share != piece) {
                         share = piece;                            // those of the shares' length are too many
                         return COUNT_AGAIN;
                     }
@@ -769,7 +769,10 @@ struct Work {
 
     // Where a partial result goes, of `size` floats each; tells the join of a tile that begins here.
     __device__ __forceinline__ float* part(const AttnArgs& A, int size) const {
-        if (done == 0 && threadIdx.x == 0) A.shared[me] = SharedTile{q.first, x.r0, x.rows, head, (int)divide(u + n - 1, share)};
+        if (done == 0 && threadIdx.x == 0) {
+            const int last = min((int)divide(u + n - 1, share), (int)gridDim.x - 1);
+            A.shared[me] = SharedTile{q.first, x.r0, x.rows, head, last};
+        }
         return A.part + ((int64_t)me * 2 + (done == 0 ? 1 : 0)) * size;
     }
 
@@ -946,7 +949,6 @@ template <int DIM, int RB>
 struct ShareSize {
     static constexpr int ROWS = ATTN_WAVES * 16 * RB;
     static constexpr int LDS = 2 * AttnShare<DIM>::BYTES;
-    static constexpr int WAVES_EU = DIM <= 128 ? 2 : 1;
     static constexpr int PART = ROWS * (DIM + 2);
     static_assert(LDS >= ROWS * DIM * 2, "a tile's results go through the blocks' places");
 };
@@ -954,7 +956,7 @@ struct ShareSize {
 // Many rows a sequence: each wave has rows of its own, all go through a tile's blocks
 // together, with one barrier a block; the next block is on its way meanwhile.
 template <int DIM, bool BF16, int RB>
-__global__ __launch_bounds__(ATTN_WAVES * 64, (ShareSize<DIM, RB>::WAVES_EU)) void fp8_attention_rows_kernel(AttnArgs A) {
+__global__ __launch_bounds__(ATTN_WAVES * 64, 2) void fp8_attention_rows_kernel(AttnArgs A) {
     typedef ShareSize<DIM, RB> Z;
     constexpr int OWN = 16 * RB;
     extern __shared__ __attribute__((aligned(16))) char share_lds[];

@@ -26,15 +26,33 @@ static int check_cache(const void* k, const void* k_scale, const void* v, const 
 
 static int log2_of(int64_t v) { return 63 - __builtin_clzll((unsigned long long)v); }
 
-// Work is shared out where there are fewer than two tiles a CU.
+// Rows of a tile, and the kernel with it, by the rows that a sequence and cache head have on average.  16 and 32: the
+// waves divide a tile's keys; 64 and 128: they have rows of their own and share the keys in LDS.  In us, 32 query heads
+// over 8 cache heads, 64 ragged sequences of up to 8192 keys with up to 8, 16 and 32 tokens (18, 34 and 66 rows):
+//            16 rows         32 rows         64 rows         128 rows
+//   dim 64   88, 144, 255    76, 106, 170    100, 105, 231   112, 139, 153
+//   dim 128  168, 286, 498   199, 290, 479   143, 151, 280   160, 176, 203
+// and of 4 such sequences 25, 30, 46 / 37, 41, 50 / 31, 33, 38 / 42, 46, 49 (dim 128); 16 query heads over 4 of 256
+// channels, the 64 sequences: 170, 257, 443 / 265, 388, 606 / 152, 157, 218 (128 rows have no room in the registers).
+static int tile_rows(int64_t rows, int64_t dim, int64_t pairs, int64_t cus) {
+    if (rows <= 16) return 16;
+    if (dim <= 64) return rows <= 64 ? 32 : 128;
+    if (dim <= 128 && rows <= 32 && pairs < cus / 2) return 16;
+    return dim > 128 || rows <= 64 ? 64 : 128;
+}
+
+// Work is shared out over the workgroups that run at once, two a CU, where the waves divide the keys, and where there are
+// fewer than four tiles a CU: one tile's length more or less counts then (64 sequences of up to 8192 keys, 512 tiles of
+// 128 rows: 222 -> 174 us; with up to 16 tiles a CU four prompts of up to 3000 tokens, 2000 tiles, go from 230 to 401).
 static AttnPlan plan_attention(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t keys) {
     const int64_t group = heads / kv_heads, rows = (tokens + seqs - 1) / seqs * group, cus = device_cus();
     AttnPlan P{};
-    P.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : ATTN_MANY;
+    P.rows = tile_rows(rows, dim, std::min(seqs, tokens) * kv_heads, cus);
+    const bool few = P.rows <= 32;
     const int64_t tiles = tokens * group / P.rows + std::min(seqs, tokens), blocks = (keys + ATTN_KEYS - 1) / ATTN_KEYS;
     P.tiles = (unsigned)tiles;
-    if (tiles * kv_heads < 2 * cus || P.rows < ATTN_MANY) {
-        const int64_t each = P.rows < ATTN_MANY ? ATTN_WAVES : 1, units = tiles * kv_heads * std::max<int64_t>(blocks, 1);
+    if (tiles * kv_heads < 4 * cus || few) {
+        const int64_t each = few ? ATTN_WAVES : 1, units = tiles * kv_heads * std::max<int64_t>(blocks, 1);
         P.shares = (unsigned)std::max<int64_t>(1, std::min(2 * cus, (units + each - 1) / each + tiles * kv_heads));
         P.least = (int)each;
         P.most = (int)(2 * cus);

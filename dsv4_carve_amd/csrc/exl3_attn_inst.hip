@@ -28,14 +28,25 @@ static int launch_few(const AttnArgs& A, const AttnPlan& P, hipStream_t s) {
     return launch<DIM, BF16, Z::ROWS, Z::LDS>(fp8_attention_kernel<DIM, BF16, RB>, A, P, ready, s);
 }
 
+template <int DIM, bool BF16, int RB>
+static int launch_many(const AttnArgs& A, const AttnPlan& P, hipStream_t s) {
+    static std::atomic<uint64_t> ready{0};
+    typedef ShareSize<DIM, RB> Z;
+    return launch<DIM, BF16, Z::ROWS, Z::LDS>(fp8_attention_rows_kernel<DIM, BF16, RB>, A, P, ready, s);
+}
+
+// The tiles that plan_attention takes for heads of up to DIM values.
 template <int DIM, bool BF16>
 static int launch(const AttnArgs& A, const AttnPlan& P, hipStream_t s) {
     if (P.rows == 16) return launch_few<DIM, BF16, 1>(A, P, s);
-    if (P.rows == 32) return launch_few<DIM, BF16, 2>(A, P, s);
-    static std::atomic<uint64_t> ready{0};
-    typedef ShareSize<DIM, 2> Z;
-    static_assert(Z::ROWS == ATTN_MANY, "rows of a tile");
-    return launch<DIM, BF16, Z::ROWS, Z::LDS>(fp8_attention_rows_kernel<DIM, BF16, 2>, A, P, ready, s);
+    if constexpr (DIM <= 64) {
+        if (P.rows == 32) return launch_few<DIM, BF16, 2>(A, P, s);
+        return launch_many<DIM, BF16, 2>(A, P, s);
+    } else {
+        if constexpr (DIM <= 128)
+            if (P.rows == 128) return launch_many<DIM, BF16, 2>(A, P, s);
+        return launch_many<DIM, BF16, 1>(A, P, s);
+    }
 }
 
 #define EXL3_ATTN_CAT_(a, b) a##b

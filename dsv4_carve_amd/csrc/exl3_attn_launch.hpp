@@ -7,10 +7,8 @@
 
 namespace exl3 {
 
-constexpr int ATTN_MANY = 128;
-
 struct AttnPlan {
-    int rows;                    // of a tile: 16, 32 or ATTN_MANY
+    int rows;                    // of a tile: 16, 32, 64 or 128
     unsigned shares;             // workgroups of a launch that share the work, or 0: a workgroup a tile
     unsigned tiles;              // tiles at most, for a workgroup a tile
     int least;                   // units that a workgroup has at least
