@@ -624,7 +624,12 @@ __device__ __forceinline__ float finish_row(const AttnArgs& A, int head, float m
 __device__ __forceinline__ void clear_rows(const AttnArgs& A) {
     const CacheView& C = A.c;
     if (!A.clear || !C.starts) return;
-    const int a = min(max(C.starts[0], 0), C.tokens), b = min(max(C.starts[C.seqs], a), C.tokens);
+    int largest = 0;
+    for (int s0 = 0; s0 <= C.seqs; s0 += 64) {
+        const int s = s0 + (threadIdx.x & 63);
+        largest = max(largest, s <= C.seqs ? get_start(C, s) : 0);
+    }
+    const int a = get_start(C, 0), b = read_lane(wave_max_scan(largest), 63);
     const int rows = C.tokens - (b - a);
     const int64_t each = (int64_t)A.heads * C.dim / 8;
     for (int i = blockIdx.x; i < rows; i += gridDim.x) {
@@ -784,12 +789,14 @@ struct Work {
         done = 0;
         if (++t == tiles_of(A, q, ROWS)) {
             t = 0;
+            int before = q.first + q.n;
             do {
                 if (++s == C.seqs) {
-                    s = 0;
+                    s = before = 0;
                     ++head;
                 }
-                q = get_seq(C, s);
+                q = get_seq(C, s, before);
+                before = q.first + q.n;
             } while (q.n == 0);
         }
         x = get_tile(A, q, t, ROWS);

@@ -27,17 +27,20 @@ struct CacheView {
 };
 
 // A sequence's tokens in a call and its length.  What a table, a length or a start
-// names past its range is cut to it: no index leaves a buffer.
+// names past its range is cut to it: no index leaves a buffer.  A start that is less
+// than one before it counts as the largest before it: no token has two sequences.
 struct Seq {
     int first, n, len;
 };
 
-__device__ __forceinline__ Seq get_seq(const CacheView& C, int s) {
+__device__ __forceinline__ int get_start(const CacheView& C, int s) { return min(max(C.starts[s], 0), C.tokens); }
+
+// before: the largest start before sequence s
+__device__ __forceinline__ Seq get_seq(const CacheView& C, int s, int before) {
     Seq q;
     if (C.starts) {
-        const int a = C.starts[s], b = C.starts[s + 1];
-        q.first = min(max(a, 0), C.tokens);
-        q.n = max(min(b, C.tokens) - q.first, 0);
+        q.first = max(get_start(C, s), before);
+        q.n = max(get_start(C, s + 1) - q.first, 0);
     } else {
         q.first = s;
         q.n = 1;
@@ -65,6 +68,27 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v) {
     v += lane_of<0x142, 0xa>(v, (int64_t)0);        // row_bcast:15, 31
     v += lane_of<0x143, 0xc>(v, (int64_t)0);
     return v;
+}
+
+// Inclusive largest values, of values that are not negative.
+__device__ __forceinline__ int wave_max_scan(int v) {
+    v = max(v, lane_of<0x111, 0xf>(v, 0));
+    v = max(v, lane_of<0x112, 0xf>(v, 0));
+    v = max(v, lane_of<0x114, 0xf>(v, 0));
+    v = max(v, lane_of<0x118, 0xf>(v, 0));
+    v = max(v, lane_of<0x142, 0xa>(v, 0));
+    return max(v, lane_of<0x143, 0xc>(v, 0));
+}
+
+// Each lane's of the sequences s0 .. s0 + 63; `before` goes on to the next 64.
+__device__ __forceinline__ Seq lane_seq(const CacheView& C, int s0, int& before) {
+    const int s = s0 + (threadIdx.x & 63);
+    int first = before;
+    if (C.starts) {
+        first = max(before, wave_max_scan(s < C.seqs ? get_start(C, s) : 0));
+        before = read_lane(first, 63);
+    }
+    return s < C.seqs ? get_seq(C, s, first) : Seq{0, 0, 0};
 }
 
 // a / b, 0 <= a, 0 < b; in 32 bits where both fit, and else bit by bit: a short call
@@ -97,9 +121,7 @@ struct Found {
 
 template <typename Count, typename At>
 __device__ __forceinline__ Found find_seq(const CacheView& C, Count&& count, At&& at) {
-    const int lane = threadIdx.x & 63;
-    const Seq none{0, 0, 0};
-    Found f{-1, 0, none};
+    Found f{-1, 0, Seq{0, 0, 0}};
     const auto look = [&](int s0, const Seq& q, int64_t c, int64_t before, int64_t sum, int64_t want) {
         before += sum - c;
         const uint64_t hit = __builtin_amdgcn_ballot_w64(want >= before && want < before + c);
@@ -110,7 +132,7 @@ __device__ __forceinline__ Found find_seq(const CacheView& C, Count&& count, At&
         f.q = Seq{read_lane(q.first, l), read_lane(q.n, l), read_lane(q.len, l)};
     };
     if (C.seqs == 1) {
-        f.q = get_seq(C, 0);
+        f.q = get_seq(C, 0, 0);
         for (;;) {
             const int64_t c = uniform(count(f.q)), want = at(c);
             if (want == COUNT_AGAIN) continue;
@@ -119,7 +141,8 @@ __device__ __forceinline__ Found find_seq(const CacheView& C, Count&& count, At&
             break;
         }
     } else if (C.seqs <= 64) {
-        const Seq q = lane < C.seqs ? get_seq(C, lane) : none;
+        int before = 0;
+        const Seq q = lane_seq(C, 0, before);
         for (;;) {
             const int64_t c = count(q), sum = wave_scan(c), want = at(read_lane(sum, 63));
             if (want == COUNT_AGAIN) continue;
@@ -130,12 +153,14 @@ __device__ __forceinline__ Found find_seq(const CacheView& C, Count&& count, At&
         int64_t want;
         do {
             int64_t c = 0;
-            for (int s = lane; s < C.seqs; s += 64) c += count(get_seq(C, s));
+            int start = 0;
+            for (int s0 = 0; s0 < C.seqs; s0 += 64) c += count(lane_seq(C, s0, start));
             want = at(read_lane(wave_scan(c), 63));
         } while (want == COUNT_AGAIN);
         int64_t before = 0;
+        int start = 0;
         for (int s0 = 0; s0 < C.seqs && want >= before && f.s < 0; s0 += 64) {
-            const Seq q = s0 + lane < C.seqs ? get_seq(C, s0 + lane) : none;
+            const Seq q = lane_seq(C, s0, start);
             const int64_t n = count(q), sum = wave_scan(n);
             look(s0, q, n, before, sum, want);
             before += read_lane(sum, 63);
@@ -226,7 +251,7 @@ __global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(App
         nth = (int)f.unit;
         q = f.q;
     } else {
-        q = get_seq(C, s);
+        q = get_seq(C, s, 0);
     }
     const int page = 1 << C.page_shift, base = q.len - q.n, from = max(base, 0);
     if (q.len <= from) return;

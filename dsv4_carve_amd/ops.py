@@ -1150,13 +1150,14 @@ def fp8_cache_append(k: torch.Tensor, v: torch.Tensor, cache: Fp8Cache, table: t
     table int32 [seqs, n]: a sequence's pages, in order; lengths int32 [seqs]: its
     tokens, the new ones counted, which are its last; starts int32 [seqs + 1]:
     sequence s has the call's tokens starts[s] .. starts[s + 1] - 1 (None: one token
-    each).  A page's scale is the smallest power of two that is not below its largest
-    magnitude / 448: over the new tokens, and where the page holds tokens of the
-    sequence already, not below the one it has; where it grows, their codes are
-    rounded to it.  A NaN or an infinity is kept as a NaN.  What the tables name out
-    of range is left out: tokens before position 0 or behind the table's room, pages
-    outside the cache.  A page that two sequences of one call write has a mixture of
-    both: sequences share pages that are full.  Returns the cache."""
+    each; a start less than one before it counts as the largest before it).  A page's
+    scale is the smallest power of two that is not below its largest magnitude / 448:
+    over the new tokens, and where the page holds tokens of the sequence already, not
+    below the one it has; where it grows, their codes are rounded to it.  A NaN or an
+    infinity is kept as a NaN.  What the tables name out of range is left out: tokens
+    before position 0 or behind the table's room, pages outside the cache.  A page
+    that two sequences of one call write has a mixture of both: sequences share pages
+    that are full.  Returns the cache."""
     _check(k.dim() == 3 and k.dtype in OUT_KIND, "k must be fp16, bf16 or fp32 [tokens, kv_heads, dim]")
     _check(v.dtype == k.dtype and v.shape == k.shape and v.device == k.device, "v must be of k's shape, dtype and device")
     _check_cache(cache, table, lengths, starts, k.shape[0], k.device)

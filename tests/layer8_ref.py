@@ -42,11 +42,12 @@ def sequences(table, lengths, starts, tokens, page):
     """(first token, new tokens, length) of each sequence, out-of-range values cut as documented."""
     room = table.shape[1] * page
     out = []
+    largest = 0                                            # starts that decrease count as the largest before them
     for s, length in enumerate(lengths.tolist()):
         if starts is None:
             first, n = s, 1
         else:
-            first = min(max(int(starts[s]), 0), tokens)
+            first = largest = max(largest, min(max(int(starts[s]), 0), tokens))
             n = max(min(int(starts[s + 1]), tokens) - first, 0)
         out.append((first, n, min(max(length, 0), room)))
     return out
