@@ -106,22 +106,14 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t u) {       // 0x80 in eac
 // less counts as nothing beside the row's largest.)  The denominator is the sum of w
 // 2^-k.  Sums are fp32.  A 16-bit weight has 11 bits, three more than a bf16 result;
 // for an fp16 result the rest of the weight goes through the product as well (FINE).
-//
-// PARTS, where rows are many and the conversions of codes cost more than the products:
-// the keys are multiplied as the codes that they are.  A bf16 value, over a power of two
-// near its row's largest, is then the sum of two e4m3 values, the second in units of
-// 2^-5: exact down to 2^-14 of the row's largest, and below that 2^-22 of it off at most.
-template <int DIM, bool BF16, int RB, bool PARTS = false>
+template <int DIM, bool BF16, int RB>
 struct AttnRows {
-    static_assert(!PARTS || (BF16 && DIM % 128 == 0), "two parts have the bits of a bf16 value; products of 128 channels");
     static constexpr bool FINE = !BF16;
     static constexpr int ROWS = 16 * RB, KC = DIM / 64, DT = DIM / 16;
     typedef Half16<BF16> H;
     typedef Half16<false> W;
 
-    typename H::vec8 qf[PARTS ? 1 : RB][KC][2];
-    int8x32_t qp[PARTS ? RB : 1][PARTS ? DIM / 128 : 1][2];    // in parts: 128 channels, as the keys' (16 of each 64 a lane)
-    float unit[RB];                                            // of the parts, for the logits
+    typename H::vec8 qf[RB][KC][2];
     int see_lo[RB], see_hi[RB];
     float4_t o[DT][RB];
     float m[RB], top[RB], c[RB], l[RB];
@@ -135,20 +127,18 @@ struct AttnRows {
             const bool in = row < rows;
             const int of = r0 + (in ? row : 0), at = of / A.group, hg = of - at * A.group;
             const uint16_t* p = A.q + (int64_t)(q.first + at) * A.q_token + (int64_t)(head * A.group + hg) * A.q_head;
-            u32x4_t z[KC][2];
 #pragma unroll
             for (int k = 0; k < KC; ++k)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int d = 64 * k + 16 * g + 8 * u;
                     const bool is = in && d < A.c.dim;
-                    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(p + (d < A.c.dim ? d : 0));
+                    const u32x4_t z = *reinterpret_cast<const u32x4_t*>(p + (d < A.c.dim ? d : 0));
+                    u32x4_t v;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) z[k][u][i] = is ? A.negative ? x[i] ^ 0x80008000u : x[i] : 0u;
-                    if constexpr (!PARTS) qf[rb][k][u] = __builtin_bit_cast(typename H::vec8, z[k][u]);
+                    for (int i = 0; i < 4; ++i) v[i] = is ? A.negative ? z[i] ^ 0x80008000u : z[i] : 0u;
+                    qf[rb][k][u] = __builtin_bit_cast(typename H::vec8, v);
                 }
-            unit[rb] = 1.f;
-            if constexpr (PARTS) divide_in_parts(z, rb);
             see_hi[rb] = in ? min(base + at + 1, q.len) : 0;
             see_lo[rb] = in && A.window ? base + at + 1 - A.window : 0;
             m[rb] = top[rb] = ATTN_LOW;
@@ -156,41 +146,6 @@ struct AttnRows {
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d][rb] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
-    }
-
-    __device__ __forceinline__ void divide_in_parts(const u32x4_t (&z)[KC][2], int rb) {
-        int most = 0;
-#pragma unroll
-        for (int k = 0; k < KC; ++k)
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) most = max(most, max((int)(z[k][u][i] << 16 & 0x7fff0000u), (int)(z[k][u][i] & 0x7fff0000u)));
-        most = max(most, __shfl_xor(most, 16));
-        most = max(most, __shfl_xor(most, 32));
-        const bool finite = most < 0x7f800000;                 // a row that is not has NaN logits only
-        const int up = 134 - max(most >> 23, 1);               // the largest value becomes less than 256
-        unit[rb] = ldexpf(1.f, -up);
-#pragma unroll
-        for (int k = 0; k < KC; ++k)
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                    float v[4];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        v[2 * j] = ldexpf(__uint_as_float(z[k][u][i + j] << 16), up);
-                        v[2 * j + 1] = ldexpf(__uint_as_float(z[k][u][i + j] & 0xffff0000u), up);
-                    }
-                    const uint32_t a = pack_e4m3(v[0], v[1], v[2], v[3]);
-                    const uint32_t b = pack_e4m3((v[0] - __builtin_amdgcn_cvt_f32_fp8((int)a, 0)) * 32.f,
-                                                 (v[1] - __builtin_amdgcn_cvt_f32_fp8((int)a, 1)) * 32.f,
-                                                 (v[2] - __builtin_amdgcn_cvt_f32_fp8((int)a, 2)) * 32.f,
-                                                 (v[3] - __builtin_amdgcn_cvt_f32_fp8((int)a, 3)) * 32.f);
-                    qp[rb][k / 2][0][4 * (k & 1) + 2 * u + i / 2] = finite ? (int)a : 0x7f7f7f7f;
-                    qp[rb][k / 2][1][4 * (k & 1) + 2 * u + i / 2] = finite ? (int)b : 0x7f7f7f7f;
-                }
     }
 
     // What no row of [lo, hi) sees may hold anything: its bytes become zeros (a weight of 0 would leave a NaN one).
@@ -219,9 +174,9 @@ struct AttnRows {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) p[t][rb] = float4_t{0.f, 0.f, 0.f, 0.f};
         // Two reads from LDS are on their way while the last two are multiplied: piece n of the keys is t = 2 n % 4 and the
-        // next, k = n / 2, or in parts t = n % 4, k = 2 (n / 4) and the next; the values' follow.
+        // next, k = n / 2; the values' follow.
         u32x4_t z[2][2];
-        const auto read_key = [&](int n, int i) { return PARTS ? key(n % 4, n / 4 * 2 + i) : key(2 * n % 4 + i, n / 2); };
+        const auto read_key = [&](int n, int i) { return key(2 * n % 4 + i, n / 2); };
 #pragma unroll
         for (int i = 0; i < 2; ++i) z[0][i] = read_key(0, i);
         // Products first: the other waves' other work goes on beside them (a chunk of 512 tokens, 16384 keys: 174.8 -> 167 us;
@@ -232,38 +187,25 @@ struct AttnRows {
 #pragma unroll
             for (int i = 0; i < 2; ++i) z[(n + 1) & 1][i] = n + 1 < 2 * KC ? read_key(n + 1, i) : value(i);
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (PARTS) {
-                const int8x32_t w = join(__builtin_bit_cast(i32x4_t, z[n & 1][0]), __builtin_bit_cast(i32x4_t, z[n & 1][1]));
-#pragma unroll
-                for (int part = 0; part < 2; ++part)
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb)
-                        p[n % 4][rb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                            w, qp[rb][n / 4][part], p[n % 4][rb], 0, 0, 0, 127, 0, part ? 127 - 5 : 127);
-                __builtin_amdgcn_sched_barrier(0);
-                continue;
-            }
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const typename H::vec8 w = H::widen(z[n & 1][i][2 * u], z[n & 1][i][2 * u + 1]);
 #pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) p[2 * n % 4 + i][rb] = H::mfma(w, qf[PARTS ? 0 : rb][n / 2][u], p[2 * n % 4 + i][rb]);
+                    for (int rb = 0; rb < RB; ++rb) p[2 * n % 4 + i][rb] = H::mfma(w, qf[rb][n / 2][u], p[2 * n % 4 + i][rb]);
                 }
             __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_setprio(0);
-        float kc[RB];
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) kc[rb] = __builtin_amdgcn_fmed3f(ks * A.qk_scale * unit[rb], 0x1p-126f, 0x1.fffffep127f);
+        float kc = fmaxf(ks * A.qk_scale, 0x1p-126f);
         uint32_t keep[4] = {};
         if (masked) {
             here = here && key0 + 15 >= lo && key0 < hi;
+            kc = here ? kc : 1.f;
             vs = here ? vs : 1.f;
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-                kc[rb] = here ? kc[rb] : 1.f;
                 const int from = here ? see_lo[rb] - key0 : 16, n = see_hi[rb] - key0;
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
@@ -286,7 +228,7 @@ struct AttnRows {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (t + i) a = fmaxf(a, p[t][rb][i]);
-            most[rb] = a * kc[rb];
+            most[rb] = a * kc;
             grew |= most[rb] > m[rb] + ATTN_SLACK || most[rb] + lv > top[rb] + ATTN_SLACK;
         }
         if (__builtin_amdgcn_ballot_w64(grew)) {
@@ -317,8 +259,8 @@ struct AttnRows {
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
-                    const float w0 = __builtin_amdgcn_exp2f(fmaf(p[t][rb][i], kc[rb], add));
-                    const float w1 = __builtin_amdgcn_exp2f(fmaf(p[t][rb][i + 1], kc[rb], add));
+                    const float w0 = __builtin_amdgcn_exp2f(fmaf(p[t][rb][i], kc, add));
+                    const float w1 = __builtin_amdgcn_exp2f(fmaf(p[t][rb][i + 1], kc, add));
                     sum[i] = t ? sum[i] + w0 : w0;
                     sum[i + 1] = t ? sum[i + 1] + w1 : w1;
                     const int at = 4 * (t & 1) + i;
@@ -978,7 +920,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void fp8_attention_rows_kernel(
         // this wave's rows; a wave without any takes the first one's, and stores nothing
         const int rows = w.x.rows - wave * OWN;
         const Tile x = get_tile(A, w.q, w.t * ATTN_WAVES + (rows > 0 ? wave : 0), OWN);
-        AttnRows<DIM, BF16, RB, BF16 && DIM % 128 == 0> R;
+        AttnRows<DIM, BF16, RB> R;
         R.begin(A, w.q, x.r0, x.rows, w.head);
         const Pages P(C, w.q, w.s);
         bool nans = false;

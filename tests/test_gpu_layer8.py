@@ -92,6 +92,19 @@ def test_norm_extremes(dev, k):
 
 @pytest.mark.parametrize("k", [384, 380])
 @pytest.mark.parametrize("pow2", [False, True])
+def test_norm_groups_of_any_size(dev, k, pow2):
+    """Groups of a row whose largest values are 2^250 apart, and products with the weight past fp32's range."""
+    gen = gen_of(dev, k + 1)
+    x, w = normal(gen, 90, k, dtype=torch.float32, spread=False), normal(gen, k, dtype=torch.float32, spread=False)
+    for exponents in ((-120, 60, 0), (60, -130, 10), (-100, -101, -99), (100, 99, 101), (40, 40, 40)):
+        size = torch.tensor(exponents, device=dev).repeat_interleave(128)[:k]
+        check_norm(torch.ldexp(x, size), w, pow2=pow2, eps=1e-30)
+        check_norm(x, torch.ldexp(w, size), pow2=pow2)
+        check_norm(torch.ldexp(x, size // 2), torch.ldexp(w, size), pow2=pow2)
+
+
+@pytest.mark.parametrize("k", [384, 380])
+@pytest.mark.parametrize("pow2", [False, True])
 def test_norm_rows_that_are_not_finite(dev, k, pow2):
     """They stay by themselves: a NaN row is NaN under the least scale, a row with an infinity 0 and NaN; 0 / 0 is NaN."""
     gen = gen_of(dev, k)
@@ -181,6 +194,19 @@ def test_append(dev, page, dtype, kv, dim):
     k, v = normal(gen, sum(counts), kv, dim, dtype=dtype), normal(gen, sum(counts), kv, dim, dtype=dtype)
     k *= torch.exp2(torch.randint(-12, 6, (sum(counts), 1, 1), generator=gen, device=dev)).to(dtype)
     check_append(k, v, cache_on(gen, pages, kv, page, dim, 6), table, lengths_of(dev, lengths), starts_of(dev, counts))
+
+
+@pytest.mark.parametrize("page,dim,dtype", [(16, 32, torch.bfloat16), (256, 256, torch.float32), (256, 240, torch.float16),
+                                            (128, 144, torch.bfloat16)])
+def test_append_many_sequences(dev, page, dim, dtype):
+    """More sequences than a wave has lanes, most of few tokens, some of whole pages."""
+    gen = gen_of(dev, page + dim)
+    counts = [(0, 1, 2, 5)[i % 4] for i in range(150)]
+    counts[70], counts[131] = page + 7, 2 * page
+    lengths = [c + (i * 13) % 20 for i, c in enumerate(counts)]
+    table, pages = L8.make_table(gen, lengths, page)
+    k, v = normal(gen, sum(counts), 1, dim, dtype=dtype), normal(gen, sum(counts), 1, dim, dtype=dtype)
+    check_append(k, v, cache_on(gen, pages, 1, page, dim, 6), table, lengths_of(dev, lengths), starts_of(dev, counts))
 
 
 @pytest.mark.parametrize("page", [16, 64])
@@ -323,6 +349,70 @@ def test_attention_prompts(dev):
     gen = gen_of(dev, 3)
     check_attention(*problem(gen, [700, 1, 333, 1000], [700, 1, 333, 1300], heads=16, kv=8, dim=64, page=16))
     check_attention(*problem(gen, [900, 500], [900, 2100], heads=8, kv=8, dim=128, page=64, dtype=torch.float16))
+
+
+@pytest.mark.parametrize("dim", [48, 64, 96, 128, 160, 256])
+@pytest.mark.parametrize("counts", [[2, 5, 3], [1 + i % 4 for i in range(70)], [9, 4, 0, 11], [60, 3, 20]])
+def test_attention_tiles_of_each_size(dev, dim, counts):
+    """About 27, 20, 48 and 221 rows a sequence and cache head, of few such pairs and of many."""
+    gen = gen_of(dev, dim + len(counts))
+    lengths = [c + (i * 37) % 150 for i, c in enumerate(counts)]
+    sinks = torch.randn(16, generator=gen, device=dev)
+    for dtype, page in ((torch.bfloat16, 16), (torch.float16, 64)):
+        p = problem(gen, counts, lengths, heads=16, kv=2, dim=dim, page=page, dtype=dtype)
+        check_attention(*p)
+        check_attention(*p, window=30, sinks=sinks)
+
+
+@pytest.mark.parametrize("heads,kv,dim,tokens", [(8, 1, 16, 17000), (16, 4, 128, 8500), (16, 8, 64, 8500), (16, 16, 96, 8500),
+                                                 (6, 3, 128, 22500), (16, 4, 256, 4300)])
+def test_attention_a_workgroup_a_tile(dev, heads, kv, dim, tokens):
+    """More tiles than four a CU, in each order of heads and tiles; some sequences behind a context, one of one token."""
+    gen = gen_of(dev, tokens + kv)
+    counts = [1] + [tokens // 16] * 16
+    lengths = [1 if i == 0 else c + 40 * (i % 3) for i, c in enumerate(counts)]
+    p = problem(gen, counts, lengths, heads=heads, kv=kv, dim=dim, page=64, dtype=torch.bfloat16 if kv != 4 else torch.float16)
+    check_attention(*p, window=None if kv % 3 else 70)
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+def test_attention_queries_of_far_apart_values(dev, dim):
+    """Values down to 2^-30 of a row's largest, a largest one that meets zeros only, rows of any size."""
+    gen = gen_of(dev, dim + 11)
+    q, cache, table, n, starts = problem(gen, [150, 20], [200, 300], heads=4, kv=2, dim=dim, page=32)
+    q *= torch.exp2(torch.randint(-30, 1, q.shape, generator=gen, device=dev)).to(q.dtype)
+    check_attention(q, cache, table, n, starts)
+    q[:, :, 3] = 2.0 ** 9                                     # beside a channel of the keys that is 0
+    cache.k.view(torch.uint8)[..., 3] = 0
+    check_attention(q, cache, table, n, starts)
+    q *= torch.exp2(torch.randint(-100, 1, (170, 4, 1), generator=gen, device=dev)).to(q.dtype)
+    q[5], q[6, 1], q[7, :, 5:] = 0.0, 2.0 ** -133, 0.0
+    check_attention(q, cache, table, n, starts)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [1] * 70, [9, 4, 11], [60, 3, 20]])
+def test_attention_pages_that_no_query_sees(dev, dim, counts):
+    """The cache's first page and pages of other sequences hold NaNs and NaN scales; so do a sequence's pages before its windows."""
+    gen = gen_of(dev, dim + len(counts))
+    lengths = [c + 90 + (i * 37) % 60 for i, c in enumerate(counts)]
+    q, cache, table, n, starts = problem(gen, counts, lengths, heads=4, kv=2, dim=dim, page=16)
+    own = table[table >= 0]
+    away = ops.Fp8Cache(*(torch.cat([t.view(torch.uint8)[:1], t.view(torch.uint8), t.view(torch.uint8)[:1]]).view(t.dtype)
+                          if t.dtype == R.E4M3 else torch.cat([t[:1], t, t[:1]]) for t in cache))
+    moved = torch.where(table >= 0, table + 1, table)
+    unseen = torch.ones(away.k.shape[0], dtype=torch.bool, device=dev)
+    unseen[own.long() + 1] = False
+    for window in (None, 20):
+        clean = ops.fp8_attention(q, cache, table, n, starts, window=window)
+        for i, (c, length) in enumerate(zip(counts, lengths)):
+            if window:
+                unseen[moved[i, :max(length - c - window, 0) // 16].long()] = True
+        for t in (away.k, away.v):
+            t.view(torch.uint8)[unseen] = 0x7f
+        for t in (away.k_scale, away.v_scale):
+            t[unseen] = torch.nan
+        assert torch.equal(ops.fp8_attention(q, away, moved, n, starts, window=window), clean)
 
 
 def test_attention_rows_without_keys(dev):
