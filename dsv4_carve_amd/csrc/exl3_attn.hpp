@@ -179,8 +179,8 @@ struct AttnRows {
         const auto read_key = [&](int n, int i) { return key(2 * n % 4 + i, n / 2); };
 #pragma unroll
         for (int i = 0; i < 2; ++i) z[0][i] = read_key(0, i);
-        // Products first: the other waves' other work goes on beside them (a chunk of 512 tokens, 16384 keys: 174.8 -> 167 us;
-        // the other way round 170).
+        // Products first: the other waves' other work goes on beside them (four prompts of up to 3000 tokens 236 -> 230 us, the
+        // other way round 240; a chunk of 512 behind 16384 keys 185, 184 and 180).
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int n = 0; n < 2 * KC; ++n) {
@@ -749,7 +749,11 @@ struct Work {
 };
 
 // Few rows a sequence: the four waves of a workgroup go through a tile's blocks in
-// turn, each with a place of its own in LDS, and join their sums there.
+// turn, each with a place of its own in LDS, and join their sums there.  Bound by memory
+// where there is much of it: 64 ragged contexts of up to 8192, 593 MB, 119 us (5.0 TB/s);
+// one of 131072, 268 MB, 48 us and 5 for the join.  A short call is a chain: lookup,
+// first loads, a block's instructions, join (one token of 1000 keys: 10.7 us with the
+// join kernel).  Two workgroups of heads of up to 128 channels are on a CU.
 template <int DIM, bool BF16, int RB>
 __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) void fp8_attention_kernel(AttnArgs A) {
     typedef AttnSize<DIM, RB> Z;
@@ -903,7 +907,13 @@ struct ShareSize {
 };
 
 // Many rows a sequence: each wave has rows of its own, all go through a tile's blocks
-// together, with one barrier a block; the next block is on its way meanwhile.
+// together, with one barrier a block; the next block is on its way meanwhile.  Bound by
+// vector instructions: a wave widens the codes of a whole block for its 32 rows (16 where
+// heads are wider than 128, for the registers: 329 us where 32 rows spilled in 522), and
+// the exponentials come on top.  512 tokens behind 16384 keys, 32 heads over 8 of 128:
+// 180 us, 750 TFLOP/s, the matrix unit 41% busy.  The 8-bit product on the codes as they
+// are (queries in two e4m3 parts) took 167, but its sums are not fp32's: logits were up to
+// 2^-16 of their terms' sum off.  256 rows a workgroup of eight waves: no faster.
 template <int DIM, bool BF16, int RB>
 __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void fp8_attention_rows_kernel(AttnArgs A) {
     typedef ShareSize<DIM, RB> Z;
@@ -1033,7 +1043,9 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void fp8_attention_rows_kernel(
 // A tile that several workgroups share, joined: blockIdx.x is the workgroup that
 // begins it, blockIdx.y takes every gridDim.y-th row.  A row's threads are groups that
 // each take some of the partial results, four channels a thread; the groups' sums
-// meet in LDS.
+// meet in LDS.  3 to 5 us, mostly a launch's; 9 where the partial results are 34 MB (512
+// workgroups of 128 rows).  A launch of its own: the last workgroup to come would need
+// counters that are zero, and the caller's scratch is not.
 template <int DIM, bool BF16, int ROWS>
 __global__ __launch_bounds__(ATTN_WAVES * 64) void fp8_attention_join_kernel(AttnArgs A) {
     constexpr int PART = ROWS * (DIM + 2), QUADS = DIM / 4, GROUPS = ATTN_WAVES * 64 / QUADS;

@@ -31,9 +31,9 @@ static int log2_of(int64_t v) { return 63 - __builtin_clzll((unsigned long long)
 // over 8 cache heads, 64 ragged sequences of up to 8192 keys with up to 8, 16 and 32 tokens (18, 34 and 66 rows):
 //            16 rows         32 rows         64 rows         128 rows
 //   dim 64   88, 144, 255    76, 106, 170    100, 105, 231   112, 139, 153
-//   dim 128  168, 286, 498   199, 290, 479   143, 151, 280   160, 176, 203
-// and of 4 such sequences 25, 30, 46 / 37, 41, 50 / 31, 33, 38 / 42, 46, 49 (dim 128); 16 query heads over 4 of 256
-// channels, the 64 sequences: 170, 257, 443 / 265, 388, 606 / 152, 157, 218 (128 rows have no room in the registers).
+//   dim 128  169, 289, 500   199, 290, 479   144, 158, 324   159, 186, 207
+// and of 4 such sequences 25, 30, 46 / 37, 41, 50 / 31, 33, 39 / 43, 46, 49 (dim 128); 16 query heads over 4 of 256
+// channels, the 64 sequences: 172, 260, 451 / 265, 388, 606 / 152, 158, 234 (128 rows have no room in the registers).
 static int tile_rows(int64_t rows, int64_t dim, int64_t pairs, int64_t cus) {
     if (rows <= 16) return 16;
     if (dim <= 64) return rows <= 64 ? 32 : 128;
@@ -43,7 +43,7 @@ static int tile_rows(int64_t rows, int64_t dim, int64_t pairs, int64_t cus) {
 
 // Work is shared out over the workgroups that run at once, two a CU, where the waves divide the keys, and where there are
 // fewer than four tiles a CU: one tile's length more or less counts then (64 sequences of up to 8192 keys, 512 tiles of
-// 128 rows: 222 -> 174 us; with up to 16 tiles a CU four prompts of up to 3000 tokens, 2000 tiles, go from 230 to 401).
+// 128 rows: 259 -> 184 us; with up to 16 tiles a CU four prompts of up to 3000 tokens, 2000 tiles, go from 230 to 401).
 static AttnPlan plan_attention(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t keys) {
     const int64_t group = heads / kv_heads, rows = (tokens + seqs - 1) / seqs * group, cus = device_cus();
     AttnPlan P{};

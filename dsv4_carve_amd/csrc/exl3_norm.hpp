@@ -136,7 +136,10 @@ __device__ __forceinline__ void load16_any(const void* p, int kind, int64_t at, 
 
 // Rows of a multiple of 16 values up to 1024 * WAVES * CHUNKS, 16-byte aligned: WAVES
 // waves have a row, a lane 16 neighbouring values in each of CHUNKS pieces, held
-// in registers from the sum to the quotients.
+// in registers from the sum to the quotients.  Bound by memory where rows are many
+// (8000 rows of 4096 in bf16 with a residual: 42.4 us, 5.4 TB/s; all quotients in 64
+// bits 52.6, of instructions), by one chain of loads, sum and stores where they are few
+// (1 row: 3.2 us).
 template <int X, int R, int WAVES, int CHUNKS>
 __global__ __launch_bounds__(256) void fp8_norm_kernel(NormArgs A) {
     __shared__ double part[4];
