@@ -567,6 +567,7 @@ __device__ __forceinline__ void clear_rows(const AttnArgs& A) {
     const CacheView& C = A.c;
     if (!A.clear || !C.starts) return;
     int largest = 0;
+#pragma unroll 4
     for (int s0 = 0; s0 <= C.seqs; s0 += 64) {
         const int s = s0 + (threadIdx.x & 63);
         largest = max(largest, s <= C.seqs ? get_start(C, s) : 0);
@@ -647,7 +648,7 @@ struct Work {
                     share = piece = A.least;
                     pieces = 1;
                     if (all > (wgs - tiles) * piece) {
-                        share = max(share, divide(all + wgs - 1, wgs));
+                        share = max((int64_t)1, divide(all + wgs - 1, wgs));
                         // no more than wgs pieces have this length, or the rest of a tile
                         if (wgs > tiles) piece = max(piece, divide(all + wgs - tiles - 1, wgs - tiles));
                         pieces = wgs > tiles && piece <= share + 4 * A.least;
@@ -693,8 +694,8 @@ struct Work {
             tile_by_xcd(blockIdx.x, A.tiles, C.kv, tile, head);
             if (tile >= A.tiles || head >= C.kv) return false;
             const int64_t at = A.tiles - 1 - tile;
-            const Found f = find_seq(C, [&](const Seq& x) { return (int64_t)tiles_of(A, x, ROWS); }, [&](int64_t) { return at; });
-            if (f.s < 0) return false;
+            const Found f = find_slot(C, at, [&](int64_t token, int64_t i) { return token * A.group / ROWS + i; });
+            if (f.s < 0 || f.unit >= tiles_of(A, f.q, ROWS)) return false;
             s = f.s;
             q = f.q;
             t = (int)f.unit;

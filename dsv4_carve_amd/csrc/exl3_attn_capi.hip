@@ -50,8 +50,8 @@ static AttnPlan plan_attention(int64_t tokens, int64_t heads, int64_t kv_heads, 
     P.rows = tile_rows(rows, dim, std::min(seqs, tokens) * kv_heads, cus);
     const bool few = P.rows <= 32;
     const int64_t tiles = tokens * group / P.rows + std::min(seqs, tokens), blocks = (keys + ATTN_KEYS - 1) / ATTN_KEYS;
-    P.tiles = (unsigned)tiles;
-    if (tiles * kv_heads < 4 * cus || few) {
+    P.tiles = (unsigned)(tokens * group / P.rows + seqs);                // as the kernels' find_slot counts
+    if (tiles * kv_heads < 4 * cus || few || P.tiles * kv_heads > MAX_GRID / 2) {     // or more than a launch takes
         const int64_t each = few ? ATTN_WAVES : 1, units = tiles * kv_heads * std::max<int64_t>(blocks, 1);
         P.shares = (unsigned)std::max<int64_t>(1, std::min(2 * cus, (units + each - 1) / each + tiles * kv_heads));
         P.least = (int)each;
@@ -75,19 +75,31 @@ static int64_t keys_of(int64_t width, int64_t page_size, int64_t tokens, int64_t
     return window ? std::min(width * page_size, window + tokens + 2 * ATTN_KEYS) : width * page_size;
 }
 
-template <int K>
-static int launch_append(const AppendArgs& A, dim3 grid, hipStream_t s) {
+template <int K, int TEAM>
+static int launch_append(const AppendArgs& A, int64_t slots, hipStream_t s) {
     static std::atomic<uint64_t> ready{0};           // devices that know of the LDS size
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= MAX_DEVICES) return fail("no HIP device");
     if (!(ready.load() >> dev & 1)) {
-        if (hipFuncSetAttribute(reinterpret_cast<const void*>(fp8_cache_append_kernel<K>),
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(fp8_cache_append_kernel<K, TEAM>),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, append_lds(256, 256)) != hipSuccess)
             return fail("the device does not give the kernel its LDS");
         ready.fetch_or(1ull << dev);
     }
-    hipLaunchKernelGGL(fp8_cache_append_kernel<K>, grid, dim3(APPEND_WAVES * 64), append_lds(1 << A.c.page_shift, A.c.dim), s, A);
+    constexpr int TEAMS = APPEND_WAVES * 64 / TEAM;
+    hipLaunchKernelGGL((fp8_cache_append_kernel<K, TEAM>), dim3((unsigned)slots, (unsigned)((A.c.kv + TEAMS - 1) / TEAMS), 2),
+                       dim3(APPEND_WAVES * 64), TEAMS * append_lds(1 << A.c.page_shift, A.c.dim), s, A);
     return check_launch();
+}
+
+// A wave a page and head where sequences are many, have few tokens and the waves' pages have room in LDS.  In us, pages of
+// 64, 8 heads of 128 channels, a workgroup each and a wave each: 1, 64, 256 and 1024 sequences of a token 5.0, 6.5, 13.5, 36.3
+// and 5.7, 6.4, 10.0, 28.0; 16, 256 and 1024 of 3 tokens 5.6, 24.3, 125.5 and 6.2, 15.9, 58.4; 64 of 16 8.5 and 8.1.
+template <int K>
+static int launch_append(const AppendArgs& A, int64_t slots, hipStream_t s) {
+    const bool waves = A.c.tokens <= 16 * (int64_t)A.c.seqs && slots * A.c.kv * 2 > 4 * device_cus() &&
+                       APPEND_WAVES * append_lds(1 << A.c.page_shift, A.c.dim) <= 64 * 1024;
+    return waves ? launch_append<K, 64>(A, slots, s) : launch_append<K, APPEND_WAVES * 64>(A, slots, s);
 }
 
 extern "C" {
@@ -109,13 +121,11 @@ int exl3_fp8_cache_append(const void* k, int64_t k_token, int64_t k_head, const 
     const AppendArgs A{{k_cache, k_scale, v_cache, v_scale, table, table_stride, lengths, starts, (int)seqs, (int)tokens,
                         (int)kv_heads, (int)dim, log2_of(page_size), (int)width, (int)pages},
                        k, v, k_token, k_head, v_token, v_head};
-    // pages that may be touched: each sequence's first and last one, and those that its tokens fill
-    const int64_t bound = starts ? std::min(tokens, tokens / page_size + 2 * seqs) : tokens;
+    const int64_t slots = starts ? tokens / page_size + 2 * seqs : tokens;     // as the kernel's find_slot counts
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const dim3 grid((unsigned)bound, (unsigned)kv_heads, 2);
-    if (kind == OUT_F16) return launch_append<OUT_F16>(A, grid, s);
-    if (kind == OUT_BF16) return launch_append<OUT_BF16>(A, grid, s);
-    return launch_append<OUT_F32>(A, grid, s);
+    if (kind == OUT_F16) return launch_append<OUT_F16>(A, slots, s);
+    if (kind == OUT_BF16) return launch_append<OUT_BF16>(A, slots, s);
+    return launch_append<OUT_F32>(A, slots, s);
 }
 
 int64_t exl3_fp8_attention_scratch_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs,

@@ -35,6 +35,12 @@ struct Seq {
 
 __device__ __forceinline__ int get_start(const CacheView& C, int s) { return min(max(C.starts[s], 0), C.tokens); }
 
+__device__ __forceinline__ int get_length(const CacheView& C, int s) {
+    const int64_t room = (int64_t)C.width << C.page_shift;
+    const int len = max(C.lengths[s], 0);
+    return (int64_t)len < room ? len : (int)room;
+}
+
 // before: the largest start before sequence s
 __device__ __forceinline__ Seq get_seq(const CacheView& C, int s, int before) {
     Seq q;
@@ -45,9 +51,7 @@ __device__ __forceinline__ Seq get_seq(const CacheView& C, int s, int before) {
         q.first = s;
         q.n = 1;
     }
-    const int64_t room = (int64_t)C.width << C.page_shift;
-    const int len = max(C.lengths[s], 0);
-    q.len = (int64_t)len < room ? len : (int)room;
+    q.len = get_length(C, s);
     return q;
 }
 
@@ -150,21 +154,68 @@ __device__ __forceinline__ Found find_seq(const CacheView& C, Count&& count, At&
             break;
         }
     } else {
-        int64_t want;
-        do {
-            int64_t c = 0;
-            int start = 0;
-            for (int s0 = 0; s0 < C.seqs; s0 += 64) c += count(lane_seq(C, s0, start));
-            want = at(read_lane(wave_scan(c), 63));
-        } while (want == COUNT_AGAIN);
-        int64_t before = 0;
+        // A lane counts `each` neighbouring sequences; those of the lane that has the unit are then a lane each.
+        const int lane = threadIdx.x & 63, each = (C.seqs + 63) / 64, from = min(lane * each, C.seqs), to = min(from + each, C.seqs);
         int start = 0;
-        for (int s0 = 0; s0 < C.seqs && want >= before && f.s < 0; s0 += 64) {
-            const Seq q = lane_seq(C, s0, start);
-            const int64_t n = count(q), sum = wave_scan(n);
-            look(s0, q, n, before, sum, want);
-            before += read_lane(sum, 63);
+        if (C.starts) {
+            for (int s = from; s < to; ++s) start = max(start, get_start(C, s));
+            start = __shfl_up(wave_max_scan(start), 1);
+            start = lane ? start : 0;                                         // the largest before the lane's
         }
+        int64_t c, sum, want;
+        do {
+            c = 0;
+            int before = start;
+            for (int s = from; s < to; ++s) {
+                const Seq q = get_seq(C, s, before);
+                before = q.first;
+                c += count(q);
+            }
+            sum = wave_scan(c);
+            want = at(read_lane(sum, 63));
+        } while (want == COUNT_AGAIN);
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(want >= sum - c && want < sum);
+        if (!hit) return f;
+        const int l = __builtin_ctzll(hit);
+        int64_t before = read_lane(sum - c, l);
+        int first = read_lane(start, l);
+        for (int s0 = l * each; f.s < 0 && s0 < (l + 1) * each && s0 < C.seqs; s0 += 64) {
+            const Seq q = lane_seq(C, s0, first);
+            const int64_t n = s0 + lane < (l + 1) * each ? count(q) : 0, sums = wave_scan(n);
+            look(s0, q, n, before, sums, want);
+            before += read_lane(sums, 63);
+        }
+    }
+    return f;
+}
+
+// The sequence that has the workgroups before(first token, s) up to before(first token
+// behind it, s + 1), x among them: some more than it needs, but starts alone tell them,
+// and the look ends where it is found (append to 1024 sequences of 3 tokens, 33000
+// workgroups: 195 -> 123 us).
+template <typename Before>
+__device__ __forceinline__ Found find_slot(const CacheView& C, int64_t x, Before&& before) {
+    Found f{-1, 0, Seq{0, 0, 0}};
+    const int lane = threadIdx.x & 63;
+    int start = 0;
+    for (int s0 = 0; s0 < C.seqs; s0 += 64) {
+        const int s = s0 + lane;
+        int first = s, end = s + 1;
+        if (C.starts) {
+            first = max(start, wave_max_scan(s < C.seqs ? get_start(C, s) : 0));
+            end = max(first, s < C.seqs ? get_start(C, s + 1) : 0);
+            start = read_lane(first, 63);
+        }
+        const int64_t lo = before((int64_t)first, (int64_t)s);
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(s < C.seqs && x >= lo && x < before((int64_t)end, (int64_t)s + 1));
+        if (!hit) continue;
+        const int l = __builtin_ctzll(hit);
+        f.s = s0 + l;
+        f.unit = x - read_lane(lo, l);
+        f.q.first = read_lane(first, l);
+        f.q.n = read_lane(end, l) - f.q.first;
+        f.q.len = get_length(C, f.s);
+        break;
     }
     return f;
 }
@@ -224,32 +275,35 @@ __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
     w[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
-// A workgroup has one page of one head, of the keys or of the values: the new
-// tokens' largest magnitude, the scale, the old codes where it grew, the new ones.
-// The inputs stay in registers in between, the first APPEND_HOLD * 256 chunks of eight
-// (64 tokens of 256, 128 of 128); what a page has more is read twice.  A value's codes
+// A workgroup, or each wave of it where tokens are few (TEAM threads), has one page of
+// one head, of the keys or of the values: the new tokens' largest magnitude, the scale,
+// the old codes where it grew, the new ones.  The inputs stay in registers in between,
+// the first APPEND_HOLD * TEAM chunks of eight (a workgroup's: 64 tokens of 256 values,
+// 128 of 128); what a page has more is read twice.  A value's codes
 // are turned in LDS: tokens of a channel are neighbours in the cache.  Four chunks of
 // up to 2000 tokens, 8 heads of 128 (30 MB): 11.3 us; read twice and values gathered two
 // bytes a load 18.4.
 // 13 single tokens: 4.2 us, a chain of lookup, page, inputs, reduction and store.
 constexpr int APPEND_HOLD = 8;
 
-inline int append_lds(int page, int dim) { return page * (dim + 4); }
+__host__ __device__ inline int append_lds(int page, int dim) { return page * (dim + 4); }
 
-template <int K>
+template <int K, int TEAM>
 __global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(AppendArgs A) {
-    constexpr int THREADS = APPEND_WAVES * 64;
-    extern __shared__ __attribute__((aligned(16))) char append_codes[];           // values: [page][dim + 4]
+    constexpr int THREADS = TEAM, TEAMS = APPEND_WAVES * 64 / TEAM;
+    extern __shared__ __attribute__((aligned(16))) char append_lds_[];
     __shared__ float most_of[APPEND_WAVES];
     const CacheView& C = A.c;
-    const int tid = threadIdx.x, head = blockIdx.y;
+    const int tid = threadIdx.x % TEAM, team = uniform((int)threadIdx.x / TEAM), head = blockIdx.y * TEAMS + team;
+    char* append_codes = append_lds_ + team * append_lds(1 << C.page_shift, C.dim);        // values: [page][dim + 4]
     const bool values = blockIdx.z;
+    if (head >= C.kv) return;
     int s = blockIdx.x, nth = 0;
     Seq q;
     if (C.starts) {
-        const Found f = find_seq(C, [&](const Seq& x) { return (int64_t)touched_pages(C, x); },
-                                 [](int64_t) { return (int64_t)blockIdx.x; });
-        if (f.s < 0) return;
+        // pages that new tokens lie in: at most two more than they fill
+        const Found f = find_slot(C, blockIdx.x, [&](int64_t token, int64_t i) { return (token >> C.page_shift) + 2 * i; });
+        if (f.s < 0 || f.unit >= touched_pages(C, f.q)) return;
         s = f.s;
         nth = (int)f.unit;
         q = f.q;
@@ -318,10 +372,12 @@ __global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(App
         largest(v);
     }
     most = wave_max(most, 0.f);
-    if ((tid & 63) == 0) most_of[tid >> 6] = most;
-    __syncthreads();
+    if constexpr (TEAM > 64) {
+        if ((tid & 63) == 0) most_of[tid >> 6] = most;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < APPEND_WAVES; ++w) most = fmaxf(most, most_of[w]);
+        for (int w = 0; w < APPEND_WAVES; ++w) most = fmaxf(most, most_of[w]);
+    }
     const float now = fmaxf(QuantGroup(most, true).scale, before);
     const float inverse = 1.0f / now, by = before / now;
     const bool grew = lo && by != 1.0f;
@@ -358,7 +414,8 @@ __global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(App
                 reinterpret_cast<u32x4_t*>(code)[i] = u;
             }
     } else {
-        __syncthreads();
+        if constexpr (TEAM > 64) __syncthreads();
+        else asm volatile("" ::: "memory");                     // LDS keeps a wave's order, the compiler has to
         const int first = grew ? 0 : lo >> 4;
         for (int i = tid; i < fours; i += THREADS) {
             const int group = i & ((1 << lg) - 1), d = i >> lg << 2, t0 = group * 16;

@@ -209,6 +209,18 @@ def test_append_many_sequences(dev, page, dim, dtype):
     check_append(k, v, cache_on(gen, pages, 1, page, dim, 6), table, lengths_of(dev, lengths), starts_of(dev, counts))
 
 
+@pytest.mark.parametrize("page,kv,dim", [(16, 7, 128), (64, 3, 80), (128, 8, 16), (256, 5, 32)])
+def test_append_a_wave_a_page(dev, page, kv, dim):
+    """Many sequences of few tokens, and heads that are no multiple of a workgroup's waves; one with pages of tokens."""
+    gen = gen_of(dev, page + kv)
+    for counts in ([1] * 400, [1 + i % 3 for i in range(399)] + [2 * page + 5], [6 * (i % 2) for i in range(300)]):
+        lengths = [c + (i * 29) % (2 * page) for i, c in enumerate(counts)]
+        table, pages = L8.make_table(gen, lengths, page)
+        k, v = normal(gen, sum(counts), kv, dim), normal(gen, sum(counts), kv, dim)
+        starts = None if max(counts) == 1 else starts_of(dev, counts)
+        check_append(k, v, cache_on(gen, pages, kv, page, dim, 6), table, lengths_of(dev, lengths), starts)
+
+
 @pytest.mark.parametrize("page", [16, 64])
 def test_append_token_by_token(dev, page):
     """Scales grow and stay as the tokens come, and each page begins anew."""
