@@ -281,7 +281,7 @@ __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
 // the first APPEND_HOLD * TEAM chunks of eight (a workgroup's: 64 tokens of 256 values,
 // 128 of 128); what a page has more is read twice.  A value's codes
 // are turned in LDS: tokens of a channel are neighbours in the cache.  Four chunks of
-// up to 2000 tokens, 8 heads of 128 (30 MB): 11.3 us; read twice and values gathered two
+// up to 2000 tokens, 8 heads of 128 (30 MB): 12 us; read twice and values gathered two
 // bytes a load 18.4.
 // 13 single tokens: 4.2 us, a chain of lookup, page, inputs, reduction and store.
 constexpr int APPEND_HOLD = 8;
