@@ -619,9 +619,19 @@ __device__ __forceinline__ void tile_by_xcd(int b, int tiles, int heads, int& ti
 // where the tile began before its share, in its second where it goes on behind it.
 // Without a place for partial results a workgroup has a tile, the last, longest ones
 // first.
+//
+// Two workgroups are on a CU, and the waves of the first go first: where instructions
+// bound it, 65 blocks of 64 keys and 128 rows take the first 112 us and the second 154.
+// So there the first ones (the first half of an XCD's) have ATTN_FIRST : 16 - ATTN_FIRST
+// of the units, where these are 16 a workgroup at least (a chunk of 512 behind 16384
+// keys: 171-176 us, 180 with equal shares; 10 : 6 is like 9 : 7).
+constexpr int ATTN_FIRST = 9;
+
 template <int ROWS>
 struct Work {
-    int64_t u, u1, share;        // units: the next, the end of the workgroup's, how many a workgroup has
+    static constexpr bool UNEVEN = ROWS >= 64;
+    int64_t all, u, u1, share;   // units: of the call, the next, the end of the workgroup's, how many a workgroup has
+    bool uneven;
     int me, s, t, head;
     int done, n, here;           // of the tile: blocks before the next unit, all of them, those of this workgroup
     Seq q;
@@ -630,11 +640,12 @@ struct Work {
     // False if there is nothing for this workgroup.
     __device__ __forceinline__ bool find(const AttnArgs& A) {
         const CacheView& C = A.c;
-        u = u1 = share = 0;
+        all = u = u1 = share = 0;
+        uneven = false;
         me = blockIdx.x;
         t = head = done = 0;
         if (A.part) {
-            int64_t all = 0, mine = 0, piece = 0;                 // units; tiles of this lane's sequences
+            int64_t mine = 0, piece = 0;                          // tiles of this lane's sequences
             int pieces = -1;                                      // a share is of one tile; -1: not known yet
             const Found f = find_seq(C, [&](const Seq& x) {
                 if (pieces < 0) mine += tiles_of(A, x, ROWS);
@@ -663,11 +674,13 @@ struct Work {
                     }
                 } else {
                     busy = divide(all + share - 1, share);
+                    uneven = UNEVEN && all >= 16 * (int64_t)A.most && (int)gridDim.x == A.most && A.most % (2 * XCDS) == 0;
+                    if (uneven) busy = A.most;
                 }
                 if (me >= busy) return (int64_t)-1;
                 me = by_xcd(me, (int)busy);
-                u = share * me;
-                u1 = u + share < all ? u + share : all;
+                u = begin_of(A, me);
+                u1 = min(begin_of(A, me + 1), all);
                 const int64_t at = pieces ? me : u;
                 head = (int)divide(at, total);
                 return at - head * total;
@@ -707,6 +720,13 @@ struct Work {
         return true;
     }
 
+    // The first unit of workgroup j.
+    __device__ __forceinline__ int64_t begin_of(const AttnArgs& A, int j) const {
+        if (!UNEVEN || !uneven) return share * j;
+        const int half = A.most / (2 * XCDS), p = j % (2 * half);
+        return divide(all * (8 * (j - p) + min(p, half) * ATTN_FIRST + max(p - half, 0) * (16 - ATTN_FIRST)), 8 * A.most);
+    }
+
     __device__ __forceinline__ void measure() {
         const int64_t want = u1 - u;
         here = (int)(n - done < want ? n - done : want);
@@ -718,7 +738,12 @@ struct Work {
     // Where a partial result goes, of `size` floats each; tells the join of a tile that begins here.
     __device__ __forceinline__ float* part(const AttnArgs& A, int size) const {
         if (done == 0 && threadIdx.x == 0) {
-            const int last = min((int)divide(u + n - 1, share), (int)gridDim.x - 1);
+            int last = me;
+            if (UNEVEN && uneven)
+                while (begin_of(A, last + 1) < u + n) ++last;
+            else
+                last = (int)divide(u + n - 1, share);
+            last = min(last, (int)gridDim.x - 1);
             A.shared[me] = SharedTile{q.first, x.r0, x.rows, head, last};
         }
         return A.part + ((int64_t)me * 2 + (done == 0 ? 1 : 0)) * size;
@@ -912,9 +937,9 @@ struct ShareSize {
 // vector instructions: a wave widens the codes of a whole block for its 32 rows (16 where
 // heads are wider than 128, for the registers: 329 us where 32 rows spilled in 522), and
 // the exponentials come on top.  512 tokens behind 16384 keys, 32 heads over 8 of 128:
-// 180 us, 750 TFLOP/s, the matrix unit 41% busy.  The 8-bit product on the codes as they
-// are (queries in two e4m3 parts) took 167, but its sums are not fp32's: logits were up to
-// 2^-16 of their terms' sum off.  256 rows a workgroup of eight waves: no faster.
+// 171-176 us, 780 TFLOP/s, the matrix unit 41% busy.  The 8-bit product on the codes as
+// they are (queries in two e4m3 parts) took 167 for 180, but its sums are not fp32's:
+// logits were up to 2^-16 of their terms' sum off.  256 rows a workgroup of eight waves: no faster.
 template <int DIM, bool BF16, int RB>
 __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void fp8_attention_rows_kernel(AttnArgs A) {
     typedef ShareSize<DIM, RB> Z;

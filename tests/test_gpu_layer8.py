@@ -387,6 +387,16 @@ def test_attention_a_workgroup_a_tile(dev, heads, kv, dim, tokens):
     check_attention(*p, window=None if kv % 3 else 70)
 
 
+@pytest.mark.parametrize("dim,heads,kv", [(64, 32, 8), (128, 32, 8), (256, 16, 4)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_a_chunk_behind_a_long_context(dev, dim, heads, kv, dtype):
+    """Shares of about 70 units, of one tile or of two, beside a short sequence."""
+    gen = gen_of(dev, dim)
+    p = problem(gen, [300, 2], [28000, 500], heads=heads, kv=kv, dim=dim, page=64, dtype=dtype)
+    check_attention(*p)
+    check_attention(*p, window=20000)
+
+
 @pytest.mark.parametrize("dim", [128, 256])
 def test_attention_queries_of_far_apart_values(dev, dim):
     """Values down to 2^-30 of a row's largest, a largest one that meets zeros only, rows of any size."""
