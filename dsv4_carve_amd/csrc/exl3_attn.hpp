@@ -392,7 +392,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t page_part(const CacheView& C, 
                                                             bool on) {
     const int id = __builtin_amdgcn_readlane(ids, 16 * g);
     const bool is = on && valid_page(C, id);
-    const uint32_t bytes = (uint32_t)C.dim << C.page_shift;                   // below 2^16, and 1024 heads of it below 2^32
+    const uint32_t bytes = (uint32_t)C.dim << C.page_shift;                   // 2^16 at most, and 1024 heads of it 2^26
     return __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>(p) + (uint64_t)(uint32_t)(is ? id : 0) * ((uint32_t)C.kv * bytes) + (head * bytes + at), 0,
         is ? bytes - at : 0, 0x27000);

@@ -1156,8 +1156,8 @@ def fp8_cache_append(k: torch.Tensor, v: torch.Tensor, cache: Fp8Cache, table: t
     below the one it has; where it grows, their codes are rounded to it.  A NaN or an
     infinity is kept as a NaN.  What the tables name out of range is left out: tokens
     before position 0 or behind the table's room, pages outside the cache.  A page
-    that two sequences of one call write has a mixture of both: sequences share pages
-    that are full.  Returns the cache."""
+    that a call writes twice (two sequences, or one that names it twice) has a mixture
+    of both: sequences share pages that are full.  Returns the cache."""
     _check(k.dim() == 3 and k.dtype in OUT_KIND, "k must be fp16, bf16 or fp32 [tokens, kv_heads, dim]")
     _check(v.dtype == k.dtype and v.shape == k.shape and v.device == k.device, "v must be of k's shape, dtype and device")
     _check_cache(cache, table, lengths, starts, k.shape[0], k.device)

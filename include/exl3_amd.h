@@ -385,8 +385,8 @@ int exl3_fp8_norm(const void* x, int x_kind, const void* residual, int residual_
  * of the call included.  starts int32 [seqs + 1]: sequence s has the call's tokens
  * starts[s] .. starts[s + 1] - 1, which are its last ones; null for one token each
  * (tokens == seqs).  All four are read on the device: a length past the table's row
- * counts as the row's room, a page outside the cache is left out, and starts are cut
- * to 0..tokens.
+ * counts as the row's room, a page outside the cache is left out, starts are cut to
+ * 0..tokens, and one less than a start before it counts as the largest before it.
  *
  * exl3_fp8_cache_append writes the call's keys and values (strides in values, rows
  * 16-byte aligned; kind 0 = fp16, 1 = bf16, 2 = fp32).  A page's scale becomes the
@@ -394,7 +394,7 @@ int exl3_fp8_norm(const void* x, int x_kind, const void* residual, int residual_
  * NaN and infinities left out), or stays where the page holds tokens of the sequence
  * already and has a larger one; where it grows, their codes are rounded to it.  A NaN
  * or an infinity becomes a NaN.  Tokens before position 0 are left out.  A page that
- * two sequences of one call write has a mixture of both.
+ * a call writes twice (two sequences, or one that names it twice) has a mixture of both.
  */
 int exl3_fp8_cache_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
                           int64_t v_head, int kind, int64_t tokens, uint8_t* k_cache, float* k_scale,
