@@ -1117,21 +1117,21 @@ def _check_cache(cache: Fp8Cache, table, lengths, starts, tokens: int, device: t
     _check(page in FP8_CACHE_PAGES, "page must be 16, 32, 64, 128 or 256")
     _check(dim % 16 == 0 and 16 <= dim <= FP8_CACHE_MAX_DIM, "dim must be a multiple of 16 in 16..256")
     _check(pages >= 1 and 1 <= heads <= 1024, "the cache must have a page and 1..1024 heads")
-    _check(v.dtype == E4M3 and v.is_contiguous() and v.device == device and tuple(v.shape) == (pages, heads, dim, page),
+    _check(v.dtype == E4M3 and v.is_contiguous() and v.device == device and v.shape == (pages, heads, dim, page),
            "the cache's v must be contiguous float8_e4m3fn [pages, kv_heads, dim, page] on the input device")
     for t in (k_scale, v_scale):
-        _check(t.dtype == torch.float32 and t.is_contiguous() and t.device == device and tuple(t.shape) == (pages, heads),
+        _check(t.dtype == torch.float32 and t.is_contiguous() and t.device == device and t.shape == (pages, heads),
                "the cache's scales must be contiguous fp32 [pages, kv_heads] on the input device")
     _check(table.dim() == 2 and table.dtype == torch.int32 and table.device == device and table.stride(1) == 1 and
            table.shape[1] >= 1, "table must be int32 [seqs, pages] on the input device, rows contiguous")
     seqs = table.shape[0]
     _check(lengths.dtype == torch.int32 and lengths.is_contiguous() and lengths.device == device and
-           tuple(lengths.shape) == (seqs,), "lengths must be contiguous int32 [seqs] on the input device")
+           lengths.shape == (seqs,), "lengths must be contiguous int32 [seqs] on the input device")
     if starts is None:
         _check(tokens == seqs, "without starts there is one token for each sequence")
     else:
         _check(starts.dtype == torch.int32 and starts.is_contiguous() and starts.device == device and
-               tuple(starts.shape) == (seqs + 1,), "starts must be contiguous int32 [seqs + 1] on the input device")
+               starts.shape == (seqs + 1,), "starts must be contiguous int32 [seqs + 1] on the input device")
 
 
 def _token_rows(t: torch.Tensor) -> torch.Tensor:
@@ -1204,17 +1204,18 @@ def fp8_attention(q: torch.Tensor, cache: Fp8Cache, table: torch.Tensor, lengths
         _check(sinks.dtype == torch.float32 and sinks.is_contiguous() and sinks.device == q.device and
                tuple(sinks.shape) == (heads,), "sinks must be contiguous fp32 [heads] on q's device")
     clear = out is None
-    if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
-    _check(out.dtype == q.dtype and out.device == q.device and out.is_contiguous() and out.shape == q.shape,
-           "out must be contiguous, of q's shape, dtype and device")
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    if clear:
+        out = q.new_empty((tokens, heads, dim))
+    else:
+        _check(out.dtype == q.dtype and out.device == q.device and out.is_contiguous() and out.shape == q.shape,
+               "out must be contiguous, of q's shape, dtype and device")
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     if tokens and table.shape[0]:
         scratch = None
         if q.is_cuda:
             nbytes = _fp8_attention_scratch_bytes(q.device.index, tokens, heads, kv_heads, dim, table.shape[0], table.shape[1],
                                                   page, window or 0)
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+            scratch = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         torch.ops.exl3_amd.fp8_attention(_token_rows(q), *cache, table, lengths, starts, scale, window or 0, sinks, out, lse,
                                          clear, scratch)
     elif clear:
