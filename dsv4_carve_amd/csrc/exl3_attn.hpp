@@ -707,11 +707,18 @@ struct Work {
             tile_by_xcd(blockIdx.x, A.tiles, C.kv, tile, head);
             if (tile >= A.tiles || head >= C.kv) return false;
             const int64_t at = A.tiles - 1 - tile;
-            const Found f = find_slot(C, at, [&](int64_t token, int64_t i) { return token * A.group / ROWS + i; });
-            if (f.s < 0 || f.unit >= tiles_of(A, f.q, ROWS)) return false;
-            s = f.s;
-            q = f.q;
-            t = (int)f.unit;
+            if (C.starts) {
+                const Found f = find_slot(C, at, [&](int64_t token, int64_t i) { return token * A.group / ROWS + i; });
+                if (f.s < 0 || f.unit >= tiles_of(A, f.q, ROWS)) return false;
+                s = f.s;
+                q = f.q;
+                t = (int)f.unit;
+            } else {
+                const int each = (A.group + ROWS - 1) / ROWS;
+                s = (int)at / each;
+                t = (int)at - s * each;
+                q = get_seq(C, s, 0);
+            }
             x = get_tile(A, q, t, ROWS);
             n = blocks_of(x);
             u1 = n;

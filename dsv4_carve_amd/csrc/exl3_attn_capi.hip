@@ -44,14 +44,17 @@ static int tile_rows(int64_t rows, int64_t dim, int64_t pairs, int64_t cus) {
 // Work is shared out over the workgroups that run at once, two a CU, where the waves divide the keys, and where there are
 // fewer than four tiles a CU: one tile's length more or less counts then (64 sequences of up to 8192 keys, 512 tiles of
 // 128 rows: 259 -> 184 us; with up to 16 tiles a CU four prompts of up to 3000 tokens, 2000 tiles, go from 230 to 401).
+// Single tokens of many sequences have a workgroup a tile too: a second tile costs a workgroup more than a new one does
+// (8 heads of 128: 256 sequences of up to 500, 1000 and 4000 keys 49, 72 and 217 us, shared out 60, 83 and 224; 128 of up to
+// 2000 and 8192 64 and 257, shared out 72 and 247: fewer are not even enough).
 static AttnPlan plan_attention(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t keys) {
     const int64_t group = heads / kv_heads, rows = (tokens + seqs - 1) / seqs * group, cus = device_cus();
     AttnPlan P{};
     P.rows = tile_rows(rows, dim, std::min(seqs, tokens) * kv_heads, cus);
-    const bool few = P.rows <= 32;
+    const bool few = P.rows <= 32, single = tokens == seqs;
     const int64_t tiles = tokens * group / P.rows + std::min(seqs, tokens), blocks = (keys + ATTN_KEYS - 1) / ATTN_KEYS;
     P.tiles = (unsigned)(tokens * group / P.rows + seqs);                // as the kernels' find_slot counts
-    if (tiles * kv_heads < 4 * cus || few || P.tiles * kv_heads > MAX_GRID / 2) {     // or more than a launch takes
+    if (tiles * kv_heads <= 4 * cus || (few && !single) || P.tiles * kv_heads > MAX_GRID / 2) {   // or more than a launch takes
         const int64_t each = few ? ATTN_WAVES : 1, units = tiles * kv_heads * std::max<int64_t>(blocks, 1);
         P.shares = (unsigned)std::max<int64_t>(1, std::min(2 * cus, (units + each - 1) / each + tiles * kv_heads));
         P.least = (int)each;
@@ -155,7 +158,8 @@ int exl3_fp8_attention(const void* q, int kind, int64_t q_token, int64_t q_head,
     if (!std::isfinite(scale)) return fail("scale must be finite");
     if (window < 0 || window > INT32_MAX / 2) return fail("window must be in 0..2^30");
     if (!aligned16(q) || !aligned16(out) || q_token % 8 || q_head % 8) return fail("rows of q and out must be 16-byte aligned");
-    const AttnPlan P = plan_attention(tokens, heads, kv_heads, dim, seqs, keys_of(width, page_size, tokens, window));
+    AttnPlan P = plan_attention(tokens, heads, kv_heads, dim, seqs, keys_of(width, page_size, tokens, window));
+    if (!starts) P.tiles = (unsigned)(seqs * ((heads / kv_heads + P.rows - 1) / P.rows));
     const int64_t need = attention_scratch(P, dim);
     if (need && !scratch) return fail("null pointer");
     if (!aligned16(scratch)) return fail("scratch must be 16-byte aligned");

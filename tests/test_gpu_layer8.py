@@ -350,6 +350,23 @@ def test_attention_many_sequences_share_the_work(dev):
     check_attention(*problem(gen, counts, lengths, heads=8, kv=2, dim=128, page=64, dtype=torch.float16))
 
 
+@pytest.mark.parametrize("dim,heads,kv,seqs", [(64, 64, 32, 40), (64, 320, 16, 40), (128, 48, 24, 50), (128, 32, 32, 40),
+                                               (208, 64, 16, 70)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_a_workgroup_a_sequence(dev, dim, heads, kv, seqs, dtype):
+    """As many tokens as sequences, one each or not, where a workgroup has a tile; some sequences without keys."""
+    gen = gen_of(dev, dim + kv)
+    lengths = [(i * 37) % 200 for i in range(seqs)]
+    q, cache, table, n, _ = problem(gen, [1] * seqs, lengths, heads=heads, kv=kv, dim=dim, page=32, dtype=dtype)
+    assert ops._fp8_attention_scratch_bytes(dev.index or 0, seqs, heads, kv, dim, seqs, table.shape[1], 32, 0) == 0
+    sinks = torch.randn(heads, generator=gen, device=dev)
+    alone, _ = check_attention(q, cache, table, n, sinks=sinks)
+    counts = [(2, 0, 1, 1)[i % 4] for i in range(seqs - seqs % 4)] + [1] * (seqs % 4)
+    check_attention(q, cache, table, n, starts_of(dev, counts), sinks=sinks, window=40)
+    same = ops.fp8_attention(q, cache, table, n, starts_of(dev, [1] * seqs), sinks=sinks)
+    assert torch.equal(same, alone)
+
+
 def test_attention_one_long_sequence(dev):
     gen = gen_of(dev, 2)
     for heads, counts in ((4, [1]), (32, [2]), (8, [40])):
