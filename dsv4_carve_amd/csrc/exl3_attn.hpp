@@ -104,11 +104,15 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t u) {       // 0x80 in eac
 // scale) + HEADROOM - c, where c follows the row's largest log2 of weight times scale:
 // so it neither overflows nor loses a row whose values are small.  (k is -64 at least:
 // less counts as nothing beside the row's largest.)  The denominator is the sum of w
-// 2^-k.  Sums are fp32.  A 16-bit weight has 11 bits, three more than a bf16 result;
-// for an fp16 result the rest of the weight goes through the product as well (FINE).
-template <int DIM, bool BF16, int RB>
+// 2^-k.  Sums are fp32.  A 16-bit weight has 11 bits; with FINE the rest of it goes
+// through the product as well (22 bits).  That is nearly free where memory bounds a call
+// (few rows, 64 tokens of up to 8192: 119.6 -> 121.3 us; one of 1000: 10.8 -> 10.9), and
+// costs 22% where instructions do (a chunk of 512 behind 16384 keys: 171-175 -> 210): so
+// many rows with a bf16 result, which has three bits less than the weight, go without.
+// Against 64 bits the chunk's error, the result's rounding in it, is 1.6596e-3 of the
+// result without the rest and 1.6568e-3 with it.
+template <int DIM, bool BF16, int RB, bool FINE>
 struct AttnRows {
-    static constexpr bool FINE = !BF16;
     static constexpr int ROWS = 16 * RB, KC = DIM / 64, DT = DIM / 16;
     typedef Half16<BF16> H;
     typedef Half16<false> W;
@@ -492,7 +496,7 @@ struct AttnStage {
 // Blocks first, first + step, ... < last of a tile's keys for one wave.  No branch divides lanes in here: the compiler may
 // leave them apart in the loop around the products, and may place copies of other lanes' registers before they are back.
 template <int DIM, bool BF16, int RB>
-__device__ __forceinline__ void attend(const AttnArgs& A, const AttnStage<DIM>& S, AttnRows<DIM, BF16, RB>& R, const Seq& q,
+__device__ __forceinline__ void attend(const AttnArgs& A, const AttnStage<DIM>& S, AttnRows<DIM, BF16, RB, true>& R, const Seq& q,
                                        const Tile& x, int s, int head, int first, int last, int step) {
     constexpr int DT = DIM / 16;
     if (first >= last) return;
@@ -801,7 +805,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) voi
     float* ml = lds + ATTN_WAVES * Z::ROWS * Z::PITCH;          // [wave][row][2]
     for (;;) {
         {
-            AttnRows<DIM, BF16, RB> R;
+            AttnRows<DIM, BF16, RB, true> R;
             R.begin(A, w.q, w.x.r0, w.x.rows, w.head);
             attend(A, S, R, w.q, w.x, w.s, w.head, w.first() + wave, w.last(), ATTN_WAVES);
             __syncthreads();
@@ -963,7 +967,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void fp8_attention_rows_kernel(
         // this wave's rows; a wave without any takes the first one's, and stores nothing
         const int rows = w.x.rows - wave * OWN;
         const Tile x = get_tile(A, w.q, w.t * ATTN_WAVES + (rows > 0 ? wave : 0), OWN);
-        AttnRows<DIM, BF16, RB> R;
+        AttnRows<DIM, BF16, RB, !BF16> R;
         R.begin(A, w.q, x.r0, x.rows, w.head);
         const Pages P(C, w.q, w.s);
         bool nans = false;

@@ -1,0 +1,47 @@
+"""Borders of the 8-bit cache and the attention over it on the GPU, against 64-bit references."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from dsv4_carve_amd import ops
+from tests import layer8_ref as L8
+from tests.test_gpu_fp8 import gen_of
+from tests.test_gpu_layer8 import problem
+
+pytestmark = pytest.mark.gpu
+
+
+def rounded_from(got, ref, tol):
+    """got is what some value within tol of ref rounds to; 2^-22 of ref for fp32 on the way to a bf16 bound."""
+    tol = tol + ref.abs() * 2.0 ** -22
+    lo, hi = (ref - tol).to(got.dtype).double(), (ref + tol).to(got.dtype).double()
+    off = int(((got.double() < lo) | (got.double() > hi)).sum())
+    assert off == 0, f"{off} of {got.numel()} values are rounded from elsewhere"
+
+
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("count", [1, 5])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_few_rows_keep_the_weights_bits(dev, dim, count, dtype):
+    """A result of few rows is the fp32 one rounded.
+
+    One channel of the query is not zero and is 1/4 at most, keys are 3.5 at most: the bound of an fp32 query counts
+    dim + 2 steps of 2^-23 of the product and 6 more, twice, for a weight's logit, 1.1e-4 for 256 channels at most, and
+    the sums' 60 steps: 2^-13.  An 11-bit weight is off by up to 2^-12, so that with 64 channels, where the bound is
+    2^-14.6, some results of bf16 would be rounded from outside it."""
+    gen = gen_of(dev, dim + count)
+    counts = [count] * 48
+    lengths = [count + 1 + i % 15 for i in range(48)]
+    q, cache, table, n, starts = problem(gen, counts, lengths, heads=8, kv=2, dim=dim, page=16, dtype=dtype, octaves=0)
+    q[..., 1:] = 0
+    q.clamp_(-0.25, 0.25)
+    out = ops.fp8_attention(q, cache, table, n, starts, scale=1.0)
+    ref, tol, *_ = L8.attention(q.float(), cache, table, n, starts, scale=1.0)
+    if dim > 128 and count > 1 and dtype == torch.bfloat16:
+        # 20 rows of a wide head go through the kernel for many rows, whose weights have 11 bits for a bf16 result: each
+        # is off by up to 2^-12 of itself, so the result by that of its weighted magnitudes, which are the largest value's
+        # at most
+        tol = tol + 2.0 ** -12 * 448 * float(cache.v_scale.max())
+    rounded_from(out, ref, tol + 2.0 ** -25 * (dtype == torch.float16))
