@@ -37,7 +37,7 @@ struct AttnArgs {
     int tiles;                                // tiles at most
     int least;                                // units that a workgroup has at least
     int most;                                 // workgroups that the units are divided over at most
-    bool clear;                               // rows that no sequence has are zeroed
+    int clear;                                // rows that no sequence has: 1: zeros, and -inf for the logarithm; 2: this alone
 };
 
 // Rows of a tile: ROWS neighbouring (query, head of the group) pairs of one sequence and cache head.
@@ -566,7 +566,7 @@ __device__ __forceinline__ float finish_row(const AttnArgs& A, int head, float m
     return l == 0.f ? 0.f : f / l;
 }
 
-// Rows of q whose tokens no sequence has: zeros, and -inf for the logarithm.
+// Rows of q whose tokens no sequence has, by A.clear.
 __device__ __forceinline__ void clear_rows(const AttnArgs& A) {
     const CacheView& C = A.c;
     if (!A.clear || !C.starts) return;
@@ -581,8 +581,9 @@ __device__ __forceinline__ void clear_rows(const AttnArgs& A) {
     const int64_t each = (int64_t)A.heads * C.dim / 8;
     for (int i = blockIdx.x; i < rows; i += gridDim.x) {
         const int64_t t = i < a ? i : i + (b - a);
-        for (int64_t j = threadIdx.x; j < each; j += blockDim.x)
-            reinterpret_cast<u32x4_t*>(A.out + t * A.heads * C.dim)[j] = u32x4_t{0, 0, 0, 0};
+        if (A.clear == 1)
+            for (int64_t j = threadIdx.x; j < each; j += blockDim.x)
+                reinterpret_cast<u32x4_t*>(A.out + t * A.heads * C.dim)[j] = u32x4_t{0, 0, 0, 0};
         if (A.lse)
             for (int j = threadIdx.x; j < A.heads; j += blockDim.x) A.lse[t * A.heads + j] = -__builtin_inff();
     }

@@ -170,7 +170,7 @@ int exl3_fp8_attention(const void* q, int kind, int64_t q_token, int64_t q_head,
                static_cast<const uint16_t*>(q), q_token, q_head, (int)heads, (int)(heads / kv_heads),
                std::fabs(scale) * 1.4426950408889634f, scale < 0.f, (int)window, sinks, static_cast<uint16_t*>(out), lse,
                P.shares ? static_cast<float*>(scratch) : nullptr,
-               reinterpret_cast<SharedTile*>(static_cast<char*>(scratch) + part_bytes(P, dim)), (int)P.tiles, P.least, P.most, clear != 0};
+               reinterpret_cast<SharedTile*>(static_cast<char*>(scratch) + part_bytes(P, dim)), (int)P.tiles, P.least, P.most, clear == 2 ? 2 : clear != 0};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const bool bf16 = kind == OUT_BF16;
     if (dim <= 64) return launch_attention_64(A, P, bf16, s);

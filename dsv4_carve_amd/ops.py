@@ -1011,7 +1011,7 @@ _LIB.define("fp8_cache_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!)
             "Tensor(d!) v_scale, Tensor table, Tensor lengths, Tensor? starts) -> ()")
 _LIB.define("fp8_attention(Tensor q, Tensor k_cache, Tensor k_scale, Tensor v_cache, Tensor v_scale, Tensor table, "
             "Tensor lengths, Tensor? starts, float scale, int window, Tensor? sinks, Tensor(a!) out, Tensor(b!)? lse, "
-            "bool clear, Tensor(c!)? scratch) -> ()")
+            "int clear, Tensor(c!)? scratch) -> ()")
 
 
 def _fp8_norm_impl(x, residual, weight, eps, pow2, q, scale, total, normed):
@@ -1189,8 +1189,8 @@ def fp8_attention(q: torch.Tensor, cache: Fp8Cache, table: torch.Tensor, lengths
     denominator, fp32 [tokens, heads].  A query that sees no key has 0 (and -inf, or
     its sink); a key that it does not see has no part in its result, whatever the
     cache holds there.  Tokens outside every sequence are left as they were in an
-    `out` given, and are 0 otherwise.  Scratch is the call's own (stream-ordered,
-    capturable)."""
+    `out` given, and are 0 otherwise; their logarithm is -inf.  Scratch is the call's
+    own (stream-ordered, capturable)."""
     _check(q.dim() == 3 and q.dtype in X_KIND, "q must be fp16 or bf16 [tokens, heads, dim]")
     tokens, heads, dim = q.shape
     _check_cache(cache, table, lengths, starts, tokens, q.device)
@@ -1203,8 +1203,8 @@ def fp8_attention(q: torch.Tensor, cache: Fp8Cache, table: torch.Tensor, lengths
     if sinks is not None:
         _check(sinks.dtype == torch.float32 and sinks.is_contiguous() and sinks.device == q.device and
                tuple(sinks.shape) == (heads,), "sinks must be contiguous fp32 [heads] on q's device")
-    clear = out is None
-    if clear:
+    clear = 1 if out is None else 2 if return_lse else 0       # what is the call's own has no rows left as they were
+    if out is None:
         out = q.new_empty((tokens, heads, dim))
     else:
         _check(out.dtype == q.dtype and out.device == q.device and out.is_contiguous() and out.shape == q.shape,
@@ -1218,8 +1218,9 @@ def fp8_attention(q: torch.Tensor, cache: Fp8Cache, table: torch.Tensor, lengths
             scratch = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         torch.ops.exl3_amd.fp8_attention(_token_rows(q), *cache, table, lengths, starts, scale, window or 0, sinks, out, lse,
                                          clear, scratch)
-    elif clear:
-        out.zero_()
+    else:
+        if clear == 1:
+            out.zero_()
         if lse is not None:
             lse.fill_(float("-inf"))
     return (out, lse) if return_lse else out

@@ -412,7 +412,7 @@ int exl3_fp8_cache_append(const void* k, int64_t k_token, int64_t k_head, const 
  * fp32 [tokens][heads] or null: the logarithm of the denominator.  A query that sees
  * nothing has out 0 and lse -inf (its sink, where there is one).  A key that a query
  * does not see has no part in its result, whatever its bytes.  Tokens outside every
- * sequence are left as they were; with `clear` they become 0 and -inf.
+ * sequence are left as they were (clear 0), become 0 and -inf (1), or only their lse -inf (2).
  * scratch: >= exl3_fp8_attention_scratch_bytes(...) bytes, asked for with the call's
  * device current, 16-byte aligned, no zeroing needed (may be null where the size is
  * 0); one call at a time per buffer.

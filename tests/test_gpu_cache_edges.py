@@ -45,3 +45,27 @@ def test_attention_few_rows_keep_the_weights_bits(dev, dim, count, dtype):
         # at most
         tol = tol + 2.0 ** -12 * 448 * float(cache.v_scale.max())
     rounded_from(out, ref, tol + 2.0 ** -25 * (dtype == torch.float16))
+
+
+@pytest.mark.parametrize("counts,heads,kv,dim", [([1, 1, 1], 4, 2, 64), ([40, 7], 8, 1, 128), ([300, 1], 4, 4, 256)])
+def test_attention_logarithms_of_rows_that_no_sequence_has(dev, counts, heads, kv, dim):
+    """With an `out` given, whose rows stay, the logarithms are the call's own: -inf before, behind and without sequences."""
+    gen = gen_of(dev, dim)
+    q, cache, table, n, starts = problem(gen, [5, *counts, 9], [5, *(c + 60 for c in counts), 9], heads=heads, kv=kv, dim=dim,
+                                         page=16)
+    table, n, starts = table[1:-1], n[1:-1].contiguous(), starts[1:-1].contiguous()
+    mine = slice(5, 5 + sum(counts))
+    want, want_lse = ops.fp8_attention(q, cache, table, n, starts, return_lse=True)
+    none = torch.ones(q.shape[0], dtype=torch.bool, device=dev)
+    none[mine] = False
+    assert (want[none] == 0).all() and (want_lse[none] == -torch.inf).all()
+    for given in (starts, torch.zeros_like(starts)):
+        for _ in range(3):
+            out = torch.full_like(q, 7.0)
+            torch.full((q.shape[0], heads), 3.0, device=dev)          # what the logarithms' place held before
+            got, lse = ops.fp8_attention(q, cache, table, n, given, out=out, return_lse=True)
+            assert got is out
+            left = none if given is starts else torch.ones_like(none)
+            assert (out[left] == 7.0).all() and (lse[left] == -torch.inf).all()
+            assert torch.equal(out[~left], want[~left]) and torch.equal(lse[~left], want_lse[~left])
+            assert torch.equal(ops.fp8_attention(q, cache, table, n, given, out=torch.full_like(q, 7.0)), out)
