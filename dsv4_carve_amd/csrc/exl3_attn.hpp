@@ -53,7 +53,7 @@ __device__ __forceinline__ Tile get_tile(const AttnArgs& A, const Seq& q, int t,
     x.rows = min(ROWS, q.n * A.group - x.r0);
     const int base = q.len - q.n;
     const int qa = x.r0 / A.group, qb = (x.r0 + x.rows - 1) / A.group;
-    x.hi = min(max(base + qb + 1, 0), q.len);
+    x.hi = min(max(base + qb + 1, 0), q.end);
     x.full_hi = max(base + qa + 1, 0);
     x.lo = x.full_lo = 0;
     if (A.window) {
@@ -143,7 +143,7 @@ struct AttnRows {
                     for (int i = 0; i < 4; ++i) v[i] = is ? A.negative ? z[i] ^ 0x80008000u : z[i] : 0u;
                     qf[rb][k][u] = __builtin_bit_cast(typename H::vec8, v);
                 }
-            see_hi[rb] = in ? min(base + at + 1, q.len) : 0;
+            see_hi[rb] = in ? min(base + at + 1, q.end) : 0;
             see_lo[rb] = in && A.window ? base + at + 1 - A.window : 0;
             m[rb] = top[rb] = ATTN_LOW;
             c[rb] = l[rb] = 0.f;
@@ -371,7 +371,7 @@ struct Pages {
     int pages;
 
     __device__ __forceinline__ Pages(const CacheView& C, const Seq& q, int s)
-        : table(C.table + s * C.table_stride), pages((q.len + (1 << C.page_shift) - 1) >> C.page_shift) {}
+        : table(C.table + s * C.table_stride), pages((q.end + (1 << C.page_shift) - 1) >> C.page_shift) {}
 
     // The page of the 16 keys from 64 b + 16 (lane / 16) on, -1 behind the sequence's end; raw: as the table has it.
     __device__ __forceinline__ int index(const CacheView& C, int b) const { return (b * ATTN_KEYS + (threadIdx.x & 48)) >> C.page_shift; }

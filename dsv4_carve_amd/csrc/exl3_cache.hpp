@@ -26,19 +26,20 @@ struct CacheView {
     int seqs, tokens, kv, dim, page_shift, width, pages;
 };
 
-// A sequence's tokens in a call and its length.  What a table, a length or a start
-// names past its range is cut to it: no index leaves a buffer.  A start that is less
-// than one before it counts as the largest before it: no token has two sequences.
+// A sequence's tokens in a call, its length and how many of its keys have room.  A token
+// keeps its position where the length is past the table's row: those behind the room have
+// no place, and do not take that of others.  No index leaves a buffer: pages follow from
+// `end`, and starts are cut to the call's tokens.  A start that is less than one before it
+// counts as the largest before it: no token has two sequences.
 struct Seq {
-    int first, n, len;
+    int first, n, len, end;
 };
 
 __device__ __forceinline__ int get_start(const CacheView& C, int s) { return min(max(C.starts[s], 0), C.tokens); }
 
-__device__ __forceinline__ int get_length(const CacheView& C, int s) {
-    const int64_t room = (int64_t)C.width << C.page_shift;
-    const int len = max(C.lengths[s], 0);
-    return (int64_t)len < room ? len : (int)room;
+__device__ __forceinline__ void get_length(const CacheView& C, int s, Seq& q) {
+    q.len = max(C.lengths[s], 0);
+    q.end = min(q.len, C.width << C.page_shift);                // the room is below 2^31
 }
 
 // before: the largest start before sequence s
@@ -51,7 +52,7 @@ __device__ __forceinline__ Seq get_seq(const CacheView& C, int s, int before) {
         q.first = s;
         q.n = 1;
     }
-    q.len = get_length(C, s);
+    get_length(C, s, q);
     return q;
 }
 
@@ -92,7 +93,7 @@ __device__ __forceinline__ Seq lane_seq(const CacheView& C, int s0, int& before)
         first = max(before, wave_max_scan(s < C.seqs ? get_start(C, s) : 0));
         before = read_lane(first, 63);
     }
-    return s < C.seqs ? get_seq(C, s, first) : Seq{0, 0, 0};
+    return s < C.seqs ? get_seq(C, s, first) : Seq{0, 0, 0, 0};
 }
 
 // a / b, 0 <= a, 0 < b; in 32 bits where both fit, and else bit by bit: a short call
@@ -125,7 +126,7 @@ struct Found {
 
 template <typename Count, typename At>
 __device__ __forceinline__ Found find_seq(const CacheView& C, Count&& count, At&& at) {
-    Found f{-1, 0, Seq{0, 0, 0}};
+    Found f{-1, 0, Seq{0, 0, 0, 0}};
     const auto look = [&](int s0, const Seq& q, int64_t c, int64_t before, int64_t sum, int64_t want) {
         before += sum - c;
         const uint64_t hit = __builtin_amdgcn_ballot_w64(want >= before && want < before + c);
@@ -133,7 +134,7 @@ __device__ __forceinline__ Found find_seq(const CacheView& C, Count&& count, At&
         const int l = __builtin_ctzll(hit);
         f.s = s0 + l;
         f.unit = want - read_lane(before, l);
-        f.q = Seq{read_lane(q.first, l), read_lane(q.n, l), read_lane(q.len, l)};
+        f.q = Seq{read_lane(q.first, l), read_lane(q.n, l), read_lane(q.len, l), read_lane(q.end, l)};
     };
     if (C.seqs == 1) {
         f.q = get_seq(C, 0, 0);
@@ -195,7 +196,7 @@ __device__ __forceinline__ Found find_seq(const CacheView& C, Count&& count, At&
 // workgroups: 195 -> 123 us).
 template <typename Before>
 __device__ __forceinline__ Found find_slot(const CacheView& C, int64_t x, Before&& before) {
-    Found f{-1, 0, Seq{0, 0, 0}};
+    Found f{-1, 0, Seq{0, 0, 0, 0}};
     const int lane = threadIdx.x & 63;
     int start = 0;
     for (int s0 = 0; s0 < C.seqs; s0 += 64) {
@@ -214,7 +215,7 @@ __device__ __forceinline__ Found find_slot(const CacheView& C, int64_t x, Before
         f.unit = x - read_lane(lo, l);
         f.q.first = read_lane(first, l);
         f.q.n = read_lane(end, l) - f.q.first;
-        f.q.len = get_length(C, f.s);
+        get_length(C, f.s, f.q);
         break;
     }
     return f;
@@ -234,7 +235,7 @@ struct AppendArgs {
 // The pages that a sequence's new tokens lie in.
 __device__ __forceinline__ int touched_pages(const CacheView& C, const Seq& q) {
     const int from = max(q.len - q.n, 0);
-    return q.len > from ? ((q.len - 1) >> C.page_shift) - (from >> C.page_shift) + 1 : 0;
+    return q.end > from ? ((q.end - 1) >> C.page_shift) - (from >> C.page_shift) + 1 : 0;
 }
 
 // Eight neighbouring values (16-byte aligned), as they are in memory.
@@ -311,11 +312,11 @@ __global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(App
         q = get_seq(C, s, 0);
     }
     const int page = 1 << C.page_shift, base = q.len - q.n, from = max(base, 0);
-    if (q.len <= from) return;
+    if (q.end <= from) return;
     const int at = (from >> C.page_shift) + nth;                                  // the page's place in the sequence
     const int id = C.table[s * C.table_stride + at];
     if ((unsigned)id >= (unsigned)C.pages) return;
-    const int lo = max(from - (at << C.page_shift), 0), hi = min(q.len - (at << C.page_shift), page);
+    const int lo = max(from - (at << C.page_shift), 0), hi = min(q.end - (at << C.page_shift), page);
     const int64_t token = q.first + (at << C.page_shift) - base;                  // the token of the page's place 0
     const int64_t stride = values ? A.v_token : A.k_token;
     const int64_t in0 = token * stride + head * (values ? A.v_head : A.k_head);

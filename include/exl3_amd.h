@@ -384,9 +384,11 @@ int exl3_fp8_norm(const void* x, int x_kind, const void* residual, int residual_
  * [seqs][table_stride], width columns); lengths int32 [seqs] count its tokens, those
  * of the call included.  starts int32 [seqs + 1]: sequence s has the call's tokens
  * starts[s] .. starts[s + 1] - 1, which are its last ones; null for one token each
- * (tokens == seqs).  All four are read on the device: a length past the table's row
- * counts as the row's room, a page outside the cache is left out, starts are cut to
- * 0..tokens, and one less than a start before it counts as the largest before it.
+ * (tokens == seqs).  All four are read on the device: where a length is past the
+ * table's row, positions stay as they are and those behind the row's room have no key
+ * or value (nothing is written for them, no query sees them); a page outside the cache
+ * is left out, starts are cut to 0..tokens, and one less than a start before it counts
+ * as the largest before it.
  *
  * exl3_fp8_cache_append writes the call's keys and values (strides in values, rows
  * 16-byte aligned; kind 0 = fp16, 1 = bf16, 2 = fp32).  A page's scale becomes the

@@ -39,7 +39,7 @@ def norm(x, weight, residual, eps, pow2):
 
 
 def sequences(table, lengths, starts, tokens, page):
-    """(first token, new tokens, length) of each sequence, out-of-range values cut as documented."""
+    """(first token, new tokens, length, keys that have room) of each sequence, out-of-range values cut as documented."""
     room = table.shape[1] * page
     out = []
     largest = 0                                            # starts that decrease count as the largest before them
@@ -49,7 +49,7 @@ def sequences(table, lengths, starts, tokens, page):
         else:
             first = largest = max(largest, min(max(int(starts[s]), 0), tokens))
             n = max(min(int(starts[s + 1]), tokens) - first, 0)
-        out.append((first, n, min(max(length, 0), room)))
+        out.append((first, n, max(length, 0), min(max(length, 0), room)))
     return out
 
 
@@ -57,11 +57,11 @@ def append(k, v, cache, table, lengths, starts):
     """The four tensors after the write, in 64 bits; NaN codes are NaN."""
     out = [t.double().clone() for t in cache]
     pages, heads, page, dim = cache[0].shape
-    for s, (first, n, length) in enumerate(sequences(table, lengths, starts, k.shape[0], page)):
+    for s, (first, n, length, end) in enumerate(sequences(table, lengths, starts, k.shape[0], page)):
         at = max(length - n, 0)
-        while at < length:
+        while at < end:
             place, lo = divmod(at, page)
-            hi = min(length - place * page, page)
+            hi = min(end - place * page, page)
             p = int(table[s, place])
             if 0 <= p < pages:
                 token = first + at - (length - n)
@@ -96,29 +96,29 @@ def attention(q, cache, table, lengths, starts=None, *, scale=None, window=None,
     tol, lse = torch.zeros_like(out), torch.full((tokens, heads), -torch.inf, dtype=torch.float64, device=q.device)
     lse_tol, mine = torch.zeros_like(lse), torch.zeros(tokens, dtype=torch.bool, device=q.device)
     weight_eps = 2.0 ** -11 if q.dtype == torch.bfloat16 else 2.0 ** -21
-    for s, (first, n, length) in enumerate(sequences(table, lengths, starts, tokens, page)):
+    for s, (first, n, length, end) in enumerate(sequences(table, lengths, starts, tokens, page)):
         mine[first:first + n] = True
         if not n:
             continue
-        ids = table[s, :-(-length // page)].long()
-        there = ((ids >= 0) & (ids < pages)).repeat_interleave(page)[:length]
+        ids = table[s, :-(-end // page)].long()
+        there = ((ids >= 0) & (ids < pages)).repeat_interleave(page)[:end]
         ids = ids.clamp(0, pages - 1)
         i = torch.arange(length - n, length, device=q.device).view(-1, 1)
-        j = torch.arange(length, device=q.device)
+        j = torch.arange(end, device=q.device)
         seen = (j <= i) & there
         if window:
             seen &= j > i - window
         for h in range(heads):
             c = h // group
             kd = (cache[0].view(torch.uint8)[ids, c].view(E4M3).double() * cache[1][ids, c].double()[:, None, None])
-            vs = cache[3][ids, c].double().repeat_interleave(page)[:length]
-            vd = cache[2].view(torch.uint8)[ids, c].view(E4M3).double().transpose(1, 2).reshape(-1, dim)[:length]
+            vs = cache[3][ids, c].double().repeat_interleave(page)[:end]
+            vd = cache[2].view(torch.uint8)[ids, c].view(E4M3).double().transpose(1, 2).reshape(-1, dim)[:end]
             vd = vd * vs[:, None]
-            kd = kd.reshape(-1, dim)[:length]
+            kd = kd.reshape(-1, dim)[:end]
             x = q[first:first + n, h].double()
             logit = torch.where(seen, (x @ kd.t()) * scale, -torch.inf)
             size = torch.where(seen, (x.abs() @ kd.abs().t()) * abs(scale), 0.0)
-            most = logit.amax(1, keepdim=True) if length else torch.full((n, 1), -torch.inf, device=q.device).double()
+            most = logit.amax(1, keepdim=True) if end else torch.full((n, 1), -torch.inf, device=q.device).double()
             if sinks is not None:
                 most = torch.maximum(most, sinks[h].double())
             safe = torch.where(most == -torch.inf, 0.0, most)
@@ -132,17 +132,17 @@ def attention(q, cache, table, lengths, starts=None, *, scale=None, window=None,
                 o, absolute = terms.sum(1), terms.abs().sum(1)
             else:
                 o, absolute = w @ vd, w @ vd.abs()
-            off = ((dim + 2) * U * size.amax(1, keepdim=True) if length else 0.0) + 4 * U * safe.abs() + 6 * U
+            off = ((dim + 2) * U * size.amax(1, keepdim=True) if end else 0.0) + 4 * U * safe.abs() + 6 * U
             if sinks is not None:
                 off = off + 4 * U * sinks[h].double().abs()
-            eps = 2 * off + weight_eps + (length + 40) * U
-            cut = 448 * 2.0 ** -31 * length * ((w * vs).amax(1, keepdim=True) if length else 0.0)
+            eps = 2 * off + weight_eps + (end + 40) * U
+            cut = 448 * 2.0 ** -31 * end * ((w * vs).amax(1, keepdim=True) if end else 0.0)
             at = slice(first, first + n)
             out[at, h] = o / some
             tol[at, h] = (absolute * eps + cut) / some + out[at, h].abs() * half_step(q.dtype) + 2.0 ** -24 * (
                 q.dtype == torch.float16)
             lse[at, h] = (safe + torch.log(total))[:, 0]
-            lse_tol[at, h] = (off + (length + 40) * U + 4 * U * lse[at, h:h + 1].nan_to_num(0.0, neginf=0.0).abs())[:, 0]
+            lse_tol[at, h] = (off + (end + 40) * U + 4 * U * lse[at, h:h + 1].nan_to_num(0.0, neginf=0.0).abs())[:, 0]
     return out, tol, lse, lse_tol, mine
 
 

@@ -7,8 +7,8 @@ import torch
 
 from dsv4_carve_amd import ops
 from tests import layer8_ref as L8
-from tests.test_gpu_fp8 import gen_of
-from tests.test_gpu_layer8 import problem
+from tests.test_gpu_fp8 import gen_of, normal
+from tests.test_gpu_layer8 import cache_on, check_append, check_attention, lengths_of, problem, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +69,34 @@ def test_attention_logarithms_of_rows_that_no_sequence_has(dev, counts, heads, k
             assert (out[left] == 7.0).all() and (lse[left] == -torch.inf).all()
             assert torch.equal(out[~left], want[~left]) and torch.equal(lse[~left], want_lse[~left])
             assert torch.equal(ops.fp8_attention(q, cache, table, n, given, out=torch.full_like(q, 7.0)), out)
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [20, 70, 3], [1] * 70, [300, 2]])
+def test_lengths_past_the_tables_room(dev, page, counts):
+    """Tokens behind the room have no place: nothing is written for them, and they do not take the place of others."""
+    gen = gen_of(dev, page)
+    seqs, room, kv, dim = len(counts), 3 * page, 2, 64
+    table = torch.randperm(3 * seqs, generator=gen, device=dev).to(torch.int32).view(seqs, 3)
+    starts = None if max(counts) == 1 else starts_of(dev, counts)
+    k, v = normal(gen, sum(counts), kv, dim), normal(gen, sum(counts), kv, dim)
+    q = normal(gen, sum(counts), 4, dim, spread=False)
+    # all new tokens behind the room, the first of them its last place, some of them in it, none
+    for at, past in enumerate((lambda n: room + n, lambda n: room + n - 1, lambda n: room + n // 2, lambda n: room)):
+        lengths = lengths_of(dev, [past(n) for n in counts])
+        cache = cache_on(gen, 3 * seqs, kv, page, dim)
+        before = [t.clone() for t in cache]
+        check_append(k, v, cache, table, lengths, starts)
+        live = [(s, j) for s, n in enumerate(counts) for j in range(min(past(n) - n, room))]     # keys from before the call
+        ids = torch.tensor([int(table[s, j // page]) for s, j in live], device=dev)
+        slot = torch.tensor([j % page for _, j in live], device=dev)
+        full = ids[slot == page - 1]
+        for was, now in zip(before, cache):
+            assert torch.equal(now.view(torch.uint8)[full], was.view(torch.uint8)[full])
+        if at == 0:
+            assert all(torch.equal(now.view(torch.uint8), was.view(torch.uint8)) for was, now in zip(before, cache))
+        for window in (None, 5, page):
+            check_attention(q, cache, table, lengths, starts, window=window)
+    lengths = lengths_of(dev, [2 ** 31 - 1] * seqs)
+    check_append(k, v, cache, table, lengths, starts)
+    check_attention(q, cache, table, lengths, starts)
