@@ -7,6 +7,9 @@
 
 using namespace exl3;
 
+// Keys that a table's row may name: a block of them, or the next ones that a wave asks for, still ends below 2^31.
+constexpr int64_t MAX_ROOM = INT32_MAX - 1023;
+
 static int check_cache(const void* k, const void* k_scale, const void* v, const void* v_scale, int64_t pages, int64_t kv_heads,
                        int64_t page_size, int64_t dim, const void* table, int64_t width, const void* lengths,
                        const void* starts, int64_t seqs, int64_t tokens) {
@@ -16,7 +19,7 @@ static int check_cache(const void* k, const void* k_scale, const void* v, const 
     if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
         return fail("page_size must be 16, 32, 64, 128 or 256");
     if (dim < 16 || dim > 256 || dim % 16) return fail("dim must be a multiple of 16 in 16..256");
-    if (width < 1 || width > INT32_MAX / page_size) return fail("a table's row must have 1..(2^31-1)/page_size pages");
+    if (width < 1 || width > MAX_ROOM / page_size) return fail("a table's row must have 1..(2^31-1024)/page_size pages");
     if (seqs < 1 || seqs > (1 << 20)) return fail("seqs must be in 1..2^20");
     if (tokens < 1 || tokens > (1 << 22)) return fail("tokens must be in 1..2^22");
     if (!starts && tokens != seqs) return fail("without starts there is one token for each sequence");
@@ -136,7 +139,7 @@ int64_t exl3_fp8_attention_scratch_bytes(int64_t tokens, int64_t heads, int64_t 
     clear_error();
     if (tokens < 1 || tokens > (1 << 22) || seqs < 1 || seqs > (1 << 20) || kv_heads < 1 || heads < kv_heads ||
         heads % kv_heads || heads > 65536 || dim < 16 || dim > 256 || dim % 16 || page_size < 16 || page_size > 256 ||
-        width < 1 || width > INT32_MAX / page_size || window < 0)
+        width < 1 || width > MAX_ROOM / page_size || window < 0)
         return fail("sizes out of range");
     return attention_scratch(plan_attention(tokens, heads, kv_heads, dim, seqs, keys_of(width, page_size, tokens, window)), dim);
 }

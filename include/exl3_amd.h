@@ -381,7 +381,7 @@ int exl3_fp8_norm(const void* x, int x_kind, const void* residual, int residual_
  *   v [pages][kv_heads][dim][page_size]   v_scale [pages][kv_heads]
  * k and v 16-byte aligned; page_size 16, 32, 64, 128 or 256, dim a multiple of 16 up
  * to 256.  A sequence's pages are the first ones of its row of `table` (int32
- * [seqs][table_stride], width columns); lengths int32 [seqs] count its tokens, those
+ * [seqs][table_stride], width columns, width * page_size <= 2^31 - 1024); lengths int32 [seqs] count its tokens, those
  * of the call included.  starts int32 [seqs + 1]: sequence s has the call's tokens
  * starts[s] .. starts[s + 1] - 1, which are its last ones; null for one token each
  * (tokens == seqs).  All four are read on the device: where a length is past the

@@ -5,8 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from dsv4_carve_amd import ops
-from tests.test_layer8 import args, i32, z
+from dsv4_carve_amd import _lib, ops
+from tests.test_layer8 import CACHE, P, args, cache_of, i32, refused, z
 
 
 @pytest.mark.parametrize("given", [False, True])
@@ -22,3 +22,15 @@ def test_attention_without_sequences_fills_the_logarithms(given, tokens):
         torch.use_deterministic_algorithms(False)
     assert lse.shape == (tokens, 4) and (lse == -torch.inf).all()
     assert (made == (7.0 if given else 0.0)).all() and (not given or made is out)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+def test_a_tables_room_ends_before_the_kernels_32_bit_places_do(page):
+    """Blocks of 64 keys, and those that a wave asks for ahead (up to 8 blocks), are counted in 32 bits."""
+    L, most = _lib.load(), ((1 << 31) - 1024) // page
+    assert most * page + 64 * 9 < 1 << 31
+    assert L.exl3_fp8_attention_scratch_bytes(3, 4, 2, 64, 3, most, page, 0) > 0
+    refused(L.exl3_fp8_attention_scratch_bytes(3, 4, 2, 64, 3, most + 1, page, 0), "out of range")
+    a = {**CACHE, "page": page, "width": most + 1}
+    refused(L.exl3_fp8_cache_append(P, 128, 64, P, 128, 64, 1, 3, *cache_of(a), None), "2^31-1024")
+    refused(L.exl3_fp8_attention(P, 1, 256, 64, 3, 4, *cache_of(a), 1.0, 0, None, P, None, 0, P, 1 << 40, None), "2^31-1024")
