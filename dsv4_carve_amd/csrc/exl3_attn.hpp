@@ -92,6 +92,11 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t u) {       // 0x80 in eac
     return ((u & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
 
+// A page's scale that is NaN, infinite or negative: what sees the page is NaN.
+__device__ __forceinline__ bool bad_scale(float s) {
+    return __builtin_amdgcn_classf(s, 0x3 | 0x4 | 0x8 | 0x10 | 0x200);     // NaNs, -infinity, -normal, -subnormal, infinity
+}
+
 // One wave's rows against blocks of 64 keys.  The products are transposed: keys are
 // the rows of S^T = K Q^T, so that a lane has logits of one row only (row lane % 16 of
 // each 16), and lane group g = lane / 16 has keys 16 g .. 16 g + 15 of the block: key
@@ -167,8 +172,9 @@ struct AttnRows {
 
     // A block of keys, key0 = its first plus 16 (lane / 16).  key(t, k): 16 bytes of key 16 (lane % 16 / 4) + 4 t + lane % 4
     // from channel 64 k + 16 (lane / 16) on; value(d): 16 tokens, from key0 on, of channel 16 d + lane % 16.  ks, vs: the
-    // scales of the lane's 16 keys.  masked: not every row sees it whole; the lane's keys are in a page (`here`) and the rows
-    // see [lo, hi) at most.  Returns whether a value that some rows see is a NaN: it is left out (counted by add_nans).
+    // scales of the lane's 16 keys.  masked: not every row sees it whole, or a scale is none; the lane's keys are in a page
+    // (`here`) and the rows see [lo, hi) at most.  Returns whether a value that some rows see is a NaN, by itself or by its
+    // scale: it is left out (counted by add_nans).
     template <typename K, typename V>
     __device__ __forceinline__ bool step(const AttnArgs& A, bool masked, float ks, float vs, bool here, int key0, int lo, int hi, K&& key,
                                          V&& value) {
@@ -203,11 +209,13 @@ struct AttnRows {
         }
         __builtin_amdgcn_s_setprio(0);
         float kc = fmaxf(ks * A.qk_scale, 0x1p-126f);
-        uint32_t keep[4] = {};
+        uint32_t keep[4] = {}, nan = 0;
         if (masked) {
             here = here && key0 + 15 >= lo && key0 < hi;
-            kc = here ? kc : 1.f;
-            vs = here ? vs : 1.f;
+            const float poison = bad_scale(ks) ? __builtin_nanf("") : 0.f;
+            kc = here && !bad_scale(ks) ? kc : 1.f;
+            nan = here && bad_scale(vs) ? 1u : 0u;
+            vs = here && !bad_scale(vs) ? vs : 1.f;
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 const int from = here ? see_lo[rb] - key0 : 16, n = see_hi[rb] - key0;
@@ -216,7 +224,7 @@ struct AttnRows {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int at = 4 * t + i;
-                        p[t][rb][i] = at >= from && at < n ? p[t][rb][i] : -__builtin_inff();
+                        p[t][rb][i] = at >= from && at < n ? p[t][rb][i] + poison : -__builtin_inff();
                     }
             }
             keep_bytes(keep, here, key0, lo, hi);
@@ -279,7 +287,6 @@ struct AttnRows {
             asm volatile("" : "+v"(l[rb]));                     // now: the weights would be kept until behind the products
             __builtin_amdgcn_sched_barrier(0);
         }
-        uint32_t nan = 0;
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int n = 0; n < DT / 2; ++n) {
@@ -318,9 +325,10 @@ struct AttnRows {
         return masked && __builtin_amdgcn_ballot_w64(nan != 0) != 0;
     }
 
-    // The NaN values of a masked block, counted for the rows that see them in products of their own.
+    // The NaN values of a masked block (all of the lane's, if their scale vs is none), counted for the rows that see them in
+    // products of their own.
     template <typename V>
-    __device__ __forceinline__ void add_nans(bool here, int key0, int lo, int hi, V&& value) {
+    __device__ __forceinline__ void add_nans(bool here, float vs, int key0, int lo, int hi, V&& value) {
         uint32_t keep[4];
         here = here && key0 + 15 >= lo && key0 < hi;
         keep_bytes(keep, here, key0, lo, hi);
@@ -336,7 +344,9 @@ struct AttnRows {
                 }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const u32x4_t z = value(d);
+                u32x4_t z = value(d);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) z[j] = bad_scale(vs) ? 0x7f7f7f7fu : z[j];
                 float4_t n = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
@@ -385,9 +395,10 @@ __device__ __forceinline__ float scale_of(const CacheView& C, const float* p, in
     return p[(int64_t)(valid_page(C, id) ? id : 0) * C.kv + head];
 }
 
-// Whether some row of a tile does not see a block whole.
-__device__ __forceinline__ bool masked_block(const CacheView& C, const Tile& x, int b, int id) {
-    return b * ATTN_KEYS < x.full_lo || (b + 1) * ATTN_KEYS > x.full_hi || __builtin_amdgcn_ballot_w64(valid_page(C, id)) != ~0ull;
+// Whether some row of a tile does not see a block whole, or a scale is none.
+__device__ __forceinline__ bool masked_block(const CacheView& C, const Tile& x, int b, int id, float ks, float vs) {
+    return b * ATTN_KEYS < x.full_lo || (b + 1) * ATTN_KEYS > x.full_hi ||
+           __builtin_amdgcn_ballot_w64(valid_page(C, id) && !bad_scale(ks) && !bad_scale(vs)) != ~0ull;
 }
 
 // Bytes of a page and head from `at` on, as a buffer that ends with the page; none where ids' lane group g names no
@@ -524,7 +535,7 @@ __device__ __forceinline__ void attend(const AttnArgs& A, const AttnStage<DIM>& 
         S.put_v(vreg);
         S.load_v(C, head, b + step, ids, more, vreg);
         // one step for both kinds of blocks: with one each, the compiler keeps the sums twice
-        const bool masked = uniform((int)masked_block(C, x, b, id)) != 0;
+        const bool masked = uniform((int)masked_block(C, x, b, id, ks_now, vs_now)) != 0;
         nans |= R.step(A, masked, ks_now, vs_now, !masked || valid_page(C, id), b * ATTN_KEYS + g16, x.lo, x.hi, key, value);
     }
     if (!nans) return;
@@ -532,7 +543,7 @@ __device__ __forceinline__ void attend(const AttnArgs& A, const AttnStage<DIM>& 
         const int id = P.of(C, b);
         S.load_v(C, head, b, id, true, vreg);
         S.put_v(vreg);
-        R.add_nans(valid_page(C, id), b * ATTN_KEYS + g16, x.lo, x.hi, value);
+        R.add_nans(valid_page(C, id), scale_of(C, C.v_scale, id, head), b * ATTN_KEYS + g16, x.lo, x.hi, value);
     }
 }
 
@@ -996,7 +1007,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void fp8_attention_rows_kernel(
                 vs = scale_of(C, C.v_scale, ids, w.head);
                 S.load(C, w.head, b + 1, ids, b + 1 < last, place ^ 1);
                 if (uniform((int)(rows <= 0 || b * ATTN_KEYS >= x.hi || (b + 1) * ATTN_KEYS <= x.lo))) return 0;
-                return uniform(masked_block(C, x, b, id) ? 2 : 1);
+                return uniform(masked_block(C, x, b, id, ks_now, vs_now) ? 2 : 1);
             };
             const auto key = [&](int t, int k) { return S.key(place, t, k); };
             const auto value = [&](int d) { return S.value(place, d); };
@@ -1019,7 +1030,8 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void fp8_attention_rows_kernel(
                     S.load(C, w.head, b, id, true, 0);
                     wait_loads();
                     bare_barrier();
-                    R.add_nans(valid_page(C, id), b * ATTN_KEYS + (lane & 48), x.lo, x.hi, [&](int d) { return S.value(0, d); });
+                    R.add_nans(valid_page(C, id), scale_of(C, C.v_scale, id, w.head), b * ATTN_KEYS + (lane & 48), x.lo, x.hi,
+                               [&](int d) { return S.value(0, d); });
                     wait_loads();
                     bare_barrier();
                 }

@@ -1188,7 +1188,8 @@ def fp8_attention(q: torch.Tensor, cache: Fp8Cache, table: torch.Tensor, lengths
     that joins each row's denominator.  With return_lse also the logarithm of the
     denominator, fp32 [tokens, heads].  A query that sees no key has 0 (and -inf, or
     its sink); a key that it does not see has no part in its result, whatever the
-    cache holds there.  Positions behind the table's room have no key.  Tokens outside every sequence are left as they were in an
+    cache holds there; a page that it sees and whose scale is NaN, infinite or negative
+    makes it NaN.  Positions behind the table's room have no key.  Tokens outside every sequence are left as they were in an
     `out` given, and are 0 otherwise; their logarithm is -inf.  Scratch is the call's
     own (stream-ordered, capturable)."""
     _check(q.dim() == 3 and q.dtype in X_KIND, "q must be fp16 or bf16 [tokens, heads, dim]")

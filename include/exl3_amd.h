@@ -413,7 +413,9 @@ int exl3_fp8_cache_append(const void* k, int64_t k_token, int64_t k_head, const 
  * [heads][dim] of the same kind, 16-byte aligned; sinks fp32 [heads] or null; lse
  * fp32 [tokens][heads] or null: the logarithm of the denominator.  A query that sees
  * nothing has out 0 and lse -inf (its sink, where there is one).  A key that a query
- * does not see has no part in its result, whatever its bytes.  Tokens outside every
+ * does not see has no part in its result, whatever its bytes.  A page whose scale is
+ * NaN, infinite or negative makes the rows that see a key of it NaN (the logarithms
+ * too, if it is the keys' scale).  Tokens outside every
  * sequence are left as they were (clear 0), become 0 and -inf (1), or only their lse -inf (2).
  * scratch: >= exl3_fp8_attention_scratch_bytes(...) bytes, asked for with the call's
  * device current, 16-byte aligned, no zeroing needed (may be null where the size is

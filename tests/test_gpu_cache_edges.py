@@ -7,7 +7,7 @@ import torch
 
 from dsv4_carve_amd import ops
 from tests import layer8_ref as L8
-from tests.test_gpu_fp8 import gen_of, normal
+from tests.test_gpu_fp8 import gen_of, normal, within
 from tests.test_gpu_layer8 import cache_on, check_append, check_attention, lengths_of, problem, starts_of
 
 pytestmark = pytest.mark.gpu
@@ -100,3 +100,38 @@ def test_lengths_past_the_tables_room(dev, page, counts):
     lengths = lengths_of(dev, [2 ** 31 - 1] * seqs)
     check_append(k, v, cache, table, lengths, starts)
     check_attention(q, cache, table, lengths, starts)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [1] * 70, [9, 4, 11], [300, 20]])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_scales_that_are_none(dev, dim, counts, dtype):
+    """A page whose scale is NaN, infinite or negative: the rows that see a key of it are NaN, and nobody else."""
+    gen = gen_of(dev, dim + len(counts))
+    heads, kv, page = 8, 2, 16
+    lengths = [c + 130 + 17 * (i % 3) for i, c in enumerate(counts)]
+    q, cache, table, n, starts = problem(gen, counts, lengths, heads=heads, kv=kv, dim=dim, page=page, dtype=dtype)
+    for case, bad in enumerate((torch.nan, torch.inf, -torch.inf, -0.5, -2.0 ** -130)):
+        for window in (None, 40):
+            ref, tol, ref_lse, lse_tol, _ = L8.attention(q, cache, table, n, starts, window=window)
+            s, c = case % len(counts), case % kv
+            place = (1, 3, (lengths[s] - 1) // page, max(lengths[s] - counts[s] - 20, 0) // page, 0)[case]
+            p = int(table[s, place])
+            position = torch.arange(lengths[s] - counts[s], lengths[s], device=dev)
+            sees = position >= place * page
+            if window:
+                sees &= position - window < (place + 1) * page - 1
+            hit = torch.zeros((sum(counts), heads), dtype=torch.bool, device=dev)
+            hit[int(starts[s]):int(starts[s + 1]), c * heads // kv:(c + 1) * heads // kv] = sees[:, None]
+            for scales in (cache.k_scale, cache.v_scale):
+                was = scales[p, c].clone()
+                scales[p, c] = bad
+                out, lse = ops.fp8_attention(q, cache, table, n, starts, window=window, return_lse=True)
+                scales[p, c] = was
+                assert out[hit].isnan().all()
+                within(out[~hit], ref[~hit], tol[~hit], "out")
+                if scales is cache.k_scale:
+                    assert lse[hit].isnan().all()
+                    within(lse[~hit], ref_lse[~hit], lse_tol[~hit], "lse")
+                else:
+                    within(lse, ref_lse, lse_tol, "lse")
