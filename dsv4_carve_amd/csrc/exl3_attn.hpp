@@ -5,6 +5,7 @@
 #pragma once
 
 #include "exl3_cache.hpp"
+#include "exl3_xcd.hpp"
 
 namespace exl3 {
 
@@ -600,32 +601,6 @@ __device__ __forceinline__ void clear_rows(const AttnArgs& A) {
     }
 }
 
-// Workgroups go to the XCDs in turn (workgroup b to XCD b % 8), and what one reads its
-// neighbours on the XCD find in L2: so an XCD's workgroups take neighbouring work.
-constexpr int XCDS = 8;
-
-// Workgroup b's place where each XCD's workgroups are next to each other.
-__device__ __forceinline__ int by_xcd(int b, int n) {
-    const int x = b % XCDS, each = n / XCDS, more = n % XCDS;
-    return x * each + min(x, more) + b / XCDS;
-}
-
-// A workgroup a tile: a head's tiles in turn on the XCDs that the head has, or an XCD's heads one after another.
-__device__ __forceinline__ void tile_by_xcd(int b, int tiles, int heads, int& tile, int& head) {
-    const int x = b % XCDS, i = b / XCDS;
-    if (heads < XCDS && XCDS % heads == 0) {
-        const int of = XCDS / heads;
-        head = x / of;
-        tile = i * of + x % of;
-    } else if (heads % XCDS == 0) {
-        head = x * (heads / XCDS) + i / tiles;
-        tile = i % tiles;
-    } else {
-        head = b / tiles;
-        tile = b % tiles;
-    }
-}
-
 // Units are (cache head, tile, block of keys), in this order; a workgroup has an
 // equal share of them, next to each other, whatever sequences they are of.  Where the
 // shares are hardly larger then, a share is of one tile: a second one costs a workgroup
@@ -720,8 +695,7 @@ struct Work {
             done = (int)left;
         } else {
             int tile;
-            tile_by_xcd(blockIdx.x, A.tiles, C.kv, tile, head);
-            if (tile >= A.tiles || head >= C.kv) return false;
+            if (!tile_by_xcd(blockIdx.x, A.tiles, C.kv, tile, head)) return false;
             const int64_t at = A.tiles - 1 - tile;
             if (C.starts) {
                 const Found f = find_slot(C, at, [&](int64_t token, int64_t i) { return token * A.group / ROWS + i; });

@@ -13,7 +13,7 @@ static int launch(void (*kernel)(AttnArgs), const AttnArgs& A, const AttnPlan& P
             return fail("the device does not give the kernel its LDS");
         ready.fetch_or(1ull << dev);
     }
-    const unsigned grid = P.shares ? P.shares : (P.tiles + XCDS - 1) / XCDS * XCDS * A.c.kv;
+    const unsigned grid = P.shares ? P.shares : tile_grid((int)P.tiles, A.c.kv);
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(ATTN_WAVES * 64), LDS, s, A);
     if (check_launch()) return -1;
     if (P.shares < 2) return 0;

@@ -35,6 +35,7 @@
 
 #include "exl3_gemv.hpp"
 #include "exl3_prefill.hpp"
+#include "exl3_xcd.hpp"
 
 using exl3::u32x4_t;
 
@@ -734,6 +735,16 @@ int exl3_probe_isa(int op, int blocks, int iters, uint32_t* sink, uint64_t* clk,
 }
 
 int exl3_probe_isa_ops(void) { return ISA_OPS; }
+
+// The work of workgroup b, on the host: its place among n where each XCD's workgroups
+// are next to each other, and the tile (tile * heads + head; -1: none) that it has of a
+// launch of exl3_probe_tile_grid workgroups, one a tile.
+int exl3_probe_by_xcd(int b, int n) { return exl3::by_xcd(b, n); }
+int exl3_probe_tile_grid(int tiles, int heads) { return (int)exl3::tile_grid(tiles, heads); }
+int exl3_probe_tile_by_xcd(int b, int tiles, int heads) {
+    int tile, head;
+    return exl3::tile_by_xcd(b, tiles, heads, tile, head) ? tile * heads + head : -1;
+}
 
 // Launches `blocks` single-wave workgroups of the row-block probe at `bits`
 // (2 or 3; MCG) for configuration `cfg` (0-7: (row blocks, column divisor) =

@@ -2,10 +2,12 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
-from dsv4_carve_amd import _lib, ops
+from dsv4_carve_amd import _lib, build, ops
 from tests.test_layer8 import CACHE, P, args, cache_of, i32, refused, z
 
 
@@ -34,3 +36,22 @@ def test_a_tables_room_ends_before_the_kernels_32_bit_places_do(page):
     a = {**CACHE, "page": page, "width": most + 1}
     refused(L.exl3_fp8_cache_append(P, 128, 64, P, 128, 64, 1, 3, *cache_of(a), None), "2^31-1024")
     refused(L.exl3_fp8_attention(P, 1, 256, 64, 3, 4, *cache_of(a), 1.0, 0, None, P, None, 0, P, 1 << 40, None), "2^31-1024")
+
+
+@pytest.mark.parametrize("heads", [1, 2, 3, 4, 5, 7, 8, 9, 16, 24, 32, 40, 128])
+def test_every_tile_has_one_workgroup(heads):
+    """A workgroup a tile: the launch's padding has no tile a second time, and none is left out."""
+    probe = ctypes.CDLL(build.PROBE_LIB)
+    for tiles in [*range(1, 42), 127, 128, 129, 300, 1025]:
+        grid = probe.exl3_probe_tile_grid(tiles, heads)
+        got = [probe.exl3_probe_tile_by_xcd(b, tiles, heads) for b in range(grid)]
+        assert sorted(t for t in got if t >= 0) == list(range(tiles * heads)), tiles
+
+
+def test_workgroups_of_an_xcd_are_neighbours():
+    probe = ctypes.CDLL(build.PROBE_LIB)
+    for n in [*range(1, 70), 511, 512, 513]:
+        assert sorted(probe.exl3_probe_by_xcd(b, n) for b in range(n)) == list(range(n))
+        for x in range(min(8, n)):
+            mine = [probe.exl3_probe_by_xcd(b, n) for b in range(x, n, 8)]
+            assert mine == list(range(mine[0], mine[0] + len(mine)))
