@@ -608,8 +608,8 @@ __device__ __forceinline__ void clear_rows(const AttnArgs& A) {
 // 24 sequences of 1 token: 25.8 -> 20.7).  A tile whose blocks one workgroup has all is
 // finished; of the others each workgroup leaves a partial result: in its first place
 // where the tile began before its share, in its second where it goes on behind it.
-// Without a place for partial results a workgroup has a tile, the last, longest ones
-// first.
+// Without a place for partial results a workgroup has a tile, the last ones first (of a
+// prompt the longest).
 //
 // Two workgroups are on a CU, and the waves of the first go first: where instructions
 // bound it, 65 blocks of 64 keys and 128 rows take the first 112 us and the second 154.

@@ -47,15 +47,19 @@ static int tile_rows(int64_t rows, int64_t dim, int64_t pairs, int64_t cus) {
 // Work is shared out over the workgroups that run at once, two a CU, where the waves divide the keys, and where there are
 // fewer than four tiles a CU: one tile's length more or less counts then (64 sequences of up to 8192 keys, 512 tiles of
 // 128 rows: 259 -> 184 us; with up to 16 tiles a CU four prompts of up to 3000 tokens, 2000 tiles, go from 230 to 401).
-// Single tokens of many sequences have a workgroup a tile too: a second tile costs a workgroup more than a new one does
-// (8 heads of 128: 256 sequences of up to 500, 1000 and 4000 keys 49, 72 and 217 us, shared out 60, 83 and 224; 128 of up to
-// 2000 and 8192 64 and 257, shared out 72 and 247: fewer are not even enough).
+// Single tokens of many sequences have a workgroup a tile too, if their tables have room for few keys: a second tile costs a
+// workgroup more than a new one does (8 heads of 128: 256 sequences of up to 500, 1000 and 4000 keys 51, 76 and 218 us, shared
+// out 60, 85 and 225; 128 of up to 2000 69 and 75), but then the longest sequence bounds the call.  So its run, 6.6 us for
+// 1024 keys, is to be no longer than the launch's rounds of two workgroups a CU, which take 7 us and more each.  Past that
+// 300 sequences of 500 keys with one of 131072 take 140 us shared out and 870-910 otherwise, 128 and 256 even ones of up to
+// 8192 242 and 473 against 255 and 483; and 300 of 500 alone, in tables with room for 131072, 85 where 74 would do.
 static AttnPlan plan_attention(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t keys) {
     const int64_t group = heads / kv_heads, rows = (tokens + seqs - 1) / seqs * group, cus = device_cus();
     AttnPlan P{};
     P.rows = tile_rows(rows, dim, std::min(seqs, tokens) * kv_heads, cus);
-    const bool few = P.rows <= 32, single = tokens == seqs;
+    const bool few = P.rows <= 32;
     const int64_t tiles = tokens * group / P.rows + std::min(seqs, tokens), blocks = (keys + ATTN_KEYS - 1) / ATTN_KEYS;
+    const bool single = tokens == seqs && keys * 2 * cus <= 1024 * tiles * kv_heads;
     P.tiles = (unsigned)(tokens * group / P.rows + seqs);                // as the kernels' find_slot counts
     if (tiles * kv_heads <= 4 * cus || (few && !single) || P.tiles * kv_heads > MAX_GRID / 2) {   // or more than a launch takes
         const int64_t each = few ? ATTN_WAVES : 1, units = tiles * kv_heads * std::max<int64_t>(blocks, 1);

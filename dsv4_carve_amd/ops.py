@@ -1191,7 +1191,9 @@ def fp8_attention(q: torch.Tensor, cache: Fp8Cache, table: torch.Tensor, lengths
     cache holds there; a page that it sees and whose scale is NaN, infinite or negative
     makes it NaN.  Positions behind the table's room have no key.  Tokens outside every sequence are left as they were in an
     `out` given, and are 0 otherwise; their logarithm is -inf.  Scratch is the call's
-    own (stream-ordered, capturable)."""
+    own (stream-ordered, capturable).  The table's width bounds the keys that a
+    sequence may have, and with it how the work is divided: columns that no sequence
+    needs cost many short single tokens up to a third of their time."""
     _check(q.dim() == 3 and q.dtype in X_KIND, "q must be fp16 or bf16 [tokens, heads, dim]")
     tokens, heads, dim = q.shape
     _check_cache(cache, table, lengths, starts, tokens, q.device)

@@ -55,3 +55,15 @@ def test_workgroups_of_an_xcd_are_neighbours():
         for x in range(min(8, n)):
             mine = [probe.exl3_probe_by_xcd(b, n) for b in range(x, n, 8)]
             assert mine == list(range(mine[0], mine[0] + len(mine)))
+
+
+@pytest.mark.parametrize("seqs,heads,kv,dim,keys,shared", [
+    (300, 32, 8, 128, 512, False), (300, 32, 8, 128, 131072, True), (129, 32, 8, 128, 16384, True), (256, 32, 8, 128, 4096, False),
+    (128, 32, 8, 128, 8192, True), (256, 32, 8, 128, 8192, True), (128, 32, 8, 128, 2048, False), (64, 32, 8, 128, 8192, True),
+    (4096, 8, 2, 128, 16384, False), (4096, 8, 2, 128, 1 << 20, True), (1 << 20, 8, 8, 64, 1 << 18, True)])
+def test_a_long_sequence_among_single_tokens_is_shared_out(seqs, heads, kv, dim, keys, shared):
+    """A workgroup a tile, which needs no scratch, only where the longest sequence that the table has room for takes no more
+    time than the launch's rounds, and the tiles are a launch (2^20 of 8 heads are not: (2^16 + 2^20) * 8 > 2^23)."""
+    need = _lib.load().exl3_fp8_attention_scratch_bytes
+    assert (need(seqs, heads, kv, dim, seqs, keys // 64, 64, 0) > 0) == shared
+    assert need(seqs, heads, kv, dim, seqs, (1 << 20) // 64, 64, 512) == need(seqs, heads, kv, dim, seqs, (1 << 24) // 64, 64, 512)

@@ -135,3 +135,17 @@ def test_attention_scales_that_are_none(dev, dim, counts, dtype):
                     within(lse[~hit], ref_lse[~hit], lse_tol[~hit], "lse")
                 else:
                     within(lse, ref_lse, lse_tol, "lse")
+
+
+@pytest.mark.parametrize("place", [0, 70, 140])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_one_long_sequence_among_many(dev, place, dtype):
+    gen = gen_of(dev, place)
+    lengths = [1 + (i * 37) % 90 for i in range(140)]
+    lengths.insert(place, 20000)
+    q, cache, table, n, _ = problem(gen, [1] * 141, lengths, heads=16, kv=8, dim=64, page=32, dtype=dtype)
+    assert ops._fp8_attention_scratch_bytes(dev.index or 0, 141, 16, 8, 64, 141, table.shape[1], 32, 0) > 0
+    check_attention(q, cache, table, n)
+    check_attention(q, cache, table, n, starts_of(dev, [1] * 141), window=33)
+    short = torch.arange(141, device=dev) != place
+    check_attention(q[short], cache, table[short][:, :3].contiguous(), n[short])
