@@ -6,7 +6,8 @@
 //
 // A power of two as the scale keeps a value's bits where the scale of a begun page
 // grows (but for those that fall below e4m3's normal range), and e4m3's relative
-// error does not depend on where in its range a value lies.
+// error does not depend on where in its range a value lies.  A begun page that has
+// another scale is written by that one.
 #pragma once
 
 #include "exl3_fp8.hpp"
@@ -260,6 +261,15 @@ struct Eight {
     }
 };
 
+// One value, from 64 bits, as an e4m3 code.
+__device__ __forceinline__ uint8_t code_of(double v) {
+    const float f = to_odd(v);
+    return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(f, f, 0, false);
+}
+__device__ __forceinline__ uint8_t rescale1(uint8_t u, float by) {
+    return code_of((double)__builtin_amdgcn_cvt_f32_fp8((int)u, 0) * (double)by);
+}
+
 // Four codes times a power of two, rounded to e4m3 again.
 __device__ __forceinline__ uint32_t rescale4(uint32_t u, float by) {
     return pack_e4m3(__builtin_amdgcn_cvt_f32_fp8((int)u, 0) * by, __builtin_amdgcn_cvt_f32_fp8((int)u, 1) * by,
@@ -382,6 +392,10 @@ __global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(App
     const float now = fmaxf(QuantGroup(most, true).scale, before);
     const float inverse = 1.0f / now, by = before / now;
     const bool grew = lo && by != 1.0f;
+    // A begun page's scale that is not this kernel's may be no power of two: then values are divided in 64 bits, where a
+    // quotient that is not on a border of e4m3 stays on its side (a product with a rounded 1 / now does not).  One by one:
+    // beside the others' code, eight a step cost every call 0.3 us (13 single tokens 4.2 -> 4.5), this costs it 0.1.
+    const bool exact = ((__float_as_uint(now) | __float_as_uint(before)) & 0x7fffffu) == 0;
     const auto put = [&](int i, const Eight<K>& v) {
         where(i, t, d);
         v.finite(x);
@@ -406,14 +420,30 @@ __global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(App
         v.load(in, in0 + t * stride + d);
         put(i, v);
     }
+    if (!exact) {
+        // each thread's own codes again
+#pragma unroll 1
+        for (int i = 0; i < ((chunks - tid + THREADS - 1) / THREADS) * 8; ++i) {
+            const int64_t from = where(tid + (i >> 3) * THREADS, t, d) + (i & 7);
+            d += i & 7;
+            const float v = load_kind<K>(in, from);
+            const uint8_t u = code_of(fabsf(v) == __builtin_inff() ? __builtin_nan("") : (double)v / (double)now);
+            if (values) append_codes[t * (C.dim + 4) + d] = (char)u;
+            else code[t * C.dim + d] = u;
+        }
+    }
     if (!values) {
-        if (grew)
+        if (grew && exact)
             for (int i = tid; i < lo * C.dim / 16; i += THREADS) {
                 u32x4_t u = reinterpret_cast<u32x4_t*>(code)[i];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) u[j] = rescale4(u[j], by);
                 reinterpret_cast<u32x4_t*>(code)[i] = u;
             }
+        if (grew && !exact) {
+#pragma unroll 1
+            for (int i = tid; i < lo * C.dim; i += THREADS) code[i] = rescale1(code[i], by);
+        }
     } else {
         if constexpr (TEAM > 64) __syncthreads();
         else asm volatile("" ::: "memory");                     // LDS keeps a wave's order, the compiler has to
@@ -443,13 +473,20 @@ __global__ __launch_bounds__(APPEND_WAVES * 64) void fp8_cache_append_kernel(App
                     const uint32_t below = bytes_before(lo - t0 - 4 * j), fresh = bytes_before(hi - t0 - 4 * j) & ~below;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint32_t u = old[e][j], moved = grew ? rescale4(u, by) : u;
+                        const uint32_t u = old[e][j], moved = grew && exact ? rescale4(u, by) : u;
                         made[e][j] = (made[e][j] & fresh) | (moved & below) | (u & ~(fresh | below));
                     }
                 }
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) *row(i, e) = made[e];
+            if (grew && !exact) {
+#pragma unroll 1
+                for (int j = 0; j < 64; ++j) {
+                    uint8_t* u = reinterpret_cast<uint8_t*>(row(i, j >> 4)) + (j & 15);
+                    if (t0 + (j & 15) < lo) *u = rescale1(*u, by);
+                }
+            }
         }
     }
     if (tid == 0) *scale = now;

@@ -177,6 +177,16 @@ struct QuantGroup {
     }
 };
 
+// v as the nearest float, but that an inexact one has its last bit set: rounding it
+// once more to fewer bits is rounding v.
+__device__ __forceinline__ float to_odd(double v) {
+    const float f = (float)v;
+    const double d = (double)f;
+    const uint32_t b = __float_as_uint(f);
+    const bool fix = d != v && !(b & 1u);
+    return __uint_as_float(fix ? (fabs(d) < fabs(v) ? b + 1 : b - 1) : b);
+}
+
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
 }

@@ -35,16 +35,6 @@ struct NormArgs {
 
 constexpr int NO_RESIDUAL = -1;
 
-// v as the nearest float, but that an inexact one has its last bit set: rounding it
-// once more to fewer bits is rounding v.
-__device__ __forceinline__ float to_odd(double v) {
-    const float f = (float)v;
-    const double d = (double)f;
-    const uint32_t b = __float_as_uint(f);
-    const bool fix = d != v && !(b & 1u);
-    return __uint_as_float(fix ? (fabs(d) < fabs(v) ? b + 1 : b - 1) : b);
-}
-
 // What a group's largest |h w| makes of its values g = h w.
 struct NormGroup {
     double mul, b;

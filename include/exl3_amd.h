@@ -394,7 +394,8 @@ int exl3_fp8_norm(const void* x, int x_kind, const void* residual, int residual_
  * 16-byte aligned; kind 0 = fp16, 1 = bf16, 2 = fp32).  A page's scale becomes the
  * smallest power of two s with max|x| <= 448 s over its new tokens (at least 2^-126;
  * NaN and infinities left out), or stays where the page holds tokens of the sequence
- * already and has a larger one; where it grows, their codes are rounded to it.  A NaN
+ * already and has a larger one (a power of two or not); where it grows, their codes are
+ * rounded to it.  A NaN
  * or an infinity becomes a NaN.  Tokens before position 0 are left out.  A page that
  * a call writes twice (two sequences, or one that names it twice) has a mixture of both.
  */

@@ -149,3 +149,42 @@ def test_attention_one_long_sequence_among_many(dev, place, dtype):
     check_attention(q, cache, table, n, starts_of(dev, [1] * 141), window=33)
     short = torch.arange(141, device=dev) != place
     check_attention(q[short], cache, table[short][:, :3].contiguous(), n[short])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("page,dim", [(16, 32), (64, 128), (256, 256)])
+@pytest.mark.parametrize("seqs", [3, 70])
+def test_append_to_pages_with_any_scale(dev, dtype, page, dim, seqs):
+    """A begun page's scale may be no power of two: values on a border of e4m3, or next to one, are rounded as quotients."""
+    gen = gen_of(dev, page + seqs)
+    kv, counts = 2, [1 + i % (page // 2) for i in range(seqs)]
+    cache = cache_on(gen, seqs, kv, page, dim)
+    table = torch.arange(seqs, device=dev, dtype=torch.int32).view(-1, 1)
+    tokens, starts = sum(counts), starts_of(dev, counts)
+    held = torch.tensor([(page - n) // 2 + 1 for n in counts], device=dev)
+    codes = torch.arange(0, 127, device=dev, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    border = (codes[1:] + codes[:-1]) / 2
+    pick = lambda *shape: border[torch.randint(len(border), shape, generator=gen, device=dev)]  # noqa: E731
+    odd = torch.tensor([1.25, 1.5, 1.75], device=dev, dtype=torch.float64)
+    scale = odd[torch.randint(3, (seqs, kv), generator=gen, device=dev)] * 0.25
+    of = torch.repeat_interleave(torch.arange(seqs, device=dev), torch.tensor(counts, device=dev))
+    # few-bit scales: the border times the scale is a 16-bit number, and lies on the border again when it is divided
+    cache.k_scale.copy_(scale)
+    cache.v_scale.copy_(scale)
+    k, v = ((pick(tokens, kv, dim) * scale[of][:, :, None]).to(dtype) for _ in range(2))
+    check_append(k, v, cache, table, (held + torch.tensor(counts, device=dev)).int(), starts)
+    # 24-bit scales, a new value that makes them grow to a power of two: an old code, a small whole number, comes next to a
+    # border, on the one side of it or the other
+    cache.k.copy_(cache.k.float().clamp(1, 15).round().to(cache.k.dtype))
+    cache.v.copy_(cache.v.float().clamp(1, 15).round().to(cache.v.dtype))
+    by = (pick(seqs, kv) / torch.randint(1, 16, (seqs, kv), generator=gen, device=dev)).float()
+    by = by / torch.exp2(torch.ceil(torch.log2(by)))                            # a half to one
+    cache.k_scale.copy_(by)
+    cache.v_scale.copy_(by)
+    k, v = (torch.randn((tokens, kv, dim), generator=gen, device=dev) for _ in range(2))
+    k[..., 0], v[..., 0] = 448, 448                                             # the scale 1
+    check_append(k.to(dtype), v.to(dtype), cache, table, (held + torch.tensor(counts, device=dev)).int(), starts)
+    # 24-bit scales that stay
+    cache.k_scale.copy_(by * 8)
+    cache.v_scale.copy_(by * 8)
+    check_append(k.to(dtype), v.to(dtype), cache, table, (held + torch.tensor(counts, device=dev)).int(), starts)
