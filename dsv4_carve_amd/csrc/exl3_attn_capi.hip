@@ -53,6 +53,10 @@ static int tile_rows(int64_t rows, int64_t dim, int64_t pairs, int64_t cus) {
 // 1024 keys, is to be no longer than the launch's rounds of two workgroups a CU, which take 7 us and more each.  Past that
 // 300 sequences of 500 keys with one of 131072 take 140 us shared out and 870-910 otherwise, 128 and 256 even ones of up to
 // 8192 242 and 473 against 255 and 483; and 300 of 500 alone, in tables with room for 131072, 85 where 74 would do.
+// Rows of a shared tile are joined by a workgroup each where a tile has more than five partial results, and by one for four
+// where it has fewer (us, a row each and four rows: one token of 131072 keys with one cache head 25.3 and 33.6, 24 tokens of a
+// 256-channel head 20.9 and 24.2, four of four tokens of 8192 23.2 and 27.4; 16 of five tokens 23.0 and 20.8, 512 tokens of
+// 1024 keys 56 and 45, of 16384 175 and 166.  64 tokens of 8192 are on the wrong side: 44 and 39).
 static AttnPlan plan_attention(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int64_t keys) {
     const int64_t group = heads / kv_heads, rows = (tokens + seqs - 1) / seqs * group, cus = device_cus();
     AttnPlan P{};

@@ -10,6 +10,10 @@
 // other side of a border.  Most values are nowhere near one, though: an fp32 quotient
 // whose both neighbours at its error's distance have the same code has that code, and
 // only a wave that holds another value divides in 64 bits (SURE).
+//
+// y in 16 bits goes by way of fp32: 2^-14 (fp16) and 2^-17 (bf16) of its values, next to
+// a border, round to the other side of it, by half a step and 2^-24.  Rounded once, 8000
+// rows of 4096 with y took 56 us instead of 53 and 333 rows of 1536 4.2 instead of 3.85.
 #pragma once
 
 #include "exl3_fp8.hpp"

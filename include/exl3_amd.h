@@ -366,10 +366,11 @@ int exl3_moe_route(const void* logits, int logits_kind, int64_t rows, int64_t n_
  * block-scaled products read it: h = x + residual (or x), y = h / sqrt(mean(h^2)
  * + eps) * weight, (q, scale) = exl3_fp8_quantize's formula on y, all of it in 64
  * bits up to each result's rounding.  sum: h in the residual's type (may be the
- * residual itself).  normed: y as normed_kind, or null.  A row whose sum of squares
- * is not finite has what 64-bit arithmetic makes of y: NaN (its scales 2^-126), or
- * 0 beside an infinity.  Kinds 0 = fp16, 1 = bf16, 2 = fp32; the residual is of x's
- * kind or fp32, or null; any rows >= 1, 1 <= k <= 2^24, 0 <= eps finite.
+ * residual itself).  normed: y as normed_kind (16 bits by way of fp32), or null.  A
+ * row whose sum of squares is not finite has what 64-bit arithmetic makes of y: NaN
+ * (its scales 2^-126), or 0 beside an infinity.  Kinds 0 = fp16, 1 = bf16, 2 = fp32;
+ * the residual is of x's kind or fp32, or null; any rows >= 1, 1 <= k <= 2^24,
+ * 0 <= eps finite.
  */
 int exl3_fp8_norm(const void* x, int x_kind, const void* residual, int residual_kind, const void* weight,
                   int weight_kind, int64_t rows, int64_t k, float eps, int pow2, uint8_t* q, float* scale, void* sum,
@@ -394,10 +395,10 @@ int exl3_fp8_norm(const void* x, int x_kind, const void* residual, int residual_
  * 16-byte aligned; kind 0 = fp16, 1 = bf16, 2 = fp32).  A page's scale becomes the
  * smallest power of two s with max|x| <= 448 s over its new tokens (at least 2^-126;
  * NaN and infinities left out), or stays where the page holds tokens of the sequence
- * already and has a larger one (a power of two or not); where it grows, their codes are
- * rounded to it.  A NaN
- * or an infinity becomes a NaN.  Tokens before position 0 are left out.  A page that
- * a call writes twice (two sequences, or one that names it twice) has a mixture of both.
+ * already and has a larger one (a power of two or not); where it grows, their codes
+ * are rounded to it.  A NaN or an infinity becomes a NaN.  Tokens before position 0
+ * are left out.  A page that a call writes twice (two sequences, or one that names it
+ * twice) has a mixture of both.
  */
 int exl3_fp8_cache_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
                           int64_t v_head, int kind, int64_t tokens, uint8_t* k_cache, float* k_scale,
