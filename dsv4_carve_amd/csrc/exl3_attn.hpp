@@ -773,9 +773,9 @@ struct Work {
 
 // Few rows a sequence: the four waves of a workgroup go through a tile's blocks in
 // turn, each with a place of its own in LDS, and join their sums there.  Bound by memory
-// where there is much of it: 64 ragged contexts of up to 8192, 593 MB, 119 us (5.0 TB/s);
+// where there is much of it: 64 ragged contexts of up to 8192, 593 MB, 121 us (4.9 TB/s);
 // one of 131072, 268 MB, 48 us and 5 for the join.  A short call is a chain: lookup,
-// first loads, a block's instructions, join (one token of 1000 keys: 10.7 us with the
+// first loads, a block's instructions, join (one token of 1000 keys: 11 us with the
 // join kernel).  Two workgroups of heads of up to 128 channels are on a CU.
 template <int DIM, bool BF16, int RB>
 __global__ __launch_bounds__(ATTN_WAVES * 64, (AttnSize<DIM, RB>::WAVES_EU)) void fp8_attention_kernel(AttnArgs A) {
@@ -934,7 +934,7 @@ struct ShareSize {
 // vector instructions: a wave widens the codes of a whole block for its 32 rows (16 where
 // heads are wider than 128, for the registers: 329 us where 32 rows spilled in 522), and
 // the exponentials come on top.  512 tokens behind 16384 keys, 32 heads over 8 of 128:
-// 171-176 us, 780 TFLOP/s, the matrix unit 41% busy.  The 8-bit product on the codes as
+// 165-175 us, 790 TFLOP/s, the matrix unit 41% busy.  The 8-bit product on the codes as
 // they are (queries in two e4m3 parts) took 167 for 180, but its sums are not fp32's:
 // logits were up to 2^-16 of their terms' sum off.  256 rows a workgroup of eight waves: no faster.
 template <int DIM, bool BF16, int RB>

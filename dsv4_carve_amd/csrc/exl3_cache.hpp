@@ -294,7 +294,7 @@ __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
 // are turned in LDS: tokens of a channel are neighbours in the cache.  Four chunks of
 // up to 2000 tokens, 8 heads of 128 (30 MB): 12 us; read twice and values gathered two
 // bytes a load 18.4.
-// 13 single tokens: 4.2 us, a chain of lookup, page, inputs, reduction and store.
+// 13 single tokens: 4.4 us, a chain of lookup, page, inputs, reduction and store.
 constexpr int APPEND_HOLD = 8;
 
 __host__ __device__ inline int append_lds(int page, int dim) { return page * (dim + 4); }
