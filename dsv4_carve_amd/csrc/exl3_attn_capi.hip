@@ -52,7 +52,8 @@ static int tile_rows(int64_t rows, int64_t dim, int64_t pairs, int64_t cus) {
 // out 60, 85 and 225; 128 of up to 2000 69 and 75), but then the longest sequence bounds the call.  So its run, 6.6 us for
 // 1024 keys, is to be no longer than the launch's rounds of two workgroups a CU, which take 7 us and more each.  Past that
 // 300 sequences of 500 keys with one of 131072 take 140 us shared out and 870-910 otherwise, 128 and 256 even ones of up to
-// 8192 242 and 473 against 255 and 483; and 300 of 500 alone, in tables with room for 131072, 85 where 74 would do.
+// 8192 242 and 473 against 255 and 483; but in tables with room for 131072, 300 of 500 take 85 where 74 would do, and 1024 of
+// up to 128 with two cache heads 50 instead of 34.
 // Rows of a shared tile are joined by a workgroup each where a tile has more than five partial results, and by one for four
 // where it has fewer (us, a row each and four rows: one token of 131072 keys with one cache head 25.3 and 33.6, 24 tokens of a
 // 256-channel head 20.9 and 24.2, four of four tokens of 8192 23.2 and 27.4; 16 of five tokens 23.0 and 20.8, 512 tokens of

@@ -1193,7 +1193,7 @@ def fp8_attention(q: torch.Tensor, cache: Fp8Cache, table: torch.Tensor, lengths
     `out` given, and are 0 otherwise; their logarithm is -inf.  Scratch is the call's
     own (stream-ordered, capturable).  The table's width bounds the keys that a
     sequence may have, and with it how the work is divided: columns that no sequence
-    needs cost many short single tokens up to a third of their time."""
+    needs cost single tokens of many short sequences up to half as much time again."""
     _check(q.dim() == 3 and q.dtype in X_KIND, "q must be fp16 or bf16 [tokens, heads, dim]")
     tokens, heads, dim = q.shape
     _check_cache(cache, table, lengths, starts, tokens, q.device)
