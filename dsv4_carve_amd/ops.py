@@ -1189,11 +1189,12 @@ def fp8_attention(q: torch.Tensor, cache: Fp8Cache, table: torch.Tensor, lengths
     denominator, fp32 [tokens, heads].  A query that sees no key has 0 (and -inf, or
     its sink); a key that it does not see has no part in its result, whatever the
     cache holds there; a page that it sees and whose scale is NaN, infinite or negative
-    makes it NaN.  Positions behind the table's room have no key.  Tokens outside every sequence are left as they were in an
-    `out` given, and are 0 otherwise; their logarithm is -inf.  Scratch is the call's
-    own (stream-ordered, capturable).  The table's width bounds the keys that a
-    sequence may have, and with it how the work is divided: columns that no sequence
-    needs cost single tokens of many short sequences up to half as much time again."""
+    makes it NaN.  Positions behind the table's room have no key.  Tokens outside every
+    sequence are left as they were in an `out` given, and are 0 otherwise; their
+    logarithm is -inf.  Scratch is the call's own (stream-ordered, capturable).  The
+    table's width bounds the keys that a sequence may have, and with it how the work is
+    divided: columns that no sequence needs cost single tokens of many short sequences
+    up to half as much time again."""
     _check(q.dim() == 3 and q.dtype in X_KIND, "q must be fp16 or bf16 [tokens, heads, dim]")
     tokens, heads, dim = q.shape
     _check_cache(cache, table, lengths, starts, tokens, q.device)
